@@ -48,6 +48,13 @@ class BnLlamaLayer(C.Structure):
                                           "k_cache", "v_cache")]
 
 
+class BnPagedKV(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "page_table", "seq_lens")] + \
+               [(n, C.c_int64) for n in ("page_stride", "head_stride", "row_stride", "table_stride")] + \
+               [(n, C.c_int32) for n in ("dtype", "batch", "n_pages", "max_pages", "page_size",
+                                         "n_kv_heads", "head_dim")]
+
+
 class BnError(RuntimeError):
     def __init__(self, status, msg):
         super().__init__(msg)
@@ -74,7 +81,7 @@ def lib():
     except ImportError:
         pass
     L = C.CDLL(LIB_PATH)
-    vp, V = C.c_void_p, C.POINTER(BnView)
+    vp, V, P = C.c_void_p, C.POINTER(BnView), C.POINTER(BnPagedKV)
     i, f, i64, sz = C.c_int, C.c_float, C.c_int64, C.c_size_t
     sig = {
         "bn_abi_version": ([], i), "bn_last_error": ([], C.c_char_p),
@@ -116,6 +123,11 @@ def lib():
         "bn_gqa_decode_planned": ([i, vp, vp, vp, vp, vp, vp] + [i] * 5 + [f, vp, sz, vp], i),
         "bn_gqa_decode_planned_strided": ([i, vp, vp, vp, vp, vp, vp] + [i] * 5 + [i64] * 3 +
                                           [f, vp, sz, vp], i),
+        "bn_paged_append": ([P, vp, vp, vp, vp, vp, i, i] + [i64] * 4 + [f, vp], i),
+        "bn_paged_workspace_size": ([P, i, i, i], sz),
+        "bn_paged_decode": ([P, vp, vp, i, i64, i64, f, vp, sz, vp], i),
+        "bn_paged_prefill": ([P, vp, vp, vp, i, i, i64, i64, f, vp, sz, vp], i),
+        "bn_paged_decode_shared": ([P, vp, vp, i, i64, i64, f, vp, i, vp, sz, vp], i),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -335,3 +347,151 @@ def decode_workspace(B, Lmax, H, D=64):
     import torch
     n = lib().bn_gqa_decode_workspace_size(B, Lmax, H, D)
     return torch.empty(max(n, 4), dtype=torch.uint8, device="cuda")
+
+
+# ----------------------------------------------------------- paged KV cache
+class PagedKV:
+    """A paged KV cache as the ``paged_*`` calls take it: k_pages and v_pages
+    [n_pages, Hkv, page_size, D] (any strides, rows contiguous: the token-major
+    pool [n_pages, page_size, Hkv, D] is passed as its ``transpose(1, 2)``),
+    page_table int32 [B, max_pages] and seq_lens int32 [B] on the device.  The
+    tensors are the caller's: the calls read the table and the lengths that
+    stand there when they run."""
+
+    def __init__(self, k_pages, v_pages, page_table, seq_lens):
+        import torch
+        if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride():
+            raise ValueError("PagedKV: k_pages and v_pages must be [n_pages, Hkv, page_size, D] of the "
+                             "same shape and strides")
+        if k_pages.stride(3) != 1:
+            raise ValueError("PagedKV: key rows must be contiguous (stride 1 along head_dim)")
+        if k_pages.dtype not in (torch.float32, torch.bfloat16) or v_pages.dtype != k_pages.dtype:
+            raise ValueError("PagedKV: pools must be float32 or bfloat16, both alike")
+        if page_table.dim() != 2 or seq_lens.shape != page_table.shape[:1]:
+            raise ValueError("PagedKV: page_table must be [B, max_pages] and seq_lens [B]")
+        if page_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+            raise ValueError("PagedKV: page_table and seq_lens must be int32")
+        if (page_table.shape[1] > 1 and page_table.stride(1) != 1) or not seq_lens.is_contiguous():
+            raise ValueError("PagedKV: page_table rows and seq_lens must be contiguous")
+        if len({t.device for t in (k_pages, v_pages, page_table, seq_lens)}) != 1:
+            raise ValueError("PagedKV: tensors on different devices")
+        self.k_pages, self.v_pages, self.page_table, self.seq_lens = k_pages, v_pages, page_table, seq_lens
+        n_pages, hkv, page_size, d = k_pages.shape
+        batch, max_pages = page_table.shape
+        self.view = BnPagedKV(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+                              seq_lens.data_ptr(), k_pages.stride(0), k_pages.stride(1), k_pages.stride(2),
+                              page_table.stride(0), _torch_dtype_code(k_pages), batch, n_pages, max_pages,
+                              page_size, hkv, d)
+        self.ref = C.byref(self.view)
+
+
+def _paged_rows(what, t, cache, rows, heads=None):
+    """(pointer, row stride) of a [rows, heads, D] tensor whose heads are
+    contiguous within a row, of the cache's type."""
+    v = cache.view
+    if t.dim() != 3 or t.shape[2] != v.head_dim or (heads is not None and t.shape[1] != heads) or \
+            (rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{what}: expected [{'rows' if rows is None else rows}, "
+                         f"{'heads' if heads is None else heads}, {v.head_dim}], got {tuple(t.shape)}")
+    if t.dtype != cache.k_pages.dtype or t.device != cache.k_pages.device:
+        raise ValueError(f"{what}: dtype and device must be the cache's")
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError(f"{what}: a row's heads must be contiguous")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _cache_stream(cache, stream):
+    import torch
+    return stream_of(torch.cuda.current_stream(cache.k_pages.device) if stream is None else stream)
+
+
+def _row_starts(what, row_starts, cache, n_rows):
+    import torch
+    if row_starts is None:
+        if n_rows != cache.view.batch:
+            raise ValueError(f"{what}: without row_starts there is one row per sequence")
+        return None
+    if row_starts.dtype != torch.int32 or tuple(row_starts.shape) != (cache.view.batch + 1,) or \
+            not row_starts.is_contiguous() or row_starts.device != cache.k_pages.device:
+        raise ValueError(f"{what}: row_starts must be int32 [B + 1] on the cache's device")
+    return row_starts.data_ptr()
+
+
+def _workspace(workspace):
+    return (None, 0) if workspace is None else (workspace.data_ptr(),
+                                                workspace.numel() * workspace.element_size())
+
+
+def paged_workspace(cache, n_heads, n_rows, prefix_len=0):
+    """A workspace for the attention calls over the cache with up to n_rows
+    query rows (and prefix_len common keys); one per call in flight."""
+    import torch
+    n = lib().bn_paged_workspace_size(cache.ref, n_heads, n_rows, prefix_len)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k_pages.device)
+
+
+def paged_append(cache, k, v, q=None, q_out=None, row_starts=None, theta=10000.0, stream=None):
+    """Rotates the new rows' keys (and queries) by their positions and stores
+    keys and values in the pages: k, v [rows, Hkv, D], q [rows, H, D] torch
+    tensors, each with contiguous heads and a row stride of its own; rows of
+    sequence b: row_starts[b] .. row_starts[b+1]-1 (None: one row each), the
+    last of them at position seq_lens[b] - 1.  Returns q_out (default: in
+    place), or None without q."""
+    n = k.shape[0]
+    kp, ks = _paged_rows("paged_append: k", k, cache, n, cache.view.n_kv_heads)
+    vp, vs = _paged_rows("paged_append: v", v, cache, n, cache.view.n_kv_heads)
+    qp, qs, op, os_, heads = None, 0, None, 0, 0
+    if q is not None:
+        q_out = q if q_out is None else q_out
+        heads = q.shape[1]
+        qp, qs = _paged_rows("paged_append: q", q, cache, n)
+        op, os_ = _paged_rows("paged_append: q_out", q_out, cache, n, heads)
+    elif q_out is not None:
+        raise ValueError("paged_append: q_out without q")
+    call("bn_paged_append", cache.ref, kp, vp, qp, op, _row_starts("paged_append", row_starts, cache, n),
+         n, heads, ks, vs, qs, os_, theta, _cache_stream(cache, stream))
+    return q_out
+
+
+def paged_decode(q, cache, o=None, scale=None, workspace=None, stream=None):
+    """One query row per sequence over its pages: q, o [B, H, D]."""
+    import torch
+    o = torch.empty_like(q) if o is None else o
+    qp, qs = _paged_rows("paged_decode: q", q, cache, cache.view.batch)
+    op, os_ = _paged_rows("paged_decode: o", o, cache, cache.view.batch, q.shape[1])
+    call("bn_paged_decode", cache.ref, qp, op, q.shape[1], qs, os_,
+         1.0 / math.sqrt(q.shape[2]) if scale is None else scale, *_workspace(workspace), _cache_stream(cache, stream))
+    return o
+
+
+def paged_prefill(q, cache, row_starts=None, o=None, scale=None, workspace=None, stream=None):
+    """The new rows of a ragged batch over the cache, causal: q, o [rows, H, D],
+    rows of sequence b row_starts[b] .. row_starts[b+1]-1, the last of them
+    at position seq_lens[b] - 1 (rows of no sequence are left as they are)."""
+    import torch
+    o = torch.empty_like(q) if o is None else o
+    n = q.shape[0]
+    qp, qs = _paged_rows("paged_prefill: q", q, cache, None)
+    op, os_ = _paged_rows("paged_prefill: o", o, cache, n, q.shape[1])
+    call("bn_paged_prefill", cache.ref, qp, op, _row_starts("paged_prefill", row_starts, cache, n), n,
+         q.shape[1], qs, os_, 1.0 / math.sqrt(q.shape[2]) if scale is None else scale,
+         *_workspace(workspace), _cache_stream(cache, stream))
+    return o
+
+
+def paged_decode_shared(q, cache, prefix_pages, prefix_len, o=None, scale=None, workspace=None, stream=None):
+    """paged_decode of a batch whose sequences begin with the same prefix_len
+    keys, those of prefix_pages (int32, device), read once for all."""
+    import torch
+    o = torch.empty_like(q) if o is None else o
+    qp, qs = _paged_rows("paged_decode_shared: q", q, cache, cache.view.batch)
+    op, os_ = _paged_rows("paged_decode_shared: o", o, cache, cache.view.batch, q.shape[1])
+    if prefix_pages.dtype != torch.int32 or prefix_pages.dim() != 1 or not prefix_pages.is_contiguous() or \
+            prefix_pages.device != cache.k_pages.device or prefix_len < 0 or \
+            prefix_pages.shape[0] < -(-prefix_len // cache.view.page_size):
+        raise ValueError("paged_decode_shared: prefix_pages must be int32 [ceil(prefix_len / page_size)] "
+                         "on the cache's device")
+    call("bn_paged_decode_shared", cache.ref, qp, op, q.shape[1], qs, os_,
+         1.0 / math.sqrt(q.shape[2]) if scale is None else scale, prefix_pages.data_ptr(), prefix_len,
+         *_workspace(workspace), _cache_stream(cache, stream))
+    return o

@@ -440,6 +440,97 @@ int bn_gqa_decode_noalloc(int dtype, const void *q, const void *k_cache,
                           int batch, int max_len, int n_heads, int n_kv_heads,
                           int head_dim, float scale, void *stream);
 
+/* ----------------------------------------------------------- paged KV cache
+ * No counterpart in the reference (it keeps no cache, llama_model.py:135-141
+ * recomputes the prefix): keys and values of many sequences in one pool of
+ * pages, so that a sequence takes memory as it grows and sequences can have
+ * pages in common.  Key j of sequence b lies in page
+ * page_table[b*table_stride + j / page_size], slot j % page_size; element d of
+ * KV head g of a page's slot s is
+ *   pool[page*page_stride + g*head_stride + s*row_stride + d]
+ * (strides in elements, multiples of 16 bytes, the same for K and V; a
+ * [n_pages, n_kv_heads, page_size, 64] pool streams fastest, a [n_pages,
+ * page_size, n_kv_heads, 64] one is as good a layout).  seq_lens[b] keys of
+ * sequence b are in the cache, the rows of the present call included: a row
+ * is appended, and attends to itself, under a length that counts it.  Both
+ * arrays are device int32, read on the device by every call (nothing is kept
+ * from one call for the next): a length below 1 is an empty sequence, one
+ * above max_pages*page_size counts as that many keys.  A page number outside
+ * [0, n_pages) has no memory: its keys are not stored and are hidden from every
+ * query (a page that was given up, an entry not yet set).  Entries past a
+ * sequence's last key are not looked at.  page_size: a power of two.
+ * head_dim must be 64, and dtype BN_F32 or BN_BF16 for the pools, the queries
+ * and the outputs alike; sums and softmax statistics are fp32.  Any number of
+ * query heads per KV head; query head h reads KV head h / (n_heads /
+ * n_kv_heads).
+ *
+ * New rows of a ragged batch lie one after another: sequence b's are rows
+ * row_starts[b] .. row_starts[b+1] - 1 (device int32 [batch + 1], not
+ * decreasing), row i of its n at position seq_lens[b] - n + i.  row_starts
+ * NULL: one row per sequence (n_rows == batch).  n_rows counts the rows that
+ * the tensors have; rows below row_starts[0] and from row_starts[batch] on are
+ * padding, neither read nor written. */
+typedef struct bn_paged_kv {
+  void *k, *v;               /* pools (device) */
+  const int32_t *page_table; /* device [batch, table_stride], max_pages entries a row */
+  const int32_t *seq_lens;   /* device [batch] */
+  int64_t page_stride, head_stride, row_stride, table_stride; /* elements */
+  int32_t dtype, batch, n_pages, max_pages, page_size, n_kv_heads, head_dim;
+} bn_paged_kv;
+
+/* Appends a batch's new keys and values to the cache and rotates its new
+ * queries, in one launch: with pos the row's position and the angle
+ * pos * theta^(-2p/64) formed in 64 bits, pair p of every head of k and q
+ * turns as bn_rope turns it, (x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos); K
+ * and V go to the row's place in the pools, q to q_out (which may be q).
+ * theta 0: nothing is turned.  k, v: [n_rows, n_kv_heads, 64] with row
+ * strides of their own (column ranges of a QKV projection's output are such
+ * tensors); q, q_out: [n_rows, n_heads, 64] or both NULL.  A row whose position
+ * lies outside the table, or on a page without memory, is not stored (its q
+ * is written all the same); two rows that land on one place leave either's
+ * elements there.  k, v, q and q_out must not lie in the pools. */
+int bn_paged_append(const bn_paged_kv *cache, const void *k, const void *v,
+                    const void *q, void *q_out, const int32_t *row_starts,
+                    int n_rows, int n_heads, int64_t k_row_stride,
+                    int64_t v_row_stride, int64_t q_row_stride,
+                    int64_t q_out_row_stride, float theta, void *stream);
+
+/* Workspace of the three attention calls below for up to n_rows query rows
+ * (decode: the batch) and prefix_len common keys (0 without): bytes of device
+ * memory, 16-byte aligned, any contents.  NULL there: the pool supplies it.
+ * Calls in flight at once need workspaces of their own. */
+size_t bn_paged_workspace_size(const bn_paged_kv *cache, int n_heads, int n_rows,
+                               int prefix_len);
+
+/* One query row per sequence over its seq_lens[b] keys: bn_gqa_decode over a
+ * paged cache.  q, o: [batch, n_heads, 64] with row strides.  A sequence with
+ * no visible key gives zeros. */
+int bn_paged_decode(const bn_paged_kv *cache, const void *q, void *o, int n_heads,
+                    int64_t q_row_stride, int64_t o_row_stride, float scale,
+                    void *workspace, size_t workspace_bytes, void *stream);
+
+/* The new rows of a ragged batch over the cache, causal: the row at position
+ * pos sees the keys 0 .. pos (prompts, chunks behind cached keys, or a few rows
+ * per sequence).  q, o: [n_rows, n_heads, 64] with row strides.  Rows that see
+ * no key give zeros. */
+int bn_paged_prefill(const bn_paged_kv *cache, const void *q, void *o,
+                     const int32_t *row_starts, int n_rows, int n_heads,
+                     int64_t q_row_stride, int64_t o_row_stride, float scale,
+                     void *workspace, size_t workspace_bytes, void *stream);
+
+/* bn_paged_decode for a batch whose sequences begin with the same prefix_len
+ * keys (a system prompt, the samples of one prompt): keys below prefix_len
+ * are those of prefix_pages (device int32, ceil(prefix_len / page_size)
+ * entries) for every sequence, read once for all of them; the others come from
+ * the sequence's own table, whose entries for pages wholly below prefix_len
+ * are not looked at.  seq_lens counts the prefix; a sequence shorter than it
+ * sees its first seq_lens[b] keys of it. */
+int bn_paged_decode_shared(const bn_paged_kv *cache, const void *q, void *o,
+                           int n_heads, int64_t q_row_stride,
+                           int64_t o_row_stride, float scale,
+                           const int32_t *prefix_pages, int prefix_len,
+                           void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,552 @@
+"""The paged KV cache's operators against their plain form in 64 bits (paged_util): lengths around
+every tile and page border, empty sequences, ragged rows with padding around them, pages without
+memory, places that hold NaN and infinities, odd strides and layouts, any group of heads; then
+graphs, streams, shared workspaces and the operators together as a server uses them."""
+import numpy as np
+import pytest
+import torch
+
+import bnhip as B
+from gpu_util import require_gpu
+from paged_util import D, TD, Case, attention64, check, rotate64, rows_of, starts_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    require_gpu()
+
+
+def wide(x, pad, fill=float("nan")):
+    """x [n, heads, D] on the device as a column range of a wider tensor (and that tensor)."""
+    n, h, d = x.shape
+    base = torch.full((n, h * d + pad), fill, dtype=x.dtype, device="cuda")
+    v = base[:, pad // 2:pad // 2 + h * d].unflatten(1, (h, d))
+    v.copy_(x)
+    return v, base
+
+
+def host(t):
+    torch.cuda.synchronize()
+    return t.double().cpu().numpy()
+
+
+def bits(t):
+    return t.contiguous().view(torch.int16 if t.dtype == torch.bfloat16 else torch.int32)
+
+
+# ------------------------------------------------------------------- append
+APPENDS = [
+    # dtype, lens (after), new rows, Hkv, H, page, layout, theta, q: None / "out" / "in place"
+    ("bf16", [1, 17, 300], [1, 1, 1], 4, 32, 16, True, 1e4, "out"),
+    ("f32", [1, 17, 300], [1, 1, 1], 4, 32, 16, False, 1e4, "in place"),
+    ("bf16", [40, 0, 33, 9], [40, 0, 2, 9], 2, 6, 8, "gaps", 1e4, "out"),
+    ("f32", [65, 64, 63], [65, 1, 40], 1, 1, 64, True, 5e5, None),
+    ("bf16", [70, 3], [70, 5], 3, 15, 1, False, 0.0, "in place"),      # more rows than the length
+    ("f32", [1000, 700], [900, 650], 2, 4, 32, True, 1e4, "out"),      # many rows a workgroup
+    ("bf16", [1200, 400, 64], [1200, 1, 64], 4, 8, 128, False, 1e4, "in place"),
+    ("bf16", [-3, 5], [2, 5], 2, 2, 16, True, 1e4, "out"),             # a negative length is empty
+]
+
+
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("case", APPENDS, ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_append(case, pad):
+    dtype, lens, rows, Hkv, H, page, layout, theta, q_how = case
+    print("append", case, pad, flush=True)
+    drop = [(0, 0)] if pad else []
+    c = Case(dtype, lens, Hkv, page, layout, seed=len(lens), drop=drop, junk=2**31 - 1, pad_table=pad)
+    total = sum(rows) + 2 * pad
+    n64 = {w: rows_of(dtype, total, h, 7 + i) for i, (w, h) in enumerate((("k", Hkv), ("v", Hkv), ("q", H)))}
+    cache = c.cuda(B)
+    k, _ = wide(n64["k"].cuda(), 16)
+    v, _ = wide(n64["v"].cuda(), 48)
+    q, qbase = wide(n64["q"].cuda(), 16)
+    out, obase = wide(torch.full_like(n64["q"], 7.0).cuda(), 32, 7.0)
+    st = starts_of(rows, pad)
+    starts = None if not pad and all(n == 1 for n in rows) else torch.from_numpy(st).cuda()
+    want_k, want_v = c.k.double().numpy(), c.v.double().numpy()
+    tol_k = np.zeros_like(want_k)
+    eps = torch.finfo(TD[dtype]).eps / 2
+    want_q = n64["q"].double().numpy().copy() if q_how == "in place" else np.full((total, H, D), 7.0)
+    tol_q = np.zeros_like(want_q)
+
+    def tol(x, y):  # cos and sin off by 2 2^-24 (units: up to 1), two products, a sum; then the type's half step
+        pair = np.abs(x).reshape(x.shape[0], -1, 2).sum(2, keepdims=True).repeat(2, 2).reshape(x.shape)
+        return 0 * y if theta == 0 else pair * 6 * 2.0 ** -24 + (np.abs(y) + pair * 2.0 ** -21) * eps
+
+    for b, n in enumerate(rows):
+        for i in range(n):
+            row, pos = pad + sum(rows[:b]) + i, max(lens[b], 0) - n + i
+            xq, xk = n64["q"][row].double().numpy(), n64["k"][row].double().numpy()
+            want_q[row] = rotate64(xq, pos, theta)
+            tol_q[row] = tol(xq, want_q[row])
+            at = c.place(b, pos)
+            if at:
+                want_k[at[0], :, at[1]] = rotate64(xk, pos, theta)
+                tol_k[at[0], :, at[1]] = tol(xk, want_k[at[0], :, at[1]])
+                want_v[at[0], :, at[1]] = n64["v"][row].double().numpy()
+    got = B.paged_append(cache, k, v, q=q if q_how else None, q_out=out if q_how == "out" else None,
+                         row_starts=starts, theta=theta)
+    gk, gv = host(c.kd), host(c.vd)
+    for g, w, t, what in ((gk, want_k, tol_k, "k"), (gv, want_v, 0 * tol_k, "v")):
+        same = np.isnan(g) & np.isnan(w) | (g == w)
+        off = np.abs(np.where(same, 0, np.where(same, 0, g) - np.where(same, 0, w)))
+        assert (off <= t).all(), f"{what}: {int((~(off <= t)).sum())} wrong, worst {np.nanmax(off - t):.2e}"
+    if q_how:
+        assert got is (out if q_how == "out" else q)
+        off = np.abs(host(got) - want_q)
+        assert (off <= tol_q).all(), f"q: worst {np.max(off - tol_q):.2e}"
+        if q_how == "out":   # around the output nothing was touched
+            assert (host(obase)[:, :16] == 7.0).all() and (host(obase)[:, -16:] == 7.0).all()
+            assert torch.equal(bits(q), bits(n64["q"].cuda()))
+    else:
+        assert got is None
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_append_far_positions(dtype):
+    """Angles of far positions: a 32-bit product of position and frequency would be off by 0.06 rad
+    at 2^20 and by a whole turn and more at 2^29."""
+    page, last = 1 << 15, (1 << 30) - 1
+    pos = [2 ** 20 + 1, 123456789, last, 2 ** 24 + 3]
+    Bn, Hkv, H = len(pos), 1, 2
+    table = np.full((Bn, (1 << 30) // page), -1, np.int32)
+    for b, p in enumerate(pos):
+        table[b, p // page] = b
+    kd = torch.zeros((Bn, Hkv, page, D), dtype=TD[dtype], device="cuda")
+    vd = torch.zeros_like(kd)
+    cache = B.PagedKV(kd, vd, torch.from_numpy(table).cuda(),
+                      torch.tensor([p + 1 for p in pos], dtype=torch.int32, device="cuda"))
+    k, v, q = (rows_of(dtype, Bn, h, 3 + h) for h in (1, 1, 2))
+    out = B.paged_append(cache, k.cuda(), v.cuda(), q=q.cuda())
+    eps = torch.finfo(TD[dtype]).eps / 2
+    for b, p in enumerate(pos):
+        for got, x in ((out[b], q[b]), (kd[b, :, p % page], k[b])):
+            w = rotate64(x.double().numpy(), p, 1e4)
+            # the test's own angle, in 64 bits: off by 2^30 2^-52 at most
+            t = np.abs(x.double().numpy()).sum() * (6 * 2.0 ** -24 + 2.0 ** -20 * (dtype == "f32") * 2.0 ** -1) + np.abs(w) * eps
+            assert (np.abs(host(got) - w) <= t).all(), (b, p)
+    assert torch.equal(vd[range(Bn), :, [p % page for p in pos]], v.cuda())
+
+
+# ------------------------------------------------------------------- decode
+EDGES = [0, 1, 2, 7, 8, 15, 16, 17, 31, 32, 33, 63, 64, 65, 95, 96, 97, 127, 128, 129, 255, 256, 257, 300]
+DECODES = [
+    # dtype, lens, Hkv, H, page, layout, dropped pages (sequence, index)
+    ("bf16", EDGES, 2, 16, 16, True, []),
+    ("f32", EDGES, 2, 16, 16, True, []),
+    ("bf16", EDGES, 1, 3, 8, False, [(20, 3), (23, 0)]),
+    ("f32", EDGES, 3, 15, 32, "gaps", [(20, 3), (23, 0), (2, 0)]),
+    ("bf16", EDGES, 1, 16, 64, "gaps", [(16, 0), (20, 1)]),
+    ("bf16", EDGES, 1, 20, 128, True, []),             # more heads a KV head than a tile holds
+    ("f32", EDGES, 2, 66, 1, False, []),
+    ("bf16", EDGES[:14], 5, 5, 1, True, [(13, 11), (13, 63)]),
+    ("bf16", [1000], 1, 8, 256, True, [(0, 1)]),
+    ("bf16", [513] * 3 + [2000], 4, 32, 16, True, []),
+    ("f32", [513] * 3 + [2000], 4, 32, 16, False, []),
+    ("bf16", [-7, 0, 0], 2, 2, 16, True, []),           # nothing at all
+    ("f32", [50, 2 ** 31 - 1, -2 ** 31], 2, 4, 16, True, []),  # lengths past the table
+    ("bf16", [3] * 70 + [1], 8, 8, 16, True, []),
+]
+
+
+@pytest.mark.parametrize("case", DECODES, ids=lambda c: f"{c[0]}-{len(c[1])}x{max(c[1])}-{c[2]}-{c[3]}-p{c[4]}-{c[5]}-d{len(c[6])}")
+def test_decode(case):
+    dtype, lens, Hkv, H, page, layout, drop = case
+    print("decode", case, flush=True)
+    big = max(lens) > 10 ** 6
+    c = Case(dtype, lens, Hkv, page, layout, drop=drop, seed=H, max_pages=4 if big else None,
+             junk=2 ** 31 - 1, pad_table=5)
+    q = rows_of(dtype, len(lens), H, 1)
+    ref, tol = attention64(c, q, [1] * len(lens))
+    cache = c.cuda(B)
+    qd, _ = wide(q.cuda(), 32)
+    o, obase = wide(torch.full_like(q, 7.0).cuda(), 48, 7.0)
+    assert B.paged_decode(qd, cache, o=o, scale=0.125) is o
+    check(host(o), ref, tol, "decode")
+    assert (host(obase)[:, :24] == 7.0).all() and (host(obase)[:, -24:] == 7.0).all()
+    ws = B.paged_workspace(cache, H, len(lens))
+    ws.fill_(255)                                       # any contents
+    for _ in range(3):                                  # and what an earlier call left
+        o2 = B.paged_decode(qd, cache, scale=0.125, workspace=ws)
+        assert torch.equal(bits(o2), bits(o)), "a second call differs"
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[20011], [9000, 1, 0, 33], [5000, 40, 7000, 1234, 4000]],
+                         ids=lambda x: "-".join(map(str, x)))
+def test_decode_long(dtype, lens):
+    """Caches cut over many workgroups."""
+    print("decode long", dtype, lens, flush=True)
+    c = Case(dtype, lens, 2, 64, True, drop=[(0, 17)], seed=3)
+    q = rows_of(dtype, len(lens), 8, 5)
+    ref, tol = attention64(c, q, [1] * len(lens))
+    cache = c.cuda(B)
+    ws = B.paged_workspace(cache, 8, len(lens))
+    for _ in range(2):
+        check(host(B.paged_decode(q.cuda(), cache, scale=0.125, workspace=ws)), ref, tol, "decode")
+
+
+def test_decode_many_sequences():
+    """More sequences than one wave scans at a time, in no order of length."""
+    lens = [int(x) for x in np.random.default_rng(0).integers(0, 90, 1300)]
+    lens[700] = 3000
+    c = Case("bf16", lens, 2, 16, True, seed=1)
+    q = rows_of("bf16", len(lens), 4, 2)
+    ref, tol = attention64(c, q, [1] * len(lens))
+    check(host(B.paged_decode(q.cuda(), c.cuda(B), scale=0.125)), ref, tol, "decode")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_decode_extreme_scores(dtype):
+    """Scores far apart, equal, and -inf: a key of -inf weighs nothing, keys of -inf alone give zeros
+    (where V is finite, 0 is what their weights of 0 give)."""
+    c = Case(dtype, [200, 70, 40], 1, 16, True, seed=4, nan=False)
+    q = rows_of(dtype, 3, 4, 6)
+    q[0] *= 300.0
+    q[1] = 0.0
+    q[2] = 0.0
+    q[2, :, 0] = 1.0
+    for j in range(40):
+        pg, sl = c.place(2, j)
+        c.k[pg, :, sl, 0] = float("-inf") if j != 33 else 1.0
+    ref, tol = attention64(c, q, [1] * 3)
+    got = host(B.paged_decode(q.cuda(), c.cuda(B), scale=0.125))
+    check(got[:2], ref[:2], tol[:2], "decode")
+    pg, sl = c.place(2, 33)
+    assert (got[2] == c.v[pg, 0, sl].double().numpy()).all()
+    c.k[pg, :, sl, 0] = float("-inf")
+    got = host(B.paged_decode(q.cuda(), c.cuda(B), scale=0.125))
+    assert (got[2] == 0.0).all()
+
+
+def test_decode_offsets_past_32_bits():
+    """A pool whose elements pass 2^32: pages far apart, and keys at both ends."""
+    n_pages, page, Hkv = 70000, 512, 1
+    free, _ = torch.cuda.mem_get_info()
+    kd = torch.empty((n_pages, page, Hkv, D), dtype=torch.bfloat16, device="cuda").transpose(1, 2)
+    vd = kd.clone()
+    assert kd.numel() > 2 ** 31 and free > 4 * kd.numel()
+    table = torch.tensor([[n_pages - 1, 0, n_pages // 2], [69000, 12, 41000]], dtype=torch.int32)
+    lens = [3 * page, 2 * page + 5]
+    r = torch.Generator().manual_seed(0)
+    ks, vs = (torch.randn((2, 3 * page, Hkv, D), generator=r).bfloat16() for _ in range(2))
+    for b in range(2):
+        for i in range(3):
+            for pool, x in ((kd, ks), (vd, vs)):
+                pool[int(table[b, i]), 0] = x[b, i * page:(i + 1) * page, 0].cuda()
+    cache = B.PagedKV(kd, vd, table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    q = torch.randn((2, 8, D), generator=r).bfloat16()
+    got = host(B.paged_decode(q.cuda(), cache, scale=0.125))
+    st = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    got2 = host(B.paged_prefill(q.cuda(), cache, st, scale=0.125))
+    got3 = host(B.paged_decode_shared(q[:1].expand(2, 8, D).contiguous().cuda(),
+                                      B.PagedKV(kd, vd, table[:1].expand(2, 3).contiguous().cuda(),
+                                                cache.seq_lens), table[0, :2].contiguous().cuda(), 2 * page,
+                                      scale=0.125))
+    for b in range(2):
+        k, v = ks[b, :lens[b], 0].double(), vs[b, :lens[b], 0].double()
+        p = torch.softmax(0.125 * q[b].double() @ k.T, 1)
+        A = (p @ v.abs()).numpy()
+        for g in (got, got2):
+            assert (np.abs(g[b] - (p @ v).numpy()) <= A * (4 * 2.0 ** -8)).all()
+        k, v = ks[0, :lens[b], 0].double(), vs[0, :lens[b], 0].double()
+        p = torch.softmax(0.125 * q[0].double() @ k.T, 1)
+        assert (np.abs(got3[b] - (p @ v).numpy()) <= (p @ v.abs()).numpy() * (4 * 2.0 ** -8)).all()
+
+
+# ------------------------------------------------------------------- prefill
+PREFILLS = [
+    # dtype, lens (with the new rows), rows, Hkv, H, page, layout, dropped pages, padding rows
+    ("bf16", [1, 2, 17, 33], [1, 2, 17, 33], 2, 16, 16, True, [], 0),
+    ("f32", [1, 2, 17, 33], [1, 2, 17, 33], 2, 16, 16, True, [], 0),
+    ("bf16", [130, 0, 65, 129], [130, 0, 65, 129], 1, 8, 16, False, [(3, 2)], 3),
+    ("f32", [130, 0, 65, 129], [130, 0, 65, 129], 1, 4, 16, False, [(3, 2)], 3),
+    ("bf16", [300, 40, 257], [3, 17, 200], 2, 12, 8, "gaps", [(0, 0), (2, 30)], 1),
+    ("f32", [300, 40, 257], [3, 17, 200], 2, 10, 64, "gaps", [(0, 0)], 1),
+    ("bf16", [200, 64], [199, 64], 1, 1, 128, True, [], 0),
+    ("bf16", [100, 31], [64, 31], 1, 20, 1, True, [(0, 50)], 0),
+    ("bf16", [10, 5], [12, 9], 2, 8, 16, True, [], 2),      # more rows than keys: the first see nothing
+    ("f32", [10, -5], [12, 9], 2, 6, 16, True, [], 2),
+    ("bf16", [1000, 700, 3], [5, 1, 1], 4, 32, 32, True, [], 0),   # a few rows behind long caches
+    ("f32", [1000, 700, 3], [5, 1, 1], 4, 8, 32, False, [], 0),
+    ("bf16", [600, 500], [400, 300], 2, 8, 16, False, [], 0),
+    ("f32", [400, 300], [400, 100], 1, 3, 256, True, [], 0),
+    ("bf16", [2 ** 31 - 1, 40], [70, 40], 1, 4, 16, True, [], 0),  # a length past the table
+]
+
+
+@pytest.mark.parametrize("case", PREFILLS, ids=lambda c: f"{c[0]}-{'_'.join(map(str, c[2]))}of{max(c[1])}-{c[3]}-{c[4]}-p{c[5]}-{c[6]}-d{len(c[7])}-{c[8]}")
+def test_prefill(case):
+    dtype, lens, rows, Hkv, H, page, layout, drop, pad = case
+    print("prefill", case, flush=True)
+    big = max(lens) > 10 ** 6
+    c = Case(dtype, lens, Hkv, page, layout, drop=drop, seed=H, max_pages=9 if big else None, junk=-5)
+    total = sum(rows) + 2 * pad
+    q = rows_of(dtype, total, H, 11)
+    ref, tol = attention64(c, q, rows, pad)
+    cache = c.cuda(B)
+    qd, _ = wide(q.cuda(), 32)
+    o, obase = wide(torch.full_like(q, 7.0).cuda(), 16, 7.0)
+    st = torch.from_numpy(starts_of(rows, pad)).cuda()
+    assert B.paged_prefill(qd, cache, st, o=o, scale=0.125) is o
+    got = host(o)
+    check(got, ref, tol, "prefill")
+    for side in (got[:pad], got[total - pad:], host(obase)[:, :8], host(obase)[:, -8:]):
+        assert (side == 7.0).all(), "wrote outside its rows"
+    ws = B.paged_workspace(cache, H, total)
+    ws.fill_(255)
+    for _ in range(3):
+        o2 = torch.full_like(q, 7.0).cuda()
+        B.paged_prefill(qd, cache, st, o=o2, scale=0.125, workspace=ws)
+        assert torch.equal(bits(o2), bits(o)), "a second call differs"
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("what", ["nan", "inf"])
+def test_prefill_hidden_values(dtype, what):
+    """The value of a key that a later row sees stays out of the rows before it, whatever it is."""
+    n = 140
+    c = Case(dtype, [n + 20], 1, 16, True, seed=8, nan=False)
+    for j in (45, 90, 131, 159):
+        pg, sl = c.place(0, j)
+        c.v[pg, 0, sl, ::3] = float(what)
+    q = rows_of(dtype, n, 4, 9)
+    got = host(B.paged_prefill(q.cuda(), c.cuda(B), torch.tensor([0, n], dtype=torch.int32).cuda(), scale=0.125))
+    clean = torch.nan_to_num(c.v.double(), nan=0.0, posinf=0.0)
+    whole, c.v = c.v, clean.to(TD[dtype])
+    ref, tol = attention64(c, q, [n])
+    sees = np.arange(n) + 20 >= 45
+    bad = np.zeros(D, bool)
+    bad[::3] = True
+    check(got[~sees], ref[~sees], tol[~sees], "rows that do not see it")
+    check(got[sees][:, :, ~bad], ref[sees][:, :, ~bad], tol[sees][:, :, ~bad], "the other columns")
+    assert not np.isfinite(got[sees][:, :, bad]).any()
+    c.v = whole
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_prefill_extreme_scores(dtype):
+    """Growing scores (the running maximum moves at every tile), then huge ones."""
+    n = 150
+    c = Case(dtype, [n + 70], 1, 16, True, seed=8, nan=False)
+    for j in range(n + 70):
+        pg, sl = c.place(0, j)
+        c.k[pg, 0, sl] = c.k[pg, 0, sl] * (1 + j)
+    q = rows_of(dtype, n, 8, 9)
+    ref, tol = attention64(c, q, [n])
+    got = host(B.paged_prefill(q.cuda(), c.cuda(B), torch.tensor([0, n], dtype=torch.int32).cuda(), scale=0.125))
+    check(got, ref, tol, "prefill")
+
+
+def test_prefill_without_starts_is_decode():
+    c = Case("bf16", [5, 100, 64], 2, 16, True, seed=2)
+    q = rows_of("bf16", 3, 16, 3)
+    ref, tol = attention64(c, q, [1] * 3)
+    check(host(B.paged_prefill(q.cuda(), c.cuda(B), scale=0.125)), ref, tol, "prefill")
+
+
+# ------------------------------------------------------------------- shared prefix
+SHARED = [
+    # dtype, prefix, own keys per sequence, Hkv, H, page, layout
+    ("bf16", 0, [1, 40, 5], 2, 16, 16, True),
+    ("bf16", 1, [1, 40, 5], 2, 16, 16, True),
+    ("f32", 33, [1, 40, 5], 2, 6, 16, False),
+    ("bf16", 64, [1, 70, 0, 5, 129], 1, 8, 64, True),
+    ("f32", 64, [1, 70, 0, 5, 129], 1, 8, 64, True),
+    ("bf16", 300, [3, 1, 1, 90] * 9, 2, 16, 16, False),
+    ("f32", 300, [3, 1, 1, 90] * 9, 2, 4, 8, "gaps"),
+    ("bf16", 1000, [10], 1, 20, 32, True),
+    ("bf16", 129, [-100, -129, -1, 20, -300], 2, 12, 16, "gaps"),   # shorter than the prefix, empty
+    ("f32", 129, [-100, -129, -1, 20, -300], 2, 12, 16, True),
+    ("bf16", 2500, [1] * 40 + [700], 1, 3, 128, True),
+    ("bf16", 70, [0] * 300, 1, 8, 1, True),
+]
+
+
+@pytest.mark.parametrize("case", SHARED, ids=lambda c: f"{c[0]}-P{c[1]}-{len(c[2])}-{c[3]}-{c[4]}-p{c[5]}-{c[6]}")
+def test_shared(case):
+    dtype, P, own, Hkv, H, page, layout = case
+    print("shared", case, flush=True)
+    lens = [P + n for n in own]
+    c = Case(dtype, lens, Hkv, page, layout, seed=P, nan=False)
+    # the common keys in pages of their own; what the tables say of pages wholly below P is not looked at
+    n_prefix = -(-P // page)
+    r = np.random.default_rng(P + 1)
+    extra = [torch.from_numpy(r.standard_normal((n_prefix, Hkv, page, D)).astype(np.float32)).to(TD[dtype])
+             for _ in range(2)]
+    prefix = np.arange(c.n_pages, c.n_pages + n_prefix, dtype=np.int32)
+    c.k, c.v = torch.cat([c.k, extra[0]]), torch.cat([c.v, extra[1]])
+    c.n_pages += n_prefix
+    c.table[:, :P // page] = 2 ** 31 - 1
+    if P % page:
+        c.v[-1, :, P % page:] = float("nan")
+        for b in range(len(lens)):      # and a shared page's part of the sequence's copy neither
+            if 0 <= c.table[b, P // page] < c.n_pages:
+                c.v[int(c.table[b, P // page]), :, :P % page] = float("nan")
+    q = rows_of(dtype, len(lens), H, 1)
+    ref, tol = attention64(c, q, [1] * len(lens), prefix=prefix, prefix_len=P)
+    cache = c.cuda(B)
+    qd, _ = wide(q.cuda(), 32)
+    o, obase = wide(torch.full_like(q, 7.0).cuda(), 48, 7.0)
+    pd = torch.from_numpy(prefix).cuda()
+    assert B.paged_decode_shared(qd, cache, pd, P, o=o, scale=0.125) is o
+    check(host(o), ref, tol, "shared")
+    assert (host(obase)[:, :24] == 7.0).all() and (host(obase)[:, -24:] == 7.0).all()
+    ws = B.paged_workspace(cache, H, len(lens), P)
+    ws.fill_(255)
+    for _ in range(3):
+        o2 = B.paged_decode_shared(qd, cache, pd, P, scale=0.125, workspace=ws)
+        assert torch.equal(bits(o2), bits(o)), "a second call differs"
+
+
+def test_shared_prefix_page_without_memory():
+    c = Case("bf16", [90, 120, 70], 2, 16, True, seed=2)
+    prefix = c.table[0, :4].copy()
+    prefix[1] = -1
+    q = rows_of("bf16", 3, 8, 3)
+    ref, tol = attention64(c, q, [1] * 3, prefix=prefix, prefix_len=64)
+    got = B.paged_decode_shared(q.cuda(), c.cuda(B), torch.from_numpy(prefix).cuda(), 64, scale=0.125)
+    check(host(got), ref, tol, "shared")
+
+
+# ------------------------------------------------------------------- graphs, streams
+def big_case():
+    c = Case("bf16", [3000, 17, 900, 2100], 2, 16, True, seed=5, nan=False)
+    return c, c.cuda(B)
+
+
+@pytest.mark.parametrize("op", ["decode", "prefill", "shared"])
+def test_graphs_share_a_workspace(op):
+    """Two graphs with one workspace, replayed in turn with eager calls on it and changed lengths
+    in between: each replay equals the eager call."""
+    c, cache = big_case()
+    q = rows_of("bf16", 8, 16, 6).cuda()
+    st = torch.tensor([0, 4, 5, 5, 8], dtype=torch.int32).cuda()
+    pages = cache.page_table[0, :40].contiguous()
+    ws = B.paged_workspace(cache, 16, 8, 600)
+    ws.fill_(77)
+
+    def call(x, o):
+        if op == "decode":
+            B.paged_decode(x[:4], cache, o=o[:4], scale=0.125, workspace=ws)
+        elif op == "prefill":
+            B.paged_prefill(x, cache, st, o=o, scale=0.125, workspace=ws)
+        else:
+            B.paged_decode_shared(x[:4], cache, pages, 600, o=o[:4], scale=0.125, workspace=ws)
+
+    xs, outs, graphs = [q, (q * 0.5)], [], []
+    s = torch.cuda.Stream()
+    for x in xs:
+        o = torch.zeros_like(q)
+        with torch.cuda.stream(s):
+            call(x, o)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(x, o)
+        outs.append(o)
+        graphs.append(g)
+    for step, lens in enumerate(([3000, 17, 900, 2100], [1, 0, 640, 3000], [2999, 300, 601, 5], [3000, 17, 900, 2100])):
+        cache.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        for x, o, g in zip(xs, outs, graphs):
+            o.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            got = o.clone()
+            want = torch.zeros_like(q)
+            call(x, want)
+            torch.cuda.synchronize()
+            assert torch.equal(bits(got), bits(want)), f"step {step}"
+            junk = torch.empty_like(ws)
+            if step == 1:
+                ws.copy_(junk.random_(0, 256))
+
+
+def test_calls_on_two_streams():
+    """Calls in flight at once, each with its own workspace or the pool's."""
+    c, cache = big_case()
+    q = rows_of("bf16", 4, 16, 6).cuda()
+    want = B.paged_decode(q, cache, scale=0.125)
+    pages = cache.page_table[0, :40].contiguous()
+    want_s = B.paged_decode_shared(q, cache, pages, 600, scale=0.125)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    wss = [B.paged_workspace(cache, 16, 4, 600), B.paged_workspace(cache, 16, 4, 600), None]
+    got = []
+    for _ in range(5):
+        for s, ws in zip(streams, wss):
+            with torch.cuda.stream(s):
+                got.append((B.paged_decode(q, cache, scale=0.125, workspace=ws), want))
+                got.append((B.paged_decode_shared(q, cache, pages, 600, scale=0.125, workspace=ws), want_s))
+    torch.cuda.synchronize()
+    for g, w in got:
+        assert torch.equal(bits(g), bits(w))
+
+
+def test_host_memory_is_refused():
+    c = Case("bf16", [5, 9], 2, 16, True)
+    kv = B.PagedKV(c.k, c.v, torch.from_numpy(c.table.copy()), torch.tensor([5, 9], dtype=torch.int32))
+    q = rows_of("bf16", 2, 4, 1)
+    s, m = B.status_of("bn_paged_decode", kv.ref, q.data_ptr(), q.data_ptr(), 4, 256, 256, 0.125, None, 0, None)
+    assert s == B.BN_ERR_NOT_DEVICE and "only GPU implementation available" in m
+
+
+# ------------------------------------------------------------------- together
+@pytest.mark.parametrize("dtype,page,layout", [("f32", 16, True), ("bf16", 8, False), ("bf16", 32, True)])
+def test_a_server_run(dtype, page, layout):
+    """Prompts of three users arrive and are answered token by token: append and prefill, one more
+    chunk for one of them, then append and decode steps, and a shared-prefix decode over the same
+    tables; every output against 64 bits over the cache's own (checked) contents."""
+    Hkv, H, prompt = 2, 8, [37, 5, 64]
+    room = [120] * 3
+    c = Case(dtype, room, Hkv, page, layout, seed=21, nan=True)
+    c.k[:], c.v[:] = float("nan"), float("nan")       # nothing is there before it is appended
+    cache = c.cuda(B)
+    eps = torch.finfo(TD[dtype]).eps / 2
+    r = np.random.default_rng(5)
+    truth_k = {}
+
+    def step(rows, op):
+        c.lens = [a + n for a, n in zip(c.lens, rows)]
+        cache.seq_lens.copy_(torch.tensor(c.lens, dtype=torch.int32))
+        n = sum(rows)
+        qkv = torch.from_numpy(r.standard_normal((n, (H + 2 * Hkv) * D)).astype(np.float32)).to(TD[dtype])
+        x = qkv.cuda()
+        q, k, v = (t.unflatten(1, (-1, D)) for t in x.split([H * D, Hkv * D, Hkv * D], 1))
+        st = torch.from_numpy(starts_of(rows)).cuda()
+        B.paged_append(cache, k, v, q=q, row_starts=st)
+        o = op(q, st)
+        torch.cuda.synchronize()
+        c.k, c.v = c.kd.cpu().contiguous(), c.vd.cpu().contiguous()
+        at = 0
+        for b, m in enumerate(rows):
+            for i in range(m):
+                j = c.lens[b] - m + i
+                raw = qkv[at + i].double().numpy().reshape(-1, D)
+                turned = rotate64(raw[:H + Hkv], j, 1e4)
+                pg, sl = c.place(b, j)
+                pair = 2 * np.abs(raw).max() * 6 * 2.0 ** -24
+                assert (np.abs(c.k[pg, :, sl].double().numpy() - turned[H:]) <= pair + np.abs(turned[H:]) * eps * 1.01).all()
+                assert (c.v[pg, :, sl].double().numpy() == raw[H + Hkv:]).all()
+                assert (np.abs(host(q[at + i]) - turned[:H]) <= pair + np.abs(turned[:H]) * eps * 1.01).all()
+            at += m
+        ref, tol = attention64(c, q.cpu(), rows)
+        check(host(o), ref, tol, f"lengths {c.lens}")
+
+    c.lens = [0, 0, 0]
+    step(prompt, lambda q, st: B.paged_prefill(q, cache, st, scale=0.125))
+    step([0, 30, 2], lambda q, st: B.paged_prefill(q, cache, st, scale=0.125))
+    for _ in range(6):
+        step([1, 1, 1], lambda q, st: B.paged_decode(q.contiguous(), cache, scale=0.125))
+    # the last two users' tables start like the first one's: their copies of its pages
+    common = 32
+    for b in (1, 2):
+        for i in range(common // page):
+            cache.page_table[b, i] = cache.page_table[0, i]
+            c.table[b, i] = c.table[0, i]
+    pages = cache.page_table[0, :common // page].contiguous()
+    for _ in range(2):
+        step([1, 1, 1], lambda q, st: B.paged_decode_shared(q.contiguous(), cache, pages, common, scale=0.125))

@@ -1,0 +1,202 @@
+"""The paged KV cache's calls refuse on the host what they cannot take, before any device work
+(made-up addresses, never dereferenced: no GPU needed)."""
+import ctypes as C
+
+import pytest
+import torch
+
+import bnhip as B
+
+CACHE = dict(k=0x10000, v=0x20000, page_table=0x30000, seq_lens=0x40000, page_stride=4 * 16 * 64,
+             head_stride=16 * 64, row_stride=64, table_stride=8, dtype=B.BN_BF16, batch=3, n_pages=24,
+             max_pages=8, page_size=16, n_kv_heads=4, head_dim=64)
+
+
+def cache(**kw):
+    return B.BnPagedKV(*[{**CACHE, **kw}[n] for n, _ in B.BnPagedKV._fields_])
+
+
+def append(c=None, k=0x1000, v=0x2000, q=0x3000, qo=0x4000, starts=0x5000, n=7, H=32, ks=2560, vs=2560,
+           qs=2560, qos=2048, theta=1e4):
+    c = cache() if c is None else c
+    return B.status_of("bn_paged_append", C.byref(c) if c else None, k, v, q, qo, starts, n, H, ks, vs,
+                       qs, qos, theta, None)
+
+
+def decode(c=None, q=0x1000, o=0x2000, H=32, qs=2048, os=2048, scale=0.125, ws=None, wsb=0):
+    c = cache() if c is None else c
+    return B.status_of("bn_paged_decode", C.byref(c) if c else None, q, o, H, qs, os, scale, ws, wsb, None)
+
+
+def prefill(c=None, q=0x1000, o=0x2000, starts=0x3000, n=7, H=32, qs=2048, os=2048, scale=0.125, ws=None,
+            wsb=0):
+    c = cache() if c is None else c
+    return B.status_of("bn_paged_prefill", C.byref(c) if c else None, q, o, starts, n, H, qs, os, scale,
+                       ws, wsb, None)
+
+
+def shared(c=None, q=0x1000, o=0x2000, H=32, qs=2048, os=2048, scale=0.125, pages=0x3000, P=40, ws=None,
+           wsb=0):
+    c = cache() if c is None else c
+    return B.status_of("bn_paged_decode_shared", C.byref(c) if c else None, q, o, H, qs, os, scale,
+                       pages, P, ws, wsb, None)
+
+
+CALLS = {"Paged append": append, "Paged decode": decode, "Paged prefill": prefill,
+         "Paged decode (shared prefix)": shared}
+
+
+@pytest.mark.parametrize("kw,status,msg", [
+    (dict(dtype=B.BN_U32), B.BN_ERR_UNSUPPORTED, "dtype"),
+    (dict(batch=-1), B.BN_ERR_SHAPE, "negative"),
+    (dict(n_pages=-1), B.BN_ERR_SHAPE, "negative"),
+    (dict(max_pages=-1), B.BN_ERR_SHAPE, "negative"),
+    (dict(n_kv_heads=0), B.BN_ERR_SHAPE, "num_kv_heads"),
+    (dict(head_dim=128), B.BN_ERR_UNSUPPORTED, "head_dim must be 64"),
+    (dict(page_size=0), B.BN_ERR_UNSUPPORTED, "power of two"),
+    (dict(page_size=24), B.BN_ERR_UNSUPPORTED, "power of two"),
+    (dict(page_size=-16), B.BN_ERR_UNSUPPORTED, "power of two"),
+    (dict(max_pages=1 << 27), B.BN_ERR_UNSUPPORTED, "2^30"),
+    (dict(batch=(1 << 20) + 1), B.BN_ERR_SHAPE | B.BN_ERR_UNSUPPORTED, ""),
+    (dict(row_stride=32), B.BN_ERR_INVALID_ARG, "strides"),
+    (dict(row_stride=68), B.BN_ERR_INVALID_ARG, "strides"),
+    (dict(head_stride=0), B.BN_ERR_INVALID_ARG, "strides"),
+    (dict(page_stride=-4096), B.BN_ERR_INVALID_ARG, "strides"),
+    (dict(page_stride=(1 << 40) + 8), B.BN_ERR_INVALID_ARG, "strides"),
+    (dict(table_stride=7), B.BN_ERR_SHAPE, "overlap"),
+    (dict(k=0), B.BN_ERR_INVALID_ARG, "NULL"),
+    (dict(v=0), B.BN_ERR_INVALID_ARG, "NULL"),
+    (dict(page_table=0), B.BN_ERR_INVALID_ARG, "NULL"),
+    (dict(seq_lens=0), B.BN_ERR_INVALID_ARG, "NULL"),
+    (dict(k=0x10008), B.BN_ERR_UNSUPPORTED, "16-byte"),
+    (dict(page_table=0x30002), B.BN_ERR_UNSUPPORTED, "4-byte"),
+    (dict(seq_lens=0x40001), B.BN_ERR_UNSUPPORTED, "4-byte"),
+])
+@pytest.mark.parametrize("name", sorted(CALLS))
+def test_cache_refusals(name, kw, status, msg):
+    s, m = CALLS[name](cache(**kw))
+    if "batch" in kw and kw["batch"] > 0:  # one row each: the row counts disagree first where they are given
+        assert s in (B.BN_ERR_SHAPE, B.BN_ERR_UNSUPPORTED) and m.startswith(name + ":")
+        return
+    assert s == status, m
+    assert m.startswith(name + ":") and msg in m, m
+
+
+@pytest.mark.parametrize("name", sorted(CALLS))
+def test_null_cache_and_empty_batch(name):
+    s, m = CALLS[name](False)
+    assert s == B.BN_ERR_INVALID_ARG and "cache is NULL" in m
+    c = cache(batch=0, k=0, v=0, page_table=0, seq_lens=0)
+    assert CALLS[name](c) == (B.BN_OK, "")
+
+
+@pytest.mark.parametrize("call,kw,status,msg", [
+    (append, dict(n=-1), B.BN_ERR_SHAPE, "negative number of rows"),
+    (append, dict(starts=None), B.BN_ERR_SHAPE, "one row per sequence"),
+    (append, dict(starts=0x5002), B.BN_ERR_UNSUPPORTED, "row_starts"),
+    (append, dict(q=None), B.BN_ERR_INVALID_ARG, "together"),
+    (append, dict(qo=None), B.BN_ERR_INVALID_ARG, "together"),
+    (append, dict(H=30), B.BN_ERR_SHAPE, "num_heads"),
+    (append, dict(theta=-1.0), B.BN_ERR_INVALID_ARG, "theta"),
+    (append, dict(theta=float("nan")), B.BN_ERR_INVALID_ARG, "theta"),
+    (append, dict(theta=float("inf")), B.BN_ERR_INVALID_ARG, "theta"),
+    (append, dict(k=None), B.BN_ERR_INVALID_ARG, "k is NULL"),
+    (append, dict(v=None), B.BN_ERR_INVALID_ARG, "v is NULL"),
+    (append, dict(ks=255), B.BN_ERR_SHAPE, "k row stride"),
+    (append, dict(vs=260), B.BN_ERR_UNSUPPORTED, "v must be"),
+    (append, dict(q=0x3004), B.BN_ERR_UNSUPPORTED, "q must be"),
+    (append, dict(qos=2040), B.BN_ERR_SHAPE, "q_out row stride"),
+    (append, dict(qo=0x3000), B.BN_ERR_INVALID_ARG, "in q's place"),
+    (decode, dict(H=30), B.BN_ERR_SHAPE, "num_heads"),
+    (decode, dict(H=0), B.BN_ERR_SHAPE, "num_heads"),
+    (decode, dict(H=4 * 16384), B.BN_ERR_UNSUPPORTED, "65535"),
+    (decode, dict(scale=0.0), B.BN_ERR_INVALID_ARG, "scale"),
+    (decode, dict(scale=float("inf")), B.BN_ERR_INVALID_ARG, "scale"),
+    (decode, dict(q=None), B.BN_ERR_INVALID_ARG, "q is NULL"),
+    (decode, dict(o=None), B.BN_ERR_INVALID_ARG, "o is NULL"),
+    (decode, dict(o=0x2008), B.BN_ERR_UNSUPPORTED, "o must be"),
+    (decode, dict(qs=2044), B.BN_ERR_SHAPE, "q row stride"),
+    (decode, dict(os=2052), B.BN_ERR_UNSUPPORTED, "o must be"),
+    (decode, dict(ws=0x9008, wsb=1 << 40), B.BN_ERR_UNSUPPORTED, "workspace must be"),
+    (prefill, dict(n=-3), B.BN_ERR_SHAPE, "negative number of rows"),
+    (prefill, dict(starts=None), B.BN_ERR_SHAPE, "one row per sequence"),
+    (prefill, dict(scale=-1.0), B.BN_ERR_INVALID_ARG, "scale"),
+    (prefill, dict(q=0x1002), B.BN_ERR_UNSUPPORTED, "q must be"),
+    (shared, dict(P=-1), B.BN_ERR_SHAPE, "prefix length"),
+    (shared, dict(pages=None), B.BN_ERR_INVALID_ARG, "prefix_pages"),
+    (shared, dict(pages=0x3001), B.BN_ERR_UNSUPPORTED, "prefix_pages"),
+])
+def test_argument_refusals(call, kw, status, msg):
+    s, m = call(**kw)
+    assert s == status, m
+    assert msg in m, m
+
+
+def test_no_rows_is_nothing_to_do():
+    assert append(n=0) == (B.BN_OK, "")
+    assert prefill(n=0) == (B.BN_OK, "")
+
+
+def test_workspace_sizes():
+    L = B.lib()
+    c = cache()
+    for n in (0, 1, 7, 1000):
+        for P in (0, 1, 5000):
+            need = L.bn_paged_workspace_size(C.byref(c), 32, n, P)
+            assert need < 1 << 32
+    for bad in (cache(dtype=B.BN_U32), cache(head_dim=32), cache(n_kv_heads=0), cache(page_size=3)):
+        assert L.bn_paged_workspace_size(C.byref(bad), 32, 3, 0) == 0
+    assert L.bn_paged_workspace_size(None, 32, 3, 0) == 0
+    assert L.bn_paged_workspace_size(C.byref(c), 30, 3, 0) == 0
+    assert L.bn_paged_workspace_size(C.byref(c), 32, -1, 0) == 0
+
+
+def test_a_workspace_too_small_is_refused():
+    L = B.lib()
+    c = cache(batch=64, max_pages=1024, table_stride=1024, n_pages=4096)
+    for call, P in ((decode, 0), (shared, 5000)):
+        need = L.bn_paged_workspace_size(C.byref(c), 32, 64, P)
+        if need:
+            s, m = call(c, ws=0x9000, wsb=need - 1, **(dict(P=P) if P else {}))
+            assert s == B.BN_ERR_INVALID_ARG and "workspace" in m
+
+
+def test_python_wrappers_refuse():
+    k = torch.zeros((5, 2, 16, 64), dtype=torch.bfloat16)
+    table = torch.zeros((3, 4), dtype=torch.int32)
+    lens = torch.zeros(3, dtype=torch.int32)
+    kv = B.PagedKV(k, k.clone(), table, lens)
+    assert kv.view.page_size == 16 and kv.view.n_kv_heads == 2 and kv.view.batch == 3
+    for bad in (dict(v=k[:4]), dict(v=k.float()), dict(k=k.half(), v=k.half()), dict(table=table.long()),
+                dict(lens=lens.long()), dict(lens=lens[:2]), dict(table=table[0]), dict(k=k[..., ::2], v=k[..., ::2]),
+                dict(table=torch.zeros((3, 8), dtype=torch.int32)[:, ::2])):
+        a = dict(k=k, v=k, table=table, lens=lens, **{})
+        a.update(bad)
+        with pytest.raises(ValueError, match="PagedKV"):
+            B.PagedKV(a["k"], a["v"], a["table"], a["lens"])
+    q = torch.zeros((3, 8, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="paged_decode: q"):
+        B.paged_decode(q[:2], kv)
+    with pytest.raises(ValueError, match="dtype"):
+        B.paged_decode(q.float(), kv)
+    with pytest.raises(ValueError, match="contiguous"):
+        B.paged_decode(torch.zeros((3, 64, 8), dtype=torch.bfloat16).transpose(1, 2), kv)
+    with pytest.raises(ValueError, match="paged_decode: o"):
+        B.paged_decode(q, kv, o=q[:, :4])
+    with pytest.raises(ValueError, match="one row per sequence"):
+        B.paged_prefill(torch.zeros((7, 8, 64), dtype=torch.bfloat16), kv)
+    with pytest.raises(ValueError, match="row_starts"):
+        B.paged_prefill(q, kv, torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError, match="row_starts"):
+        B.paged_prefill(q, kv, torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(ValueError, match="prefix_pages"):
+        B.paged_decode_shared(q, kv, torch.zeros(2, dtype=torch.int32), 33)
+    with pytest.raises(ValueError, match="prefix_pages"):
+        B.paged_decode_shared(q, kv, torch.zeros(2), 3)
+    kn = torch.zeros((3, 2, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="paged_append: k"):
+        B.paged_append(kv, q, kn)
+    with pytest.raises(ValueError, match="paged_append: v"):
+        B.paged_append(kv, kn, kn[:2])
+    with pytest.raises(ValueError, match="q_out without q"):
+        B.paged_append(kv, kn, kn, q_out=q)
