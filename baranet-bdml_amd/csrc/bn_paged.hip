@@ -12,6 +12,7 @@
 // address, and lengths are clamped to what the table can hold, so that no
 // contents of those arrays lead outside the pools.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "bn_common.hpp"
@@ -169,6 +170,567 @@ struct AttnParams {
   int prefix_len;
 };
 
+// ----------------------------------------------------- decode, over pages
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ bf16x4 lds_tr16(const bf16_t *p) {
+  const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4 *)(__attribute__((address_space(3))) void *)p);
+  return __builtin_bit_cast(bf16x4, r);
+}
+
+// A tile of keys as a wave loads it: four 16-byte loads per lane of K and four
+// of V, LPR lanes a row: whole rows, 1 KB of a head-major page an instruction
+// (loads straight into the products' operands, 16 rows of 64 bytes an
+// instruction, streamed a third slower).  P: pitch of a row in LDS, elements
+// (144 and 272 bytes: the fragment reads below spread over the banks).
+template <typename T> struct DecTile;
+template <> struct DecTile<bf16_t> { static constexpr int TK = 32, LPR = 8, P = HD + 8; };
+template <> struct DecTile<float> { static constexpr int TK = 16, LPR = 16, P = HD + 4; };
+
+constexpr int kMaxRows = 16;   // query heads of a KV head that one workgroup serves
+constexpr int kRec = HD + 2;   // floats of a record's row: acc[64], m (log2 units), l
+constexpr int kHold = HD + 4;  // the same in LDS, rows 16-byte aligned
+constexpr int kHoldRows = 160; // rows of LDS for the waves' parts of sequences
+constexpr int kShareMin = 4;   // tiles of a share at least
+constexpr int kMergeBatch = 16;  // records read at once
+
+// Sums of the lanes up to and with each lane, by moves inside a row of 16
+// lanes, then of a row's last lane to the rows behind it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);  // row_bcast 15 to rows 1 and 3
+  return dpp_add<0x143, 0xc>(x);  // row_bcast 31 to rows 2 and 3
+}
+
+struct DecodeParams {
+  AttnParams a;
+  float *ws;                        // records: [bins][2][columns][rows][kRec]
+  unsigned long long *arrive_end;   // two arrival words per (sequence, column) below it
+  unsigned long long tag;           // the launch's 48-bit tag
+  int bins, hblocks, columns, k0;   // k0: keys below it are not this kernel's
+};
+
+// Counts the caller in as one of n on a pair of 64-bit words and says whether
+// it is the last.  The first word holds kArrive between launches and counts up
+// from it.  Anything else there (memory that nobody has counted in yet) sends
+// every caller of the launch to the second word, where a count starts under
+// the launch's tag.  A finished count leaves kArrive and 0, so neither fresh
+// memory nor a replayed graph needs a clearing pass.
+constexpr unsigned long long kArrive = 0x5bd1e995a93c71d4ull;
+__device__ __forceinline__ bool arrive_last(unsigned long long *word, int n, unsigned long long tag) {
+  unsigned long long old =
+      __hip_atomic_fetch_add(word, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) - kArrive;
+  bool last = old == (unsigned long long)(n - 1);
+  if (old >= (unsigned long long)n) {
+    old = __hip_atomic_load(word + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    while (old >> 16 != tag &&
+           !__hip_atomic_compare_exchange_strong(word + 1, &old, tag << 16, __ATOMIC_RELAXED,
+                                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) {
+    }
+    old = __hip_atomic_fetch_add(word + 1, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = (int)(old & 0xffff) == n - 1;
+    if (last) __hip_atomic_store(word + 1, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (last) __hip_atomic_store(word, kArrive, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return last;
+}
+
+// Two floats through to memory, past the caches (another workgroup, on another
+// XCD, reads them in the same launch), and back.
+__device__ __forceinline__ void put2(float *p, float a, float b) {
+  const unsigned long long v = (unsigned long long)__float_as_uint(a) | ((unsigned long long)__float_as_uint(b) << 32);
+  __hip_atomic_store((unsigned long long *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+__device__ __forceinline__ float2 get2(const float *p) {
+  const unsigned long long v =
+      __hip_atomic_load((const unsigned long long *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// The batch's tiles, sequences in order, are dealt in equal shares to the
+// workgroups of a column (a KV head, or up to 16 of its query heads), so that
+// any mix of lengths keeps every compute unit streaming to the end.  A
+// workgroup's four waves take its share's tiles in turn, across the borders of
+// sequences, with the loads of the next tiles and the table entries of the one
+// after them in flight; no barrier between them.  A wave leaves its part of
+// each sequence (running maximum, sum, accumulator) in LDS; when the share, or
+// as many sequences as LDS has room for, are through, the workgroup adds the
+// waves' parts.  A sequence that lies in one share is then written; of one cut
+// between shares each workgroup leaves a record in the workspace and counts
+// itself in, and the last to arrive adds the records, in the order of the keys,
+// and writes the output: one launch, and the same bits whoever arrives last.
+//
+// Per tile, with the query heads as columns of the products:
+//   S^T[key][head] = K . Q^T,  O^T[d][head] += V^T . P^T
+// on v_mfma_f32_16x16x32_bf16 (bf16 probabilities: half a step of 2^-8 each)
+// or v_mfma_f32_16x16x4_f32; a lane holds its 8 (4) keys' scores of one head,
+// which are the second product's operand as they stand.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
+  using Ti = DecTile<T>;
+  constexpr bool BF = sizeof(T) == 2;
+  constexpr int TK = Ti::TK, LPR = Ti::LPR, RPI = 64 / LPR, VEC = HD / LPR, P = Ti::P;
+  constexpr int NS = TK / 16;  // 16-key score tiles
+  constexpr int NQ = BF ? 2 : 4;
+  __shared__ __attribute__((aligned(16))) T KT[4][TK * P];
+  __shared__ __attribute__((aligned(16))) T VT[4][TK * P];
+  __shared__ __attribute__((aligned(16))) float hold[kHoldRows * kHold];
+  __shared__ int last_in[2];
+
+  const Paged &c = p.a.c;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, grp = lane >> 4;
+  const int bin = blockIdx.x / p.columns, col = blockIdx.x - bin * p.columns;
+  const int g = col / p.hblocks, hb = col - g * p.hblocks;
+  const int rows = min(kMaxRows, p.a.group - kMaxRows * hb), head0 = g * p.a.group + kMaxRows * hb;
+  const int room = kHoldRows / (4 * rows);  // sequences that LDS has room for
+  // the first tile begins at a multiple of the smallest page, so that eight rows
+  // of a tile from a multiple of eight on lie in one page
+  const int k0 = p.k0 & -8;
+  auto clamp_len = [&](int n) { return max(min(n, c.cap), 0); };
+  auto tiles_of = [&](int len) { return len > p.k0 ? (int)((uint32_t)(len - k0 + TK - 1) / TK) : 0; };
+
+  // ---- the share: every wave scans the lengths for itself, a run of
+  // `per` sequences a lane
+  const int per = (c.batch + 63) >> 6;
+  int own, some = 0;
+  auto length_of = [&](int b) __attribute__((always_inline)) {
+    const int n = c.lens[min(b, c.batch - 1)];
+    return b < c.batch ? clamp_len(n) : 0;
+  };
+  if (per == 1) {
+    some = length_of(lane);
+    own = tiles_of(some);
+  } else {
+    own = 0;
+    for (int i = 0; i < per; i += 8) {
+      int n[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) n[j] = c.lens[min(lane * per + i + j, c.batch - 1)];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        own += i + j < per && lane * per + i + j < c.batch ? tiles_of(clamp_len(n[j])) : 0;
+    }
+  }
+  const int upto = wave_scan(own);
+  const int total = __builtin_amdgcn_readlane(upto, 63);
+  const int share =
+      __builtin_amdgcn_readfirstlane(max((int)((uint32_t)(total + p.bins - 1) / (uint32_t)p.bins), kShareMin));
+  const int pos0 = (int)min((int64_t)bin * share, (int64_t)total), n_wg = min(share, total - pos0);
+
+  struct Window {  // 64 lengths from sequence b0 on, one a lane
+    int b0, len;
+  };
+  auto window = [&](int b) __attribute__((always_inline)) { return Window{b, length_of(b + lane)}; };
+  struct Tile {
+    int b, t, len, ord;  // tile t of sequence b of len keys, the share's ord-th sequence
+  };
+  // the sequence behind x's that has a tile (there is one)
+  auto next_seq = [&](Tile x, Window &w) __attribute__((always_inline)) {
+    int b = x.b + 1;
+    for (;;) {
+      if (b - w.b0 >= 64) w = window(b);
+      const unsigned long long there = __builtin_amdgcn_ballot_w64(tiles_of(w.len) > 0) >> (b - w.b0);
+      if (there) {
+        b += __builtin_ctzll(there);
+        return Tile{b, 0, __builtin_amdgcn_readlane(w.len, b - w.b0), x.ord + 1};
+      }
+      b = w.b0 + 64;
+    }
+  };
+  auto skip = [&](Tile x, int by, Window &w) __attribute__((always_inline)) {
+    x.t += by;
+    for (int nt; x.t >= (nt = tiles_of(x.len));) {
+      const int t = x.t - nt;
+      x = next_seq(x, w);
+      x.t = t;
+    }
+    return x;
+  };
+
+  // ---- loads: the RPI rows of a load instruction lie in one page, so that its
+  // table entry and address are scalars and a lane's offset to them is fixed
+  const int crow = lane / LPR, ccol = (lane % LPR) * VEC;
+  const uint32_t off = (uint32_t)((crow * c.row_stride + ccol) * sizeof(T));
+  const char *const Kg = (const char *)((const T *)c.k + g * c.head_stride);
+  const char *const Vg = (const char *)((const T *)c.v + g * c.head_stride);
+  const int slot_mask = (1 << c.shift) - 1;
+  const int64_t page_bytes = c.page_stride * (int64_t)sizeof(T);
+  const uint32_t row_bytes = (uint32_t)(c.row_stride * sizeof(T));
+  // A tile's table entries are read as scalars: they come in their own order,
+  // not behind the rows requested before them (as vector loads they held up
+  // the next rows: 64 caches of 4096 keys 51 us).
+  typedef const __attribute__((address_space(4))) int32_t *scalar_ints;
+  int ids[4];  // of rows RPI r .. of the tile to load next
+  struct Rows {
+    u32x4 k[4], v[4];  // the lane's pieces of a tile
+    int lo, hi;        // keys lo .. hi - 1 of the tile are the sequence's
+    int pages;         // bit r: rows RPI r .. have memory (else page 0 is read)
+  };
+  auto load_ids = [&](const Tile &x) __attribute__((always_inline)) {
+    const int b = __builtin_amdgcn_readfirstlane(x.b), key0 = k0 + TK * __builtin_amdgcn_readfirstlane(x.t);
+    const int last = __builtin_amdgcn_readfirstlane(x.len) - 1;
+    const scalar_ints row = (scalar_ints)(c.table + b * c.table_stride);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) ids[r] = row[min(key0 + RPI * r, last) >> c.shift];
+  };
+  int64_t at[4];  // byte offsets of the rows
+  int at_pages;   // bit r: those rows have memory (else page 0's are read)
+  auto locate_rows = [&](const Tile &x) __attribute__((always_inline)) {
+    const int key0 = k0 + TK * __builtin_amdgcn_readfirstlane(x.t);
+    at_pages = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const bool ok = (unsigned)ids[r] < (unsigned)c.n_pages;
+      at_pages |= ok << r;
+      at[r] = (ok ? ids[r] : 0) * page_bytes + (int64_t)((uint64_t)(uint32_t)((key0 + RPI * r) & slot_mask) * row_bytes);
+    }
+  };
+  auto load_rows = [&](Rows &y, const Tile &x) __attribute__((always_inline)) {
+    const int key0 = k0 + TK * x.t;
+    y.lo = p.k0 - key0;
+    y.hi = x.len - key0;
+    y.pages = at_pages;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {  // streamed once: non-temporal
+      y.k[r] = __builtin_nontemporal_load((const u32x4 *)(Kg + at[r] + off));
+      y.v[r] = __builtin_nontemporal_load((const u32x4 *)(Vg + at[r] + off));
+    }
+  };
+  T *const kt = KT[wave], *const vt = VT[wave];
+  auto store_rows = [&](Rows &y, bool masked) __attribute__((always_inline)) {
+    if (masked) {  // no key: zeros, whatever lies there (0 times an infinite value is none)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = crow + RPI * r;
+        if (row < y.lo || row >= y.hi || !(y.pages >> r & 1)) y.k[r] = y.v[r] = u32x4{0, 0, 0, 0};
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) *(u32x4 *)(kt + (crow + RPI * r) * P + ccol) = y.k[r];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) *(u32x4 *)(vt + (crow + RPI * r) * P + ccol) = y.v[r];
+  };
+  // queries: lane holds head l16's elements 8 grp + 32 t .. +7 (bf16), 16 grp .. +15 (fp32)
+  u32x4 q[NQ], qn[NQ];
+  auto load_q = [&](int b) __attribute__((always_inline)) {
+    const T *const qp = (const T *)p.a.q + b * p.a.q_rs + (head0 + min(l16, rows - 1)) * HD;
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) qn[t] = *(const u32x4 *)(qp + (BF ? 8 * grp + 32 * t : 16 * grp + 4 * t));
+  };
+
+  // ---- a tile's arithmetic.  The probabilities are taken against a reference
+  // that is the true running maximum only when it was last moved: it moves when
+  // a key's weight against it passes 2^16 (or is NaN), which saves the maximum
+  // over the lanes and the rescaling of the accumulator for most tiles.
+  float mc = -INFINITY, l = 0.f;  // of head l16: reference, log2 units; this lane's keys' sum
+  f32x4 o[4];
+  const float cl = p.a.cl;
+  auto compute = [&](bool masked, int lo, int hi, int pages) __attribute__((always_inline)) {
+    f32x4 s[NS];
+    if constexpr (BF) {
+#pragma unroll
+      for (int u = 0; u < NS; ++u) {
+        const bf16_t *kp = kt + 8 * grp + (16 * u + l16) * P;
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8 *)kp, __builtin_bit_cast(bf16x8, q[0]),
+                                                       f32x4{}, 0, 0, 0);
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8 *)(kp + 32),
+                                                       __builtin_bit_cast(bf16x8, q[1]), s[u], 0, 0, 0);
+      }
+    } else {
+      const float *kp = kt + 16 * grp + l16 * P;
+      f32x4 s2[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {  // four chains
+        const f32x4 a = *(const f32x4 *)(kp + 4 * t), b = __builtin_bit_cast(f32x4, q[t]);
+        s2[t] = f32x4{};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s2[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], s2[t], 0, 0, 0);
+      }
+      s[0] = (s2[0] + s2[1]) + (s2[2] + s2[3]);
+    }
+    // s[u][i]: key 16u + 4grp + i of the tile, head l16
+    if (masked) {
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 16 * u + 4 * grp + i;
+          if (row < lo || row >= hi || !(pages >> (row / RPI) & 1)) s[u][i] = -INFINITY;
+        }
+    }
+    float e[4 * NS], rs;
+    auto weigh = [&](float ref) __attribute__((always_inline)) {
+      rs = 0.f;
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[4 * u + i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], cl, -ref));
+          rs += e[4 * u + i];
+        }
+    };
+    weigh(mc);  // (no key yet: mc is -inf, and the sum +inf or NaN)
+    if (__builtin_amdgcn_ballot_w64(!(rs <= 65536.f)) != 0) {
+      float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+      if constexpr (NS > 1) mx = fmaxf(mx, fmaxf(fmaxf(s[NS - 1][0], s[NS - 1][1]), fmaxf(s[NS - 1][2], s[NS - 1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float m_new = fmaxf(mc, mx * cl);
+      const float ref = m_new == -INFINITY ? 0.f : m_new;  // no key above -inf yet: weights 0
+      const float alpha = __builtin_amdgcn_exp2f(mc - ref);
+      mc = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
+      weigh(ref);
+    }
+    l += rs;
+    if constexpr (BF) {
+      bf16x8 pb;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pb[i] = (__bf16)e[i];
+      // V^T: slot j of lane (grp, l16) is V[key 16(j/4) + 4grp + j%4][16dt + l16]
+      const bf16_t *vp = vt + (4 * grp + (l16 >> 2)) * P + 4 * (l16 & 3);
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) {
+        const bf16x4 x = lds_tr16(vp + 16 * dt), y = lds_tr16(vp + 16 * P + 16 * dt);
+        const bf16x8 a = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb, o[dt], 0, 0, 0);
+      }
+    } else {
+      // k slot grp of step i is key 4grp + i; row r of product dt is d = 4r + dt
+      f32x4 a[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = *(const f32x4 *)(vt + (4 * grp + i) * P + 4 * l16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][dt], e[i], o[dt], 0, 0, 0);
+    }
+  };
+
+  // ---- results: two elements of a head's row a thread
+  auto write2 = [&](int b, int h, int d, float x, float y, float sum) __attribute__((always_inline)) {
+    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+    T *const op = (T *)p.a.o + b * p.a.o_rs + (head0 + h) * HD + d;
+    if constexpr (BF)
+      *(uint32_t *)op = (uint32_t)f32_to_bf16(x * inv) | ((uint32_t)f32_to_bf16(y * inv) << 16);
+    else
+      *(float2 *)op = make_float2(x * inv, y * inv);
+  };
+  // row h of the record of a sequence's piece in bin `at` (a bin has two: the end
+  // of a sequence begun before it, and the start of one, begun in bin0, that goes on)
+  auto record = [&](int at, int bin0, int h) __attribute__((always_inline)) {
+    return p.ws + ((((int64_t)at * 2 + (at == bin0)) * p.columns + col) * kMaxRows + h) * kRec;
+  };
+  // a cut sequence: its first bin and the number of its pieces, one a bin
+  struct Cut {
+    int b, bin0, pieces;
+  };
+  Cut cuts[2] = {{0, 0, 0}, {0, 0, 0}};  // one that began before the share, one that goes on
+
+  if (n_wg > 0) {
+    Tile x;       // the wave's tile (its loads are in flight)
+    Window w;     // of the tiles to come
+    Tile seg;     // the next sequence whose parts are to be added (its t: 0), ...
+    Window sw;
+    int first;    // ... and the position of its first tile
+    {
+      const int src = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > pos0));
+      first = __builtin_amdgcn_readlane(upto - own, src);
+      if (per == 1) {
+        w = Window{0, some};
+        seg = Tile{src, 0, __builtin_amdgcn_readlane(some, src), 0};
+      } else {
+        w = window(src * per);
+        for (;;) {  // (one round unless a lane's run is longer than a window)
+          const int t = tiles_of(w.len), up = wave_scan(t);
+          const unsigned long long hit = __builtin_amdgcn_ballot_w64(first + up > pos0);
+          if (hit) {
+            const int i = __builtin_ctzll(hit);
+            first += __builtin_amdgcn_readlane(up - t, i);
+            seg = Tile{w.b0 + i, 0, __builtin_amdgcn_readlane(w.len, i), 0};
+            break;
+          }
+          first += __builtin_amdgcn_readlane(up, 63);
+          w = window(w.b0 + 64);
+        }
+      }
+      sw = w;
+    }
+    const int n = n_wg > wave ? (n_wg - wave + 3) / 4 : 0;  // the wave's tiles
+    Rows buf;
+    Tile ahead[3];  // the wave's tiles i .. i + 2 (the last one again past the end)
+    bool fresh = true;
+    if (n > 0) {
+      x = seg;
+      x.t = pos0 - first;
+      if (wave) x = skip(x, wave, w);
+      load_q(x.b);
+      load_ids(x);
+      ahead[0] = x;
+      ahead[1] = 1 < n ? skip(x, 4, w) : x;
+      locate_rows(x);
+      load_rows(buf, x);
+      load_ids(ahead[1]);
+      ahead[2] = 2 < n ? skip(ahead[1], 4, w) : ahead[1];
+    }
+    int i = 0, base = 0;  // base: the sequence in the first place of LDS
+    auto step = [&]() __attribute__((always_inline)) {
+      locate_rows(ahead[1]);
+      const int lo = buf.lo, hi = buf.hi, pages = buf.pages;
+      const bool masked = lo > 0 || hi < TK || pages != 15;
+      // a wave's LDS instructions execute in order, so its tile needs no
+      // barrier; wave_barrier keeps the compiler from moving them across
+      __builtin_amdgcn_wave_barrier();
+      store_rows(buf, masked);
+      __builtin_amdgcn_wave_barrier();
+      if (fresh) {
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) q[t] = qn[t];
+        mc = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = f32x4{};
+      }
+      x = ahead[0];
+      const bool ends = i + 1 == n || ahead[1].b != x.b;
+      if (i + 1 < n) {
+        load_rows(buf, ahead[1]);
+        if (ends) load_q(ahead[1].b);
+        load_ids(ahead[2]);
+        ahead[0] = ahead[1];
+        ahead[1] = ahead[2];
+        if (i + 3 < n) ahead[2] = skip(ahead[2], 4, w);
+      }
+      compute(masked, lo, hi, pages);
+      if (ends) {
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (l16 < rows) {
+          float *const h = hold + (((x.ord - base) * 4 + wave) * rows + l16) * kHold;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // bf16: o[j] is d = 16j + 4grp ..; fp32: o[0..3][j] is d = 16grp + 4j ..
+            *(f32x4 *)(h + (BF ? 16 * j + 4 * grp : 16 * grp + 4 * j)) =
+                BF ? o[j] : f32x4{o[0][j], o[1][j], o[2][j], o[3][j]};
+          if (grp == 0) *(float2 *)(h + HD) = make_float2(mc, l);
+        }
+      }
+      fresh = ends;
+      ++i;
+    };
+    for (;;) {
+      while (i < n && ahead[0].ord < base + room) step();
+      __syncthreads();
+      bool more = true;
+      for (int place = 0; more && place < room; ++place) {
+        const int nt = tiles_of(seg.len), i0 = max(first - pos0, 0), i1 = min(first + nt - pos0, n_wg);
+        const int bin0 = (int)((uint32_t)first / (uint32_t)share);
+        const int pieces = (int)((uint32_t)(first + nt - 1) / (uint32_t)share) - bin0 + 1;
+        if (pieces > 1) cuts[bin0 == bin] = Cut{seg.b, bin0, pieces};
+        for (int k = tid; k < rows * (HD / 2); k += 256) {
+          const int h = k / (HD / 2), d = 2 * (k % (HD / 2));
+          const float *r = hold + (place * 4 * rows + h) * kHold;
+          float2 ml[4];
+          float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            ml[v] = make_float2(-INFINITY, 0.f);  // no tile of it
+            if (((v - i0) & 3) < i1 - i0) ml[v] = *(const float2 *)(r + v * rows * kHold + HD);
+            M = fmaxf(M, ml[v].x);
+          }
+          const float Mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            if (((v - i0) & 3) >= i1 - i0) continue;
+            const float f = __builtin_amdgcn_exp2f(ml[v].x - Mu);
+            const float2 a = *(const float2 *)(r + v * rows * kHold + d);
+            L = fmaf(ml[v].y, f, L);
+            A0 = fmaf(a.x, f, A0);
+            A1 = fmaf(a.y, f, A1);
+          }
+          if (pieces == 1) {
+            write2(seg.b, h, d, A0, A1, L);
+          } else {
+            float *const to = record(bin, bin0, h);
+            put2(to + d, A0, A1);
+            if (d == 0) put2(to + HD, M, L);
+          }
+        }
+        first += nt;
+        more = first < pos0 + n_wg;
+        if (more) seg = next_seq(seg, sw);
+      }
+      if (!more) break;
+      __syncthreads();  // the places are free again
+      base += room;
+    }
+    if (cuts[0].pieces | cuts[1].pieces) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the records' stores have reached memory
+      __syncthreads();
+      if (tid < 2) {
+        const Cut u = tid ? cuts[1] : cuts[0];
+        last_in[tid] =
+            u.pieces && arrive_last(p.arrive_end - 2 * ((int64_t)u.b * p.columns + col + 1), u.pieces, p.tag);
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int side = 0; side < 2; ++side) {
+        if (!last_in[side]) continue;
+        const Cut u = side ? cuts[1] : cuts[0];
+        for (int k = tid; k < rows * (HD / 2); k += 256) {
+          const int h = k / (HD / 2), d = 2 * (k % (HD / 2));
+          float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
+          for (int n0 = 0; n0 < u.pieces; n0 += kMergeBatch) {
+            float2 ml[kMergeBatch], a[kMergeBatch];
+#pragma unroll
+            for (int v = 0; v < kMergeBatch; ++v) {
+              const float *const r = record(u.bin0 + min(n0 + v, u.pieces - 1), u.bin0, h);
+              ml[v] = get2(r + HD);
+              a[v] = get2(r + d);
+            }
+            float mx = M;
+#pragma unroll
+            for (int v = 0; v < kMergeBatch; ++v) mx = n0 + v < u.pieces ? fmaxf(mx, ml[v].x) : mx;
+            const float mu = mx == -INFINITY ? 0.f : mx, fo = __builtin_amdgcn_exp2f(M - mu);
+            L *= fo;
+            A0 *= fo;
+            A1 *= fo;
+#pragma unroll
+            for (int v = 0; v < kMergeBatch; ++v) {
+              const bool in = n0 + v < u.pieces;  // (a record past the end is never multiplied: it may hold anything)
+              const float f = __builtin_amdgcn_exp2f(ml[v].x - mu);
+              L = in ? fmaf(ml[v].y, f, L) : L;
+              A0 = in ? fmaf(a[v].x, f, A0) : A0;
+              A1 = in ? fmaf(a[v].y, f, A1) : A1;
+            }
+            M = mx;
+          }
+          write2(u.b, h, d, A0, A1, L);
+        }
+      }
+    }
+  }
+  // sequences without a key
+  for (int b = bin; b < c.batch; b += p.bins)
+    if (tiles_of(clamp_len(c.lens[b])) == 0)
+      for (int k = tid; k < rows * (HD / 2); k += 256) write2(b, k / (HD / 2), 2 * (k % (HD / 2)), 0.f, 0.f, 0.f);
+}
+
 // One wave per (row, query head), lane = element of the head: every key's
 // dot product is a wave sum.
 template <typename T>
@@ -207,12 +769,17 @@ int check_cache(const std::string &op, const bn_paged_kv *kv, Paged *c) {
     return fail(BN_ERR_SHAPE, op + ": negative batch or number of pages");
   if (kv->n_kv_heads <= 0) return fail(BN_ERR_SHAPE, op + ": num_kv_heads must be positive");
   if (kv->head_dim != HD) return fail(BN_ERR_UNSUPPORTED, op + ": head_dim must be 64");
-  if (kv->page_size <= 0 || (kv->page_size & (kv->page_size - 1)))
-    return fail(BN_ERR_UNSUPPORTED, op + ": page_size must be a power of two");
-  if ((int64_t)kv->max_pages * kv->page_size > (1 << 30))
+  if (kv->page_size < 8 || (kv->page_size & (kv->page_size - 1)))
+    return fail(BN_ERR_UNSUPPORTED, op + ": page_size must be a power of two, at least 8");
+  const int64_t keys = (int64_t)kv->max_pages * kv->page_size;
+  if (keys > (1 << 30))
     return fail(BN_ERR_UNSUPPORTED, op + ": max_pages * page_size must be at most 2^30 keys");
   if (kv->batch == 0) return BN_OK;
   if (kv->batch > (1 << 20)) return fail(BN_ERR_UNSUPPORTED, op + ": more than 2^20 sequences");
+  if (kv->batch * keys > ((int64_t)1 << 34))  // tiles of 16 keys are counted in 32 bits
+    return fail(BN_ERR_UNSUPPORTED, op + ": batch * max_pages * page_size must be at most 2^34 keys");
+  if (kv->row_stride > (1 << 24))  // (a load's rows are reached through 32-bit byte offsets)
+    return fail(BN_ERR_UNSUPPORTED, op + ": cache row stride must be at most 2^24 elements");
   const int64_t vec = kv->dtype == BN_BF16 ? 8 : 4, most = (int64_t)1 << 40;
   for (int64_t s : {kv->page_stride, kv->head_stride, kv->row_stride})
     if (s < HD || s % vec || s > most)
@@ -232,7 +799,7 @@ int check_cache(const std::string &op, const bn_paged_kv *kv, Paged *c) {
   c->batch = kv->batch; c->n_pages = kv->n_pages; c->max_pages = kv->max_pages;
   c->shift = __builtin_ctz((unsigned)kv->page_size);
   c->n_kv_heads = kv->n_kv_heads;
-  c->cap = kv->max_pages * kv->page_size;
+  c->cap = kv->n_pages > 0 ? (int)keys : 0;  // without a page there is no key
   return BN_OK;
 }
 
@@ -295,6 +862,72 @@ class DeviceScope {
   }
 };
 
+// A launch's 48-bit tag: a mixed counter (SplitMix64's finaliser), so that no
+// plausible memory contents look like this launch's arrivals.
+unsigned long long next_tag() {
+  static std::atomic<uint64_t> launches{0};
+  uint64_t z = (launches.fetch_add(1) + 1) * 0x9e3779b97f4a7c15ull + 0x517cc1b727220a95ull;
+  z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
+  z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
+  return (z ^ (z >> 31)) >> 16 | 1;
+}
+
+// The decode kernel's launch: a workgroup per share and column.
+constexpr int kDecGroups = 256;
+struct DecodePlan {
+  int hblocks, columns, bins;
+  size_t records, words;  // bytes
+};
+DecodePlan plan_decode(int batch, int n_heads, int n_kv_heads) {
+  DecodePlan d;
+  d.hblocks = (n_heads / n_kv_heads + kMaxRows - 1) / kMaxRows;
+  d.columns = d.hblocks * n_kv_heads;
+  d.bins = std::max(1, kDecGroups / d.columns);
+  d.records = d.bins == 1 ? 0 : (size_t)d.bins * 2 * d.columns * kMaxRows * kRec * sizeof(float);
+  d.words = d.bins == 1 ? 0 : (size_t)batch * d.columns * 16;
+  return d;
+}
+
+// A call's workspace: the caller's, or one from the pool until the end of the call's work.
+class Workspace {
+  void *own_ = nullptr, *stream_ = nullptr;
+
+ public:
+  void *p = nullptr;
+  int take(void *given, size_t need, void *stream) {
+    p = given;
+    if (p || need == 0) return BN_OK;
+    const int st = bn_alloc(&own_, need, stream);
+    stream_ = stream;
+    p = own_;
+    return st;
+  }
+  int release(int st) {
+    if (own_) {
+      const int st2 = bn_free(own_, stream_);
+      own_ = nullptr;
+      if (st == BN_OK) st = st2;
+    }
+    return st;
+  }
+};
+
+int launch_decode(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
+  const DecodePlan d = plan_decode(a.c.batch, a.n_heads, a.c.n_kv_heads);
+  DecodeParams p;
+  p.a = a;
+  p.ws = (float *)ws;
+  p.arrive_end = (unsigned long long *)((char *)ws + d.records + d.words);
+  p.tag = next_tag();
+  p.bins = d.bins; p.hblocks = d.hblocks; p.columns = d.columns;
+  p.k0 = 0;
+  const dim3 grid((unsigned)(d.bins * d.columns)), block(256);
+  if (dtype == BN_BF16) hipLaunchKernelGGL(paged_decode_kernel<bf16_t>, grid, block, 0, s, p);
+  else hipLaunchKernelGGL(paged_decode_kernel<float>, grid, block, 0, s, p);
+  BN_LAUNCH_CHECK();
+  return BN_OK;
+}
+
 int attention(const char *name, const bn_paged_kv *kv, const void *q, void *o, const int32_t *starts,
               int n_rows, int n_heads, int64_t q_rs, int64_t o_rs, float scale,
               const int32_t *prefix_pages, int prefix_len, void *workspace, size_t workspace_bytes,
@@ -329,13 +962,16 @@ int attention(const char *name, const bn_paged_kv *kv, const void *q, void *o, c
   p.n_rows = n_rows; p.n_heads = n_heads; p.group = n_heads / kv->n_kv_heads;
   p.cl = scale * kLog2e;
   p.prefix_pages = prefix_pages; p.prefix_len = prefix_len;
+  Workspace ws;
+  if ((st = ws.take(workspace, need, stream))) return st;
+  if (!starts && prefix_len == 0) return ws.release(launch_decode(p, kv->dtype, ws.p, as_stream(stream)));
   const dim3 grid(n_rows, n_heads);
   if (kv->dtype == BN_BF16)
     hipLaunchKernelGGL(paged_rows_kernel<bf16_t>, grid, dim3(64), 0, as_stream(stream), p);
   else
     hipLaunchKernelGGL(paged_rows_kernel<float>, grid, dim3(64), 0, as_stream(stream), p);
-  BN_LAUNCH_CHECK();
-  return BN_OK;
+  const hipError_t e = hipGetLastError();
+  return ws.release(e == hipSuccess ? BN_OK : hip_fail(e, __FILE__, __LINE__));
 }
 
 }  // namespace
@@ -388,8 +1024,12 @@ int bn_paged_append(const bn_paged_kv *cache, const void *k, const void *v, cons
 }
 
 size_t bn_paged_workspace_size(const bn_paged_kv *cache, int n_heads, int n_rows, int prefix_len) {
-  (void)cache; (void)n_heads; (void)n_rows; (void)prefix_len;
-  return 0;
+  Paged c;
+  if (n_rows <= 0 || prefix_len < 0 || !cache || check_cache("", cache, &c) || cache->batch == 0 ||
+      check_heads("", n_heads, cache->n_kv_heads))
+    return 0;
+  const DecodePlan d = plan_decode(cache->batch, n_heads, cache->n_kv_heads);
+  return d.records + d.words;
 }
 
 int bn_paged_decode(const bn_paged_kv *cache, const void *q, void *o, int n_heads, int64_t q_row_stride,

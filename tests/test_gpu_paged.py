@@ -43,7 +43,7 @@ APPENDS = [
     ("f32", [1, 17, 300], [1, 1, 1], 4, 32, 16, False, 1e4, "in place"),
     ("bf16", [40, 0, 33, 9], [40, 0, 2, 9], 2, 6, 8, "gaps", 1e4, "out"),
     ("f32", [65, 64, 63], [65, 1, 40], 1, 1, 64, True, 5e5, None),
-    ("bf16", [70, 3], [70, 5], 3, 15, 1, False, 0.0, "in place"),      # more rows than the length
+    ("bf16", [70, 3], [70, 5], 3, 15, 8, False, 0.0, "in place"),      # more rows than the length
     ("f32", [1000, 700], [900, 650], 2, 4, 32, True, 1e4, "out"),      # many rows a workgroup
     ("bf16", [1200, 400, 64], [1200, 1, 64], 4, 8, 128, False, 1e4, "in place"),
     ("bf16", [-3, 5], [2, 5], 2, 2, 16, True, 1e4, "out"),             # a negative length is empty
@@ -141,8 +141,8 @@ DECODES = [
     ("f32", EDGES, 3, 15, 32, "gaps", [(20, 3), (23, 0), (2, 0)]),
     ("bf16", EDGES, 1, 16, 64, "gaps", [(16, 0), (20, 1)]),
     ("bf16", EDGES, 1, 20, 128, True, []),             # more heads a KV head than a tile holds
-    ("f32", EDGES, 2, 66, 1, False, []),
-    ("bf16", EDGES[:14], 5, 5, 1, True, [(13, 11), (13, 63)]),
+    ("f32", EDGES, 2, 66, 8, False, []),
+    ("bf16", EDGES[:14], 5, 5, 8, True, [(13, 1), (13, 7)]),
     ("bf16", [1000], 1, 8, 256, True, [(0, 1)]),
     ("bf16", [513] * 3 + [2000], 4, 32, 16, True, []),
     ("f32", [513] * 3 + [2000], 4, 32, 16, False, []),
@@ -267,7 +267,7 @@ PREFILLS = [
     ("bf16", [300, 40, 257], [3, 17, 200], 2, 12, 8, "gaps", [(0, 0), (2, 30)], 1),
     ("f32", [300, 40, 257], [3, 17, 200], 2, 10, 64, "gaps", [(0, 0)], 1),
     ("bf16", [200, 64], [199, 64], 1, 1, 128, True, [], 0),
-    ("bf16", [100, 31], [64, 31], 1, 20, 1, True, [(0, 50)], 0),
+    ("bf16", [100, 31], [64, 31], 1, 20, 8, True, [(0, 5)], 0),
     ("bf16", [10, 5], [12, 9], 2, 8, 16, True, [], 2),      # more rows than keys: the first see nothing
     ("f32", [10, -5], [12, 9], 2, 6, 16, True, [], 2),
     ("bf16", [1000, 700, 3], [5, 1, 1], 4, 32, 32, True, [], 0),   # a few rows behind long caches
@@ -362,7 +362,7 @@ SHARED = [
     ("bf16", 129, [-100, -129, -1, 20, -300], 2, 12, 16, "gaps"),   # shorter than the prefix, empty
     ("f32", 129, [-100, -129, -1, 20, -300], 2, 12, 16, True),
     ("bf16", 2500, [1] * 40 + [700], 1, 3, 128, True),
-    ("bf16", 70, [0] * 300, 1, 8, 1, True),
+    ("bf16", 70, [0] * 300, 1, 8, 8, True),
 ]
 
 

@@ -55,6 +55,8 @@ CALLS = {"Paged append": append, "Paged decode": decode, "Paged prefill": prefil
     (dict(head_dim=128), B.BN_ERR_UNSUPPORTED, "head_dim must be 64"),
     (dict(page_size=0), B.BN_ERR_UNSUPPORTED, "power of two"),
     (dict(page_size=24), B.BN_ERR_UNSUPPORTED, "power of two"),
+    (dict(page_size=4), B.BN_ERR_UNSUPPORTED, "at least 8"),
+    (dict(row_stride=(1 << 24) + 8), B.BN_ERR_UNSUPPORTED, "2^24"),
     (dict(page_size=-16), B.BN_ERR_UNSUPPORTED, "power of two"),
     (dict(max_pages=1 << 27), B.BN_ERR_UNSUPPORTED, "2^30"),
     (dict(batch=(1 << 20) + 1), B.BN_ERR_SHAPE | B.BN_ERR_UNSUPPORTED, ""),
