@@ -731,6 +731,735 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
       for (int k = tid; k < rows * (HD / 2); k += 256) write2(b, k / (HD / 2), 2 * (k % (HD / 2)), 0.f, 0.f, 0.f);
 }
 
+// ------------------------------------------------- prefill, over pages
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// The rows of a (sequence, KV head) are its new tokens' query heads of the
+// group, token by token (row r: token r / group, head r % group), so that any
+// group fills the products' rows and a few tokens take few of them.  A unit is
+// R = 32 * HW consecutive rows; its keys go in tiles of 32.
+struct PrefillParams {
+  AttnParams a;
+  float *ws;                       // records: [slot][R][kRec]
+  unsigned long long *arrive_end;  // two arrival words per slot below it
+  unsigned long long tag;
+  int slots;   // records that the workspace holds
+  int prefix;  // the rows are the batch's, the keys prefix_pages' (every piece leaves a record)
+};
+struct Piece {
+  int b, g, unit, part, parts;  // part of parts of the unit's keys
+  int row0, rows;               // the sequence's rows of the tensors
+  int last;                     // keys the sequence's last row sees, before the table's clamp
+  int slot;                     // record of the unit's first part (parts > 1)
+};
+constexpr int kPartMin = 24;      // tiles of a part at least
+constexpr int kPartsAll = 1024;   // a part is at least this share of all the call's tiles
+
+// Which piece of work is workgroup L's.  A call's units differ in length (the
+// diagonal, and the sequences themselves): a unit whose keys are more than
+// twice a 1024th part of all the call's tiles is cut into parts, as many as
+// its sequence's longest unit has such shares, so that no compute unit is left
+// with a long one at the end; sequences of no such unit are not cut.  XCDs: a
+// KV head's units go to 8 / n_kv_heads of them, whose L2s then hold its keys.
+// Every wave finds its piece itself from the lengths.  False: none.
+template <int R>
+__device__ __forceinline__ bool find_piece(const PrefillParams &p, Piece &w) {
+  const Paged &c = p.a.c;
+  const int lane = threadIdx.x & 63, hkv = c.n_kv_heads, G = p.a.group;
+  int idx;
+  if (hkv <= 8 && (8 % hkv) == 0) {
+    const int x = blockIdx.x & 7;
+    w.g = x % hkv;
+    idx = (blockIdx.x >> 3) * (8 / hkv) + x / hkv;
+  } else {
+    w.g = blockIdx.x % hkv;
+    idx = blockIdx.x / hkv;
+  }
+  struct Seq {
+    int row0, rows, last, units, steps;  // steps: tiles of its longest unit
+    float weight;                        // tiles of all its units, about
+  };
+  auto seq = [&](int b) __attribute__((always_inline)) {
+    Seq s;
+    if (p.prefix) {
+      s.row0 = 0;
+      s.rows = c.batch;
+      s.last = p.a.prefix_len;
+    } else {
+      const int bb = min(b, c.batch - 1);
+      const int s0 = p.a.starts ? p.a.starts[bb] : bb, s1 = p.a.starts ? p.a.starts[bb + 1] : bb + 1;
+      s.row0 = min(max(s0, 0), p.a.n_rows);
+      s.rows = min(max(s1, s.row0), p.a.n_rows) - s.row0;
+      s.last = max(c.lens[bb], 0) - s1 + s.row0 + s.rows;  // (s1 is past the tensors' rows: not its last)
+      if (b >= c.batch) s.rows = 0;
+    }
+    s.units = (s.rows * G + R - 1) / R;
+    const int cap = p.prefix ? p.a.prefix_len : c.cap;
+    auto tiles = [&](int n) { return (min(max(n, 0), cap) + 31) >> 5; };
+    s.steps = tiles(s.last);
+    const int first = p.prefix ? s.steps : tiles(s.last - s.rows + min(s.rows, (R + G - 1) / G));
+    s.weight = (float)s.units * (0.5f * (float)(s.steps + first) + 1.f);
+    return s;
+  };
+  const int n = p.prefix ? 1 : c.batch, per = (n + 63) >> 6;
+  Seq mine = seq(lane * per);
+  float total = lane * per < n ? mine.weight : 0.f;
+  for (int i = 1; i < per; ++i) total += lane * per + i < n ? seq(lane * per + i).weight : 0.f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+  const int share = max((int)(total * (float)hkv * (1.f / kPartsAll)), kPartMin);
+  auto parts_of = [&](const Seq &s) { return max(s.steps / share, 1); };
+  auto count = [&](const Seq &s, bool in, int &all, int &cut) __attribute__((always_inline)) {
+    const int parts = parts_of(s), k = in ? s.units * parts : 0;
+    all += k;
+    cut += parts > 1 || p.prefix ? k : 0;
+  };
+  int all = 0, cut = 0;
+  count(mine, lane * per < n, all, cut);
+  for (int i = 1; i < per; ++i) count(seq(lane * per + i), lane * per + i < n, all, cut);
+  int up = wave_scan(all), up_cut = wave_scan(cut);
+  if (idx >= __builtin_amdgcn_readlane(up, 63)) return false;
+  int src = __builtin_ctzll(__builtin_amdgcn_ballot_w64(up > idx));
+  int before = __builtin_amdgcn_readlane(up - all, src), cuts = __builtin_amdgcn_readlane(up_cut - cut, src);
+  int b = src * per;
+  while (per > 1) {  // the sequence within the lane's run, 64 at a time
+    mine = seq(b + lane);
+    all = cut = 0;
+    count(mine, b + lane < n, all, cut);
+    up = wave_scan(all);
+    up_cut = wave_scan(cut);
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(before + up > idx);
+    if (hit) {
+      src = __builtin_ctzll(hit);
+      before += __builtin_amdgcn_readlane(up - all, src);
+      cuts += __builtin_amdgcn_readlane(up_cut - cut, src);
+      b += src;
+      break;
+    }
+    before += __builtin_amdgcn_readlane(up, 63);
+    cuts += __builtin_amdgcn_readlane(up_cut, 63);
+    b += 64;
+  }
+  const int k = idx - before;
+  w.b = b;
+  w.row0 = __builtin_amdgcn_readlane(mine.row0, src);
+  w.rows = __builtin_amdgcn_readlane(mine.rows, src);
+  w.last = __builtin_amdgcn_readlane(mine.last, src);
+  const int units = __builtin_amdgcn_readlane(mine.units, src), steps = __builtin_amdgcn_readlane(mine.steps, src);
+  w.parts = __builtin_amdgcn_readfirstlane(max(steps / share, 1));
+  const int from_end = __builtin_amdgcn_readfirstlane(k / w.parts);  // longest units first
+  w.unit = units - 1 - from_end;
+  w.part = k - from_end * w.parts;
+  w.slot = (cuts + from_end * w.parts) * hkv + w.g;  // parts of a unit: hkv slots apart
+  // (row_starts that decrease could count rows twice and pass the workspace)
+  return w.parts == 1 || (int64_t)w.slot + (int64_t)(w.parts - 1) * hkv < p.slots;
+}
+
+// What the two prefill kernels share: the piece's keys, the rows' limits and
+// the scalars of the pages.
+struct PieceKeys {
+  const __attribute__((address_space(4))) int32_t *table;
+  int t0, t1;  // its tiles
+  int end;     // keys that some row of the unit sees
+  int shift;
+  __device__ __forceinline__ int entry(int key) const { return table[min(key, end - 1) >> shift]; }
+};
+template <int R>
+__device__ __forceinline__ PieceKeys piece_keys(const PrefillParams &p, const Piece &w) {
+  const Paged &c = p.a.c;
+  PieceKeys k;
+  if (p.prefix) {
+    k.end = p.a.prefix_len;
+    k.table = (const __attribute__((address_space(4))) int32_t *)p.a.prefix_pages;
+  } else {
+    const int tokens = min((w.unit * R + R - 1) / p.a.group + 1, w.rows);  // up to the unit's last row
+    k.end = min(max(w.last - w.rows + tokens, 0), c.cap);
+    k.table = (const __attribute__((address_space(4))) int32_t *)(c.table + w.b * c.table_stride);
+  }
+  k.end = __builtin_amdgcn_readfirstlane(k.end);
+  const int nt = (k.end + 31) >> 5;
+  k.t0 = __builtin_amdgcn_readfirstlane((int)((int64_t)nt * w.part / w.parts));
+  k.t1 = __builtin_amdgcn_readfirstlane((int)((int64_t)nt * (w.part + 1) / w.parts));
+  k.shift = c.shift;
+  return k;
+}
+// keys that token t of the piece's sequence sees
+__device__ __forceinline__ int key_limit(const PrefillParams &p, const Piece &w, int t) {
+  return p.prefix ? min(max(p.a.c.lens[t], 0), p.a.prefix_len)
+                  : min(max(w.last - w.rows + t + 1, 0), p.a.c.cap);
+}
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+// The end of a piece, all its waves: `sum(row, d, ml)` gives NV consecutive
+// elements of a row's accumulator and its (reference in log2 units, sum); a
+// whole unit is written, of a cut one a record is left and the last part to
+// arrive adds them, in the order of the keys, and writes.
+template <typename T, int R, int THREADS, class F>
+__device__ __forceinline__ void finish_piece(const PrefillParams &p, const Piece &w, int *last_in, F &&sum) {
+  constexpr int TPR = THREADS / R, NV = HD / TPR;  // threads a row, elements a thread
+  static_assert(THREADS % R == 0 && NV % 4 == 0, "whole quads");
+  const int tid = threadIdx.x, row = tid / TPR, d0 = (tid % TPR) * NV;
+  const int fr = w.unit * R + row, t = fr / p.a.group, h = w.g * p.a.group + fr - t * p.a.group;
+  const bool there = t < w.rows;
+  float acc[NV];
+  float2 ml = sum(row, d0, acc);
+  auto write = [&]() __attribute__((always_inline)) {
+    if (!there) return;
+    const float inv = ml.y > 0.f ? 1.0f / ml.y : 0.f;
+    T *const op = (T *)p.a.o + (int64_t)(w.row0 + t) * p.a.o_rs + h * HD + d0;
+#pragma unroll
+    for (int i = 0; i < NV; i += 4) {
+      if constexpr (sizeof(T) == 2) {
+        const uint32_t lo = (uint32_t)f32_to_bf16(acc[i] * inv) | ((uint32_t)f32_to_bf16(acc[i + 1] * inv) << 16);
+        const uint32_t hi = (uint32_t)f32_to_bf16(acc[i + 2] * inv) | ((uint32_t)f32_to_bf16(acc[i + 3] * inv) << 16);
+        *(uint2 *)(op + i) = make_uint2(lo, hi);
+      } else {
+        *(float4 *)(op + i) = make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+      }
+    }
+  };
+  if (w.parts == 1) return write();
+  const int64_t step = (int64_t)p.a.c.n_kv_heads * R * kRec;
+  float *const first = p.ws + ((int64_t)w.slot * R + row) * kRec;
+  if (there) {
+    float *const r = first + w.part * step;
+#pragma unroll
+    for (int i = 0; i < NV; i += 2) put2(r + d0 + i, acc[i], acc[i + 1]);
+    if (d0 == 0) put2(r + HD, ml.x, ml.y);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the record has reached memory
+  __syncthreads();
+  if (tid == 0) *last_in = arrive_last(p.arrive_end - 2 * ((int64_t)w.slot + 1), w.parts, p.tag);
+  __syncthreads();
+  if (!*last_in || !there) return;
+  ml = make_float2(-INFINITY, 0.f);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) acc[i] = 0.f;
+  constexpr int MB = NV >= 32 ? 2 : 4;  // records read at once
+  for (int n0 = 0; n0 < w.parts; n0 += MB) {
+    float2 m2[MB], a[MB][NV / 2];
+#pragma unroll
+    for (int v = 0; v < MB; ++v) {
+      const float *const r = first + min(n0 + v, w.parts - 1) * step;
+      m2[v] = get2(r + HD);
+#pragma unroll
+      for (int i = 0; i < NV / 2; ++i) a[v][i] = get2(r + d0 + 2 * i);
+    }
+#pragma unroll
+    for (int v = 0; v < MB; ++v) {
+      const bool in = n0 + v < w.parts;
+      const float mn = in ? fmaxf(ml.x, m2[v].x) : ml.x, mu = mn == -INFINITY ? 0.f : mn;
+      const float fo = __builtin_amdgcn_exp2f(ml.x - mu), fn = __builtin_amdgcn_exp2f(m2[v].x - mu);
+      auto add = [&](float s, float x) { return in ? fmaf(x, fn, s * fo) : s; };
+      ml.y = add(ml.y, m2[v].y);
+#pragma unroll
+      for (int i = 0; i < NV / 2; ++i) {
+        acc[2 * i] = add(acc[2 * i], a[v][i].x);
+        acc[2 * i + 1] = add(acc[2 * i + 1], a[v][i].y);
+      }
+      ml.x = mn;
+    }
+  }
+  write();
+}
+
+// bf16.  HW waves of 32 rows share each staged K/V tile, KW such parts take a
+// piece's tiles in turn; their (m, l, O) meet in LDS.  Per wave and tile
+//   S^T[key][row] = K . Q^T  (v_mfma_f32_32x32x16_bf16: 16 keys of one row a lane)
+//   O^T[d][row] += V^T . P^T, whose operand is P^T as the scores left it
+// (bf16 probabilities: half a step of 2^-8 each, in the row sum too, which the
+// matrix cores form against a 0/1 selector).  Weights are taken against a
+// reference that moves to the true maximum only when a tile's sum passes 2^16.
+constexpr float kSumLimit = 65536.f, kMoveLog2 = 8.f;
+template <int HW, int KW, int OCC>
+__global__ __launch_bounds__(64 * HW * KW, OCC) void paged_prefill_bf16_kernel(PrefillParams p) {
+  constexpr int W = HW * KW, R = 32 * HW;
+  constexpr int KP = HD + 8;           // K row pitch, elements (144 B: conflict-free b128 rows)
+  constexpr int VP = HD + 16;          // V row pitch (160 B: conflict-free transpose reads)
+  constexpr int KT = 32 * KP, VT = 32 * VP;
+  constexpr int NB = HW > 1 ? 2 : 1;   // tile buffers (HW == 1: a wave's tile is its own)
+  constexpr int OP = HD + 4, OT = 32 * OP;  // a wave's O at the end, floats
+  constexpr int LDSE = KW * NB * (KT + VT) > 2 * W * OT ? KW * NB * (KT + VT) : 2 * W * OT;  // elements
+  __shared__ __attribute__((aligned(16))) bf16_t smem[LDSE];
+  __shared__ float red_m[W][32], red_l[W][32];
+  __shared__ int last_in;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hw = wave % HW, kw = wave / HW;
+  const int r32 = lane & 31, hf = lane >> 5;
+  Piece w;
+  if (!find_piece<R>(p, w)) return;
+  const Paged &c = p.a.c;
+  const PieceKeys keys = piece_keys<R>(p, w);
+  const float cl = p.a.cl;
+  const int ni = (keys.t1 - keys.t0 + KW - 1) / KW;  // steps: tile t0 + kw + KW*i each
+
+  // this lane's row
+  const int fr = w.unit * R + 32 * hw + r32, tok = fr / p.a.group, head = fr - tok * p.a.group;
+  const bool there = tok < w.rows;
+  const int limit = there ? key_limit(p, w, tok) : 0;
+  const int all_see = wave_min(there ? limit : 0x7fffffff);  // keys that all the wave's rows see
+  bf16x8 qreg[4];
+  {
+    const bf16_t *const qp = (const bf16_t *)p.a.q + (int64_t)(w.row0 + (there ? tok : 0)) * p.a.q_rs +
+                             (w.g * p.a.group + (there ? head : 0)) * HD + 8 * hf;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      qreg[t] = *(const bf16x8 *)(qp + 16 * t);
+      if (!there) qreg[t] = bf16x8{};
+    }
+  }
+
+  // staging: the HW waves of a key part share its tile, NC chunks of 8 rows
+  // each (16-byte piece lane % 8 of row lane / 8); a chunk's rows lie in one page
+  constexpr int NC = 4 / HW;
+  const int crow = lane >> 3, ccol = (lane & 7) * 8;
+  const int slot_mask = (1 << c.shift) - 1;
+  const int64_t page_bytes = c.page_stride * 2;
+  const uint32_t row_bytes = (uint32_t)c.row_stride * 2, off = crow * row_bytes + ccol * 2;
+  const char *const Kg = (const char *)((const bf16_t *)c.k + w.g * c.head_stride);
+  const char *const Vg = (const char *)((const bf16_t *)c.v + w.g * c.head_stride);
+  u32x4 kr[NC], vr[NC];
+  int ids[4];
+  int pages = 0, pages_next = 0;  // bit r: rows 8r .. of the tile have memory; of this tile, of the next
+  auto load_ids = [&](int i) __attribute__((always_inline)) {
+    const int key0 = 32 * (keys.t0 + kw + KW * i);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) ids[r] = keys.entry(key0 + 8 * r);
+  };
+  auto gload = [&](int i) __attribute__((always_inline)) {
+    const int key0 = 32 * (keys.t0 + kw + KW * i);
+    pages_next = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) pages_next |= ((unsigned)ids[r] < (unsigned)c.n_pages) << r;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      int id = ids[j];
+      if constexpr (HW > 1) {  // (a scalar's index is a constant)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) id = NC * hw + j == r ? ids[r] : id;
+      }
+      const bool ok = (unsigned)id < (unsigned)c.n_pages;
+      const int64_t at = (ok ? id : 0) * page_bytes +
+                         (int64_t)((uint64_t)(uint32_t)((key0 + 8 * (NC * hw + j)) & slot_mask) * row_bytes);
+      kr[j] = *(const u32x4 *)(Kg + at + off);
+      vr[j] = *(const u32x4 *)(Vg + at + off);
+    }
+  };
+  auto lstore = [&](int i) __attribute__((always_inline)) {
+    const int key0 = 32 * (keys.t0 + kw + KW * i);
+    bf16_t *const kd = smem + (kw * NB + (NB > 1 ? i & 1 : 0)) * (KT + VT), *const vd = kd + KT;
+    if (key0 + 32 > keys.end || pages_next != 15) {  // no key: zeros, whatever lies there
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const int r = NC * hw + j;
+        if (!(pages_next >> r & 1) || key0 + 8 * r + crow >= keys.end) vr[j] = u32x4{0, 0, 0, 0};
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j) *(u32x4 *)(kd + (8 * (NC * hw + j) + crow) * KP + ccol) = kr[j];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) *(u32x4 *)(vd + (8 * (NC * hw + j) + crow) * VP + ccol) = vr[j];
+  };
+
+  float l = 0.f, mcv = -INFINITY;  // row sum; reference, log2 units
+  f32x16 o[2] = {f32x16{}, f32x16{}};
+  const uint32_t rs_bits = (((lane & 15) >> 2) & 1) == ((lane >> 4) & 1) ? 0x3f803f80u : 0u;
+  const int tr_off = (4 * hf + ((lane & 15) >> 2)) * VP + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  // p = exp2(s * cl - mc) as bf16 operands, and the tile's row sum over both half-waves
+  auto exps = [&](const f32x16 &s, float mc, bf16x8 (&pb)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pb[u][j] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[8 * u + j], cl, -mc));
+    uint32_t b = rs_bits;
+    asm volatile("" : "+v"(b));  // keeps the selector from being hoisted out of the loop
+    const bf16x8 sel = __builtin_bit_cast(bf16x8, u32x4{b, b, b, b});
+    const f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sel, pb[0], f32x4{}, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(sel, pb[1], d, 0, 0, 0)[0];
+  };
+  auto fixup = [&](const f32x16 &s, bf16x8 (&pb)[2]) __attribute__((always_inline)) {
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mt = fmaxf(mcv, mx * cl);  // -inf while nothing is visible
+    const bool move = mcv == -INFINITY || mt - mcv > kMoveLog2;
+    const float m_new = move ? mt : mcv;
+    const float mn = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(mcv - mn);
+    l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+    mcv = m_new;
+    return exps(s, mn, pb);
+  };
+
+  if (ni > 0) {
+    load_ids(0);
+    gload(0);
+    load_ids(1);
+    if (NB > 1) lstore(0);
+  }
+  if constexpr (NB > 1) __syncthreads();
+  for (int i = 0; i < ni; ++i) {
+    pages = pages_next;
+    if constexpr (NB == 1) {
+      // the wave's own tile: its LDS instructions execute in order, the
+      // barriers keep the compiler from moving them across
+      __builtin_amdgcn_wave_barrier();
+      lstore(i);
+      __builtin_amdgcn_wave_barrier();
+    }
+    gload(i + 1);  // past the range: the last key's page again, not used
+    load_ids(i + 2);
+    const bf16_t *const kl = smem + (kw * NB + (NB > 1 ? i & 1 : 0)) * (KT + VT), *const vl = kl + KT;
+    const int tile = keys.t0 + kw + KW * i, kb = 32 * tile;
+    if (tile < keys.t1) {  // wave-uniform
+      f32x16 s = f32x16{};
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8 *)(kl + r32 * KP + 16 * u + 8 * hf), qreg[u], s,
+                                                    0, 0, 0);
+      // V^T fragments: key slot j of 16-key chunk u is key 16u + (j/4)*8 + 4hf + j%4
+      bf16x8 va[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) {
+          const bf16x4 lo = lds_tr16(vl + 16 * u * VP + tr_off + 32 * dt);
+          const bf16x4 hi = lds_tr16(vl + (16 * u + 8) * VP + tr_off + 32 * dt);
+          va[u][dt] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        }
+      uint32_t odd = 0;  // keys of this tile with an infinite or NaN value, where some row does not see all
+      if (kb + 32 > all_see || pages != 15) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int k = (e >> 2) * 8 + hf * 4 + (e & 3);
+          if (kb + k >= limit || !(pages >> (e >> 2) & 1)) s[e] = -INFINITY;
+        }
+        uint32_t any = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int dt = 0; dt < 2; ++dt) {
+            const u32x4 x = __builtin_bit_cast(u32x4, va[u][dt]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) any |= (x[j] & 0x7f807f80u) + 0x00800080u;
+          }
+        if (__builtin_amdgcn_ballot_w64((any & 0x80008000u) != 0) != 0) {
+          // their weight in a row that does not see them is 0, but 0 times them is
+          // not: they leave the product, and are added to the rows that see them below
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              bool bad = false;
+#pragma unroll
+              for (int dt = 0; dt < 2; ++dt) {
+                const float x = (float)va[u][dt][j];
+                const bool b = !(fabsf(x) < INFINITY);
+                if (b) va[u][dt][j] = (__bf16)0.f;
+                bad |= b;
+              }
+              const unsigned long long who = __builtin_amdgcn_ballot_w64(bad);
+              const int k = 16 * u + (j >> 2) * 8 + (j & 3);
+              odd |= ((uint32_t)who != 0) << k | ((who >> 32) != 0) << (k + 4);
+            }
+        }
+      }
+      bf16x8 pb[2];
+      float rs = 0.f;
+      bool bad = i == 0;  // the first tile sets the reference
+      if (!bad) {
+        rs = exps(s, mcv, pb);
+        bad = !(rs <= kSumLimit);  // NaN included
+      }
+      if (__builtin_amdgcn_ballot_w64(bad) != 0) rs = fixup(s, pb);
+      l += rs;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt)
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[u][dt], pb[u], o[dt], 0, 0, 0);
+      while (odd) {  // (wave-uniform)
+        const int k = __builtin_ctz(odd);
+        odd &= odd - 1;
+        float pk = 0.f;  // this lane's weight of key k, if it is one of its 16
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pk = (e >> 2) * 8 + (e & 3) == (k & ~4) ? (float)pb[e >> 3][e & 7] : pk;
+        pk = __shfl(pk, r32 + 32 * (k >> 2 & 1), 64);
+        if (kb + k < limit && (pages >> (k >> 3) & 1)) {
+#pragma unroll
+          for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float x = bf16_to_f32(vl[k * VP + 32 * dt + (e >> 2) * 8 + hf * 4 + (e & 3)]);
+              if (!(fabsf(x) < INFINITY)) o[dt][e] = fmaf(pk, x, o[dt][e]);
+            }
+        }
+      }
+    }
+    if constexpr (NB > 1) {
+      lstore(i + 1);
+      __syncthreads();
+    }
+  }
+
+  // every wave scales its O to the key parts' common maximum and writes it to
+  // its own share of the LDS as [row][d]
+  if (hf == 0) {
+    red_m[wave][r32] = mcv;
+    red_l[wave][r32] = l;
+  }
+  __syncthreads();
+  float *const ot = (float *)smem;
+  float M = red_m[hw][r32];
+#pragma unroll
+  for (int v = 1; v < KW; ++v) M = fmaxf(M, red_m[v * HW + hw][r32]);
+  const float f = mcv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mcv - M);
+  {
+    float *dst = ot + wave * OT + r32 * OP + 4 * hf;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int gi = 0; gi < 4; ++gi)
+        *(float4 *)(dst + 32 * dt + 8 * gi) =
+            make_float4(o[dt][4 * gi] * f, o[dt][4 * gi + 1] * f, o[dt][4 * gi + 2] * f, o[dt][4 * gi + 3] * f);
+  }
+  __syncthreads();
+  constexpr int NV = R / W;  // = 64 elements over the row's threads
+  static_assert(NV * (64 * W / R) == HD, "a row's threads cover it");
+  finish_piece<bf16_t, R, 64 * W>(p, w, &last_in, [&](int row, int d0, float (&acc)[NV]) __attribute__((always_inline)) {
+    const int hu = row / 32, r = row % 32;
+    float Mr = red_m[hu][r];
+#pragma unroll
+    for (int v = 1; v < KW; ++v) Mr = fmaxf(Mr, red_m[v * HW + hu][r]);
+    const float Mu = Mr == -INFINITY ? 0.f : Mr;
+    float L = 0.f;
+#pragma unroll
+    for (int v = 0; v < KW; ++v) L += red_l[v * HW + hu][r] * __builtin_amdgcn_exp2f(red_m[v * HW + hu][r] - Mu);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int v = 0; v < KW; ++v)
+#pragma unroll
+      for (int i = 0; i < NV; i += 4) {
+        const float4 x = *(const float4 *)(ot + (v * HW + hu) * OT + r * OP + d0 + i);
+        acc[i] += x.x; acc[i + 1] += x.y; acc[i + 2] += x.z; acc[i + 3] += x.w;
+      }
+    return make_float2(Mr, L);
+  });
+}
+
+// fp32, v_mfma_f32_32x32x2f32: matrix-core time is all that counts.  32 rows a
+// unit, its tiles dealt to KW waves, no barrier before the merge: a wave
+// stages its own K tile in LDS one tile ahead (rows of 272 B) and reads V
+// straight from the pages as the second product's operand (two adjacent d of
+// one key row a lane), requested before the scores' products, which cover it.
+template <int KW>
+__global__ __launch_bounds__(64 * KW, 2) void paged_prefill_f32_kernel(PrefillParams p) {
+  constexpr int R = 32, KP = HD + 4;  // K row and O row pitch, floats
+  constexpr int TILE = 32 * KP;
+  __shared__ __attribute__((aligned(16))) float smem[KW * TILE];
+  __shared__ float red_m[KW][32], red_l[KW][32];
+  __shared__ int last_in;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int kw = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, hf = lane >> 5;
+  Piece w;
+  if (!find_piece<R>(p, w)) return;
+  const Paged &c = p.a.c;
+  const PieceKeys keys = piece_keys<R>(p, w);
+  const float cl = p.a.cl;
+  float *const kl = smem + kw * TILE;
+  const int fr = w.unit * R + r32, tok = fr / p.a.group, head = fr - tok * p.a.group;
+  const bool there = tok < w.rows;
+  const int limit = there ? key_limit(p, w, tok) : 0;
+  const int all_see = wave_min(there ? limit : 0x7fffffff);
+
+  const int slot_mask = (1 << c.shift) - 1;
+  const int64_t page_bytes = c.page_stride * 4;
+  const uint32_t row_bytes = (uint32_t)c.row_stride * 4;
+  const uint32_t koff = (lane >> 4) * row_bytes + (lane & 15) * 16;  // 4 rows of 256 bytes a load
+  const uint32_t voff = 4 * hf * row_bytes + r32 * 8;
+  const char *const Kg = (const char *)((const float *)c.k + w.g * c.head_stride);
+  const char *const Vg = (const char *)((const float *)c.v + w.g * c.head_stride);
+  u32x4 kr[8];
+  int ids[4];
+  int64_t at[4], vat[4];  // byte offsets of rows 8r .. of the tile to load next, of this tile
+  int pages = 0, pages_next = 0;
+  auto load_ids = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) ids[r] = keys.entry(32 * t + 8 * r);
+  };
+  auto gload_k = [&](int t) __attribute__((always_inline)) {
+    pages_next = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const bool ok = (unsigned)ids[r] < (unsigned)c.n_pages;
+      pages_next |= ok << r;
+      at[r] = (ok ? ids[r] : 0) * page_bytes + (int64_t)((uint64_t)(uint32_t)((32 * t + 8 * r) & slot_mask) * row_bytes);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) kr[2 * r + j] = *(const u32x4 *)(Kg + at[r] + (int64_t)j * 4 * row_bytes + koff);
+    }
+  };
+  float qreg[32];  // k slot (hf, t) of the score product is d = 32 hf + t
+  {
+    const float *const qp = (const float *)p.a.q + (int64_t)(w.row0 + (there ? tok : 0)) * p.a.q_rs +
+                            (w.g * p.a.group + (there ? head : 0)) * HD + 32 * hf;
+#pragma unroll
+    for (int t = 0; t < 32; t += 4) {
+      const float4 x = *(const float4 *)(qp + t);
+      qreg[t] = x.x; qreg[t + 1] = x.y; qreg[t + 2] = x.z; qreg[t + 3] = x.w;
+    }
+  }
+  float mc = -INFINITY, l = 0.f;
+  f32x16 o[2] = {f32x16{}, f32x16{}};  // o[j] row i is d = 2i + j
+  int t = keys.t0 + kw;
+  if (t < keys.t1) {
+    load_ids(t);
+    gload_k(t);
+    load_ids(t + KW);
+  }
+  for (; t < keys.t1; t += KW) {
+    pages = pages_next;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) vat[r] = at[r];
+    // the wave's own tile: its LDS instructions execute in order
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) *(u32x4 *)(kl + (4 * j + (lane >> 4)) * KP + (lane & 15) * 4) = kr[j];
+    __builtin_amdgcn_wave_barrier();
+    // this tile's V: key slot (hf, i) of the second product is key 8(i/4) + 4hf + i%4
+    float2 vr[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      vr[i] = *(const float2 *)(Vg + vat[i >> 2] + (int64_t)(i & 3) * row_bytes + voff);
+    gload_k(t + KW);  // past the range: the last key's page again, not used
+    load_ids(t + 2 * KW);
+    f32x16 s = f32x16{};
+    const float *krow = kl + r32 * KP + 32 * hf;
+#pragma unroll
+    for (int u = 0; u < 32; u += 4) {
+      const float4 a = *(const float4 *)(krow + u);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, qreg[u], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, qreg[u + 1], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, qreg[u + 2], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, qreg[u + 3], s, 0, 0, 0);
+    }
+    const int kb = 32 * t;
+    uint32_t odd = 0;  // as in the bf16 kernel
+    if (kb + 32 > all_see || pages != 15) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int k = (i >> 2) * 8 + hf * 4 + (i & 3);
+        const bool page = pages >> (i >> 2) & 1;
+        if (kb + k >= limit || !page) s[i] = -INFINITY;
+        if (kb + k >= keys.end || !page) vr[i] = make_float2(0.f, 0.f);  // no key: whatever lies there
+        const bool bx = !(fabsf(vr[i].x) < INFINITY), by = !(fabsf(vr[i].y) < INFINITY);
+        const unsigned long long who = __builtin_amdgcn_ballot_w64(bx || by);
+        if (who) {
+          if (bx) vr[i].x = 0.f;
+          if (by) vr[i].y = 0.f;
+          const int k0 = (i >> 2) * 8 + (i & 3);
+          odd |= ((uint32_t)who != 0) << k0 | ((who >> 32) != 0) << (k0 + 4);
+        }
+      }
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float m_new = fmaxf(mc, mx * cl);
+    const float ref = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(mc - ref);
+    float rs = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], cl, -ref));
+      rs += s[i];
+    }
+    l = l * alpha + rs;  // per half-wave; the halves are summed at the end
+    mc = m_new;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[j][i] *= alpha;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[i].x, s[i], o[0], 0, 0, 0);
+      o[1] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[i].y, s[i], o[1], 0, 0, 0);
+    }
+    while (odd) {  // (wave-uniform)
+      const int k = __builtin_ctz(odd);
+      odd &= odd - 1;
+      float pk = 0.f;
+      int64_t a = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) pk = (i >> 2) * 8 + (i & 3) == (k & ~4) ? s[i] : pk;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) a = r == k >> 3 ? vat[r] : a;
+      pk = __shfl(pk, r32 + 32 * (k >> 2 & 1), 64);
+      if (kb + k < limit && (pages >> (k >> 3) & 1)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 x = *(const float2 *)(Vg + a + (int64_t)(k & 7) * row_bytes + 8 * ((i >> 2) * 8 + hf * 4 + (i & 3)));
+          if (!(fabsf(x.x) < INFINITY)) o[0][i] = fmaf(pk, x.x, o[0][i]);
+          if (!(fabsf(x.y) < INFINITY)) o[1][i] = fmaf(pk, x.y, o[1][i]);
+        }
+      }
+    }
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if (hf == 0) {
+    red_m[kw][r32] = mc;
+    red_l[kw][r32] = l;
+  }
+  __syncthreads();
+  float M = red_m[0][r32];
+#pragma unroll
+  for (int v = 1; v < KW; ++v) M = fmaxf(M, red_m[v][r32]);
+  const float f = mc == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - M);
+#pragma unroll
+  for (int gi = 0; gi < 4; ++gi) {
+    float *dst = kl + r32 * KP + 2 * (8 * gi + 4 * hf);
+    *(float4 *)dst = make_float4(o[0][4 * gi] * f, o[1][4 * gi] * f, o[0][4 * gi + 1] * f, o[1][4 * gi + 1] * f);
+    *(float4 *)(dst + 4) =
+        make_float4(o[0][4 * gi + 2] * f, o[1][4 * gi + 2] * f, o[0][4 * gi + 3] * f, o[1][4 * gi + 3] * f);
+  }
+  __syncthreads();
+  constexpr int NV = HD / (2 * KW);
+  finish_piece<float, R, 64 * KW>(p, w, &last_in, [&](int row, int d0, float (&acc)[NV]) __attribute__((always_inline)) {
+    float Mr = red_m[0][row];
+#pragma unroll
+    for (int v = 1; v < KW; ++v) Mr = fmaxf(Mr, red_m[v][row]);
+    const float Mu = Mr == -INFINITY ? 0.f : Mr;
+    float L = 0.f;
+#pragma unroll
+    for (int v = 0; v < KW; ++v) L += red_l[v][row] * __builtin_amdgcn_exp2f(red_m[v][row] - Mu);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; i += 4)
+#pragma unroll
+      for (int v = 0; v < KW; ++v) {
+        const float4 x = *(const float4 *)(smem + v * TILE + row * KP + d0 + i);
+        acc[i] += x.x; acc[i + 1] += x.y; acc[i + 2] += x.z; acc[i + 3] += x.w;
+      }
+    return make_float2(Mr, L);
+  });
+}
+
 // One wave per (row, query head), lane = element of the head: every key's
 // dot product is a wave sum.
 template <typename T>
@@ -824,10 +1553,12 @@ int check_starts(const std::string &op, const int32_t *row_starts, int n_rows, i
   return BN_OK;
 }
 
-int check_heads(const std::string &op, int n_heads, int n_kv_heads) {
+int check_heads(const std::string &op, int n_heads, int n_kv_heads, int n_rows) {
   if (n_heads <= 0 || n_heads % n_kv_heads != 0)
     return fail(BN_ERR_SHAPE, op + ": num_heads must be a positive multiple of num_kv_heads");
   if (n_heads > 65535) return fail(BN_ERR_UNSUPPORTED, op + ": more than 65535 heads");
+  if ((int64_t)n_rows * n_heads > (1 << 30))
+    return fail(BN_ERR_UNSUPPORTED, op + ": n_rows * num_heads must be at most 2^30");
   return BN_OK;
 }
 
@@ -928,6 +1659,69 @@ int launch_decode(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
   return BN_OK;
 }
 
+// Which prefill kernel: by the units of 128 rows (32 in fp32) that the call has
+// at most.  Few of them: the keys of a unit are split over more waves.
+struct PrefillPlan {
+  int hw, kw;
+  int64_t groups, slots;   // workgroups of the launch, records
+  size_t records, words;   // bytes
+};
+PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv_heads, int cap, bool records) {
+  PrefillPlan d;
+  const int64_t rows = (int64_t)n_rows * (n_heads / n_kv_heads);  // of a KV head
+  const int64_t u128 = (rows / 128 + 1) * n_kv_heads, u32 = (rows / 32 + 1) * n_kv_heads;
+  if (dtype == BN_F32) {
+    d.hw = 1;
+    d.kw = u32 <= 2048 ? 4 : 2;
+  } else if (u128 < 256) {
+    d.hw = 1;
+    d.kw = u32 <= 256 ? 8 : 4;
+  } else {
+    d.hw = 4;
+    d.kw = u128 <= 768 ? 2 : 1;
+  }
+  const int R = 32 * d.hw;
+  const int64_t units = std::min((rows + R - 1) / R + n_seq, rows);  // of a KV head, over the sequences
+  // a sequence of U units, the longest of s tiles, counts U * s / 2 tiles at least and is cut
+  // into U * floor(s / share) pieces: at most 2 * total / share in all, where total is
+  // below (share + 1) * kPartsAll / n_kv_heads and share at least kPartMin
+  const int64_t most_parts = std::max(1, (cap / 32 + 1) / kPartMin);
+  const int64_t cut =
+      most_parts > 1 ? std::min<int64_t>(units * most_parts, (2 * kPartsAll + kPartsAll / 8) / n_kv_heads + 2) : 0;
+  const int64_t pieces = units + cut;
+  const int per = n_kv_heads <= 8 && 8 % n_kv_heads == 0 ? 8 / n_kv_heads : 1;
+  d.groups = (pieces + per - 1) / per * per * n_kv_heads;
+  d.slots = (records ? pieces : cut) * n_kv_heads;
+  d.records = (size_t)d.slots * R * kRec * sizeof(float);
+  d.words = (size_t)d.slots * 16 * d.hw;  // (16 are used; a call of fewer rows, whose records are smaller, needs no more)
+  return d;
+}
+
+int launch_prefill(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
+  const PrefillPlan d = plan_prefill(dtype, a.c.batch, a.n_rows, a.n_heads, a.c.n_kv_heads, a.c.cap, false);
+  PrefillParams p;
+  p.a = a;
+  p.ws = (float *)ws;
+  p.arrive_end = (unsigned long long *)((char *)ws + d.records + d.words);
+  p.tag = next_tag();
+  p.slots = (int)d.slots;
+  p.prefix = 0;
+  const dim3 grid((unsigned)d.groups);
+  if (dtype == BN_F32) {
+    if (d.kw == 4) hipLaunchKernelGGL(paged_prefill_f32_kernel<4>, grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL(paged_prefill_f32_kernel<2>, grid, dim3(128), 0, s, p);
+  } else if (d.hw == 4) {
+    if (d.kw == 2) hipLaunchKernelGGL((paged_prefill_bf16_kernel<4, 2, 4>), grid, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((paged_prefill_bf16_kernel<4, 1, 4>), grid, dim3(256), 0, s, p);
+  } else if (d.kw == 8) {
+    hipLaunchKernelGGL((paged_prefill_bf16_kernel<1, 8, 2>), grid, dim3(512), 0, s, p);
+  } else {
+    hipLaunchKernelGGL((paged_prefill_bf16_kernel<1, 4, 3>), grid, dim3(256), 0, s, p);
+  }
+  BN_LAUNCH_CHECK();
+  return BN_OK;
+}
+
 int attention(const char *name, const bn_paged_kv *kv, const void *q, void *o, const int32_t *starts,
               int n_rows, int n_heads, int64_t q_rs, int64_t o_rs, float scale,
               const int32_t *prefix_pages, int prefix_len, void *workspace, size_t workspace_bytes,
@@ -935,7 +1729,7 @@ int attention(const char *name, const bn_paged_kv *kv, const void *q, void *o, c
   const std::string op = name;
   AttnParams p;
   int st = check_cache(op, kv, &p.c);
-  if (st || (st = check_heads(op, n_heads, kv->n_kv_heads)) ||
+  if (st || (st = check_heads(op, n_heads, kv->n_kv_heads, n_rows)) ||
       (st = check_starts(op, starts, n_rows, kv->batch)))
     return st;
   if (!(scale > 0.f) || !std::isfinite(scale))
@@ -964,7 +1758,9 @@ int attention(const char *name, const bn_paged_kv *kv, const void *q, void *o, c
   p.prefix_pages = prefix_pages; p.prefix_len = prefix_len;
   Workspace ws;
   if ((st = ws.take(workspace, need, stream))) return st;
-  if (!starts && prefix_len == 0) return ws.release(launch_decode(p, kv->dtype, ws.p, as_stream(stream)));
+  if (prefix_len == 0)
+    return ws.release(starts ? launch_prefill(p, kv->dtype, ws.p, as_stream(stream))
+                             : launch_decode(p, kv->dtype, ws.p, as_stream(stream)));
   const dim3 grid(n_rows, n_heads);
   if (kv->dtype == BN_BF16)
     hipLaunchKernelGGL(paged_rows_kernel<bf16_t>, grid, dim3(64), 0, as_stream(stream), p);
@@ -990,7 +1786,7 @@ int bn_paged_append(const bn_paged_kv *cache, const void *k, const void *v, cons
   int st = check_cache(op, cache, &p.c);
   if (st || (st = check_starts(op, row_starts, n_rows, cache->batch))) return st;
   if (!q != !q_out) return fail(BN_ERR_INVALID_ARG, op + ": q and q_out must be given together");
-  if (q && (st = check_heads(op, n_heads, cache->n_kv_heads))) return st;
+  if (q && (st = check_heads(op, n_heads, cache->n_kv_heads, n_rows))) return st;
   if (!(theta >= 0.f) || !std::isfinite(theta))
     return fail(BN_ERR_INVALID_ARG, op + ": theta must be positive and finite, or 0 for no rotation");
   if (n_rows == 0 || cache->batch == 0) return BN_OK;
@@ -1026,10 +1822,11 @@ int bn_paged_append(const bn_paged_kv *cache, const void *k, const void *v, cons
 size_t bn_paged_workspace_size(const bn_paged_kv *cache, int n_heads, int n_rows, int prefix_len) {
   Paged c;
   if (n_rows <= 0 || prefix_len < 0 || !cache || check_cache("", cache, &c) || cache->batch == 0 ||
-      check_heads("", n_heads, cache->n_kv_heads))
+      check_heads("", n_heads, cache->n_kv_heads, n_rows))
     return 0;
   const DecodePlan d = plan_decode(cache->batch, n_heads, cache->n_kv_heads);
-  return d.records + d.words;
+  const PrefillPlan f = plan_prefill(cache->dtype, cache->batch, n_rows, n_heads, cache->n_kv_heads, c.cap, false);
+  return std::max(d.records + d.words, f.records + f.words);
 }
 
 int bn_paged_decode(const bn_paged_kv *cache, const void *q, void *o, int n_heads, int64_t q_row_stride,

@@ -150,3 +150,42 @@ def rotate64(x, pos, theta):
     y[:, 0::2] = x[:, 0::2] * c - x[:, 1::2] * s
     y[:, 1::2] = x[:, 0::2] * s + x[:, 1::2] * c
     return y
+
+
+def attention64_large(case, q, rows, scale=0.125, prefix=None, prefix_len=0):
+    """attention64 for large cases: (o, tol) as float64 tensors, computed on q's device by products
+    in 64 bits per sequence and head (no padding rows)."""
+    n_rows, H, _ = q.shape
+    G = H // case.Hkv
+    o = torch.zeros((n_rows, H, D), dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(o)
+    eps = torch.finfo(TD[case.dtype]).eps / 2
+    kd, vd = case.kd, case.vd
+    at = 0
+    for b, n in enumerate(rows):
+        length = min(max(case.lens[b], 0), case.max_pages * case.page)
+        pages = torch.from_numpy(case.table[b, :-(-length // case.page)].astype(np.int64)).to(q.device)
+        if prefix is not None:
+            pages[:-(-prefix_len // case.page)] = torch.from_numpy(prefix.astype(np.int64)).to(q.device)
+            if prefix_len % case.page and length > prefix_len:
+                raise ValueError("prefix must end with a page")
+        j = torch.arange(length, device=q.device)
+        hidden = j[None, :] > (length - n + torch.arange(n, device=q.device))[:, None]
+        gone = (pages < 0) | (pages >= case.n_pages)
+        hidden |= gone[j // case.page][None, :]
+        pages = pages.masked_fill(gone, 0)
+        for g in range(case.Hkv):
+            k, v = (x[pages, g].reshape(-1, D)[:length].double() for x in (kd, vd))
+            k, v = k.masked_fill(gone[j // case.page][:, None], 0), v.masked_fill(gone[j // case.page][:, None], 0)
+            for h in range(g * G, (g + 1) * G):
+                x = q[at:at + n, h].double()
+                s = (x @ k.T).mul_(scale).masked_fill_(hidden, -np.inf)
+                p = torch.softmax(s, 1).nan_to_num_(0.0)
+                o[at:at + n, h] = p @ v
+                A = p @ v.abs()
+                S = scale * (x.abs() @ k.abs().T).max(1, keepdim=True).values
+                rel = 2 * (2 * (72 * 2.0 ** -24 * S) + 2.0 ** -22 + length * 2.0 ** -24) + \
+                    (2 * eps if case.dtype == "bf16" else 0.0)
+                tol[at:at + n, h] = eps * o[at:at + n, h].abs() + rel * A
+        at += n
+    return o, tol

@@ -8,7 +8,7 @@ import torch
 
 import bnhip as B
 from gpu_util import require_gpu
-from paged_util import D, TD, Case, attention64, check, rotate64, rows_of, starts_of
+from paged_util import D, TD, Case, attention64, attention64_large, check, rotate64, rows_of, starts_of
 
 pytestmark = pytest.mark.gpu
 
@@ -302,6 +302,55 @@ def test_prefill(case):
         o2 = torch.full_like(q, 7.0).cuda()
         B.paged_prefill(qd, cache, st, o=o2, scale=0.125, workspace=ws)
         assert torch.equal(bits(o2), bits(o)), "a second call differs"
+
+
+# many rows, and rows behind long caches: each kernel that the host can pick, whole units and cut ones
+LARGE = [
+    ("bf16", [700, 433, 400], [700, 33, 400], 4, 32, 16),
+    ("bf16", [1500, 40, 2100, 900], [1500, 33, 1100, 767], 4, 32, 32),
+    ("bf16", [2900, 3300], [2500, 1001], 4, 20, 16),
+    ("bf16", [9000, 3000, 70, 20000], [5, 64, 1, 3], 2, 16, 64),
+    ("bf16", [16500, 6000], [300, 290], 4, 32, 64),
+    ("bf16", [700] * 70 + [3], [10] * 70 + [2], 2, 6, 16),
+    ("bf16", [30000], [4], 1, 1, 16),
+    ("f32", [700, 433, 400], [700, 33, 400], 2, 16, 16),
+    ("f32", [9000, 3000, 70], [5, 64, 1], 2, 6, 64),
+    ("f32", [2000, 1100], [1700, 1100], 4, 16, 16),
+    ("f32", [300] * 80, [9] * 80, 3, 3, 8),
+]
+
+
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: f"{c[0]}-{len(c[1])}x{max(c[2])}of{max(c[1])}-{c[3]}-{c[4]}-p{c[5]}")
+def test_prefill_large(case):
+    dtype, lens, rows, Hkv, H, page = case
+    print("prefill large", case, flush=True)
+    c = Case(dtype, lens, Hkv, page, True, seed=H, drop=[(0, 3)], nan=False)
+    q = rows_of(dtype, sum(rows), H, 11).cuda()
+    cache = c.cuda(B)
+    st = torch.from_numpy(starts_of(rows)).cuda()
+    ws = B.paged_workspace(cache, H, sum(rows))
+    ws.fill_(255)
+    got = [B.paged_prefill(q, cache, st, scale=0.125, workspace=w) for w in (ws, ws, None)]
+    ref, tol = attention64_large(c, q, rows)
+    over = (got[0].double() - ref).abs() - tol
+    assert (over <= 0).all(), f"{int((over > 0).sum())} past the tolerance, by {float(over.max()):.2e}"
+    assert torch.equal(bits(got[0]), bits(got[1])) and torch.equal(bits(got[0]), bits(got[2]))
+
+
+def test_prefill_starts_that_decrease_stay_inside():
+    """row_starts out of order are the caller's mistake: the rows' values are not defined, but
+    nothing outside o is written and the call returns."""
+    n = 600
+    c = Case("bf16", [4000] * 40, 2, 16, True, seed=1, nan=False, spare=0)
+    q = rows_of("bf16", n, 16, 2).cuda()
+    cache = c.cuda(B)
+    st = torch.tensor([0, n] * 20 + [0], dtype=torch.int32).cuda()
+    need = B.paged_workspace(cache, 16, n).numel()
+    ws = torch.full((need + 4096,), 77, dtype=torch.uint8, device="cuda")
+    out = torch.full((n + 64, 16, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    B.paged_prefill(q, cache, st, o=out[32:n + 32], scale=0.125, workspace=ws[:need])
+    torch.cuda.synchronize()
+    assert (out[:32] == 7.0).all() and (out[n + 32:] == 7.0).all() and (ws[need:] == 77).all()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
