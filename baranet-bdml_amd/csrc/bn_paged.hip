@@ -219,6 +219,7 @@ struct DecodeParams {
   unsigned long long *arrive_end;   // two arrival words per (sequence, column) below it
   unsigned long long tag;           // the launch's 48-bit tag
   int bins, hblocks, columns, k0;   // k0: keys below it are not this kernel's
+  float *parts;                     // not null: [batch][n_heads][kRec], instead of the output
 };
 
 // Counts the caller in as one of n on a pair of 64-bit words and says whether
@@ -277,22 +278,26 @@ __device__ __forceinline__ float2 get2(const float *p) {
 // or v_mfma_f32_16x16x4_f32; a lane holds its 8 (4) keys' scores of one head,
 // which are the second product's operand as they stand.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
+struct DecodeLds {
+  T k[4][DecTile<T>::TK * DecTile<T>::P];
+  T v[4][DecTile<T>::TK * DecTile<T>::P];
+  float hold[kHoldRows * kHold];
+  int last_in[2];
+};
+template <typename T>
+__device__ __forceinline__ void decode_body(const DecodeParams &p, DecodeLds<T> &lds, int block) {
   using Ti = DecTile<T>;
   constexpr bool BF = sizeof(T) == 2;
   constexpr int TK = Ti::TK, LPR = Ti::LPR, RPI = 64 / LPR, VEC = HD / LPR, P = Ti::P;
   constexpr int NS = TK / 16;  // 16-key score tiles
   constexpr int NQ = BF ? 2 : 4;
-  __shared__ __attribute__((aligned(16))) T KT[4][TK * P];
-  __shared__ __attribute__((aligned(16))) T VT[4][TK * P];
-  __shared__ __attribute__((aligned(16))) float hold[kHoldRows * kHold];
-  __shared__ int last_in[2];
+  float *const hold = lds.hold;
 
   const Paged &c = p.a.c;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, grp = lane >> 4;
-  const int bin = blockIdx.x / p.columns, col = blockIdx.x - bin * p.columns;
+  const int bin = block / p.columns, col = block - bin * p.columns;
   const int g = col / p.hblocks, hb = col - g * p.hblocks;
   const int rows = min(kMaxRows, p.a.group - kMaxRows * hb), head0 = g * p.a.group + kMaxRows * hb;
   const int room = kHoldRows / (4 * rows);  // sequences that LDS has room for
@@ -409,7 +414,7 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
       y.v[r] = __builtin_nontemporal_load((const u32x4 *)(Vg + at[r] + off));
     }
   };
-  T *const kt = KT[wave], *const vt = VT[wave];
+  T *const kt = lds.k[wave], *const vt = lds.v[wave];
   auto store_rows = [&](Rows &y, bool masked) __attribute__((always_inline)) {
     if (masked) {  // no key: zeros, whatever lies there (0 times an infinite value is none)
 #pragma unroll
@@ -524,7 +529,13 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
   };
 
   // ---- results: two elements of a head's row a thread
-  auto write2 = [&](int b, int h, int d, float x, float y, float sum) __attribute__((always_inline)) {
+  auto write2 = [&](int b, int h, int d, float x, float y, float ref, float sum) __attribute__((always_inline)) {
+    if (p.parts) {  // one part of the row: left for the launch that adds them
+      float *const r = p.parts + ((int64_t)b * p.a.n_heads + head0 + h) * kRec;
+      *(float2 *)(r + d) = make_float2(x, y);
+      if (d == 0) *(float2 *)(r + HD) = make_float2(ref, sum);
+      return;
+    }
     const float inv = sum > 0.f ? 1.0f / sum : 0.f;
     T *const op = (T *)p.a.o + b * p.a.o_rs + (head0 + h) * HD + d;
     if constexpr (BF)
@@ -664,7 +675,7 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
             A1 = fmaf(a.y, f, A1);
           }
           if (pieces == 1) {
-            write2(seg.b, h, d, A0, A1, L);
+            write2(seg.b, h, d, A0, A1, M, L);
           } else {
             float *const to = record(bin, bin0, h);
             put2(to + d, A0, A1);
@@ -684,13 +695,13 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
       __syncthreads();
       if (tid < 2) {
         const Cut u = tid ? cuts[1] : cuts[0];
-        last_in[tid] =
+        lds.last_in[tid] =
             u.pieces && arrive_last(p.arrive_end - 2 * ((int64_t)u.b * p.columns + col + 1), u.pieces, p.tag);
       }
       __syncthreads();
 #pragma unroll 1
       for (int side = 0; side < 2; ++side) {
-        if (!last_in[side]) continue;
+        if (!lds.last_in[side]) continue;
         const Cut u = side ? cuts[1] : cuts[0];
         for (int k = tid; k < rows * (HD / 2); k += 256) {
           const int h = k / (HD / 2), d = 2 * (k % (HD / 2));
@@ -720,7 +731,7 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
             }
             M = mx;
           }
-          write2(u.b, h, d, A0, A1, L);
+          write2(u.b, h, d, A0, A1, M, L);
         }
       }
     }
@@ -728,7 +739,12 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
   // sequences without a key
   for (int b = bin; b < c.batch; b += p.bins)
     if (tiles_of(clamp_len(c.lens[b])) == 0)
-      for (int k = tid; k < rows * (HD / 2); k += 256) write2(b, k / (HD / 2), 2 * (k % (HD / 2)), 0.f, 0.f, 0.f);
+      for (int k = tid; k < rows * (HD / 2); k += 256) write2(b, k / (HD / 2), 2 * (k % (HD / 2)), 0.f, 0.f, -INFINITY, 0.f);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
+  __shared__ __attribute__((aligned(16))) DecodeLds<T> lds;
+  decode_body<T>(p, lds, blockIdx.x);
 }
 
 // ------------------------------------------------- prefill, over pages
@@ -743,8 +759,10 @@ struct PrefillParams {
   float *ws;                       // records: [slot][R][kRec]
   unsigned long long *arrive_end;  // two arrival words per slot below it
   unsigned long long tag;
-  int slots;   // records that the workspace holds
-  int prefix;  // the rows are the batch's, the keys prefix_pages' (every piece leaves a record)
+  int slots;  // records that the workspace holds
+  // not 0: the rows are the batch's, the keys those of prefix_pages, and every unit's are
+  // cut into so many parts, whose records are left for the launch that adds them
+  int prefix_parts;
 };
 struct Piece {
   int b, g, unit, part, parts;  // part of parts of the unit's keys
@@ -763,17 +781,27 @@ constexpr int kPartsAll = 1024;   // a part is at least this share of all the ca
 // KV head's units go to 8 / n_kv_heads of them, whose L2s then hold its keys.
 // Every wave finds its piece itself from the lengths.  False: none.
 template <int R>
-__device__ __forceinline__ bool find_piece(const PrefillParams &p, Piece &w) {
+__device__ __forceinline__ bool find_piece(const PrefillParams &p, int block, Piece &w) {
   const Paged &c = p.a.c;
   const int lane = threadIdx.x & 63, hkv = c.n_kv_heads, G = p.a.group;
   int idx;
   if (hkv <= 8 && (8 % hkv) == 0) {
-    const int x = blockIdx.x & 7;
+    const int x = block & 7;
     w.g = x % hkv;
-    idx = (blockIdx.x >> 3) * (8 / hkv) + x / hkv;
+    idx = (block >> 3) * (8 / hkv) + x / hkv;
   } else {
-    w.g = blockIdx.x % hkv;
-    idx = blockIdx.x / hkv;
+    w.g = block % hkv;
+    idx = block / hkv;
+  }
+  if (p.prefix_parts) {
+    w.b = w.row0 = 0;
+    w.rows = c.batch;
+    w.last = p.a.prefix_len;
+    w.parts = p.prefix_parts;
+    w.unit = idx / w.parts;
+    w.part = idx - w.unit * w.parts;
+    w.slot = w.unit * w.parts * hkv + w.g;
+    return w.unit * R < w.rows * G;
   }
   struct Seq {
     int row0, rows, last, units, steps;  // steps: tiles of its longest unit
@@ -781,27 +809,19 @@ __device__ __forceinline__ bool find_piece(const PrefillParams &p, Piece &w) {
   };
   auto seq = [&](int b) __attribute__((always_inline)) {
     Seq s;
-    if (p.prefix) {
-      s.row0 = 0;
-      s.rows = c.batch;
-      s.last = p.a.prefix_len;
-    } else {
-      const int bb = min(b, c.batch - 1);
-      const int s0 = p.a.starts ? p.a.starts[bb] : bb, s1 = p.a.starts ? p.a.starts[bb + 1] : bb + 1;
-      s.row0 = min(max(s0, 0), p.a.n_rows);
-      s.rows = min(max(s1, s.row0), p.a.n_rows) - s.row0;
-      s.last = max(c.lens[bb], 0) - s1 + s.row0 + s.rows;  // (s1 is past the tensors' rows: not its last)
-      if (b >= c.batch) s.rows = 0;
-    }
+    const int bb = min(b, c.batch - 1), s0 = p.a.starts[bb], s1 = p.a.starts[bb + 1];
+    s.row0 = min(max(s0, 0), p.a.n_rows);
+    s.rows = min(max(s1, s.row0), p.a.n_rows) - s.row0;
+    s.last = max(c.lens[bb], 0) - s1 + s.row0 + s.rows;  // (s1 is past the tensors' rows: not its last)
+    if (b >= c.batch) s.rows = 0;
     s.units = (s.rows * G + R - 1) / R;
-    const int cap = p.prefix ? p.a.prefix_len : c.cap;
-    auto tiles = [&](int n) { return (min(max(n, 0), cap) + 31) >> 5; };
+    auto tiles = [&](int n) { return (min(max(n, 0), c.cap) + 31) >> 5; };
     s.steps = tiles(s.last);
-    const int first = p.prefix ? s.steps : tiles(s.last - s.rows + min(s.rows, (R + G - 1) / G));
+    const int first = tiles(s.last - s.rows + min(s.rows, (R + G - 1) / G));
     s.weight = (float)s.units * (0.5f * (float)(s.steps + first) + 1.f);
     return s;
   };
-  const int n = p.prefix ? 1 : c.batch, per = (n + 63) >> 6;
+  const int n = c.batch, per = (n + 63) >> 6;
   Seq mine = seq(lane * per);
   float total = lane * per < n ? mine.weight : 0.f;
   for (int i = 1; i < per; ++i) total += lane * per + i < n ? seq(lane * per + i).weight : 0.f;
@@ -812,7 +832,7 @@ __device__ __forceinline__ bool find_piece(const PrefillParams &p, Piece &w) {
   auto count = [&](const Seq &s, bool in, int &all, int &cut) __attribute__((always_inline)) {
     const int parts = parts_of(s), k = in ? s.units * parts : 0;
     all += k;
-    cut += parts > 1 || p.prefix ? k : 0;
+    cut += parts > 1 ? k : 0;
   };
   int all = 0, cut = 0;
   count(mine, lane * per < n, all, cut);
@@ -868,7 +888,7 @@ template <int R>
 __device__ __forceinline__ PieceKeys piece_keys(const PrefillParams &p, const Piece &w) {
   const Paged &c = p.a.c;
   PieceKeys k;
-  if (p.prefix) {
+  if (p.prefix_parts) {
     k.end = p.a.prefix_len;
     k.table = (const __attribute__((address_space(4))) int32_t *)p.a.prefix_pages;
   } else {
@@ -885,8 +905,8 @@ __device__ __forceinline__ PieceKeys piece_keys(const PrefillParams &p, const Pi
 }
 // keys that token t of the piece's sequence sees
 __device__ __forceinline__ int key_limit(const PrefillParams &p, const Piece &w, int t) {
-  return p.prefix ? min(max(p.a.c.lens[t], 0), p.a.prefix_len)
-                  : min(max(w.last - w.rows + t + 1, 0), p.a.c.cap);
+  return p.prefix_parts ? min(max(p.a.c.lens[t], 0), p.a.prefix_len)
+                        : min(max(w.last - w.rows + t + 1, 0), p.a.c.cap);
 }
 __device__ __forceinline__ int wave_min(int x) {
 #pragma unroll
@@ -922,7 +942,7 @@ __device__ __forceinline__ void finish_piece(const PrefillParams &p, const Piece
       }
     }
   };
-  if (w.parts == 1) return write();
+  if (w.parts == 1 && !p.prefix_parts) return write();
   const int64_t step = (int64_t)p.a.c.n_kv_heads * R * kRec;
   float *const first = p.ws + ((int64_t)w.slot * R + row) * kRec;
   if (there) {
@@ -931,6 +951,7 @@ __device__ __forceinline__ void finish_piece(const PrefillParams &p, const Piece
     for (int i = 0; i < NV; i += 2) put2(r + d0 + i, acc[i], acc[i + 1]);
     if (d0 == 0) put2(r + HD, ml.x, ml.y);
   }
+  if (p.prefix_parts) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the record has reached memory
   __syncthreads();
   if (tid == 0) *last_in = arrive_last(p.arrive_end - 2 * ((int64_t)w.slot + 1), w.parts, p.tag);
@@ -975,25 +996,33 @@ __device__ __forceinline__ void finish_piece(const PrefillParams &p, const Piece
 // matrix cores form against a 0/1 selector).  Weights are taken against a
 // reference that moves to the true maximum only when a tile's sum passes 2^16.
 constexpr float kSumLimit = 65536.f, kMoveLog2 = 8.f;
-template <int HW, int KW, int OCC>
-__global__ __launch_bounds__(64 * HW * KW, OCC) void paged_prefill_bf16_kernel(PrefillParams p) {
-  constexpr int W = HW * KW, R = 32 * HW;
-  constexpr int KP = HD + 8;           // K row pitch, elements (144 B: conflict-free b128 rows)
-  constexpr int VP = HD + 16;          // V row pitch (160 B: conflict-free transpose reads)
-  constexpr int KT = 32 * KP, VT = 32 * VP;
-  constexpr int NB = HW > 1 ? 2 : 1;   // tile buffers (HW == 1: a wave's tile is its own)
-  constexpr int OP = HD + 4, OT = 32 * OP;  // a wave's O at the end, floats
-  constexpr int LDSE = KW * NB * (KT + VT) > 2 * W * OT ? KW * NB * (KT + VT) : 2 * W * OT;  // elements
-  __shared__ __attribute__((aligned(16))) bf16_t smem[LDSE];
-  __shared__ float red_m[W][32], red_l[W][32];
-  __shared__ int last_in;
+template <int HW, int KW>
+struct PrefillLds {
+  static constexpr int W = HW * KW;
+  static constexpr int KP = HD + 8;   // K row pitch, elements (144 B: conflict-free b128 rows)
+  static constexpr int VP = HD + 16;  // V row pitch (160 B: conflict-free transpose reads)
+  static constexpr int KT = 32 * KP, VT = 32 * VP;
+  static constexpr int NB = HW > 1 ? 2 : 1;        // tile buffers (HW == 1: a wave's tile is its own)
+  static constexpr int OP = HD + 4, OT = 32 * OP;  // a wave's O at the end, floats
+  static constexpr int RING = KW * NB * (KT + VT);
+  bf16_t smem[RING > 2 * W * OT ? RING : 2 * W * OT];
+  float red_m[W][32], red_l[W][32];
+  int last_in;
+};
+template <int HW, int KW>
+__device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, PrefillLds<HW, KW> &lds, int block) {
+  using L = PrefillLds<HW, KW>;
+  constexpr int W = L::W, R = 32 * HW, KP = L::KP, VP = L::VP, KT = L::KT, VT = L::VT, NB = L::NB;
+  constexpr int OP = L::OP, OT = L::OT;
+  bf16_t *const smem = lds.smem;
+  auto &red_m = lds.red_m, &red_l = lds.red_l;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hw = wave % HW, kw = wave / HW;
   const int r32 = lane & 31, hf = lane >> 5;
   Piece w;
-  if (!find_piece<R>(p, w)) return;
+  if (!find_piece<R>(p, block, w)) return;
   const Paged &c = p.a.c;
   const PieceKeys keys = piece_keys<R>(p, w);
   const float cl = p.a.cl;
@@ -1237,15 +1266,15 @@ __global__ __launch_bounds__(64 * HW * KW, OCC) void paged_prefill_bf16_kernel(P
   __syncthreads();
   constexpr int NV = R / W;  // = 64 elements over the row's threads
   static_assert(NV * (64 * W / R) == HD, "a row's threads cover it");
-  finish_piece<bf16_t, R, 64 * W>(p, w, &last_in, [&](int row, int d0, float (&acc)[NV]) __attribute__((always_inline)) {
+  finish_piece<bf16_t, R, 64 * W>(p, w, &lds.last_in, [&](int row, int d0, float (&acc)[NV]) __attribute__((always_inline)) {
     const int hu = row / 32, r = row % 32;
     float Mr = red_m[hu][r];
 #pragma unroll
     for (int v = 1; v < KW; ++v) Mr = fmaxf(Mr, red_m[v * HW + hu][r]);
     const float Mu = Mr == -INFINITY ? 0.f : Mr;
-    float L = 0.f;
+    float sum = 0.f;
 #pragma unroll
-    for (int v = 0; v < KW; ++v) L += red_l[v * HW + hu][r] * __builtin_amdgcn_exp2f(red_m[v * HW + hu][r] - Mu);
+    for (int v = 0; v < KW; ++v) sum += red_l[v * HW + hu][r] * __builtin_amdgcn_exp2f(red_m[v * HW + hu][r] - Mu);
 #pragma unroll
     for (int i = 0; i < NV; ++i) acc[i] = 0.f;
 #pragma unroll
@@ -1255,8 +1284,13 @@ __global__ __launch_bounds__(64 * HW * KW, OCC) void paged_prefill_bf16_kernel(P
         const float4 x = *(const float4 *)(ot + (v * HW + hu) * OT + r * OP + d0 + i);
         acc[i] += x.x; acc[i + 1] += x.y; acc[i + 2] += x.z; acc[i + 3] += x.w;
       }
-    return make_float2(Mr, L);
+    return make_float2(Mr, sum);
   });
+}
+template <int HW, int KW, int OCC>
+__global__ __launch_bounds__(64 * HW * KW, OCC) void paged_prefill_bf16_kernel(PrefillParams p) {
+  __shared__ __attribute__((aligned(16))) PrefillLds<HW, KW> lds;
+  prefill_bf16_body<HW, KW>(p, lds, blockIdx.x);
 }
 
 // fp32, v_mfma_f32_32x32x2f32: matrix-core time is all that counts.  32 rows a
@@ -1265,18 +1299,23 @@ __global__ __launch_bounds__(64 * HW * KW, OCC) void paged_prefill_bf16_kernel(P
 // straight from the pages as the second product's operand (two adjacent d of
 // one key row a lane), requested before the scores' products, which cover it.
 template <int KW>
-__global__ __launch_bounds__(64 * KW, 2) void paged_prefill_f32_kernel(PrefillParams p) {
+struct PrefillLdsF32 {
+  float smem[KW * 32 * (HD + 4)];
+  float red_m[KW][32], red_l[KW][32];
+  int last_in;
+};
+template <int KW>
+__device__ __forceinline__ void prefill_f32_body(const PrefillParams &p, PrefillLdsF32<KW> &lds, int block) {
   constexpr int R = 32, KP = HD + 4;  // K row and O row pitch, floats
   constexpr int TILE = 32 * KP;
-  __shared__ __attribute__((aligned(16))) float smem[KW * TILE];
-  __shared__ float red_m[KW][32], red_l[KW][32];
-  __shared__ int last_in;
+  float *const smem = lds.smem;
+  auto &red_m = lds.red_m, &red_l = lds.red_l;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int kw = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, hf = lane >> 5;
   Piece w;
-  if (!find_piece<R>(p, w)) return;
+  if (!find_piece<R>(p, block, w)) return;
   const Paged &c = p.a.c;
   const PieceKeys keys = piece_keys<R>(p, w);
   const float cl = p.a.cl;
@@ -1439,7 +1478,7 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_prefill_f32_kernel(PrefillPa
   }
   __syncthreads();
   constexpr int NV = HD / (2 * KW);
-  finish_piece<float, R, 64 * KW>(p, w, &last_in, [&](int row, int d0, float (&acc)[NV]) __attribute__((always_inline)) {
+  finish_piece<float, R, 64 * KW>(p, w, &lds.last_in, [&](int row, int d0, float (&acc)[NV]) __attribute__((always_inline)) {
     float Mr = red_m[0][row];
 #pragma unroll
     for (int v = 1; v < KW; ++v) Mr = fmaxf(Mr, red_m[v][row]);
@@ -1459,31 +1498,111 @@ __global__ __launch_bounds__(64 * KW, 2) void paged_prefill_f32_kernel(PrefillPa
     return make_float2(Mr, L);
   });
 }
+template <int KW>
+__global__ __launch_bounds__(64 * KW, 2) void paged_prefill_f32_kernel(PrefillParams p) {
+  __shared__ __attribute__((aligned(16))) PrefillLdsF32<KW> lds;
+  prefill_f32_body<KW>(p, lds, blockIdx.x);
+}
 
-// One wave per (row, query head), lane = element of the head: every key's
-// dot product is a wave sum.
-template <typename T>
-__global__ __launch_bounds__(64) void paged_rows_kernel(AttnParams p) {
-  const int lane = threadIdx.x, row = blockIdx.x, h = blockIdx.y, g = h / p.group;
-  const int b = sequence_of(p.starts, p.c.batch, row);
-  if (b < 0) return;
-  const int end = min(position_of(p.c, p.starts, b, row) + 1, p.c.cap);
-  const float q = Elem<T>::load((const T *)p.q + row * p.q_rs + h * HD + lane) * p.cl;
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int j = 0; j < end; ++j) {
-    const int page = j < p.prefix_len ? p.prefix_pages[j >> p.c.shift]
-                                      : p.c.table[b * p.c.table_stride + (j >> p.c.shift)];
-    if ((unsigned)page >= (unsigned)p.c.n_pages) continue;
-    const int64_t at = page * p.c.page_stride + g * p.c.head_stride +
-                       (j & ((1 << p.c.shift) - 1)) * p.c.row_stride + lane;
-    const float s = wave_sum(q * Elem<T>::load((const T *)p.c.k + at));
-    const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.f : mn;
-    const float a = __builtin_amdgcn_exp2f(m - mu), e = __builtin_amdgcn_exp2f(s - mu);
-    l = l * a + e;
-    acc = fmaf(e, Elem<T>::load((const T *)p.c.v + at), acc * a);
-    m = mn;
+// ------------------------------------------------- decode, a shared prefix
+// One launch for the common keys and the sequences' own: workgroups of the
+// prefill kernel over the batch's rows and the prefix (its keys are read once
+// for 32 or 128 rows, and computed at matrix-core rates), and workgroups of
+// the decode kernel over the keys behind it, eight of one kind and eight of
+// the other in turn while both last, so that a compute unit has some of each:
+// the one kind waits for memory, the other for the matrix cores.  Both leave
+// records, which a second launch adds.
+struct SharedParams {
+  DecodeParams d;
+  PrefillParams f;
+  int n_dec, n_pre;  // workgroups (multiples of 8 but for the last of a kind)
+};
+__device__ __forceinline__ bool shared_block(const SharedParams &p, int &block) {  // true: prefix
+  const int q = blockIdx.x >> 3, x = blockIdx.x & 7;
+  const int d8 = (p.n_dec + 7) >> 3, f8 = (p.n_pre + 7) >> 3, both = min(d8, f8);
+  bool prefix = d8 < f8;
+  if (q < 2 * both) {
+    prefix = q & 1;
+    block = (q >> 1) * 8 + x;
+  } else {
+    block = (q - both) * 8 + x;
   }
-  Elem<T>::store((T *)p.o + row * p.o_rs + h * HD + lane, l > 0.f ? acc / l : 0.f);
+  return prefix;
+}
+template <int HW, int KW>
+__global__ __launch_bounds__(256, 2) void paged_shared_bf16_kernel(SharedParams p) {
+  static_assert(HW * KW == 4, "256 threads");
+  union Lds {
+    DecodeLds<bf16_t> d;
+    PrefillLds<HW, KW> f;
+  };
+  __shared__ __attribute__((aligned(16))) Lds lds;
+  int block;
+  if (shared_block(p, block)) {
+    if (block < p.n_pre) prefill_bf16_body<HW, KW>(p.f, lds.f, block);
+  } else if (block < p.n_dec) {
+    decode_body<bf16_t>(p.d, lds.d, block);
+  }
+}
+__global__ __launch_bounds__(256, 2) void paged_shared_f32_kernel(SharedParams p) {
+  union Lds {
+    DecodeLds<float> d;
+    PrefillLdsF32<4> f;
+  };
+  __shared__ __attribute__((aligned(16))) Lds lds;
+  int block;
+  if (shared_block(p, block)) {
+    if (block < p.n_pre) prefill_f32_body<4>(p.f, lds.f, block);
+  } else if (block < p.n_dec) {
+    decode_body<float>(p.d, lds.d, block);
+  }
+}
+
+// The records of a row: `parts` of the prefix, then its own keys'.  Two
+// elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_shared_add_kernel(SharedParams p, int R) {
+  const AttnParams &a = p.d.a;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int d = 2 * (int)(i % (HD / 2)), h = (int)(i / (HD / 2) % a.n_heads), b = (int)(i / (HD / 2) / a.n_heads);
+  if (b >= a.c.batch) return;
+  const int g = h / a.group, fr = b * a.group + h - g * a.group, unit = fr / R, parts = p.f.prefix_parts;
+  const float *r = p.f.ws + (((int64_t)unit * parts * a.c.n_kv_heads + g) * R + (fr - unit * R)) * kRec;
+  const int64_t step = (int64_t)a.c.n_kv_heads * R * kRec;
+  const float *const mine = p.d.parts + ((int64_t)b * a.n_heads + h) * kRec;
+  const float2 own = *(const float2 *)(mine + HD), x = *(const float2 *)(mine + d);
+  float M = own.x, L = own.y, A0 = x.x, A1 = x.y;
+  constexpr int N = 8;  // records read at once
+  for (int n0 = 0; n0 < parts; n0 += N) {
+    float2 ml[N], y[N];
+#pragma unroll
+    for (int v = 0; v < N; ++v) {
+      const float *const q = r + min(n0 + v, parts - 1) * step;
+      ml[v] = *(const float2 *)(q + HD);
+      y[v] = *(const float2 *)(q + d);
+    }
+    float mx = M;
+#pragma unroll
+    for (int v = 0; v < N; ++v) mx = n0 + v < parts ? fmaxf(mx, ml[v].x) : mx;
+    const float mu = mx == -INFINITY ? 0.f : mx, fo = __builtin_amdgcn_exp2f(M - mu);
+    L *= fo;
+    A0 *= fo;
+    A1 *= fo;
+#pragma unroll
+    for (int v = 0; v < N; ++v) {
+      const float f = n0 + v < parts ? __builtin_amdgcn_exp2f(ml[v].x - mu) : 0.f;
+      L = n0 + v < parts ? fmaf(ml[v].y, f, L) : L;
+      A0 = n0 + v < parts ? fmaf(y[v].x, f, A0) : A0;
+      A1 = n0 + v < parts ? fmaf(y[v].y, f, A1) : A1;
+    }
+    M = mx;
+  }
+  const float inv = L > 0.f ? 1.0f / L : 0.f;
+  T *const op = (T *)a.o + b * a.o_rs + h * HD + d;
+  if constexpr (sizeof(T) == 2)
+    *(uint32_t *)op = (uint32_t)f32_to_bf16(A0 * inv) | ((uint32_t)f32_to_bf16(A1 * inv) << 16);
+  else
+    *(float2 *)op = make_float2(A0 * inv, A1 * inv);
 }
 
 // ---------------------------------------------------------------- the host
@@ -1652,6 +1771,7 @@ int launch_decode(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
   p.tag = next_tag();
   p.bins = d.bins; p.hblocks = d.hblocks; p.columns = d.columns;
   p.k0 = 0;
+  p.parts = nullptr;
   const dim3 grid((unsigned)(d.bins * d.columns)), block(256);
   if (dtype == BN_BF16) hipLaunchKernelGGL(paged_decode_kernel<bf16_t>, grid, block, 0, s, p);
   else hipLaunchKernelGGL(paged_decode_kernel<float>, grid, block, 0, s, p);
@@ -1666,7 +1786,7 @@ struct PrefillPlan {
   int64_t groups, slots;   // workgroups of the launch, records
   size_t records, words;   // bytes
 };
-PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv_heads, int cap, bool records) {
+PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv_heads, int cap) {
   PrefillPlan d;
   const int64_t rows = (int64_t)n_rows * (n_heads / n_kv_heads);  // of a KV head
   const int64_t u128 = (rows / 128 + 1) * n_kv_heads, u32 = (rows / 32 + 1) * n_kv_heads;
@@ -1691,21 +1811,21 @@ PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv
   const int64_t pieces = units + cut;
   const int per = n_kv_heads <= 8 && 8 % n_kv_heads == 0 ? 8 / n_kv_heads : 1;
   d.groups = (pieces + per - 1) / per * per * n_kv_heads;
-  d.slots = (records ? pieces : cut) * n_kv_heads;
+  d.slots = cut * n_kv_heads;
   d.records = (size_t)d.slots * R * kRec * sizeof(float);
   d.words = (size_t)d.slots * 16 * d.hw;  // (16 are used; a call of fewer rows, whose records are smaller, needs no more)
   return d;
 }
 
 int launch_prefill(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
-  const PrefillPlan d = plan_prefill(dtype, a.c.batch, a.n_rows, a.n_heads, a.c.n_kv_heads, a.c.cap, false);
+  const PrefillPlan d = plan_prefill(dtype, a.c.batch, a.n_rows, a.n_heads, a.c.n_kv_heads, a.c.cap);
   PrefillParams p;
   p.a = a;
   p.ws = (float *)ws;
   p.arrive_end = (unsigned long long *)((char *)ws + d.records + d.words);
   p.tag = next_tag();
   p.slots = (int)d.slots;
-  p.prefix = 0;
+  p.prefix_parts = 0;
   const dim3 grid((unsigned)d.groups);
   if (dtype == BN_F32) {
     if (d.kw == 4) hipLaunchKernelGGL(paged_prefill_f32_kernel<4>, grid, dim3(256), 0, s, p);
@@ -1718,6 +1838,59 @@ int launch_prefill(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
   } else {
     hipLaunchKernelGGL((paged_prefill_bf16_kernel<1, 4, 3>), grid, dim3(256), 0, s, p);
   }
+  BN_LAUNCH_CHECK();
+  return BN_OK;
+}
+
+// The shared-prefix call: units of R rows, the prefix's tiles of each in
+// `parts`, about two workgroups a compute unit.
+struct SharedPlan {
+  DecodePlan d;
+  int hw, parts;
+  int64_t n_pre;
+  size_t own, records;  // bytes: the sequences' own parts, the prefix's
+};
+SharedPlan plan_shared(int dtype, int batch, int n_heads, int n_kv_heads, int prefix_len) {
+  SharedPlan s;
+  s.d = plan_decode(batch, n_heads, n_kv_heads);
+  const int64_t rows = (int64_t)batch * (n_heads / n_kv_heads);
+  s.hw = dtype == BN_BF16 && rows * n_kv_heads >= 32 * 128 ? 4 : 1;
+  const int R = 32 * s.hw, steps = (prefix_len + 31) / 32;
+  const int64_t units = (rows + R - 1) / R;
+  s.parts = (int)std::max<int64_t>(1, std::min<int64_t>((512 + units * n_kv_heads - 1) / (units * n_kv_heads), steps / 8));
+  const int per = n_kv_heads <= 8 && 8 % n_kv_heads == 0 ? 8 / n_kv_heads : 1;
+  s.n_pre = (units * s.parts + per - 1) / per * per * n_kv_heads;
+  s.own = (size_t)batch * n_heads * kRec * sizeof(float);
+  s.records = (size_t)units * s.parts * n_kv_heads * R * kRec * sizeof(float);
+  return s;
+}
+
+int launch_shared(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
+  const SharedPlan m = plan_shared(dtype, a.c.batch, a.n_heads, a.c.n_kv_heads, a.prefix_len);
+  char *at = (char *)ws;
+  SharedParams p;
+  p.d.a = p.f.a = a;
+  p.d.ws = (float *)at;
+  p.d.arrive_end = (unsigned long long *)(at + m.d.records + m.d.words);
+  p.d.tag = p.f.tag = next_tag();
+  p.d.bins = m.d.bins; p.d.hblocks = m.d.hblocks; p.d.columns = m.d.columns;
+  p.d.k0 = a.prefix_len;
+  p.d.parts = (float *)(at + m.d.records + m.d.words);
+  p.f.ws = (float *)(at + m.d.records + m.d.words + m.own);
+  p.f.arrive_end = nullptr;
+  p.f.slots = 0;
+  p.f.prefix_parts = m.parts;
+  p.n_dec = m.d.bins * m.d.columns;
+  p.n_pre = (int)m.n_pre;
+  const dim3 grid((unsigned)(((p.n_dec + 7) / 8 + (m.n_pre + 7) / 8) * 8)), block(256);
+  if (dtype == BN_F32) hipLaunchKernelGGL(paged_shared_f32_kernel, grid, block, 0, s, p);
+  else if (m.hw == 4) hipLaunchKernelGGL((paged_shared_bf16_kernel<4, 1>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((paged_shared_bf16_kernel<1, 4>), grid, block, 0, s, p);
+  BN_LAUNCH_CHECK();
+  const int64_t pairs = (int64_t)a.c.batch * a.n_heads * (HD / 2);
+  const dim3 add((unsigned)((pairs + 255) / 256));
+  if (dtype == BN_F32) hipLaunchKernelGGL(paged_shared_add_kernel<float>, add, block, 0, s, p, 32 * m.hw);
+  else hipLaunchKernelGGL(paged_shared_add_kernel<bf16_t>, add, block, 0, s, p, 32 * m.hw);
   BN_LAUNCH_CHECK();
   return BN_OK;
 }
@@ -1755,19 +1928,13 @@ int attention(const char *name, const bn_paged_kv *kv, const void *q, void *o, c
   p.q_rs = q_rs; p.o_rs = o_rs;
   p.n_rows = n_rows; p.n_heads = n_heads; p.group = n_heads / kv->n_kv_heads;
   p.cl = scale * kLog2e;
-  p.prefix_pages = prefix_pages; p.prefix_len = prefix_len;
+  p.prefix_pages = prefix_pages; p.prefix_len = std::min(prefix_len, p.c.cap);
   Workspace ws;
   if ((st = ws.take(workspace, need, stream))) return st;
-  if (prefix_len == 0)
-    return ws.release(starts ? launch_prefill(p, kv->dtype, ws.p, as_stream(stream))
-                             : launch_decode(p, kv->dtype, ws.p, as_stream(stream)));
-  const dim3 grid(n_rows, n_heads);
-  if (kv->dtype == BN_BF16)
-    hipLaunchKernelGGL(paged_rows_kernel<bf16_t>, grid, dim3(64), 0, as_stream(stream), p);
-  else
-    hipLaunchKernelGGL(paged_rows_kernel<float>, grid, dim3(64), 0, as_stream(stream), p);
-  const hipError_t e = hipGetLastError();
-  return ws.release(e == hipSuccess ? BN_OK : hip_fail(e, __FILE__, __LINE__));
+  hipStream_t s = as_stream(stream);
+  return ws.release(p.prefix_len > 0 ? launch_shared(p, kv->dtype, ws.p, s)
+                    : starts         ? launch_prefill(p, kv->dtype, ws.p, s)
+                                     : launch_decode(p, kv->dtype, ws.p, s));
 }
 
 }  // namespace
@@ -1825,8 +1992,13 @@ size_t bn_paged_workspace_size(const bn_paged_kv *cache, int n_heads, int n_rows
       check_heads("", n_heads, cache->n_kv_heads, n_rows))
     return 0;
   const DecodePlan d = plan_decode(cache->batch, n_heads, cache->n_kv_heads);
-  const PrefillPlan f = plan_prefill(cache->dtype, cache->batch, n_rows, n_heads, cache->n_kv_heads, c.cap, false);
-  return std::max(d.records + d.words, f.records + f.words);
+  const PrefillPlan f = plan_prefill(cache->dtype, cache->batch, n_rows, n_heads, cache->n_kv_heads, c.cap);
+  size_t need = std::max(d.records + d.words, f.records + f.words);
+  if (prefix_len > 0) {
+    const SharedPlan s = plan_shared(cache->dtype, cache->batch, n_heads, cache->n_kv_heads, std::min(prefix_len, c.cap));
+    need = std::max(need, s.d.records + s.d.words + s.own + s.records);
+  }
+  return need;
 }
 
 int bn_paged_decode(const bn_paged_kv *cache, const void *q, void *o, int n_heads, int64_t q_row_stride,
