@@ -52,6 +52,23 @@ __device__ __forceinline__ int position_of(const Paged &c, const int32_t *starts
   return starts ? len - starts[b + 1] + row : len - 1;
 }
 
+// Byte offset of eight rows from `key` on in their page: two 32 x 32 products.
+struct PageRows {
+  uint32_t page_bytes, row_bytes, slot_mask, n_pages;
+  template <typename T>
+  __device__ __forceinline__ static PageRows of(const Paged &c) {
+    return PageRows{(uint32_t)(c.page_stride * sizeof(T)), (uint32_t)(c.row_stride * sizeof(T)), (1u << c.shift) - 1,
+                    (uint32_t)c.n_pages};
+  }
+  __device__ __forceinline__ bool there(int id) const { return (uint32_t)id < n_pages; }
+  __device__ __forceinline__ uint64_t at(int id, int key) const {  // (no page: page 0's rows)
+    return (uint64_t)(there(id) ? (uint32_t)id : 0u) * page_bytes + (uint64_t)((uint32_t)key & slot_mask) * row_bytes;
+  }
+};
+// table entries are read as scalars
+typedef const __attribute__((address_space(4))) char *scalar_bytes;
+typedef const __attribute__((address_space(4))) int32_t *scalar_ints;
+
 // ------------------------------------------------------------------ append
 struct AppendParams {
   Paged c;
@@ -165,7 +182,8 @@ struct AttnParams {
   const int32_t *starts;  // null: one row per sequence
   int64_t q_rs, o_rs;
   int n_rows, n_heads, group;
-  float cl;  // scale * log2(e)
+  float inv_group;  // 1 / group
+  float cl;         // scale * log2(e)
   const int32_t *prefix_pages;
   int prefix_len;
 };
@@ -211,6 +229,21 @@ __device__ __forceinline__ int wave_scan(int x) {
   x = dpp_add<0x118, 0xf>(x);
   x = dpp_add<0x142, 0xa>(x);  // row_bcast 15 to rows 1 and 3
   return dpp_add<0x143, 0xc>(x);  // row_bcast 31 to rows 2 and 3
+}
+
+// The lanes' sum, the same in every wave.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_addf(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float wave_total(float x) {
+  x = dpp_addf<0x111, 0xf>(x);
+  x = dpp_addf<0x112, 0xf>(x);
+  x = dpp_addf<0x114, 0xf>(x);
+  x = dpp_addf<0x118, 0xf>(x);
+  x = dpp_addf<0x142, 0xa>(x);
+  x = dpp_addf<0x143, 0xc>(x);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
 struct DecodeParams {
@@ -371,13 +404,10 @@ __device__ __forceinline__ void decode_body(const DecodeParams &p, DecodeLds<T> 
   const uint32_t off = (uint32_t)((crow * c.row_stride + ccol) * sizeof(T));
   const char *const Kg = (const char *)((const T *)c.k + g * c.head_stride);
   const char *const Vg = (const char *)((const T *)c.v + g * c.head_stride);
-  const int slot_mask = (1 << c.shift) - 1;
-  const int64_t page_bytes = c.page_stride * (int64_t)sizeof(T);
-  const uint32_t row_bytes = (uint32_t)(c.row_stride * sizeof(T));
+  const PageRows page_rows = PageRows::of<T>(c);
   // A tile's table entries are read as scalars: they come in their own order,
   // not behind the rows requested before them (as vector loads they held up
   // the next rows: 64 caches of 4096 keys 51 us).
-  typedef const __attribute__((address_space(4))) int32_t *scalar_ints;
   int ids[4];  // of rows RPI r .. of the tile to load next
   struct Rows {
     u32x4 k[4], v[4];  // the lane's pieces of a tile
@@ -387,20 +417,19 @@ __device__ __forceinline__ void decode_body(const DecodeParams &p, DecodeLds<T> 
   auto load_ids = [&](const Tile &x) __attribute__((always_inline)) {
     const int b = __builtin_amdgcn_readfirstlane(x.b), key0 = k0 + TK * __builtin_amdgcn_readfirstlane(x.t);
     const int last = __builtin_amdgcn_readfirstlane(x.len) - 1;
-    const scalar_ints row = (scalar_ints)(c.table + b * c.table_stride);
+    const scalar_bytes row = (scalar_bytes)(c.table + b * c.table_stride);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) ids[r] = row[min(key0 + RPI * r, last) >> c.shift];
+    for (int r = 0; r < 4; ++r) ids[r] = *(scalar_ints)(row + ((uint32_t)(min(key0 + RPI * r, last) >> c.shift) << 2));
   };
-  int64_t at[4];  // byte offsets of the rows
+  uint64_t at[4];  // byte offsets of the rows
   int at_pages;   // bit r: those rows have memory (else page 0's are read)
   auto locate_rows = [&](const Tile &x) __attribute__((always_inline)) {
     const int key0 = k0 + TK * __builtin_amdgcn_readfirstlane(x.t);
     at_pages = 0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const bool ok = (unsigned)ids[r] < (unsigned)c.n_pages;
-      at_pages |= ok << r;
-      at[r] = (ok ? ids[r] : 0) * page_bytes + (int64_t)((uint64_t)(uint32_t)((key0 + RPI * r) & slot_mask) * row_bytes);
+      at_pages |= page_rows.there(ids[r]) << r;
+      at[r] = page_rows.at(ids[r], key0 + RPI * r);
     }
   };
   auto load_rows = [&](Rows &y, const Tile &x) __attribute__((always_inline)) {
@@ -769,9 +798,31 @@ struct Piece {
   int row0, rows;               // the sequence's rows of the tensors
   int last;                     // keys the sequence's last row sees, before the table's clamp
   int slot;                     // record of the unit's first part (parts > 1)
+  int tok0, rem0;               // the unit's first row: token, head of the group
 };
+// Row r of the unit (r < 256): its token and its head of the group.  rem0 + r is
+// below group + 256, where the product with 1 / group errs by less than half of that.
+__device__ __forceinline__ int token_of(const Piece &w, float inv_group, int group, int r, int &head) {
+  const int x = w.rem0 + r, q = (int)(((float)x + 0.5f) * inv_group);
+  head = x - q * group;
+  return w.tok0 + q;
+}
+__device__ __forceinline__ void first_row(Piece &w, int row, int group) {
+  w.tok0 = __builtin_amdgcn_readfirstlane((int)((uint32_t)row / (uint32_t)group));
+  w.rem0 = row - w.tok0 * group;
+}
+// Part `part` of `parts` of n: first and end.
+__device__ __forceinline__ void part_of(int n, const Piece &w, int &from, int &to) {
+  from = 0;
+  to = n;
+  if (w.parts > 1) {
+    const int q = __builtin_amdgcn_readfirstlane((int)((uint32_t)n / (uint32_t)w.parts)), r = n - q * w.parts;
+    from = w.part * q + min(w.part, r);
+    to = from + q + (w.part < r);
+  }
+}
 constexpr int kPartMin = 24;      // tiles of a part at least
-constexpr int kPartsAll = 1024;   // a part is at least this share of all the call's tiles
+constexpr int kPartsAll = 256;   // a part is at least this share of all the call's tiles
 
 // Which piece of work is workgroup L's.  A call's units differ in length (the
 // diagonal, and the sequences themselves): a unit whose keys are more than
@@ -801,6 +852,7 @@ __device__ __forceinline__ bool find_piece(const PrefillParams &p, int block, Pi
     w.unit = idx / w.parts;
     w.part = idx - w.unit * w.parts;
     w.slot = w.unit * w.parts * hkv + w.g;
+    first_row(w, w.unit * R, G);
     return w.unit * R < w.rows * G;
   }
   struct Seq {
@@ -825,10 +877,10 @@ __device__ __forceinline__ bool find_piece(const PrefillParams &p, int block, Pi
   Seq mine = seq(lane * per);
   float total = lane * per < n ? mine.weight : 0.f;
   for (int i = 1; i < per; ++i) total += lane * per + i < n ? seq(lane * per + i).weight : 0.f;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+  total = wave_total(total);
   const int share = max((int)(total * (float)hkv * (1.f / kPartsAll)), kPartMin);
-  auto parts_of = [&](const Seq &s) { return max(s.steps / share, 1); };
+  // (a division only where it can come to 2 or more)
+  auto parts_of = [&](const Seq &s) { return s.steps < 2 * share ? 1 : (int)((uint32_t)s.steps / (uint32_t)share); };
   auto count = [&](const Seq &s, bool in, int &all, int &cut) __attribute__((always_inline)) {
     const int parts = parts_of(s), k = in ? s.units * parts : 0;
     all += k;
@@ -866,11 +918,13 @@ __device__ __forceinline__ bool find_piece(const PrefillParams &p, int block, Pi
   w.rows = __builtin_amdgcn_readlane(mine.rows, src);
   w.last = __builtin_amdgcn_readlane(mine.last, src);
   const int units = __builtin_amdgcn_readlane(mine.units, src), steps = __builtin_amdgcn_readlane(mine.steps, src);
-  w.parts = __builtin_amdgcn_readfirstlane(max(steps / share, 1));
-  const int from_end = __builtin_amdgcn_readfirstlane(k / w.parts);  // longest units first
+  w.parts = steps < 2 * share ? 1 : __builtin_amdgcn_readfirstlane((int)((uint32_t)steps / (uint32_t)share));
+  const int from_end =  // longest units first
+      w.parts == 1 ? k : __builtin_amdgcn_readfirstlane((int)((uint32_t)k / (uint32_t)w.parts));
   w.unit = units - 1 - from_end;
   w.part = k - from_end * w.parts;
   w.slot = (cuts + from_end * w.parts) * hkv + w.g;  // parts of a unit: hkv slots apart
+  first_row(w, w.unit * R, G);
   // (row_starts that decrease could count rows twice and pass the workspace)
   return w.parts == 1 || (int64_t)w.slot + (int64_t)(w.parts - 1) * hkv < p.slots;
 }
@@ -878,11 +932,15 @@ __device__ __forceinline__ bool find_piece(const PrefillParams &p, int block, Pi
 // What the two prefill kernels share: the piece's keys, the rows' limits and
 // the scalars of the pages.
 struct PieceKeys {
-  const __attribute__((address_space(4))) int32_t *table;
+  const int32_t *table;
   int t0, t1;  // its tiles
   int end;     // keys that some row of the unit sees
+  int whole;   // keys that every row of the unit sees
   int shift;
-  __device__ __forceinline__ int entry(int key) const { return table[min(key, end - 1) >> shift]; }
+  // The table entry of a key (lanes may ask for different ones).  A vector load
+  // on purpose: it comes behind the rows requested before it, for which the tile
+  // waits anyway, where a scalar load would be waited for with every LDS read.
+  __device__ __forceinline__ int entry(int key) const { return table[(uint32_t)(min(key, end - 1) >> shift)]; }
 };
 template <int R>
 __device__ __forceinline__ PieceKeys piece_keys(const PrefillParams &p, const Piece &w) {
@@ -890,16 +948,18 @@ __device__ __forceinline__ PieceKeys piece_keys(const PrefillParams &p, const Pi
   PieceKeys k;
   if (p.prefix_parts) {
     k.end = p.a.prefix_len;
-    k.table = (const __attribute__((address_space(4))) int32_t *)p.a.prefix_pages;
+    k.whole = 0;
+    k.table = p.a.prefix_pages;
   } else {
-    const int tokens = min((w.unit * R + R - 1) / p.a.group + 1, w.rows);  // up to the unit's last row
+    int h;
+    const int tokens = min(__builtin_amdgcn_readfirstlane(token_of(w, p.a.inv_group, p.a.group, R - 1, h)) + 1, w.rows);
     k.end = min(max(w.last - w.rows + tokens, 0), c.cap);
-    k.table = (const __attribute__((address_space(4))) int32_t *)(c.table + w.b * c.table_stride);
+    k.whole = min(max(w.last - w.rows + w.tok0 + 1, 0), c.cap);
+    k.table = c.table + w.b * c.table_stride;
   }
   k.end = __builtin_amdgcn_readfirstlane(k.end);
-  const int nt = (k.end + 31) >> 5;
-  k.t0 = __builtin_amdgcn_readfirstlane((int)((int64_t)nt * w.part / w.parts));
-  k.t1 = __builtin_amdgcn_readfirstlane((int)((int64_t)nt * (w.part + 1) / w.parts));
+  k.whole = __builtin_amdgcn_readfirstlane(k.whole);
+  part_of((k.end + 31) >> 5, w, k.t0, k.t1);
   k.shift = c.shift;
   return k;
 }
@@ -914,16 +974,66 @@ __device__ __forceinline__ int wave_min(int x) {
   return __builtin_amdgcn_readfirstlane(x);
 }
 
+// Infinite and NaN values of keys that not every row of a workgroup sees: a row
+// that does not see one weighs it with 0, and 0 times it is not 0.  They are
+// staged as zeros (tame), and if there were any, add_odd() puts each, as it
+// is, into the rows that see it when the tiles are through (what a sum with
+// one of them in it comes to, whatever its weight): nothing of this in the loop.
+template <typename T>
+__device__ __forceinline__ bool tame(u32x4 &x) {  // true: there was one
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 2) {
+      const bool lo = (x[j] & 0x7f80u) == 0x7f80u, hi = (x[j] & 0x7f800000u) == 0x7f800000u;
+      x[j] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+      odd |= lo || hi;
+    } else {
+      const bool b = (x[j] & 0x7f800000u) == 0x7f800000u;
+      x[j] = b ? 0u : x[j];
+      odd |= b;
+    }
+  }
+  return odd;
+}
+// o[n], n < N: the lane's rows' accumulators in the order that d_of(i) gives
+// the elements of; limit[n]: keys that the rows see; keys from .. to - 1.
+template <typename T, int N, class D>
+__device__ __forceinline__ void add_odd(const PieceKeys &keys, const PageRows &rows, const char *Vg, int from, int to,
+                                        f32x16 (&o)[N][2], const int (&limit)[N], D &&d_of) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (int k = from; k < to; ++k) {
+    const int id = __builtin_amdgcn_readfirstlane(keys.entry(k));
+    if (!rows.there(id)) continue;
+    const float v = Elem<T>::load((const T *)(Vg + rows.at(id, k)) + lane);
+    unsigned long long odd = __builtin_amdgcn_ballot_w64(!(fabsf(v) < INFINITY));
+#pragma unroll 1
+    for (; odd; odd &= odd - 1) {
+      const int d = __builtin_ctzll(odd);
+      const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), d));
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (d_of(i) == d && k < limit[n]) o[n][i >> 4][i & 15] += x;
+    }
+  }
+}
+
 // The end of a piece, all its waves: `sum(row, d, ml)` gives NV consecutive
 // elements of a row's accumulator and its (reference in log2 units, sum); a
 // whole unit is written, of a cut one a record is left and the last part to
 // arrive adds them, in the order of the keys, and writes.
 template <typename T, int R, int THREADS, class F>
-__device__ __forceinline__ void finish_piece(const PrefillParams &p, const Piece &w, int *last_in, F &&sum) {
+__device__ __forceinline__ void finish_piece(const PrefillParams &p, const Piece &kept, int *last_in, F &&sum) {
+  const Piece w = kept;
   constexpr int TPR = THREADS / R, NV = HD / TPR;  // threads a row, elements a thread
   static_assert(THREADS % R == 0 && NV % 4 == 0, "whole quads");
   const int tid = threadIdx.x, row = tid / TPR, d0 = (tid % TPR) * NV;
-  const int fr = w.unit * R + row, t = fr / p.a.group, h = w.g * p.a.group + fr - t * p.a.group;
+  int h;
+  const int t = token_of(w, p.a.inv_group, p.a.group, row, h);
+  h += w.g * p.a.group;
   const bool there = t < w.rows;
   float acc[NV];
   float2 ml = sum(row, d0, acc);
@@ -960,7 +1070,7 @@ __device__ __forceinline__ void finish_piece(const PrefillParams &p, const Piece
   ml = make_float2(-INFINITY, 0.f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) acc[i] = 0.f;
-  constexpr int MB = NV >= 32 ? 2 : 4;  // records read at once
+  constexpr int MB = NV >= 32 ? 1 : 4;  // records read at once
   for (int n0 = 0; n0 < w.parts; n0 += MB) {
     float2 m2[MB], a[MB][NV / 2];
 #pragma unroll
@@ -1007,6 +1117,9 @@ struct PrefillLds {
   static constexpr int RING = KW * NB * (KT + VT);
   bf16_t smem[RING > 2 * W * OT ? RING : 2 * W * OT];
   float red_m[W][32], red_l[W][32];
+  unsigned char __attribute__((aligned(4))) chunk_ok[KW][2][4];
+  int odd[W];
+  Piece piece;  // kept here across the tiles, not in scalar registers
   int last_in;
 };
 template <int HW, int KW>
@@ -1023,13 +1136,15 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
   const int r32 = lane & 31, hf = lane >> 5;
   Piece w;
   if (!find_piece<R>(p, block, w)) return;
+  if (tid == 0) lds.piece = w;
   const Paged &c = p.a.c;
   const PieceKeys keys = piece_keys<R>(p, w);
   const float cl = p.a.cl;
   const int ni = (keys.t1 - keys.t0 + KW - 1) / KW;  // steps: tile t0 + kw + KW*i each
 
   // this lane's row
-  const int fr = w.unit * R + 32 * hw + r32, tok = fr / p.a.group, head = fr - tok * p.a.group;
+  int head;
+  const int tok = token_of(w, p.a.inv_group, p.a.group, 32 * hw + r32, head);
   const bool there = tok < w.rows;
   const int limit = there ? key_limit(p, w, tok) : 0;
   const int all_see = wave_min(there ? limit : 0x7fffffff);  // keys that all the wave's rows see
@@ -1048,56 +1163,56 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
   // each (16-byte piece lane % 8 of row lane / 8); a chunk's rows lie in one page
   constexpr int NC = 4 / HW;
   const int crow = lane >> 3, ccol = (lane & 7) * 8;
-  const int slot_mask = (1 << c.shift) - 1;
-  const int64_t page_bytes = c.page_stride * 2;
-  const uint32_t row_bytes = (uint32_t)c.row_stride * 2, off = crow * row_bytes + ccol * 2;
+  const PageRows rows = PageRows::of<bf16_t>(c);
+  const uint32_t off = crow * rows.row_bytes + ccol * 2;
   const char *const Kg = (const char *)((const bf16_t *)c.k + w.g * c.head_stride);
   const char *const Vg = (const char *)((const bf16_t *)c.v + w.g * c.head_stride);
   u32x4 kr[NC], vr[NC];
-  int ids[4];
-  int pages = 0, pages_next = 0;  // bit r: rows 8r .. of the tile have memory; of this tile, of the next
+  int entry = 0;  // lane j (mod NC): of chunk j of the tile to load next
+  bool any_odd = false;
+  int chunks_next = 0;  // bit j: the wave's chunk j of the tile loaded last has memory
+  auto key_of = [&](int i) { return 32 * (keys.t0 + kw + KW * i); };
   auto load_ids = [&](int i) __attribute__((always_inline)) {
-    const int key0 = 32 * (keys.t0 + kw + KW * i);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) ids[r] = keys.entry(key0 + 8 * r);
+    entry = keys.entry(key_of(i) + 8 * (NC * hw + (lane & (NC - 1))));
   };
   auto gload = [&](int i) __attribute__((always_inline)) {
-    const int key0 = 32 * (keys.t0 + kw + KW * i);
-    pages_next = 0;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) pages_next |= ((unsigned)ids[r] < (unsigned)c.n_pages) << r;
+    uint32_t o32 = off;
+    asm volatile("" : "+v"(o32));  // a scalar base and this offset, not a sum of pointers kept in registers
+    chunks_next = 0;
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      int id = ids[j];
-      if constexpr (HW > 1) {  // (a scalar's index is a constant)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) id = NC * hw + j == r ? ids[r] : id;
-      }
-      const bool ok = (unsigned)id < (unsigned)c.n_pages;
-      const int64_t at = (ok ? id : 0) * page_bytes +
-                         (int64_t)((uint64_t)(uint32_t)((key0 + 8 * (NC * hw + j)) & slot_mask) * row_bytes);
-      kr[j] = *(const u32x4 *)(Kg + at + off);
-      vr[j] = *(const u32x4 *)(Vg + at + off);
+      const int id = __builtin_amdgcn_readlane(entry, j);
+      chunks_next |= rows.there(id) << j;
+      const uint64_t at = rows.at(id, key_of(i) + 8 * (NC * hw + j));
+      kr[j] = *(const u32x4 *)(Kg + at + o32);
+      vr[j] = *(const u32x4 *)(Vg + at + o32);
     }
   };
+  // (HW > 1: the waves that share a tile tell each other of their chunks through LDS)
   auto lstore = [&](int i) __attribute__((always_inline)) {
-    const int key0 = 32 * (keys.t0 + kw + KW * i);
-    bf16_t *const kd = smem + (kw * NB + (NB > 1 ? i & 1 : 0)) * (KT + VT), *const vd = kd + KT;
-    if (key0 + 32 > keys.end || pages_next != 15) {  // no key: zeros, whatever lies there
+    const int key0 = key_of(i), b = NB > 1 ? i & 1 : 0;
+    bf16_t *const kd = smem + (kw * NB + b) * (KT + VT), *const vd = kd + KT;
+    if (key0 + 32 > keys.end || chunks_next != (1 << NC) - 1) {  // no key: zeros, whatever lies there
 #pragma unroll
-      for (int j = 0; j < NC; ++j) {
-        const int r = NC * hw + j;
-        if (!(pages_next >> r & 1) || key0 + 8 * r + crow >= keys.end) vr[j] = u32x4{0, 0, 0, 0};
-      }
+      for (int j = 0; j < NC; ++j)
+        if (!(chunks_next >> j & 1) || key0 + 8 * (NC * hw + j) + crow >= keys.end) vr[j] = u32x4{0, 0, 0, 0};
+    }
+    if (key0 + 32 > keys.whole) {
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) odd |= tame<bf16_t>(vr[j]);
+      any_odd |= __builtin_amdgcn_ballot_w64(odd) != 0;
     }
 #pragma unroll
     for (int j = 0; j < NC; ++j) *(u32x4 *)(kd + (8 * (NC * hw + j) + crow) * KP + ccol) = kr[j];
 #pragma unroll
     for (int j = 0; j < NC; ++j) *(u32x4 *)(vd + (8 * (NC * hw + j) + crow) * VP + ccol) = vr[j];
+    if (HW > 1 && lane == 0) lds.chunk_ok[kw][b][hw] = (unsigned char)chunks_next;
   };
 
   float l = 0.f, mcv = -INFINITY;  // row sum; reference, log2 units
-  f32x16 o[2] = {f32x16{}, f32x16{}};
+  f32x16 ow[1][2] = {{f32x16{}, f32x16{}}};
+  f32x16 (&o)[2] = ow[0];
   const uint32_t rs_bits = (((lane & 15) >> 2) & 1) == ((lane >> 4) & 1) ? 0x3f803f80u : 0u;
   const int tr_off = (4 * hf + ((lane & 15) >> 2)) * VP + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
   // p = exp2(s * cl - mc) as bf16 operands, and the tile's row sum over both half-waves
@@ -1139,7 +1254,7 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
   }
   if constexpr (NB > 1) __syncthreads();
   for (int i = 0; i < ni; ++i) {
-    pages = pages_next;
+    int pages = chunks_next;  // bit r: rows 8r .. of this tile have memory
     if constexpr (NB == 1) {
       // the wave's own tile: its LDS instructions execute in order, the
       // barriers keep the compiler from moving them across
@@ -1151,6 +1266,10 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
     load_ids(i + 2);
     const bf16_t *const kl = smem + (kw * NB + (NB > 1 ? i & 1 : 0)) * (KT + VT), *const vl = kl + KT;
     const int tile = keys.t0 + kw + KW * i, kb = 32 * tile;
+    if constexpr (HW > 1) {
+      const uint32_t ok = __builtin_amdgcn_readfirstlane(*(const uint32_t *)lds.chunk_ok[kw][i & 1]);
+      pages = (ok & 1) | (ok >> 7 & 2) | (ok >> 14 & 4) | (ok >> 21 & 8);
+    }
     if (tile < keys.t1) {  // wave-uniform
       f32x16 s = f32x16{};
 #pragma unroll
@@ -1167,41 +1286,11 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
           const bf16x4 hi = lds_tr16(vl + (16 * u + 8) * VP + tr_off + 32 * dt);
           va[u][dt] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         }
-      uint32_t odd = 0;  // keys of this tile with an infinite or NaN value, where some row does not see all
       if (kb + 32 > all_see || pages != 15) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int k = (e >> 2) * 8 + hf * 4 + (e & 3);
           if (kb + k >= limit || !(pages >> (e >> 2) & 1)) s[e] = -INFINITY;
-        }
-        uint32_t any = 0;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int dt = 0; dt < 2; ++dt) {
-            const u32x4 x = __builtin_bit_cast(u32x4, va[u][dt]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) any |= (x[j] & 0x7f807f80u) + 0x00800080u;
-          }
-        if (__builtin_amdgcn_ballot_w64((any & 0x80008000u) != 0) != 0) {
-          // their weight in a row that does not see them is 0, but 0 times them is
-          // not: they leave the product, and are added to the rows that see them below
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              bool bad = false;
-#pragma unroll
-              for (int dt = 0; dt < 2; ++dt) {
-                const float x = (float)va[u][dt][j];
-                const bool b = !(fabsf(x) < INFINITY);
-                if (b) va[u][dt][j] = (__bf16)0.f;
-                bad |= b;
-              }
-              const unsigned long long who = __builtin_amdgcn_ballot_w64(bad);
-              const int k = 16 * u + (j >> 2) * 8 + (j & 3);
-              odd |= ((uint32_t)who != 0) << k | ((who >> 32) != 0) << (k + 4);
-            }
         }
       }
       bf16x8 pb[2];
@@ -1218,23 +1307,6 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
 #pragma unroll
         for (int dt = 0; dt < 2; ++dt)
           o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[u][dt], pb[u], o[dt], 0, 0, 0);
-      while (odd) {  // (wave-uniform)
-        const int k = __builtin_ctz(odd);
-        odd &= odd - 1;
-        float pk = 0.f;  // this lane's weight of key k, if it is one of its 16
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pk = (e >> 2) * 8 + (e & 3) == (k & ~4) ? (float)pb[e >> 3][e & 7] : pk;
-        pk = __shfl(pk, r32 + 32 * (k >> 2 & 1), 64);
-        if (kb + k < limit && (pages >> (k >> 3) & 1)) {
-#pragma unroll
-          for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float x = bf16_to_f32(vl[k * VP + 32 * dt + (e >> 2) * 8 + hf * 4 + (e & 3)]);
-              if (!(fabsf(x) < INFINITY)) o[dt][e] = fmaf(pk, x, o[dt][e]);
-            }
-        }
-      }
     }
     if constexpr (NB > 1) {
       lstore(i + 1);
@@ -1248,12 +1320,25 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
     red_m[wave][r32] = mcv;
     red_l[wave][r32] = l;
   }
+  if (lane == 0) lds.odd[wave] = any_odd;
   __syncthreads();
+  any_odd = false;
+#pragma unroll
+  for (int v = 0; v < W; ++v) any_odd |= lds.odd[v] != 0;
   float *const ot = (float *)smem;
   float M = red_m[hw][r32];
 #pragma unroll
   for (int v = 1; v < KW; ++v) M = fmaxf(M, red_m[v * HW + hw][r32]);
   const float f = mcv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mcv - M);
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dt][i] *= f;
+  if (any_odd && kw == 0) {
+    const int limits[1] = {limit};
+    add_odd<bf16_t>(keys, rows, Vg, max(32 * keys.t0, keys.whole & -32), min(32 * keys.t1, keys.end), ow, limits,
+                    [&](int i) { return 32 * (i >> 4) + 8 * (i >> 2 & 3) + 4 * hf + (i & 3); });
+  }
   {
     float *dst = ot + wave * OT + r32 * OP + 4 * hf;
 #pragma unroll
@@ -1261,12 +1346,12 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
 #pragma unroll
       for (int gi = 0; gi < 4; ++gi)
         *(float4 *)(dst + 32 * dt + 8 * gi) =
-            make_float4(o[dt][4 * gi] * f, o[dt][4 * gi + 1] * f, o[dt][4 * gi + 2] * f, o[dt][4 * gi + 3] * f);
+            make_float4(o[dt][4 * gi], o[dt][4 * gi + 1], o[dt][4 * gi + 2], o[dt][4 * gi + 3]);
   }
   __syncthreads();
   constexpr int NV = R / W;  // = 64 elements over the row's threads
   static_assert(NV * (64 * W / R) == HD, "a row's threads cover it");
-  finish_piece<bf16_t, R, 64 * W>(p, w, &lds.last_in, [&](int row, int d0, float (&acc)[NV]) __attribute__((always_inline)) {
+  finish_piece<bf16_t, R, 64 * W>(p, lds.piece, &lds.last_in, [&](int row, int d0, float (&acc)[NV]) __attribute__((always_inline)) {
     const int hu = row / 32, r = row % 32;
     float Mr = red_m[hu][r];
 #pragma unroll
@@ -1293,6 +1378,413 @@ __global__ __launch_bounds__(64 * HW * KW, OCC) void paged_prefill_bf16_kernel(P
   prefill_bf16_body<HW, KW>(p, lds, blockIdx.x);
 }
 
+// bf16, calls of many rows: 256 rows a unit, two 32-row tiles a wave, so that
+// every fragment read from LDS feeds two products, and a software pipeline over
+// 32-key tiles: step t issues O += V^T P of tile t - 1 and the scores of tile
+// t + 1 on the matrix cores among the exponentials of tile t.  Blocks of 64
+// keys in two-deep K and V rings, one barrier a block.  A tile's row sums (from
+// the matrix cores) are looked at one step later, when they are long there; only
+// if one passes 2^16 does the tile run again from its scores, still at hand,
+// against the true maximum.  Tiles that every row of the workgroup sees whole
+// run a step without mask code.
+constexpr int kBK = 64;  // keys of a block
+constexpr int kPipeR = 256;
+struct PipeLds {
+  static constexpr int KP = HD + 8;   // 144 B: conflict-free b128 fragment reads
+  static constexpr int VP = HD + 32;  // 192 B: transpose reads of 8 rows x 64 B in two passes
+  static constexpr int KBUF = kBK * KP, VBUF = kBK * VP;
+  bf16_t k[2 * KBUF], v[2 * VBUF];
+  unsigned char __attribute__((aligned(8))) chunk_ok[4][8];  // block (mod 4): its chunks of 8 rows that have memory
+  int limit[kPipeR];  // keys that the rows see
+  Piece piece;
+  int odd[4], last_in;
+};
+__global__ __launch_bounds__(256, 2) void paged_prefill_pipe_kernel(PrefillParams p) {
+  constexpr int RT = 2, R = kPipeR, KP = PipeLds::KP, VP = PipeLds::VP, KBUF = PipeLds::KBUF, VBUF = PipeLds::VBUF;
+  __shared__ __attribute__((aligned(16))) PipeLds lds;
+  bf16_t *const kring = lds.k, *const vring = lds.v;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, hf = lane >> 5;
+  Piece w;
+  if (!find_piece<R>(p, blockIdx.x, w)) return;
+  if (tid == 0) lds.piece = w;
+  const Paged &c = p.a.c;
+  const float cl = p.a.cl;
+  const PieceKeys keys = piece_keys<R>(p, w);  // (its t0, t1 are not used: blocks)
+  const int end = keys.end;
+  const int nb = (end + kBK - 1) / kBK;
+  int blk0, nblk;
+  part_of(nb, w, blk0, nblk);
+  nblk -= blk0;
+  const int first = blk0 * kBK;  // the piece's keys and tiles are counted from here
+
+  // the first block with a page without memory (from it on, steps with masks)
+  int gap = nblk + 1;
+  for (int key = (first & -(1 << c.shift)) + (lane << c.shift); key < min(first + kBK * (nblk + 1), end); key += 64 << c.shift)
+    if ((unsigned)keys.entry(key) >= (unsigned)c.n_pages) gap = min(gap, (key - first) / kBK);
+  gap = max(wave_min(gap), 0);
+
+  // this lane's rows: Q^T operands, and the keys that they see
+  bf16x8 qreg[RT][4];
+  int most = 0, least = 0x7fffffff;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    int head;
+    const int tok = token_of(w, p.a.inv_group, p.a.group, 32 * (RT * wave + rt) + r32, head);
+    const bool there = tok < w.rows;
+    const int limit = there ? key_limit(p, w, tok) - first : 0;
+    lds.limit[32 * (RT * wave + rt) + r32] = limit;  // (the steps with masks read them there)
+    most = max(most, limit);
+    if (there) least = min(least, limit);
+    const bf16_t *const qp = (const bf16_t *)p.a.q + (int64_t)(w.row0 + (there ? tok : 0)) * p.a.q_rs +
+                             (w.g * p.a.group + (there ? head : 0)) * HD + 8 * hf;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      qreg[rt][t] = *(const bf16x8 *)(qp + 16 * t);
+      if (!there) qreg[rt][t] = bf16x8{};
+    }
+  }
+  least = wave_min(least);
+  if (least == 0x7fffffff) least = 0;  // no row
+  const int ntw = min((-wave_min(-most) + 31) >> 5, 2 * nblk);  // tiles that the wave's rows see
+
+  // staging: 2 x 16 B per thread of a K block and of a V block, rows crow and
+  // crow + 32: a wave's are the block's chunks `wave` and `wave + 4`
+  const int crow = tid >> 3, ccol = (tid & 7) * 8;
+  const PageRows rows = PageRows::of<bf16_t>(c);
+  const uint32_t off = (lane >> 3) * rows.row_bytes + ccol * 2;
+  const char *const Kg = (const char *)((const bf16_t *)c.k + w.g * c.head_stride);
+  const char *const Vg = (const char *)((const bf16_t *)c.v + w.g * c.head_stride);
+  u32x4 k0, k1, v0, v1;
+  bool any_odd = false;
+  int k_ok = 0, v_ok = 0;  // bit 0, 1: the chunk in k0 / k1 has memory, in v0 / v1
+  // lanes 0 and 1: the table entries of the wave's chunks of a block
+  auto entry_of = [&](int blk) __attribute__((always_inline)) {
+    return keys.entry(first + kBK * blk + 8 * wave + 32 * (lane & 1));
+  };
+  int e_k = 0;             // of the K block to load next
+  int id0 = 0, id1 = 0;    // of the K block loaded last
+  // K block blk, whose entries stand in e_k
+  auto gload_k = [&](int blk) __attribute__((always_inline)) {
+    uint32_t o32 = off;
+    asm volatile("" : "+v"(o32));  // a scalar base and this offset, not a sum of pointers kept in registers
+    id0 = __builtin_amdgcn_readlane(e_k, 0);
+    id1 = __builtin_amdgcn_readlane(e_k, 1);
+    const int key = first + kBK * blk + 8 * wave;
+    k_ok = rows.there(id0) | rows.there(id1) << 1;
+    k0 = *(const u32x4 *)(Kg + rows.at(id0, key) + o32);
+    k1 = *(const u32x4 *)(Kg + rows.at(id1, key + 32) + o32);
+  };
+  // V block blk, the K block loaded last
+  auto gload_v = [&](int blk) __attribute__((always_inline)) {
+    uint32_t o32 = off;
+    asm volatile("" : "+v"(o32));
+    const int key = first + kBK * blk + 8 * wave;
+    v_ok = rows.there(id0) | rows.there(id1) << 1;
+    v0 = *(const u32x4 *)(Vg + rows.at(id0, key) + o32);
+    v1 = *(const u32x4 *)(Vg + rows.at(id1, key + 32) + o32);
+  };
+  auto lstore_k = [&](int blk) __attribute__((always_inline)) {
+    bf16_t *ks = kring + (blk & 1) * KBUF;
+    *(u32x4 *)(ks + crow * KP + ccol) = k0;
+    *(u32x4 *)(ks + (crow + 32) * KP + ccol) = k1;
+    if (lane < 2) lds.chunk_ok[blk & 3][wave + 4 * lane] = (unsigned char)(k_ok >> lane & 1);
+  };
+  auto lstore_v = [&](int blk) __attribute__((always_inline)) {
+    bf16_t *vs = vring + (blk & 1) * VBUF;
+    if (first + kBK * (blk + 1) > end || v_ok != 3) {  // no key: zeros, whatever lies there
+      const int key = first + kBK * blk + crow;
+      if (!(v_ok & 1) || key >= end) v0 = u32x4{0, 0, 0, 0};
+      if (!(v_ok & 2) || key + 32 >= end) v1 = u32x4{0, 0, 0, 0};
+    }
+    if (first + kBK * (blk + 1) > keys.whole) {
+      const bool odd0 = tame<bf16_t>(v0), odd1 = tame<bf16_t>(v1);
+      any_odd |= __builtin_amdgcn_ballot_w64(odd0 || odd1) != 0;
+    }
+    *(u32x4 *)(vs + crow * VP + ccol) = v0;
+    *(u32x4 *)(vs + (crow + 32) * VP + ccol) = v1;
+  };
+
+  float l[RT], mcv[RT];  // row sum; reference, log2 units
+  f32x16 o[RT][2];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    mcv[rt] = -INFINITY;
+    l[rt] = 0.f;
+    o[rt][0] = f32x16{};
+    o[rt][1] = f32x16{};
+  }
+  const uint32_t rs_bits = (((lane & 15) >> 2) & 1) == ((lane >> 4) & 1) ? 0x3f803f80u : 0u;
+  const int tr_off = (4 * hf + ((lane & 15) >> 2)) * VP + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+
+  auto kfrags = [&](const bf16_t *ks, bf16x8 (&ka)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) ka[t] = *(const bf16x8 *)(ks + r32 * KP + 16 * t + 8 * hf);
+  };
+  // V^T fragments: key slot j of 16-key chunk u is key 16u + (j/4)*8 + 4hf + j%4
+  auto vfrags = [&](const bf16_t *vs, bf16x8 (&va)[2][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bf16_t *vsl = vs + 16 * u * VP + tr_off;
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt) {
+        const bf16x4 lo = lds_tr16(vsl + 32 * dt);
+        const bf16x4 hi = lds_tr16(vsl + 8 * VP + 32 * dt);
+        va[u][dt] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      }
+    }
+  };
+  auto scores = [&](const bf16x8 (&ka)[4], f32x16 (&s)[RT]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      s[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[0], qreg[rt][0], f32x16{}, 0, 0, 0);
+#pragma unroll
+      for (int t = 1; t < 4; ++t) s[rt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[t], qreg[rt][t], s[rt], 0, 0, 0);
+    }
+  };
+  auto pv = [&](const bf16x8 (&va)[2][2], const bf16x8 (&pb)[RT][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          o[rt][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[u][dt], pb[rt][u], o[rt][dt], 0, 0, 0);
+  };
+  auto exps = [&](const f32x16 &s, float mc, bf16x8 (&pb)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pb[u][j] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[8 * u + j], cl, -mc));
+  };
+  auto rowsum = [&](const bf16x8 (&pb)[2]) __attribute__((always_inline)) {
+    uint32_t b = rs_bits;
+    asm volatile("" : "+v"(b));  // keeps the selector from being hoisted out of the loop
+    const bf16x8 sel = __builtin_bit_cast(bf16x8, u32x4{b, b, b, b});
+    f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sel, pb[0], f32x4{}, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(sel, pb[1], d, 0, 0, 0)[0];
+  };
+  // bit r: rows 8r .. of tile t have memory
+  auto pages_of = [&](int t) __attribute__((always_inline)) {
+    const uint32_t ok =
+        __builtin_amdgcn_readfirstlane(*(const uint32_t *)&lds.chunk_ok[(t >> 1) & 3][4 * (t & 1)]);
+    return (ok & 1) | (ok >> 7 & 2) | (ok >> 14 & 4) | (ok >> 21 & 8);
+  };
+  auto mask = [&](int t, uint32_t pages, f32x16 (&sc)[RT]) __attribute__((always_inline)) {
+    const int kb = 32 * t;
+    if (kb + 32 > least || pages != 15) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int limit = lds.limit[32 * (RT * wave + rt) + r32] - kb - 4 * hf;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if ((i >> 2) * 8 + (i & 3) >= limit || !(pages >> (i >> 2) & 1)) sc[rt][i] = -INFINITY;
+      }
+    }
+  };
+  auto fixup = [&](int rt, const f32x16 &s, bf16x8 (&pb)[2], float &rs) __attribute__((always_inline)) {
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mt = fmaxf(mcv[rt], mx * cl);  // -inf while nothing is visible
+    const bool move = mcv[rt] == -INFINITY || mt - mcv[rt] > kMoveLog2;
+    const float m_new = move ? mt : mcv[rt];
+    const float mn = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(mcv[rt] - mn);
+    l[rt] *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[rt][dt][i] *= alpha;
+    mcv[rt] = m_new;
+    exps(s, mn, pb);
+    rs = rowsum(pb);
+  };
+  auto step = [&](auto masked_tag, int t, const bf16_t *vs, const bf16_t *ks, f32x16 (&sc)[RT], f32x16 (&sn)[RT],
+                  bf16x8 (&pp)[RT][2], bf16x8 (&pc)[RT][2], float (&rsp)[RT], float (&rsc)[RT])
+      __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
+    {
+      bool bad = false;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) bad = bad || !(rsp[rt] <= kSumLimit);  // NaN included
+      if (__builtin_amdgcn_ballot_w64(bad) != 0) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) fixup(rt, sn[rt], pp[rt], rsp[rt]);
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) l[rt] += rsp[rt];
+    }
+    if (!MASKED) {
+    } else if (t >= ntw) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[rt][i] = -INFINITY;
+    } else {
+      mask(t, pages_of(t), sc);
+    }
+    bf16x8 va[2][2], ka[4];
+    vfrags(vs, va);
+    kfrags(ks, ka);
+    pv(va, pp);
+    scores(ka, sn);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) exps(sc[rt], mcv[rt], pc[rt]);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) rsc[rt] = rowsum(pc[rt]);
+    __builtin_amdgcn_sched_group_barrier(0x100, 12, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+#pragma unroll
+    for (int i = 0; i < 10 * RT; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+    }
+  };
+
+  f32x16 sa[RT], sb[RT];
+  bf16x8 pa[RT][2], pbb[RT][2];
+  float rsa[RT], rsb[RT];
+  if (nblk > 0) {
+    // entries of the first three blocks in one load, then their rows in one round trip
+    const int e = keys.entry(first + kBK * (lane >> 1) + 8 * wave + 32 * (lane & 1));
+    e_k = e;
+    gload_k(0);
+    gload_v(0);
+    const u32x4 ka = k0, kb = k1, va = v0, vb = v1;
+    const int ok0 = k_ok;
+    e_k = __shfl(e, 2 + (lane & 1), 64);
+    gload_k(1);
+    gload_v(1);
+    const u32x4 kc = k0, kd = k1, vc = v0, vd = v1;
+    const int ok1 = k_ok;
+    e_k = __shfl(e, 4 + (lane & 1), 64);
+    gload_k(2);
+    const u32x4 ke = k0, kf = k1;
+    const int ok2 = k_ok;
+    e_k = entry_of(3);
+    k0 = ka; k1 = kb; v0 = va; v1 = vb;
+    k_ok = v_ok = ok0;
+    lstore_k(0);
+    lstore_v(0);
+    k0 = kc; k1 = kd; v0 = vc; v1 = vd;
+    k_ok = v_ok = ok1;
+    lstore_k(1);
+    k0 = ke; k1 = kf;
+    k_ok = ok2;
+  }
+  __syncthreads();
+  if (nblk > 0) {  // step 0: scores of tiles 0 and 1, softmax of tile 0 against its true maximum
+    bf16x8 ka[4];
+    kfrags(kring, ka);
+    scores(ka, sa);
+    kfrags(kring + 32 * KP, ka);
+    scores(ka, sb);
+    mask(0, pages_of(0), sa);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) fixup(rt, sa[rt], pa[rt], rsa[rt]);
+  }
+  __syncthreads();  // iteration 0 stores K_2 where step 0 read K_0
+  // iteration j: steps 2j+1 and 2j+2, which read only V_j and K_{j+1}; it
+  // stores K_{j+2} and V_{j+1} where K_j and V_{j-1} were, last read one
+  // iteration before: one barrier a block
+  const int t_safe = min(least, kBK * nblk) >> 5;
+  const int j_safe = min(min(nblk, max(0, (t_safe - 1) / 2)), max(gap - 1, 0));
+  auto iteration = [&](auto masked_tag, int j) __attribute__((always_inline)) {
+    const bf16_t *vc = vring + (j & 1) * VBUF;
+    const bf16_t *kn = kring + ((j + 1) & 1) * KBUF;
+    step(masked_tag, 2 * j + 1, vc, kn, sb, sa, pa, pbb, rsa, rsb);
+    step(masked_tag, 2 * j + 2, vc + 32 * VP, kn + 32 * KP, sa, sb, pbb, pa, rsb, rsa);
+    lstore_k(j + 2);
+    lstore_v(j + 1);
+    gload_v(j + 2);
+    gload_k(j + 3);  // (past the end: the last key's page again)
+    e_k = entry_of(j + 4);
+    __syncthreads();
+  };
+  int j = 0;
+  for (; j < j_safe; ++j) iteration(std::false_type{}, j);
+  for (; j < nblk; ++j) iteration(std::true_type{}, j);
+
+  if (lane == 0) lds.odd[wave] = any_odd;
+  __syncthreads();
+  if (lds.odd[0] | lds.odd[1] | lds.odd[2] | lds.odd[3]) {
+    const int *const limit = lds.limit + 32 * RT * wave + r32;
+    const int limits[RT] = {limit[0] + first, limit[32] + first};
+    add_odd<bf16_t>(keys, rows, Vg, max(first, keys.whole & -kBK), min(first + kBK * nblk, end), o, limits,
+                    [&](int i) { return 32 * (i >> 4) + 8 * (i >> 2 & 3) + 4 * hf + (i & 3); });
+  }
+  // ---- results: lane holds row (rt, r32)'s elements 32 dt + 8 gi + 4 hf .. +3
+  const Piece f = lds.piece;
+  auto write = [&](int t, int h, int rt, float sum) __attribute__((always_inline)) {
+    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+    bf16_t *const op = (bf16_t *)p.a.o + (int64_t)(f.row0 + t) * p.a.o_rs + h * HD;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int gi = 0; gi < 4; ++gi) {
+        const f32x16 &x = o[rt][dt];
+        const uint32_t lo = (uint32_t)f32_to_bf16(x[4 * gi] * inv) | ((uint32_t)f32_to_bf16(x[4 * gi + 1] * inv) << 16);
+        const uint32_t hi = (uint32_t)f32_to_bf16(x[4 * gi + 2] * inv) | ((uint32_t)f32_to_bf16(x[4 * gi + 3] * inv) << 16);
+        *(uint2 *)(op + 32 * dt + 8 * gi + 4 * hf) = make_uint2(lo, hi);
+      }
+  };
+  const int64_t rec_step = (int64_t)c.n_kv_heads * R * kRec;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    int h;
+    const int row = 32 * (RT * wave + rt) + r32, t = token_of(f, p.a.inv_group, p.a.group, row, h);
+    if (t >= f.rows) continue;
+    h += f.g * p.a.group;
+    if (f.parts == 1) {
+      write(t, h, rt, l[rt]);
+    } else {
+      float *const r = p.ws + ((int64_t)f.slot * R + row) * kRec + f.part * rec_step;
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) put2(r + 32 * dt + 8 * (i >> 2) + 4 * hf + (i & 3), o[rt][dt][i], o[rt][dt][i + 1]);
+      if (hf == 0) put2(r + HD, mcv[rt], l[rt]);
+    }
+  }
+  if (f.parts == 1) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the records have reached memory
+  __syncthreads();
+  if (tid == 0) lds.last_in = arrive_last(p.arrive_end - 2 * ((int64_t)f.slot + 1), f.parts, p.tag);
+  __syncthreads();
+  if (!lds.last_in) return;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    int h;
+    const int row = 32 * (RT * wave + rt) + r32, t = token_of(f, p.a.inv_group, p.a.group, row, h);
+    if (t >= f.rows) continue;
+    h += f.g * p.a.group;
+    const float *const r0 = p.ws + ((int64_t)f.slot * R + row) * kRec;
+    float M = -INFINITY, L = 0.f;
+    o[rt][0] = o[rt][1] = f32x16{};
+    for (int n = 0; n < f.parts; ++n) {
+      const float *const r = r0 + n * rec_step;
+      const float2 ml = get2(r + HD);
+      float2 x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = get2(r + 32 * (i >> 3) + 8 * ((i >> 1) & 3) + 4 * hf + 2 * (i & 1));
+      const float mn = fmaxf(M, ml.x), mu = mn == -INFINITY ? 0.f : mn;
+      const float fo = __builtin_amdgcn_exp2f(M - mu), fn = __builtin_amdgcn_exp2f(ml.x - mu);
+      L = fmaf(ml.y, fn, L * fo);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        o[rt][i >> 3][2 * (i & 7)] = fmaf(x[i].x, fn, o[rt][i >> 3][2 * (i & 7)] * fo);
+        o[rt][i >> 3][2 * (i & 7) + 1] = fmaf(x[i].y, fn, o[rt][i >> 3][2 * (i & 7) + 1] * fo);
+      }
+      M = mn;
+    }
+    write(t, h, rt, L);
+  }
+}
+
 // fp32, v_mfma_f32_32x32x2f32: matrix-core time is all that counts.  32 rows a
 // unit, its tiles dealt to KW waves, no barrier before the merge: a wave
 // stages its own K tile in LDS one tile ahead (rows of 272 B) and reads V
@@ -1302,6 +1794,8 @@ template <int KW>
 struct PrefillLdsF32 {
   float smem[KW * 32 * (HD + 4)];
   float red_m[KW][32], red_l[KW][32];
+  int odd[KW];
+  Piece piece;
   int last_in;
 };
 template <int KW>
@@ -1316,39 +1810,36 @@ __device__ __forceinline__ void prefill_f32_body(const PrefillParams &p, Prefill
   const int r32 = lane & 31, hf = lane >> 5;
   Piece w;
   if (!find_piece<R>(p, block, w)) return;
+  if (tid == 0) lds.piece = w;
   const Paged &c = p.a.c;
   const PieceKeys keys = piece_keys<R>(p, w);
   const float cl = p.a.cl;
   float *const kl = smem + kw * TILE;
-  const int fr = w.unit * R + r32, tok = fr / p.a.group, head = fr - tok * p.a.group;
+  int head;
+  const int tok = token_of(w, p.a.inv_group, p.a.group, r32, head);
   const bool there = tok < w.rows;
   const int limit = there ? key_limit(p, w, tok) : 0;
-  const int all_see = wave_min(there ? limit : 0x7fffffff);
 
-  const int slot_mask = (1 << c.shift) - 1;
-  const int64_t page_bytes = c.page_stride * 4;
-  const uint32_t row_bytes = (uint32_t)c.row_stride * 4;
+  const PageRows rows = PageRows::of<float>(c);
+  const uint32_t row_bytes = rows.row_bytes;
   const uint32_t koff = (lane >> 4) * row_bytes + (lane & 15) * 16;  // 4 rows of 256 bytes a load
   const uint32_t voff = 4 * hf * row_bytes + r32 * 8;
   const char *const Kg = (const char *)((const float *)c.k + w.g * c.head_stride);
   const char *const Vg = (const char *)((const float *)c.v + w.g * c.head_stride);
   u32x4 kr[8];
-  int ids[4];
-  int64_t at[4], vat[4];  // byte offsets of rows 8r .. of the tile to load next, of this tile
+  int entry = 0;  // lane r (mod 4): of rows 8r .. of the tile to load next
+  uint64_t at[4], vat[4];  // byte offsets of rows 8r .. of the tile to load next, of this tile
   int pages = 0, pages_next = 0;
-  auto load_ids = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) ids[r] = keys.entry(32 * t + 8 * r);
-  };
+  auto load_ids = [&](int t) __attribute__((always_inline)) { entry = keys.entry(32 * t + 8 * (lane & 3)); };
   auto gload_k = [&](int t) __attribute__((always_inline)) {
     pages_next = 0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const bool ok = (unsigned)ids[r] < (unsigned)c.n_pages;
-      pages_next |= ok << r;
-      at[r] = (ok ? ids[r] : 0) * page_bytes + (int64_t)((uint64_t)(uint32_t)((32 * t + 8 * r) & slot_mask) * row_bytes);
+      const int id = __builtin_amdgcn_readlane(entry, r);
+      pages_next |= rows.there(id) << r;
+      at[r] = rows.at(id, 32 * t + 8 * r);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) kr[2 * r + j] = *(const u32x4 *)(Kg + at[r] + (int64_t)j * 4 * row_bytes + koff);
+      for (int j = 0; j < 2; ++j) kr[2 * r + j] = *(const u32x4 *)(Kg + at[r] + (uint64_t)(j * 4u) * row_bytes + koff);
     }
   };
   float qreg[32];  // k slot (hf, t) of the score product is d = 32 hf + t
@@ -1362,7 +1853,9 @@ __device__ __forceinline__ void prefill_f32_body(const PrefillParams &p, Prefill
     }
   }
   float mc = -INFINITY, l = 0.f;
-  f32x16 o[2] = {f32x16{}, f32x16{}};  // o[j] row i is d = 2i + j
+  f32x16 ow[1][2] = {{f32x16{}, f32x16{}}};  // ow[0][j] row i is d = 2i + j
+  f32x16 (&o)[2] = ow[0];
+  bool any_odd = false;
   int t = keys.t0 + kw;
   if (t < keys.t1) {
     load_ids(t);
@@ -1382,7 +1875,7 @@ __device__ __forceinline__ void prefill_f32_body(const PrefillParams &p, Prefill
     float2 vr[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      vr[i] = *(const float2 *)(Vg + vat[i >> 2] + (int64_t)(i & 3) * row_bytes + voff);
+      vr[i] = *(const float2 *)(Vg + vat[i >> 2] + (uint64_t)(i & 3u) * row_bytes + voff);
     gload_k(t + KW);  // past the range: the last key's page again, not used
     load_ids(t + 2 * KW);
     f32x16 s = f32x16{};
@@ -1396,8 +1889,8 @@ __device__ __forceinline__ void prefill_f32_body(const PrefillParams &p, Prefill
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, qreg[u + 3], s, 0, 0, 0);
     }
     const int kb = 32 * t;
-    uint32_t odd = 0;  // as in the bf16 kernel
-    if (kb + 32 > all_see || pages != 15) {
+    if (kb + 32 > keys.whole || pages != 15) {
+      bool odd = false;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int k = (i >> 2) * 8 + hf * 4 + (i & 3);
@@ -1405,14 +1898,10 @@ __device__ __forceinline__ void prefill_f32_body(const PrefillParams &p, Prefill
         if (kb + k >= limit || !page) s[i] = -INFINITY;
         if (kb + k >= keys.end || !page) vr[i] = make_float2(0.f, 0.f);  // no key: whatever lies there
         const bool bx = !(fabsf(vr[i].x) < INFINITY), by = !(fabsf(vr[i].y) < INFINITY);
-        const unsigned long long who = __builtin_amdgcn_ballot_w64(bx || by);
-        if (who) {
-          if (bx) vr[i].x = 0.f;
-          if (by) vr[i].y = 0.f;
-          const int k0 = (i >> 2) * 8 + (i & 3);
-          odd |= ((uint32_t)who != 0) << k0 | ((who >> 32) != 0) << (k0 + 4);
-        }
+        vr[i] = make_float2(bx ? 0.f : vr[i].x, by ? 0.f : vr[i].y);
+        odd |= bx || by;
       }
+      any_odd |= __builtin_amdgcn_ballot_w64(odd) != 0;
     }
     float mx = s[0];
 #pragma unroll
@@ -1438,25 +1927,6 @@ __device__ __forceinline__ void prefill_f32_body(const PrefillParams &p, Prefill
       o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[i].x, s[i], o[0], 0, 0, 0);
       o[1] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[i].y, s[i], o[1], 0, 0, 0);
     }
-    while (odd) {  // (wave-uniform)
-      const int k = __builtin_ctz(odd);
-      odd &= odd - 1;
-      float pk = 0.f;
-      int64_t a = 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) pk = (i >> 2) * 8 + (i & 3) == (k & ~4) ? s[i] : pk;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) a = r == k >> 3 ? vat[r] : a;
-      pk = __shfl(pk, r32 + 32 * (k >> 2 & 1), 64);
-      if (kb + k < limit && (pages >> (k >> 3) & 1)) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 x = *(const float2 *)(Vg + a + (int64_t)(k & 7) * row_bytes + 8 * ((i >> 2) * 8 + hf * 4 + (i & 3)));
-          if (!(fabsf(x.x) < INFINITY)) o[0][i] = fmaf(pk, x.x, o[0][i]);
-          if (!(fabsf(x.y) < INFINITY)) o[1][i] = fmaf(pk, x.y, o[1][i]);
-        }
-      }
-    }
   }
 
   l += __shfl_xor(l, 32, 64);
@@ -1464,21 +1934,33 @@ __device__ __forceinline__ void prefill_f32_body(const PrefillParams &p, Prefill
     red_m[kw][r32] = mc;
     red_l[kw][r32] = l;
   }
+  if (lane == 0) lds.odd[kw] = any_odd;
   __syncthreads();
+  any_odd = false;
+#pragma unroll
+  for (int v = 0; v < KW; ++v) any_odd |= lds.odd[v] != 0;
   float M = red_m[0][r32];
 #pragma unroll
   for (int v = 1; v < KW; ++v) M = fmaxf(M, red_m[v][r32]);
   const float f = mc == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - M);
 #pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[j][i] *= f;
+  if (any_odd && kw == 0) {
+    const int limits[1] = {limit};
+    add_odd<float>(keys, rows, Vg, max(32 * keys.t0, keys.whole & -32), min(32 * keys.t1, keys.end), ow, limits,
+                   [&](int i) { return 2 * (8 * (i >> 2 & 3) + 4 * hf + (i & 3)) + (i >> 4); });
+  }
+#pragma unroll
   for (int gi = 0; gi < 4; ++gi) {
     float *dst = kl + r32 * KP + 2 * (8 * gi + 4 * hf);
-    *(float4 *)dst = make_float4(o[0][4 * gi] * f, o[1][4 * gi] * f, o[0][4 * gi + 1] * f, o[1][4 * gi + 1] * f);
-    *(float4 *)(dst + 4) =
-        make_float4(o[0][4 * gi + 2] * f, o[1][4 * gi + 2] * f, o[0][4 * gi + 3] * f, o[1][4 * gi + 3] * f);
+    *(float4 *)dst = make_float4(o[0][4 * gi], o[1][4 * gi], o[0][4 * gi + 1], o[1][4 * gi + 1]);
+    *(float4 *)(dst + 4) = make_float4(o[0][4 * gi + 2], o[1][4 * gi + 2], o[0][4 * gi + 3], o[1][4 * gi + 3]);
   }
   __syncthreads();
   constexpr int NV = HD / (2 * KW);
-  finish_piece<float, R, 64 * KW>(p, w, &lds.last_in, [&](int row, int d0, float (&acc)[NV]) __attribute__((always_inline)) {
+  finish_piece<float, R, 64 * KW>(p, lds.piece, &lds.last_in, [&](int row, int d0, float (&acc)[NV]) __attribute__((always_inline)) {
     float Mr = red_m[0][row];
 #pragma unroll
     for (int v = 1; v < KW; ++v) Mr = fmaxf(Mr, red_m[v][row]);
@@ -1626,8 +2108,10 @@ int check_cache(const std::string &op, const bn_paged_kv *kv, Paged *c) {
   if (kv->batch > (1 << 20)) return fail(BN_ERR_UNSUPPORTED, op + ": more than 2^20 sequences");
   if (kv->batch * keys > ((int64_t)1 << 34))  // tiles of 16 keys are counted in 32 bits
     return fail(BN_ERR_UNSUPPORTED, op + ": batch * max_pages * page_size must be at most 2^34 keys");
-  if (kv->row_stride > (1 << 24))  // (a load's rows are reached through 32-bit byte offsets)
-    return fail(BN_ERR_UNSUPPORTED, op + ": cache row stride must be at most 2^24 elements");
+  // (a load's rows are reached through 32-bit byte offsets, pages by 32 x 32-bit products)
+  if (kv->row_stride > (1 << 24) || kv->page_stride >= (1 << 30))
+    return fail(BN_ERR_UNSUPPORTED,
+                op + ": cache row stride must be at most 2^24 elements, page stride below 2^30");
   const int64_t vec = kv->dtype == BN_BF16 ? 8 : 4, most = (int64_t)1 << 40;
   for (int64_t s : {kv->page_stride, kv->head_stride, kv->row_stride})
     if (s < HD || s % vec || s > most)
@@ -1782,7 +2266,7 @@ int launch_decode(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
 // Which prefill kernel: by the units of 128 rows (32 in fp32) that the call has
 // at most.  Few of them: the keys of a unit are split over more waves.
 struct PrefillPlan {
-  int hw, kw;
+  int hw, kw;  // (hw 8: the pipelined kernel)
   int64_t groups, slots;   // workgroups of the launch, records
   size_t records, words;   // bytes
 };
@@ -1796,6 +2280,9 @@ PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv
   } else if (u128 < 256) {
     d.hw = 1;
     d.kw = u32 <= 256 ? 8 : 4;
+  } else if (u128 >= 2048) {
+    d.hw = 8;
+    d.kw = 1;
   } else {
     d.hw = 4;
     d.kw = u128 <= 768 ? 2 : 1;
@@ -1830,6 +2317,8 @@ int launch_prefill(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
   if (dtype == BN_F32) {
     if (d.kw == 4) hipLaunchKernelGGL(paged_prefill_f32_kernel<4>, grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL(paged_prefill_f32_kernel<2>, grid, dim3(128), 0, s, p);
+  } else if (d.hw == 8) {
+    hipLaunchKernelGGL(paged_prefill_pipe_kernel, grid, dim3(256), 0, s, p);
   } else if (d.hw == 4) {
     if (d.kw == 2) hipLaunchKernelGGL((paged_prefill_bf16_kernel<4, 2, 4>), grid, dim3(512), 0, s, p);
     else hipLaunchKernelGGL((paged_prefill_bf16_kernel<4, 1, 4>), grid, dim3(256), 0, s, p);
@@ -1927,6 +2416,7 @@ int attention(const char *name, const bn_paged_kv *kv, const void *q, void *o, c
   p.q = q; p.o = o; p.starts = starts;
   p.q_rs = q_rs; p.o_rs = o_rs;
   p.n_rows = n_rows; p.n_heads = n_heads; p.group = n_heads / kv->n_kv_heads;
+  p.inv_group = 1.0f / (float)p.group;
   p.cl = scale * kLog2e;
   p.prefix_pages = prefix_pages; p.prefix_len = std::min(prefix_len, p.c.cap);
   Workspace ws;

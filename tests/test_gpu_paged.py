@@ -308,6 +308,9 @@ def test_prefill(case):
 LARGE = [
     ("bf16", [700, 433, 400], [700, 33, 400], 4, 32, 16),
     ("bf16", [1500, 40, 2100, 900], [1500, 33, 1100, 767], 4, 32, 32),
+    ("bf16", [2500, 40, 2800, 3900], [2500, 33, 1100, 1767], 4, 32, 16),
+    ("bf16", [1200] * 6, [1200] * 6, 8, 24, 8),
+    ("bf16", [40000, 9000], [300, 8500], 4, 20, 32),
     ("bf16", [2900, 3300], [2500, 1001], 4, 20, 16),
     ("bf16", [9000, 3000, 70, 20000], [5, 64, 1, 3], 2, 16, 64),
     ("bf16", [16500, 6000], [300, 290], 4, 32, 64),
@@ -374,6 +377,31 @@ def test_prefill_hidden_values(dtype, what):
     check(got[sees][:, :, ~bad], ref[sees][:, :, ~bad], tol[sees][:, :, ~bad], "the other columns")
     assert not np.isfinite(got[sees][:, :, bad]).any()
     c.v = whole
+
+
+@pytest.mark.parametrize("dtype,Hkv,H,rows", [("f32", 2, 8, 500), ("bf16", 4, 32, 1100), ("bf16", 4, 32, 9000)])
+def test_prefill_hidden_values_large(dtype, Hkv, H, rows):
+    """The same in calls that the host gives to its other kernels: a value in the middle of the new
+    rows, in one column and one KV head."""
+    past, j = 70, 70 + rows // 2
+    c = Case(dtype, [past + rows], Hkv, 16, True, seed=8, nan=False)
+    q = rows_of(dtype, rows, H, 9).cuda()
+    st = torch.tensor([0, rows], dtype=torch.int32).cuda()
+    cache = c.cuda(B)
+    want = B.paged_prefill(q, cache, st, scale=0.125)
+    pg, sl = c.place(0, j)
+    old = c.vd[pg, 1, sl, 5].clone()
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        c.vd[pg, 1, sl, 5] = bad
+        got = B.paged_prefill(q, cache, st, scale=0.125)
+        G = H // Hkv
+        hit = torch.zeros(got.shape, dtype=torch.bool, device="cuda")
+        hit[j - past:, G:2 * G, 5] = True
+        assert not torch.isfinite(got[hit]).any()
+        if bad == bad:
+            assert (got[hit] == bad).all()
+        assert torch.equal(bits(got[~hit]), bits(want[~hit]))
+    c.vd[pg, 1, sl, 5] = old
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])

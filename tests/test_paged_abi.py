@@ -64,7 +64,7 @@ CALLS = {"Paged append": append, "Paged decode": decode, "Paged prefill": prefil
     (dict(row_stride=68), B.BN_ERR_INVALID_ARG, "strides"),
     (dict(head_stride=0), B.BN_ERR_INVALID_ARG, "strides"),
     (dict(page_stride=-4096), B.BN_ERR_INVALID_ARG, "strides"),
-    (dict(page_stride=(1 << 40) + 8), B.BN_ERR_INVALID_ARG, "strides"),
+    (dict(page_stride=1 << 30), B.BN_ERR_UNSUPPORTED, "2^30"),
     (dict(table_stride=7), B.BN_ERR_SHAPE, "overlap"),
     (dict(k=0), B.BN_ERR_INVALID_ARG, "NULL"),
     (dict(v=0), B.BN_ERR_INVALID_ARG, "NULL"),
