@@ -231,6 +231,16 @@ __device__ __forceinline__ int wave_scan(int x) {
   return dpp_add<0x143, 0xc>(x);  // row_bcast 31 to rows 2 and 3
 }
 
+// The lanes' smallest value.
+template <int CTRL>
+__device__ __forceinline__ int dpp_min(int x) {
+  return min(x, __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ int wave_min(int x) {
+  x = dpp_min<0x140>(dpp_min<0x141>(dpp_min<0x4E>(dpp_min<0xB1>(x))));  // within a row of 16
+  return min(min(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
+             min(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+}
 // The lanes' sum, the same in every wave.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ float dpp_addf(float x) {
@@ -838,8 +848,10 @@ __device__ __forceinline__ bool find_piece(const PrefillParams &p, int block, Pi
   int idx;
   if (hkv <= 8 && (8 % hkv) == 0) {
     const int x = block & 7;
+    int j = block >> 3;  // a compute unit that got a long piece of one round gets a short one of the next
+    if ((j & 32) && !p.prefix_parts) j = (j & ~31) + 31 - (j & 31);
     w.g = x % hkv;
-    idx = (block >> 3) * (8 / hkv) + x / hkv;
+    idx = j * (8 / hkv) + x / hkv;
   } else {
     w.g = block % hkv;
     idx = block / hkv;
@@ -891,28 +903,58 @@ __device__ __forceinline__ bool find_piece(const PrefillParams &p, int block, Pi
   for (int i = 1; i < per; ++i) count(seq(lane * per + i), lane * per + i < n, all, cut);
   int up = wave_scan(all), up_cut = wave_scan(cut);
   if (idx >= __builtin_amdgcn_readlane(up, 63)) return false;
-  int src = __builtin_ctzll(__builtin_amdgcn_ballot_w64(up > idx));
-  int before = __builtin_amdgcn_readlane(up - all, src), cuts = __builtin_amdgcn_readlane(up_cut - cut, src);
-  int b = src * per;
-  while (per > 1) {  // the sequence within the lane's run, 64 at a time
-    mine = seq(b + lane);
-    all = cut = 0;
-    count(mine, b + lane < n, all, cut);
-    up = wave_scan(all);
-    up_cut = wave_scan(cut);
-    const unsigned long long hit = __builtin_amdgcn_ballot_w64(before + up > idx);
-    if (hit) {
-      src = __builtin_ctzll(hit);
-      before += __builtin_amdgcn_readlane(up - all, src);
-      cuts += __builtin_amdgcn_readlane(up_cut - cut, src);
-      b += src;
-      break;
+  int src, b, k, cuts;  // lane and number of the sequence, piece of it, pieces of cut sequences before it
+  if (per == 1) {
+    // The longest first over all sequences: from one unit to the one before it
+    // the keys fall by the same R / group in every sequence, so that a sequence's
+    // units take a run of levels, one each, from the level of its longest on.
+    const int parts = parts_of(mine), units = lane < n ? mine.units : 0;
+    const int at = max(mine.last, -(1 << 29)), top = -wave_min(units ? -at : 1 << 29);
+    const int off = units ? (int)((float)(top - at) * ((float)G * (1.f / R))) : 0;
+    auto pieces_above = [&](int level) __attribute__((always_inline)) {
+      return __builtin_amdgcn_readlane(wave_scan(parts * min(max(level - off, 0), units)), 63);
+    };
+    int lo = 0, hi = -wave_min(-(off + units)), below = 0;  // pieces_above(lo) <= idx < pieces_above(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1, n_mid = pieces_above(mid);
+      if (n_mid <= idx) {
+        lo = mid;
+        below = n_mid;
+      } else {
+        hi = mid;
+      }
     }
-    before += __builtin_amdgcn_readlane(up, 63);
-    cuts += __builtin_amdgcn_readlane(up_cut, 63);
-    b += 64;
+    const int here = off <= lo && lo < off + units ? parts : 0, to = wave_scan(here);
+    src = __builtin_ctzll(__builtin_amdgcn_ballot_w64(to > idx - below));
+    b = src;
+    k = (lo - __builtin_amdgcn_readlane(off, src)) * __builtin_amdgcn_readlane(parts, src) + idx - below -
+        __builtin_amdgcn_readlane(to - here, src);
+    cuts = __builtin_amdgcn_readlane(up_cut - cut, src);
+  } else {
+    src = __builtin_ctzll(__builtin_amdgcn_ballot_w64(up > idx));
+    int before = __builtin_amdgcn_readlane(up - all, src);
+    cuts = __builtin_amdgcn_readlane(up_cut - cut, src);
+    b = src * per;
+    for (;;) {  // the sequence within the lane's run, 64 at a time
+      mine = seq(b + lane);
+      all = cut = 0;
+      count(mine, b + lane < n, all, cut);
+      up = wave_scan(all);
+      up_cut = wave_scan(cut);
+      const unsigned long long hit = __builtin_amdgcn_ballot_w64(before + up > idx);
+      if (hit) {
+        src = __builtin_ctzll(hit);
+        before += __builtin_amdgcn_readlane(up - all, src);
+        cuts += __builtin_amdgcn_readlane(up_cut - cut, src);
+        b += src;
+        break;
+      }
+      before += __builtin_amdgcn_readlane(up, 63);
+      cuts += __builtin_amdgcn_readlane(up_cut, 63);
+      b += 64;
+    }
+    k = idx - before;
   }
-  const int k = idx - before;
   w.b = b;
   w.row0 = __builtin_amdgcn_readlane(mine.row0, src);
   w.rows = __builtin_amdgcn_readlane(mine.rows, src);
@@ -968,12 +1010,6 @@ __device__ __forceinline__ int key_limit(const PrefillParams &p, const Piece &w,
   return p.prefix_parts ? min(max(p.a.c.lens[t], 0), p.a.prefix_len)
                         : min(max(w.last - w.rows + t + 1, 0), p.a.c.cap);
 }
-__device__ __forceinline__ int wave_min(int x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
-  return __builtin_amdgcn_readfirstlane(x);
-}
-
 // Infinite and NaN values of keys that not every row of a workgroup sees: a row
 // that does not see one weighs it with 0, and 0 times it is not 0.  They are
 // staged as zeros (tame), and if there were any, add_odd() puts each, as it
@@ -2297,7 +2333,9 @@ PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv
       most_parts > 1 ? std::min<int64_t>(units * most_parts, (2 * kPartsAll + kPartsAll / 8) / n_kv_heads + 2) : 0;
   const int64_t pieces = units + cut;
   const int per = n_kv_heads <= 8 && 8 % n_kv_heads == 0 ? 8 / n_kv_heads : 1;
-  d.groups = (pieces + per - 1) / per * per * n_kv_heads;
+  // (whole rounds of 32 pieces an XCD, which are taken in reverse order every second time)
+  d.groups = per > 1 || n_kv_heads == 8 || n_kv_heads == 1 ? ((pieces + per - 1) / per + 31) / 32 * 32 * per * n_kv_heads
+                                                           : pieces * n_kv_heads;
   d.slots = cut * n_kv_heads;
   d.records = (size_t)d.slots * R * kRec * sizeof(float);
   d.words = (size_t)d.slots * 16 * d.hw;  // (16 are used; a call of fewer rows, whose records are smaller, needs no more)
