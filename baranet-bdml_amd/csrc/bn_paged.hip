@@ -262,7 +262,11 @@ struct DecodeParams {
   unsigned long long *arrive_end;   // two arrival words per (sequence, column) below it
   unsigned long long tag;           // the launch's 48-bit tag
   int bins, hblocks, columns, k0;   // k0: keys below it are not this kernel's
-  float *parts;                     // not null: [batch][n_heads][kRec], instead of the output
+  // not null: nothing is added or written here.  A sequence that lies in one share leaves
+  // its record in parts [batch][n_heads][kRec], a cut one its pieces' in ws, and either says
+  // where in cuts [batch][columns]: its number of pieces << 16 | its first bin.
+  float *parts;
+  int *cuts;
 };
 
 // Counts the caller in as one of n on a pair of 64-bit words and says whether
@@ -691,7 +695,11 @@ __device__ __forceinline__ void decode_body(const DecodeParams &p, DecodeLds<T> 
         const int nt = tiles_of(seg.len), i0 = max(first - pos0, 0), i1 = min(first + nt - pos0, n_wg);
         const int bin0 = (int)((uint32_t)first / (uint32_t)share);
         const int pieces = (int)((uint32_t)(first + nt - 1) / (uint32_t)share) - bin0 + 1;
-        if (pieces > 1) cuts[bin0 == bin] = Cut{seg.b, bin0, pieces};
+        if (p.parts) {
+          if (tid == 0 && bin0 == bin) p.cuts[seg.b * p.columns + col] = pieces << 16 | bin0;
+        } else if (pieces > 1) {
+          cuts[bin0 == bin] = Cut{seg.b, bin0, pieces};
+        }
         for (int k = tid; k < rows * (HD / 2); k += 256) {
           const int h = k / (HD / 2), d = 2 * (k % (HD / 2));
           const float *r = hold + (place * 4 * rows + h) * kHold;
@@ -778,7 +786,10 @@ __device__ __forceinline__ void decode_body(const DecodeParams &p, DecodeLds<T> 
   // sequences without a key
   for (int b = bin; b < c.batch; b += p.bins)
     if (tiles_of(clamp_len(c.lens[b])) == 0)
-      for (int k = tid; k < rows * (HD / 2); k += 256) write2(b, k / (HD / 2), 2 * (k % (HD / 2)), 0.f, 0.f, -INFINITY, 0.f);
+      for (int k = tid; k < rows * (HD / 2); k += 256) {
+        write2(b, k / (HD / 2), 2 * (k % (HD / 2)), 0.f, 0.f, -INFINITY, 0.f);
+        if (k == 0 && p.parts) p.cuts[b * p.columns + col] = 1 << 16;
+      }
 }
 template <typename T>
 __global__ __launch_bounds__(256) void paged_decode_kernel(DecodeParams p) {
@@ -795,7 +806,12 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // R = 32 * HW consecutive rows; its keys go in tiles of 32.
 struct PrefillParams {
   AttnParams a;
-  float *ws;                       // records: [slot][R][kRec]
+  // Records.  Of a cut unit's part [slot][33][R] pairs of floats: the accumulators' pairs of
+  // elements, row by row, then (reference, sum) -- through to memory 8 bytes a lane, which rows
+  // of a record next to each other make whole lines (row by row they were not: the prefix of
+  // 16387 keys for 200 sequences 112 us, its rows now 272 bytes apart through the caches).
+  // Of a prefix's part [slot][R][kRow]: the same by rows, for the launch that adds them.
+  float *ws;
   unsigned long long *arrive_end;  // two arrival words per slot below it
   unsigned long long tag;
   int slots;  // records that the workspace holds
@@ -832,6 +848,7 @@ __device__ __forceinline__ void part_of(int n, const Piece &w, int &from, int &t
   }
 }
 constexpr int kPartMin = 24;      // tiles of a part at least
+constexpr int kRow = HD + 4;      // floats of a prefix record's row
 constexpr int kPartsAll = 256;   // a part is at least this share of all the call's tiles
 
 // Which piece of work is workgroup L's.  A call's units differ in length (the
@@ -990,7 +1007,11 @@ __device__ __forceinline__ PieceKeys piece_keys(const PrefillParams &p, const Pi
   PieceKeys k;
   if (p.prefix_parts) {
     k.end = p.a.prefix_len;
-    k.whole = 0;
+    k.whole = p.a.prefix_len;  // unless a sequence is shorter
+    int h;
+    const int to = min(token_of(w, p.a.inv_group, p.a.group, R - 1, h) + 1, w.rows);
+    for (int t = w.tok0 + (int)(threadIdx.x & 63); t < to; t += 64) k.whole = min(k.whole, max(c.lens[t], 0));
+    k.whole = wave_min(k.whole);
     k.table = p.a.prefix_pages;
   } else {
     int h;
@@ -1089,15 +1110,22 @@ __device__ __forceinline__ void finish_piece(const PrefillParams &p, const Piece
     }
   };
   if (w.parts == 1 && !p.prefix_parts) return write();
+  if (p.prefix_parts) {
+    if (!there) return;
+    float *const r = p.ws + (((int64_t)w.slot + (int64_t)w.part * p.a.c.n_kv_heads) * R + row) * kRow;
+#pragma unroll
+    for (int i = 0; i < NV; i += 4) *(float4 *)(r + d0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+    if (d0 == 0) *(float2 *)(r + HD) = ml;
+    return;
+  }
   const int64_t step = (int64_t)p.a.c.n_kv_heads * R * kRec;
-  float *const first = p.ws + ((int64_t)w.slot * R + row) * kRec;
+  float *const first = p.ws + (int64_t)w.slot * R * kRec + 2 * row;  // pair k: 2 R k floats on
   if (there) {
     float *const r = first + w.part * step;
 #pragma unroll
-    for (int i = 0; i < NV; i += 2) put2(r + d0 + i, acc[i], acc[i + 1]);
-    if (d0 == 0) put2(r + HD, ml.x, ml.y);
+    for (int i = 0; i < NV; i += 2) put2(r + R * (d0 + i), acc[i], acc[i + 1]);
+    if (d0 == 0) put2(r + R * HD, ml.x, ml.y);
   }
-  if (p.prefix_parts) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the record has reached memory
   __syncthreads();
   if (tid == 0) *last_in = arrive_last(p.arrive_end - 2 * ((int64_t)w.slot + 1), w.parts, p.tag);
@@ -1112,9 +1140,9 @@ __device__ __forceinline__ void finish_piece(const PrefillParams &p, const Piece
 #pragma unroll
     for (int v = 0; v < MB; ++v) {
       const float *const r = first + min(n0 + v, w.parts - 1) * step;
-      m2[v] = get2(r + HD);
+      m2[v] = get2(r + R * HD);
 #pragma unroll
-      for (int i = 0; i < NV / 2; ++i) a[v][i] = get2(r + d0 + 2 * i);
+      for (int i = 0; i < NV / 2; ++i) a[v][i] = get2(r + R * (d0 + 2 * i));
     }
 #pragma unroll
     for (int v = 0; v < MB; ++v) {
@@ -1182,7 +1210,7 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
   int head;
   const int tok = token_of(w, p.a.inv_group, p.a.group, 32 * hw + r32, head);
   const bool there = tok < w.rows;
-  const int limit = there ? key_limit(p, w, tok) : 0;
+  const int limit = there ? key_limit(p, w, tok) : keys.end;  // (0: a fix of its reference in every tile)
   const int all_see = wave_min(there ? limit : 0x7fffffff);  // keys that all the wave's rows see
   bf16x8 qreg[4];
   {
@@ -1435,16 +1463,15 @@ struct PipeLds {
   Piece piece;
   int odd[4], last_in;
 };
-__global__ __launch_bounds__(256, 2) void paged_prefill_pipe_kernel(PrefillParams p) {
+__device__ __forceinline__ void prefill_pipe_body(const PrefillParams &p, PipeLds &lds, int block) {
   constexpr int RT = 2, R = kPipeR, KP = PipeLds::KP, VP = PipeLds::VP, KBUF = PipeLds::KBUF, VBUF = PipeLds::VBUF;
-  __shared__ __attribute__((aligned(16))) PipeLds lds;
   bf16_t *const kring = lds.k, *const vring = lds.v;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, hf = lane >> 5;
   Piece w;
-  if (!find_piece<R>(p, blockIdx.x, w)) return;
+  if (!find_piece<R>(p, block, w)) return;
   if (tid == 0) lds.piece = w;
   const Paged &c = p.a.c;
   const float cl = p.a.cl;
@@ -1470,7 +1497,8 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_pipe_kernel(PrefillParam
     int head;
     const int tok = token_of(w, p.a.inv_group, p.a.group, 32 * (RT * wave + rt) + r32, head);
     const bool there = tok < w.rows;
-    const int limit = there ? key_limit(p, w, tok) - first : 0;
+    // (no row there: as if it saw all, since one that sees nothing has its reference fixed in every step)
+    const int limit = (there ? key_limit(p, w, tok) : end) - first;
     lds.limit[32 * (RT * wave + rt) + r32] = limit;  // (the steps with masks read them there)
     most = max(most, limit);
     if (there) least = min(least, limit);
@@ -1483,7 +1511,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_pipe_kernel(PrefillParam
     }
   }
   least = wave_min(least);
-  if (least == 0x7fffffff) least = 0;  // no row
+  const bool idle = least == 0x7fffffff;  // no row: the wave only loads for the others
   const int ntw = min((-wave_min(-most) + 31) >> 5, 2 * nblk);  // tiles that the wave's rows see
 
   // staging: 2 x 16 B per thread of a K block and of a V block, rows crow and
@@ -1729,11 +1757,7 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_pipe_kernel(PrefillParam
   // iteration before: one barrier a block
   const int t_safe = min(least, kBK * nblk) >> 5;
   const int j_safe = min(min(nblk, max(0, (t_safe - 1) / 2)), max(gap - 1, 0));
-  auto iteration = [&](auto masked_tag, int j) __attribute__((always_inline)) {
-    const bf16_t *vc = vring + (j & 1) * VBUF;
-    const bf16_t *kn = kring + ((j + 1) & 1) * KBUF;
-    step(masked_tag, 2 * j + 1, vc, kn, sb, sa, pa, pbb, rsa, rsb);
-    step(masked_tag, 2 * j + 2, vc + 32 * VP, kn + 32 * KP, sa, sb, pbb, pa, rsb, rsa);
+  auto stage = [&](int j) __attribute__((always_inline)) {
     lstore_k(j + 2);
     lstore_v(j + 1);
     gload_v(j + 2);
@@ -1741,7 +1765,16 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_pipe_kernel(PrefillParam
     e_k = entry_of(j + 4);
     __syncthreads();
   };
+  auto iteration = [&](auto masked_tag, int j) __attribute__((always_inline)) {
+    const bf16_t *vc = vring + (j & 1) * VBUF;
+    const bf16_t *kn = kring + ((j + 1) & 1) * KBUF;
+    step(masked_tag, 2 * j + 1, vc, kn, sb, sa, pa, pbb, rsa, rsb);
+    step(masked_tag, 2 * j + 2, vc + 32 * VP, kn + 32 * KP, sa, sb, pbb, pa, rsb, rsa);
+    stage(j);
+  };
   int j = 0;
+  if (idle)
+    for (; j < nblk; ++j) stage(j);
   for (; j < j_safe; ++j) iteration(std::false_type{}, j);
   for (; j < nblk; ++j) iteration(std::true_type{}, j);
 
@@ -1775,18 +1808,30 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_pipe_kernel(PrefillParam
     const int row = 32 * (RT * wave + rt) + r32, t = token_of(f, p.a.inv_group, p.a.group, row, h);
     if (t >= f.rows) continue;
     h += f.g * p.a.group;
-    if (f.parts == 1) {
+    if (f.parts == 1 && !p.prefix_parts) {
       write(t, h, rt, l[rt]);
     } else {
-      float *const r = p.ws + ((int64_t)f.slot * R + row) * kRec + f.part * rec_step;
+      if (p.prefix_parts) {
+        float *const r = p.ws + (((int64_t)f.slot + (int64_t)f.part * c.n_kv_heads) * R + row) * kRow;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const f32x16 &x = o[rt][i >> 2];
+          const int e = 4 * (i & 3);
+          *(float4 *)(r + 32 * (i >> 2) + 8 * (i & 3) + 4 * hf) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        }
+        if (hf == 0) *(float2 *)(r + HD) = make_float2(mcv[rt], l[rt]);
+        continue;
+      }
+      float *const r = p.ws + (int64_t)f.slot * R * kRec + 2 * row + f.part * rec_step;
 #pragma unroll
       for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) put2(r + 32 * dt + 8 * (i >> 2) + 4 * hf + (i & 3), o[rt][dt][i], o[rt][dt][i + 1]);
-      if (hf == 0) put2(r + HD, mcv[rt], l[rt]);
+        for (int i = 0; i < 16; i += 2)
+          put2(r + R * (32 * dt + 8 * (i >> 2) + 4 * hf + (i & 3)), o[rt][dt][i], o[rt][dt][i + 1]);
+      if (hf == 0) put2(r + R * HD, mcv[rt], l[rt]);
     }
   }
-  if (f.parts == 1) return;
+  if (f.parts == 1 || p.prefix_parts) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the records have reached memory
   __syncthreads();
   if (tid == 0) lds.last_in = arrive_last(p.arrive_end - 2 * ((int64_t)f.slot + 1), f.parts, p.tag);
@@ -1798,15 +1843,15 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_pipe_kernel(PrefillParam
     const int row = 32 * (RT * wave + rt) + r32, t = token_of(f, p.a.inv_group, p.a.group, row, h);
     if (t >= f.rows) continue;
     h += f.g * p.a.group;
-    const float *const r0 = p.ws + ((int64_t)f.slot * R + row) * kRec;
+    const float *const r0 = p.ws + (int64_t)f.slot * R * kRec + 2 * row;
     float M = -INFINITY, L = 0.f;
     o[rt][0] = o[rt][1] = f32x16{};
     for (int n = 0; n < f.parts; ++n) {
       const float *const r = r0 + n * rec_step;
-      const float2 ml = get2(r + HD);
+      const float2 ml = get2(r + R * HD);
       float2 x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = get2(r + 32 * (i >> 3) + 8 * ((i >> 1) & 3) + 4 * hf + 2 * (i & 1));
+      for (int i = 0; i < 16; ++i) x[i] = get2(r + R * (32 * (i >> 3) + 8 * ((i >> 1) & 3) + 4 * hf + 2 * (i & 1)));
       const float mn = fmaxf(M, ml.x), mu = mn == -INFINITY ? 0.f : mn;
       const float fo = __builtin_amdgcn_exp2f(M - mu), fn = __builtin_amdgcn_exp2f(ml.x - mu);
       L = fmaf(ml.y, fn, L * fo);
@@ -1819,6 +1864,10 @@ __global__ __launch_bounds__(256, 2) void paged_prefill_pipe_kernel(PrefillParam
     }
     write(t, h, rt, L);
   }
+}
+__global__ __launch_bounds__(256, 2) void paged_prefill_pipe_kernel(PrefillParams p) {
+  __shared__ __attribute__((aligned(16))) PipeLds lds;
+  prefill_pipe_body(p, lds, blockIdx.x);
 }
 
 // fp32, v_mfma_f32_32x32x2f32: matrix-core time is all that counts.  32 rows a
@@ -1854,7 +1903,7 @@ __device__ __forceinline__ void prefill_f32_body(const PrefillParams &p, Prefill
   int head;
   const int tok = token_of(w, p.a.inv_group, p.a.group, r32, head);
   const bool there = tok < w.rows;
-  const int limit = there ? key_limit(p, w, tok) : 0;
+  const int limit = there ? key_limit(p, w, tok) : keys.end;
 
   const PageRows rows = PageRows::of<float>(c);
   const uint32_t row_bytes = rows.row_bytes;
@@ -2062,6 +2111,19 @@ __global__ __launch_bounds__(256, 2) void paged_shared_bf16_kernel(SharedParams 
     decode_body<bf16_t>(p.d, lds.d, block);
   }
 }
+__global__ __launch_bounds__(256, 2) void paged_shared_pipe_kernel(SharedParams p) {
+  union Lds {
+    DecodeLds<bf16_t> d;
+    PipeLds f;
+  };
+  __shared__ __attribute__((aligned(16))) Lds lds;
+  int block;
+  if (shared_block(p, block)) {
+    if (block < p.n_pre) prefill_pipe_body(p.f, lds.f, block);
+  } else if (block < p.n_dec) {
+    decode_body<bf16_t>(p.d, lds.d, block);
+  }
+}
 __global__ __launch_bounds__(256, 2) void paged_shared_f32_kernel(SharedParams p) {
   union Lds {
     DecodeLds<float> d;
@@ -2076,51 +2138,65 @@ __global__ __launch_bounds__(256, 2) void paged_shared_f32_kernel(SharedParams p
   }
 }
 
-// The records of a row: `parts` of the prefix, then its own keys'.  Two
+// The records of a row, the prefix's parts and then its own keys' pieces: two
 // elements a thread.
+struct RowSum {
+  float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
+  // records rec(0) .. rec(n - 1), eight at a time
+  template <class F>
+  __device__ __forceinline__ void add(int n, int d, F &&rec) {
+    constexpr int N = 8;
+    for (int n0 = 0; n0 < n; n0 += N) {
+      float2 ml[N], y[N];
+#pragma unroll
+      for (int v = 0; v < N; ++v) {
+        const float *const q = rec(min(n0 + v, n - 1));
+        ml[v] = *(const float2 *)(q + HD);
+        y[v] = *(const float2 *)(q + d);
+      }
+      float mx = M;
+#pragma unroll
+      for (int v = 0; v < N; ++v) mx = n0 + v < n ? fmaxf(mx, ml[v].x) : mx;
+      const float mu = mx == -INFINITY ? 0.f : mx, fo = __builtin_amdgcn_exp2f(M - mu);
+      L *= fo;
+      A0 *= fo;
+      A1 *= fo;
+#pragma unroll
+      for (int v = 0; v < N; ++v) {
+        const bool in = n0 + v < n;
+        const float f = __builtin_amdgcn_exp2f(ml[v].x - mu);
+        L = in ? fmaf(ml[v].y, f, L) : L;
+        A0 = in ? fmaf(y[v].x, f, A0) : A0;
+        A1 = in ? fmaf(y[v].y, f, A1) : A1;
+      }
+      M = mx;
+    }
+  }
+};
 template <typename T>
 __global__ __launch_bounds__(256) void paged_shared_add_kernel(SharedParams p, int R) {
   const AttnParams &a = p.d.a;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int d = 2 * (int)(i % (HD / 2)), h = (int)(i / (HD / 2) % a.n_heads), b = (int)(i / (HD / 2) / a.n_heads);
   if (b >= a.c.batch) return;
-  const int g = h / a.group, fr = b * a.group + h - g * a.group, unit = fr / R, parts = p.f.prefix_parts;
-  const float *r = p.f.ws + (((int64_t)unit * parts * a.c.n_kv_heads + g) * R + (fr - unit * R)) * kRec;
-  const int64_t step = (int64_t)a.c.n_kv_heads * R * kRec;
-  const float *const mine = p.d.parts + ((int64_t)b * a.n_heads + h) * kRec;
-  const float2 own = *(const float2 *)(mine + HD), x = *(const float2 *)(mine + d);
-  float M = own.x, L = own.y, A0 = x.x, A1 = x.y;
-  constexpr int N = 8;  // records read at once
-  for (int n0 = 0; n0 < parts; n0 += N) {
-    float2 ml[N], y[N];
-#pragma unroll
-    for (int v = 0; v < N; ++v) {
-      const float *const q = r + min(n0 + v, parts - 1) * step;
-      ml[v] = *(const float2 *)(q + HD);
-      y[v] = *(const float2 *)(q + d);
-    }
-    float mx = M;
-#pragma unroll
-    for (int v = 0; v < N; ++v) mx = n0 + v < parts ? fmaxf(mx, ml[v].x) : mx;
-    const float mu = mx == -INFINITY ? 0.f : mx, fo = __builtin_amdgcn_exp2f(M - mu);
-    L *= fo;
-    A0 *= fo;
-    A1 *= fo;
-#pragma unroll
-    for (int v = 0; v < N; ++v) {
-      const float f = n0 + v < parts ? __builtin_amdgcn_exp2f(ml[v].x - mu) : 0.f;
-      L = n0 + v < parts ? fmaf(ml[v].y, f, L) : L;
-      A0 = n0 + v < parts ? fmaf(y[v].x, f, A0) : A0;
-      A1 = n0 + v < parts ? fmaf(y[v].y, f, A1) : A1;
-    }
-    M = mx;
-  }
-  const float inv = L > 0.f ? 1.0f / L : 0.f;
+  const int g = h / a.group, hg = h - g * a.group, col = g * p.d.hblocks + hg / kMaxRows, row = hg % kMaxRows;
+  const int cut = p.d.cuts[b * p.d.columns + col], bin0 = min(cut & 0xffff, p.d.bins - 1);
+  const int pieces = min(max(cut >> 16, 1), p.d.bins - bin0);
+  const int fr = b * a.group + hg, unit = fr / R, parts = p.f.prefix_parts;
+  const float *const r = p.f.ws + (((int64_t)unit * parts * a.c.n_kv_heads + g) * R + (fr - unit * R)) * kRow;
+  const int64_t step = (int64_t)a.c.n_kv_heads * R * kRow;
+  RowSum s;
+  s.add(parts, d, [&](int n) { return r + n * step; });
+  s.add(pieces, d, [&](int n) {
+    return pieces == 1 ? p.d.parts + ((int64_t)b * a.n_heads + h) * kRec
+                       : p.d.ws + ((((int64_t)(bin0 + n) * 2 + (n == 0)) * p.d.columns + col) * kMaxRows + row) * kRec;
+  });
+  const float inv = s.L > 0.f ? 1.0f / s.L : 0.f;
   T *const op = (T *)a.o + b * a.o_rs + h * HD + d;
   if constexpr (sizeof(T) == 2)
-    *(uint32_t *)op = (uint32_t)f32_to_bf16(A0 * inv) | ((uint32_t)f32_to_bf16(A1 * inv) << 16);
+    *(uint32_t *)op = (uint32_t)f32_to_bf16(s.A0 * inv) | ((uint32_t)f32_to_bf16(s.A1 * inv) << 16);
   else
-    *(float2 *)op = make_float2(A0 * inv, A1 * inv);
+    *(float2 *)op = make_float2(s.A0 * inv, s.A1 * inv);
 }
 
 // ---------------------------------------------------------------- the host
@@ -2292,6 +2368,7 @@ int launch_decode(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
   p.bins = d.bins; p.hblocks = d.hblocks; p.columns = d.columns;
   p.k0 = 0;
   p.parts = nullptr;
+  p.cuts = nullptr;
   const dim3 grid((unsigned)(d.bins * d.columns)), block(256);
   if (dtype == BN_BF16) hipLaunchKernelGGL(paged_decode_kernel<bf16_t>, grid, block, 0, s, p);
   else hipLaunchKernelGGL(paged_decode_kernel<float>, grid, block, 0, s, p);
@@ -2375,20 +2452,26 @@ struct SharedPlan {
   DecodePlan d;
   int hw, parts;
   int64_t n_pre;
-  size_t own, records;  // bytes: the sequences' own parts, the prefix's
+  size_t own, cuts, records;  // bytes: the sequences' own parts and where they are, the prefix's parts
 };
 SharedPlan plan_shared(int dtype, int batch, int n_heads, int n_kv_heads, int prefix_len) {
   SharedPlan s;
   s.d = plan_decode(batch, n_heads, n_kv_heads);
   const int64_t rows = (int64_t)batch * (n_heads / n_kv_heads);
-  s.hw = dtype == BN_BF16 && rows * n_kv_heads >= 32 * 128 ? 4 : 1;
+  s.hw = dtype == BN_BF16 && rows * n_kv_heads >= 32 * 128 ? 8 : 1;
   const int R = 32 * s.hw, steps = (prefix_len + 31) / 32;
   const int64_t units = (rows + R - 1) / R;
-  s.parts = (int)std::max<int64_t>(1, std::min<int64_t>((512 + units * n_kv_heads - 1) / (units * n_kv_heads), steps / 8));
+  // pieces: one per compute unit, of 8 tiles at least; two of the large kernel's if they keep 32
+  // tiles each (1024 rows behind 16384 keys 80 -> 74 us, behind 4096 42 -> 37 with one;
+  // 256 rows behind 2048, 32 rows a piece: 21.9 us with two, 17.5 with one)
+  int64_t parts = 512 / (units * n_kv_heads);
+  if (s.hw == 1 || parts < 1 || steps / parts < 32) parts = 256 / (units * n_kv_heads);
+  s.parts = (int)std::max<int64_t>(1, std::min<int64_t>(parts, steps / 8));
   const int per = n_kv_heads <= 8 && 8 % n_kv_heads == 0 ? 8 / n_kv_heads : 1;
   s.n_pre = (units * s.parts + per - 1) / per * per * n_kv_heads;
-  s.own = (size_t)batch * n_heads * kRec * sizeof(float);
-  s.records = (size_t)units * s.parts * n_kv_heads * R * kRec * sizeof(float);
+  s.own = ((size_t)batch * n_heads * kRec * sizeof(float) + 15) / 16 * 16;
+  s.cuts = ((size_t)batch * s.d.columns * sizeof(int) + 15) / 16 * 16;
+  s.records = (size_t)units * s.parts * n_kv_heads * R * kRow * sizeof(float);
   return s;
 }
 
@@ -2404,6 +2487,7 @@ int launch_shared(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
   p.d.k0 = a.prefix_len;
   p.d.parts = (float *)(at + m.d.records + m.d.words);
   p.f.ws = (float *)(at + m.d.records + m.d.words + m.own);
+  p.d.cuts = (int *)(at + m.d.records + m.d.words + m.own + m.records);
   p.f.arrive_end = nullptr;
   p.f.slots = 0;
   p.f.prefix_parts = m.parts;
@@ -2411,7 +2495,7 @@ int launch_shared(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
   p.n_pre = (int)m.n_pre;
   const dim3 grid((unsigned)(((p.n_dec + 7) / 8 + (m.n_pre + 7) / 8) * 8)), block(256);
   if (dtype == BN_F32) hipLaunchKernelGGL(paged_shared_f32_kernel, grid, block, 0, s, p);
-  else if (m.hw == 4) hipLaunchKernelGGL((paged_shared_bf16_kernel<4, 1>), grid, block, 0, s, p);
+  else if (m.hw == 8) hipLaunchKernelGGL(paged_shared_pipe_kernel, grid, block, 0, s, p);
   else hipLaunchKernelGGL((paged_shared_bf16_kernel<1, 4>), grid, block, 0, s, p);
   BN_LAUNCH_CHECK();
   const int64_t pairs = (int64_t)a.c.batch * a.n_heads * (HD / 2);
@@ -2524,7 +2608,7 @@ size_t bn_paged_workspace_size(const bn_paged_kv *cache, int n_heads, int n_rows
   size_t need = std::max(d.records + d.words, f.records + f.words);
   if (prefix_len > 0) {
     const SharedPlan s = plan_shared(cache->dtype, cache->batch, n_heads, cache->n_kv_heads, std::min(prefix_len, c.cap));
-    need = std::max(need, s.d.records + s.d.words + s.own + s.records);
+    need = std::max(need, s.d.records + s.d.words + s.own + s.records + s.cuts);
   }
   return need;
 }

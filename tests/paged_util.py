@@ -174,6 +174,9 @@ def attention64_large(case, q, rows, scale=0.125, prefix=None, prefix_len=0):
         gone = (pages < 0) | (pages >= case.n_pages)
         hidden |= gone[j // case.page][None, :]
         pages = pages.masked_fill(gone, 0)
+        if length == 0:
+            at += n
+            continue
         for g in range(case.Hkv):
             k, v = (x[pages, g].reshape(-1, D)[:length].double() for x in (kd, vd))
             k, v = k.masked_fill(gone[j // case.page][:, None], 0), v.masked_fill(gone[j // case.page][:, None], 0)

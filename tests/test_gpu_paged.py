@@ -479,6 +479,35 @@ def test_shared(case):
         assert torch.equal(bits(o2), bits(o)), "a second call differs"
 
 
+@pytest.mark.parametrize("case", [("bf16", 2048, 200, 700, 4, 32, 16), ("bf16", 4096, 150, 3000, 8, 8, 32),
+                                  ("bf16", 640, 700, 90, 4, 20, 64), ("f32", 1024, 70, 900, 4, 16, 16)],
+                         ids=lambda c: "-".join(map(str, c)))
+def test_shared_large(case):
+    """Large batches (the pipelined kernel) and own keys cut over workgroups; some sequences shorter
+    than the prefix, some empty, a page of the prefix and one of a sequence without memory."""
+    dtype, P, Bn, own, Hkv, H, page = case
+    r = np.random.default_rng(P)
+    lens = [P + int(x) for x in r.integers(0, own + 1, Bn)]
+    lens[3], lens[5], lens[7], lens[11] = 0, P - 100, P, 17
+    c = Case(dtype, lens, Hkv, page, True, seed=P, nan=False, drop=[(9, P // page)])
+    prefix = c.table[Bn - 1, :P // page].copy()
+    prefix[2] = -1
+    q = rows_of(dtype, Bn, H, 1).cuda()
+    cache = c.cuda(B)
+    pd = torch.from_numpy(prefix).cuda()
+    ws = B.paged_workspace(cache, H, Bn, P)
+    ws.fill_(255)
+    got = [B.paged_decode_shared(q, cache, pd, P, scale=0.125, workspace=w) for w in (ws, ws, None)]
+    pages_of = c.table.copy()
+    for b in range(Bn):     # attention64_large takes the prefix from each table
+        c.table[b, :P // page] = prefix
+    ref, tol = attention64_large(c, q, [1] * Bn)
+    c.table[:] = pages_of
+    over = (got[0].double() - ref).abs() - tol
+    assert (over <= 0).all(), f"{int((over > 0).sum())} past the tolerance, by {float(over.max()):.2e}"
+    assert torch.equal(bits(got[0]), bits(got[1])) and torch.equal(bits(got[0]), bits(got[2]))
+
+
 def test_shared_prefix_page_without_memory():
     c = Case("bf16", [90, 120, 70], 2, 16, True, seed=2)
     prefix = c.table[0, :4].copy()
