@@ -383,43 +383,57 @@ class PagedKV:
                               page_table.stride(0), _torch_dtype_code(k_pages), batch, n_pages, max_pages,
                               page_size, hkv, d)
         self.ref = C.byref(self.view)
+        # what every call compares its tensors with
+        self.dtype, self.device, self.batch, self.kv_heads, self.head_dim = k_pages.dtype, k_pages.device, \
+            batch, hkv, d
 
 
 def _paged_rows(what, t, cache, rows, heads=None):
     """(pointer, row stride) of a [rows, heads, D] tensor whose heads are
     contiguous within a row, of the cache's type."""
-    v = cache.view
-    if t.dim() != 3 or t.shape[2] != v.head_dim or (heads is not None and t.shape[1] != heads) or \
-            (rows is not None and t.shape[0] != rows):
+    shape, stride, d = t.shape, t.stride(), cache.head_dim
+    if len(shape) != 3 or shape[2] != d or (heads is not None and shape[1] != heads) or \
+            (rows is not None and shape[0] != rows):
         raise ValueError(f"{what}: expected [{'rows' if rows is None else rows}, "
-                         f"{'heads' if heads is None else heads}, {v.head_dim}], got {tuple(t.shape)}")
-    if t.dtype != cache.k_pages.dtype or t.device != cache.k_pages.device:
+                         f"{'heads' if heads is None else heads}, {d}], got {tuple(shape)}")
+    if t.dtype != cache.dtype or t.device != cache.device:
         raise ValueError(f"{what}: dtype and device must be the cache's")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    if stride[2] != 1 or (shape[1] > 1 and stride[1] != d):
         raise ValueError(f"{what}: a row's heads must be contiguous")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return t.data_ptr(), stride[0] if shape[0] > 1 else shape[1] * d
 
 
 def _cache_stream(cache, stream):
+    """The stream as the library takes it; None: the current one of the cache's
+    device, asked for without a torch.cuda.Stream made of it (2 us a call)."""
     import torch
-    return stream_of(torch.cuda.current_stream(cache.k_pages.device) if stream is None else stream)
+    if cache.device.type != "cuda":
+        raise ValueError("paged KV cache: its tensors are not on a GPU")
+    if stream is not None:
+        if stream.device != cache.device:
+            raise ValueError("paged KV cache: the stream is another device's")
+        return stream.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(cache.device.index)
 
 
 def _row_starts(what, row_starts, cache, n_rows):
     import torch
     if row_starts is None:
-        if n_rows != cache.view.batch:
+        if n_rows != cache.batch:
             raise ValueError(f"{what}: without row_starts there is one row per sequence")
         return None
-    if row_starts.dtype != torch.int32 or tuple(row_starts.shape) != (cache.view.batch + 1,) or \
-            not row_starts.is_contiguous() or row_starts.device != cache.k_pages.device:
+    if row_starts.dtype != torch.int32 or tuple(row_starts.shape) != (cache.batch + 1,) or \
+            not row_starts.is_contiguous() or row_starts.device != cache.device:
         raise ValueError(f"{what}: row_starts must be int32 [B + 1] on the cache's device")
     return row_starts.data_ptr()
 
 
-def _workspace(workspace):
-    return (None, 0) if workspace is None else (workspace.data_ptr(),
-                                                workspace.numel() * workspace.element_size())
+def _workspace(workspace, cache):
+    if workspace is None:
+        return None, 0
+    if workspace.device != cache.device or not workspace.is_contiguous():
+        raise ValueError("paged KV cache: the workspace must be contiguous memory of the cache's device")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def paged_workspace(cache, n_heads, n_rows, prefix_len=0):
@@ -427,7 +441,7 @@ def paged_workspace(cache, n_heads, n_rows, prefix_len=0):
     query rows (and prefix_len common keys); one per call in flight."""
     import torch
     n = lib().bn_paged_workspace_size(cache.ref, n_heads, n_rows, prefix_len)
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k_pages.device)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.device)
 
 
 def paged_append(cache, k, v, q=None, q_out=None, row_starts=None, theta=10000.0, stream=None):
@@ -438,8 +452,8 @@ def paged_append(cache, k, v, q=None, q_out=None, row_starts=None, theta=10000.0
     last of them at position seq_lens[b] - 1.  Returns q_out (default: in
     place), or None without q."""
     n = k.shape[0]
-    kp, ks = _paged_rows("paged_append: k", k, cache, n, cache.view.n_kv_heads)
-    vp, vs = _paged_rows("paged_append: v", v, cache, n, cache.view.n_kv_heads)
+    kp, ks = _paged_rows("paged_append: k", k, cache, n, cache.kv_heads)
+    vp, vs = _paged_rows("paged_append: v", v, cache, n, cache.kv_heads)
     qp, qs, op, os_, heads = None, 0, None, 0, 0
     if q is not None:
         q_out = q if q_out is None else q_out
@@ -457,10 +471,11 @@ def paged_decode(q, cache, o=None, scale=None, workspace=None, stream=None):
     """One query row per sequence over its pages: q, o [B, H, D]."""
     import torch
     o = torch.empty_like(q) if o is None else o
-    qp, qs = _paged_rows("paged_decode: q", q, cache, cache.view.batch)
-    op, os_ = _paged_rows("paged_decode: o", o, cache, cache.view.batch, q.shape[1])
+    qp, qs = _paged_rows("paged_decode: q", q, cache, cache.batch)
+    op, os_ = _paged_rows("paged_decode: o", o, cache, cache.batch, q.shape[1])
     call("bn_paged_decode", cache.ref, qp, op, q.shape[1], qs, os_,
-         1.0 / math.sqrt(q.shape[2]) if scale is None else scale, *_workspace(workspace), _cache_stream(cache, stream))
+         1.0 / math.sqrt(q.shape[2]) if scale is None else scale,
+         *_workspace(workspace, cache), _cache_stream(cache, stream))
     return o
 
 
@@ -475,7 +490,7 @@ def paged_prefill(q, cache, row_starts=None, o=None, scale=None, workspace=None,
     op, os_ = _paged_rows("paged_prefill: o", o, cache, n, q.shape[1])
     call("bn_paged_prefill", cache.ref, qp, op, _row_starts("paged_prefill", row_starts, cache, n), n,
          q.shape[1], qs, os_, 1.0 / math.sqrt(q.shape[2]) if scale is None else scale,
-         *_workspace(workspace), _cache_stream(cache, stream))
+         *_workspace(workspace, cache), _cache_stream(cache, stream))
     return o
 
 
@@ -484,14 +499,14 @@ def paged_decode_shared(q, cache, prefix_pages, prefix_len, o=None, scale=None, 
     keys, those of prefix_pages (int32, device), read once for all."""
     import torch
     o = torch.empty_like(q) if o is None else o
-    qp, qs = _paged_rows("paged_decode_shared: q", q, cache, cache.view.batch)
-    op, os_ = _paged_rows("paged_decode_shared: o", o, cache, cache.view.batch, q.shape[1])
+    qp, qs = _paged_rows("paged_decode_shared: q", q, cache, cache.batch)
+    op, os_ = _paged_rows("paged_decode_shared: o", o, cache, cache.batch, q.shape[1])
     if prefix_pages.dtype != torch.int32 or prefix_pages.dim() != 1 or not prefix_pages.is_contiguous() or \
-            prefix_pages.device != cache.k_pages.device or prefix_len < 0 or \
+            prefix_pages.device != cache.device or prefix_len < 0 or \
             prefix_pages.shape[0] < -(-prefix_len // cache.view.page_size):
         raise ValueError("paged_decode_shared: prefix_pages must be int32 [ceil(prefix_len / page_size)] "
                          "on the cache's device")
     call("bn_paged_decode_shared", cache.ref, qp, op, q.shape[1], qs, os_,
          1.0 / math.sqrt(q.shape[2]) if scale is None else scale, prefix_pages.data_ptr(), prefix_len,
-         *_workspace(workspace), _cache_stream(cache, stream))
+         *_workspace(workspace, cache), _cache_stream(cache, stream))
     return o

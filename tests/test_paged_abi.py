@@ -202,3 +202,20 @@ def test_python_wrappers_refuse():
         B.paged_append(kv, kn, kn[:2])
     with pytest.raises(ValueError, match="q_out without q"):
         B.paged_append(kv, kn, kn, q_out=q)
+
+
+def test_python_wrappers_refuse_other_devices():
+    from types import SimpleNamespace
+    k = torch.zeros((5, 2, 16, 64), dtype=torch.bfloat16)
+    kv = B.PagedKV(k, k.clone(), torch.zeros((3, 4), dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
+    q = torch.zeros((3, 8, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="not on a GPU"):
+        B.paged_decode(q, kv)
+    with pytest.raises(ValueError, match="workspace"):
+        B.paged_decode(q, kv, workspace=torch.empty(1 << 20, dtype=torch.uint8, device="meta"))
+    with pytest.raises(ValueError, match="workspace"):
+        B.paged_prefill(q, kv, workspace=torch.empty((1 << 10, 2), dtype=torch.uint8)[:, 0])
+    kv.device = torch.device("cuda:0")  # what follows looks at the stream alone
+    with pytest.raises(ValueError, match="stream"):
+        B._cache_stream(kv, SimpleNamespace(device=torch.device("cuda:1"), cuda_stream=0))
+    assert B._cache_stream(kv, SimpleNamespace(device=torch.device("cuda:0"), cuda_stream=7)) == 7
