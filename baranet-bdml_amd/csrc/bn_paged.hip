@@ -13,6 +13,7 @@
 // contents of those arrays lead outside the pools.
 #include <algorithm>
 #include <atomic>
+
 #include <cmath>
 
 #include "bn_common.hpp"
@@ -110,66 +111,73 @@ __device__ __forceinline__ u32x4 rotate<bf16_t>(u32x4 x, const float2 *cs) {
   return y;
 }
 
-// RB rows per workgroup of 256 threads.  First a (row, pair) per thread: the
-// row's place and the pair's cosine and sine, into LDS.  The angle is formed
-// in turns and in 64 bits and reduced to an eighth of a turn before it is
-// rounded to 32: at position 2^20 a 32-bit angle would be off by 0.06 rad.
-// Then the rows' 16-byte pieces, Q heads, K heads, V heads, consecutive
-// threads on consecutive pieces, 256 / RB threads a row.
-template <typename T, int RB>
+// A row per workgroup.  32 threads form the pairs' cosines and sines: the
+// angle in turns and in 64 bits, reduced to an eighth of a turn before it is
+// rounded to 32 (at position 2^20 a 32-bit angle would be off by 0.06 rad).
+// All take the row's 16-byte pieces, Q heads, K heads, V heads, consecutive
+// threads on consecutive pieces, the first kBatch of a thread on their way
+// while the angles are formed.  Bound by memory: 16384 bf16 rows of 32 + 2 * 4
+// heads 33 us, 5.0 TB/s read and written, as fast as a copy; 16 rows 3.5 us, a
+// launch and the chain row -> sequence -> position -> page.  (Eight rows a
+// workgroup, a piece of a thread at a time: 41 us, and 1250 fp32 rows 13.7
+// where this takes 8.3; one, three or four pieces a thread: the same to 6% more.)
+constexpr int kBatch = 4;
+template <typename T>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   constexpr int PIECES = HD * sizeof(T) / 16;  // per head
   constexpr int VEC = 16 / sizeof(T);
-  constexpr int TPR = 256 / RB;
-  __shared__ float2 cs[RB][HD / 2];
-  __shared__ int64_t place[RB];  // element offset of the row's slot in KV head 0 (-1: none)
-  __shared__ int owner[RB];      // the row's sequence (-1: padding)
-  const int tid = threadIdx.x;
-  const int row0 = blockIdx.x * RB;
-  if (tid < RB * (HD / 2)) {
-    const int r = tid / (HD / 2), pair = tid % (HD / 2);
-    const int row = row0 + r;
-    const int b = row < p.n_rows ? sequence_of(p.starts, p.c.batch, row) : -1;
+  __shared__ float2 cs[HD / 2];
+  __shared__ int64_t place;  // element offset of the row's slot in KV head 0 (-1: none)
+  __shared__ int owner;      // the row's sequence (-1: padding)
+  const int tid = threadIdx.x, row = blockIdx.x, stride = blockDim.x;
+  const int hkv = p.c.n_kv_heads, kv0 = p.n_heads, v0 = kv0 + hkv, pieces = (v0 + hkv) * PIECES;
+  const T *const Q = (const T *)p.q + row * p.q_rs, *const K = (const T *)p.k + row * p.k_rs,
+          *const V = (const T *)p.v + row * p.v_rs;
+  u32x4 x[kBatch];
+  auto load = [&](int first) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n) {
+      const int i = first + n * stride, h = i / PIECES, e = (i % PIECES) * VEC;
+      if (i < pieces) x[n] = *(const u32x4 *)((h < kv0 ? Q + h * HD : h < v0 ? K + (h - kv0) * HD : V + (h - v0) * HD) + e);
+    }
+  };
+  load(tid);
+  if (tid < HD / 2) {
+    const int b = sequence_of(p.starts, p.c.batch, row);
     const int pos = b < 0 ? 0 : position_of(p.c, p.starts, b, row);
-    if (pair == 0) {
+    if (tid == 0) {
       int64_t at = -1;
       if (b >= 0 && pos >= 0 && pos < p.c.cap) {
         const int page = p.c.table[b * p.c.table_stride + (pos >> p.c.shift)];
         if ((unsigned)page < (unsigned)p.c.n_pages)
           at = page * p.c.page_stride + (pos & ((1 << p.c.shift) - 1)) * p.c.row_stride;
       }
-      place[r] = at;
-      owner[r] = b;
+      place = at;
+      owner = b;
     }
-    const double turns = (double)pos * p.f[pair];
+    const double turns = (double)pos * p.f[tid];
     const double quarter = rint(4.0 * turns);
     float s, c;
     sincospif(2.f * (float)(turns - 0.25 * quarter), &s, &c);
     const int quadrant = (int)((int64_t)quarter & 3);
     const float cq = quadrant & 1 ? -s : c, sq = quadrant & 1 ? c : s;
-    cs[r][pair] = quadrant & 2 ? make_float2(-cq, -sq) : make_float2(cq, sq);
+    cs[tid] = quadrant & 2 ? make_float2(-cq, -sq) : make_float2(cq, sq);
   }
   __syncthreads();
-  const int r = tid / TPR, row = row0 + r;
-  if (row >= p.n_rows || owner[r] < 0) return;
-  const int64_t at = place[r];
-  const int hkv = p.c.n_kv_heads, kv0 = p.n_heads, v0 = kv0 + hkv, pieces = (v0 + hkv) * PIECES;
+  if (owner < 0) return;
+  const int64_t at = place;
   T *const Kd = (T *)p.c.k + at, *const Vd = (T *)p.c.v + at;
-  const T *const Q = (const T *)p.q + row * p.q_rs, *const K = (const T *)p.k + row * p.k_rs,
-          *const V = (const T *)p.v + row * p.v_rs;
   T *const Qo = (T *)p.qo + row * p.qo_rs;
-  for (int i = tid % TPR; i < pieces; i += TPR) {
-    const int h = i / PIECES, e = (i % PIECES) * VEC;
-    if (h < kv0) {
-      u32x4 x = *(const u32x4 *)(Q + h * HD + e);
-      if (p.turn) x = rotate<T>(x, &cs[r][e / 2]);
-      *(u32x4 *)(Qo + h * HD + e) = x;
-    } else if (at >= 0 && h < v0) {
-      u32x4 x = *(const u32x4 *)(K + (h - kv0) * HD + e);
-      if (p.turn) x = rotate<T>(x, &cs[r][e / 2]);
-      *(u32x4 *)(Kd + (h - kv0) * p.c.head_stride + e) = x;
-    } else if (at >= 0) {
-      *(u32x4 *)(Vd + (h - v0) * p.c.head_stride + e) = *(const u32x4 *)(V + (h - v0) * HD + e);
+  for (int first = tid; first < pieces; first += kBatch * stride) {
+    if (first != tid) load(first);
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n) {
+      const int i = first + n * stride, h = i / PIECES, e = (i % PIECES) * VEC;
+      if (i >= pieces) break;
+      if (p.turn && h < v0) x[n] = rotate<T>(x[n], &cs[e / 2]);
+      if (h < kv0) *(u32x4 *)(Qo + h * HD + e) = x[n];
+      else if (at >= 0)
+        *(u32x4 *)((h < v0 ? Kd + (h - kv0) * p.c.head_stride : Vd + (h - v0) * p.c.head_stride) + e) = x[n];
     }
   }
 }
@@ -2566,6 +2574,7 @@ int bn_paged_append(const bn_paged_kv *cache, const void *k, const void *v, cons
   if (st || (st = check_starts(op, row_starts, n_rows, cache->batch))) return st;
   if (!q != !q_out) return fail(BN_ERR_INVALID_ARG, op + ": q and q_out must be given together");
   if (q && (st = check_heads(op, n_heads, cache->n_kv_heads, n_rows))) return st;
+  if (n_rows > (1 << 23)) return fail(BN_ERR_UNSUPPORTED, op + ": more than 2^23 rows");
   if (!(theta >= 0.f) || !std::isfinite(theta))
     return fail(BN_ERR_INVALID_ARG, op + ": theta must be positive and finite, or 0 for no rotation");
   if (n_rows == 0 || cache->batch == 0) return BN_OK;
@@ -2585,15 +2594,10 @@ int bn_paged_append(const bn_paged_kv *cache, const void *k, const void *v, cons
   for (int i = 0; i < HD / 2; ++i)
     p.f[i] = theta > 0.f ? std::pow((double)theta, -2.0 * i / HD) / (2.0 * M_PI) : 0.0;
   hipStream_t s = as_stream(stream);
-  const bool few = n_rows < 1024;
-  const dim3 grid(few ? n_rows : (n_rows + 7) / 8), block(256);
-  if (cache->dtype == BN_BF16) {
-    if (few) hipLaunchKernelGGL((paged_append_kernel<bf16_t, 1>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((paged_append_kernel<bf16_t, 8>), grid, block, 0, s, p);
-  } else {
-    if (few) hipLaunchKernelGGL((paged_append_kernel<float, 1>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((paged_append_kernel<float, 8>), grid, block, 0, s, p);
-  }
+  const int pieces = (p.n_heads + 2 * cache->n_kv_heads) * HD * (cache->dtype == BN_BF16 ? 2 : 4) / 16;
+  const dim3 grid(n_rows), block(std::min(256, (pieces + 127) / 128 * 64));
+  if (cache->dtype == BN_BF16) hipLaunchKernelGGL(paged_append_kernel<bf16_t>, grid, block, 0, s, p);
+  else hipLaunchKernelGGL(paged_append_kernel<float>, grid, block, 0, s, p);
   BN_LAUNCH_CHECK();
   return BN_OK;
 }

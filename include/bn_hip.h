@@ -469,7 +469,7 @@ int bn_gqa_decode_noalloc(int dtype, const void *q, const void *k_cache,
  * decreasing), row i of its n at position seq_lens[b] - n + i.  row_starts
  * NULL: one row per sequence (n_rows == batch).  n_rows counts the rows that
  * the tensors have; rows below row_starts[0] and from row_starts[batch] on are
- * padding, neither read nor written. */
+ * padding, left as they are. */
 typedef struct bn_paged_kv {
   void *k, *v;               /* pools (device) */
   const int32_t *page_table; /* device [batch, table_stride], max_pages entries a row */
@@ -488,7 +488,8 @@ typedef struct bn_paged_kv {
  * tensors); q, q_out: [n_rows, n_heads, 64] or both NULL.  A row whose position
  * lies outside the table, or on a page without memory, is not stored (its q
  * is written all the same); two rows that land on one place leave either's
- * elements there.  k, v, q and q_out must not lie in the pools. */
+ * elements there.  k, v, q and q_out must not lie in the pools.  At most 2^23
+ * rows. */
 int bn_paged_append(const bn_paged_kv *cache, const void *k, const void *v,
                     const void *q, void *q_out, const int32_t *row_starts,
                     int n_rows, int n_heads, int64_t k_row_stride,

@@ -94,6 +94,7 @@ def test_null_cache_and_empty_batch(name):
 
 @pytest.mark.parametrize("call,kw,status,msg", [
     (append, dict(n=-1), B.BN_ERR_SHAPE, "negative number of rows"),
+    (append, dict(n=(1 << 23) + 1), B.BN_ERR_UNSUPPORTED, "2^23 rows"),
     (append, dict(starts=None), B.BN_ERR_SHAPE, "one row per sequence"),
     (append, dict(starts=0x5002), B.BN_ERR_UNSUPPORTED, "row_starts"),
     (append, dict(q=None), B.BN_ERR_INVALID_ARG, "together"),
