@@ -822,7 +822,8 @@ struct PrefillParams {
   float *ws;
   unsigned long long *arrive_end;  // two arrival words per slot below it
   unsigned long long tag;
-  int slots;  // records that the workspace holds
+  int slots;      // records that the workspace holds
+  int parts_all;  // a part is at least 1 / parts_all of all the call's tiles
   // not 0: the rows are the batch's, the keys those of prefix_pages, and every unit's are
   // cut into so many parts, whose records are left for the launch that adds them
   int prefix_parts;
@@ -857,7 +858,6 @@ __device__ __forceinline__ void part_of(int n, const Piece &w, int &from, int &t
 }
 constexpr int kPartMin = 24;      // tiles of a part at least
 constexpr int kRow = HD + 4;      // floats of a prefix record's row
-constexpr int kPartsAll = 256;   // a part is at least this share of all the call's tiles
 
 // Which piece of work is workgroup L's.  A call's units differ in length (the
 // diagonal, and the sequences themselves): a unit whose keys are more than
@@ -915,7 +915,7 @@ __device__ __forceinline__ bool find_piece(const PrefillParams &p, int block, Pi
   float total = lane * per < n ? mine.weight : 0.f;
   for (int i = 1; i < per; ++i) total += lane * per + i < n ? seq(lane * per + i).weight : 0.f;
   total = wave_total(total);
-  const int share = max((int)(total * (float)hkv * (1.f / kPartsAll)), kPartMin);
+  const int share = max((int)(total * (float)hkv / (float)p.parts_all), kPartMin);
   // (a division only where it can come to 2 or more)
   auto parts_of = [&](const Seq &s) { return s.steps < 2 * share ? 1 : (int)((uint32_t)s.steps / (uint32_t)share); };
   auto count = [&](const Seq &s, bool in, int &all, int &cut) __attribute__((always_inline)) {
@@ -1854,21 +1854,29 @@ __device__ __forceinline__ void prefill_pipe_body(const PrefillParams &p, PipeLd
     const float *const r0 = p.ws + (int64_t)f.slot * R * kRec + 2 * row;
     float M = -INFINITY, L = 0.f;
     o[rt][0] = o[rt][1] = f32x16{};
-    for (int n = 0; n < f.parts; ++n) {
-      const float *const r = r0 + n * rec_step;
-      const float2 ml = get2(r + R * HD);
-      float2 x[16];
+    constexpr int MB = 2;  // records on their way together
+    for (int n0 = 0; n0 < f.parts; n0 += MB) {
+      float2 ml[MB], x[MB][16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = get2(r + R * (32 * (i >> 3) + 8 * ((i >> 1) & 3) + 4 * hf + 2 * (i & 1)));
-      const float mn = fmaxf(M, ml.x), mu = mn == -INFINITY ? 0.f : mn;
-      const float fo = __builtin_amdgcn_exp2f(M - mu), fn = __builtin_amdgcn_exp2f(ml.x - mu);
-      L = fmaf(ml.y, fn, L * fo);
+      for (int v = 0; v < MB; ++v) {
+        const float *const r = r0 + min(n0 + v, f.parts - 1) * rec_step;
+        ml[v] = get2(r + R * HD);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        o[rt][i >> 3][2 * (i & 7)] = fmaf(x[i].x, fn, o[rt][i >> 3][2 * (i & 7)] * fo);
-        o[rt][i >> 3][2 * (i & 7) + 1] = fmaf(x[i].y, fn, o[rt][i >> 3][2 * (i & 7) + 1] * fo);
+        for (int i = 0; i < 16; ++i) x[v][i] = get2(r + R * (32 * (i >> 3) + 8 * ((i >> 1) & 3) + 4 * hf + 2 * (i & 1)));
       }
-      M = mn;
+#pragma unroll
+      for (int v = 0; v < MB; ++v) {
+        if (n0 + v >= f.parts) break;
+        const float mn = fmaxf(M, ml[v].x), mu = mn == -INFINITY ? 0.f : mn;
+        const float fo = __builtin_amdgcn_exp2f(M - mu), fn = __builtin_amdgcn_exp2f(ml[v].x - mu);
+        L = fmaf(ml[v].y, fn, L * fo);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          o[rt][i >> 3][2 * (i & 7)] = fmaf(x[v][i].x, fn, o[rt][i >> 3][2 * (i & 7)] * fo);
+          o[rt][i >> 3][2 * (i & 7) + 1] = fmaf(x[v][i].y, fn, o[rt][i >> 3][2 * (i & 7) + 1] * fo);
+        }
+        M = mn;
+      }
     }
     write(t, h, rt, L);
   }
@@ -2385,9 +2393,18 @@ int launch_decode(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
 }
 
 // Which prefill kernel: by the units of 128 rows (32 in fp32) that the call has
-// at most.  Few of them: the keys of a unit are split over more waves.
+// at most.  Few of them: the keys of a unit are split over more waves.  The
+// pipelined kernel's units of 256 rows take twice as long a unit and need more
+// work to fill the card: many rows (2048 x 2 sequences 103 us, units of 128
+// 107; one of 2048 behind nothing 42, units of 128 37), or long sequences, which
+// the host knows only by what the table holds (behind 16384 keys 256 rows 95 ->
+// 61 us, 2048 rows 319 -> 275; behind nothing 1024 rows 21 -> 30 where the
+// table has room for 16384).  parts_all: one piece per compute unit, two of the
+// pipelined kernel's (2048 rows of 16384 317 -> 275 us) unless that makes many
+// records of few units (256 rows 61 -> 73).
 struct PrefillPlan {
   int hw, kw;  // (hw 8: the pipelined kernel)
+  int parts_all;
   int64_t groups, slots;   // workgroups of the launch, records
   size_t records, words;   // bytes
 };
@@ -2398,24 +2415,25 @@ PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv
   if (dtype == BN_F32) {
     d.hw = 1;
     d.kw = u32 <= 2048 ? 4 : 2;
+  } else if (u128 >= 2048 || (cap >= 16384 && u128 * cap >= 1 << 20)) {
+    d.hw = 8;
+    d.kw = 1;
   } else if (u128 < 256) {
     d.hw = 1;
     d.kw = u32 <= 256 ? 8 : 4;
-  } else if (u128 >= 2048) {
-    d.hw = 8;
-    d.kw = 1;
   } else {
     d.hw = 4;
     d.kw = u128 <= 768 ? 2 : 1;
   }
+  d.parts_all = d.hw == 8 && u128 >= 256 ? 512 : 256;
   const int R = 32 * d.hw;
   const int64_t units = std::min((rows + R - 1) / R + n_seq, rows);  // of a KV head, over the sequences
   // a sequence of U units, the longest of s tiles, counts U * s / 2 tiles at least and is cut
   // into U * floor(s / share) pieces: at most 2 * total / share in all, where total is
-  // below (share + 1) * kPartsAll / n_kv_heads and share at least kPartMin
+  // below (share + 1) * parts_all / n_kv_heads and share at least kPartMin
   const int64_t most_parts = std::max(1, (cap / 32 + 1) / kPartMin);
   const int64_t cut =
-      most_parts > 1 ? std::min<int64_t>(units * most_parts, (2 * kPartsAll + kPartsAll / 8) / n_kv_heads + 2) : 0;
+      most_parts > 1 ? std::min<int64_t>(units * most_parts, (2 * d.parts_all + d.parts_all / 8) / n_kv_heads + 2) : 0;
   const int64_t pieces = units + cut;
   const int per = n_kv_heads <= 8 && 8 % n_kv_heads == 0 ? 8 / n_kv_heads : 1;
   // (whole rounds of 32 pieces an XCD, which are taken in reverse order every second time)
@@ -2435,6 +2453,7 @@ int launch_prefill(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
   p.arrive_end = (unsigned long long *)((char *)ws + d.records + d.words);
   p.tag = next_tag();
   p.slots = (int)d.slots;
+  p.parts_all = d.parts_all;
   p.prefix_parts = 0;
   const dim3 grid((unsigned)d.groups);
   if (dtype == BN_F32) {

@@ -340,6 +340,27 @@ def test_prefill_large(case):
     assert torch.equal(bits(got[0]), bits(got[1])) and torch.equal(bits(got[0]), bits(got[2]))
 
 
+@pytest.mark.parametrize("lens,rows,Hkv,H", [
+    ([1, 0, 17, 300, 1000], [1, 0, 17, 200, 1000], 4, 32),
+    ([2000, 65, 64, 63], [700, 65, 1, 63], 4, 20),
+    ([5000], [513], 8, 64),
+    ([33] * 90, [3] * 90, 8, 64),
+], ids=str)
+def test_prefill_of_a_roomy_table(lens, rows, Hkv, H):
+    """Short sequences in a table with room for long ones, whose kernel runs then; what no row
+    sees is NaN and infinite."""
+    c = Case("bf16", lens, Hkv, 32, False, seed=H, drop=[(0, 0)], spare=1100)
+    q = rows_of("bf16", sum(rows), H, 3).cuda()
+    cache = c.cuda(B)
+    st = torch.from_numpy(starts_of(rows)).cuda()
+    ws = B.paged_workspace(cache, H, sum(rows))
+    got = [B.paged_prefill(q, cache, st, scale=0.125, workspace=w) for w in (ws, None)]
+    ref, tol = attention64_large(c, q, rows)
+    over = (got[0].double() - ref).abs() - tol
+    assert (over <= 0).all(), f"{int((over > 0).sum())} past the tolerance, by {float(over.max()):.2e}"
+    assert torch.equal(bits(got[0]), bits(got[1]))
+
+
 def test_prefill_starts_that_decrease_stay_inside():
     """row_starts out of order are the caller's mistake: the rows' values are not defined, but
     nothing outside o is written and the call returns."""

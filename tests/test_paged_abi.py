@@ -154,6 +154,17 @@ def test_workspace_sizes():
     assert L.bn_paged_workspace_size(C.byref(c), 32, -1, 0) == 0
 
 
+@pytest.mark.parametrize("dtype", [B.BN_F32, B.BN_BF16])
+def test_a_workspace_does_for_fewer_rows(dtype):
+    L = B.lib()
+    for pages, batch, hkv in ((8, 3, 2), (600, 3, 4), (1024, 70, 4), (4096, 1, 3), (9000, 5, 8)):
+        c = cache(dtype=dtype, batch=batch, max_pages=pages, table_stride=pages, n_kv_heads=hkv)
+        rows = sorted({n + d for n in (*range(0, 40), *(2 ** i * j for i in range(6, 15) for j in (4, 5, 6, 7)))
+                       for d in (0, 1)})
+        need = [L.bn_paged_workspace_size(C.byref(c), 8 * hkv, n, 0) for n in rows]
+        assert need == sorted(need)
+
+
 def test_a_workspace_too_small_is_refused():
     L = B.lib()
     c = cache(batch=64, max_pages=1024, table_stride=1024, n_pages=4096)
