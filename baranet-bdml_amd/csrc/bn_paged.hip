@@ -2394,12 +2394,12 @@ int launch_decode(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
 
 // Which prefill kernel: by the units of 128 rows (32 in fp32) that the call has
 // at most.  Few of them: the keys of a unit are split over more waves.  The
-// pipelined kernel's units of 256 rows take twice as long a unit and need more
-// work to fill the card: many rows (2048 x 2 sequences 103 us, units of 128
-// 107; one of 2048 behind nothing 42, units of 128 37), or long sequences, which
-// the host knows only by what the table holds (behind 16384 keys 256 rows 95 ->
-// 61 us, 2048 rows 319 -> 275; behind nothing 1024 rows 21 -> 30 where the
-// table has room for 16384).  parts_all: one piece per compute unit, two of the
+// pipelined kernel's units of 256 rows take longer to start and to fill the card:
+// it is for many rows in sequences of 512 new ones or more (one prompt of 2048
+// rows 42 us, units of 128 rows 37; of 4096 100 and 105; 64 prompts of 128 rows
+// 54 and 28), or for long sequences, which the host knows only by what the
+// table holds (behind 16384 keys 256 rows 95 -> 61 us, 2048 rows 319 -> 275;
+// behind nothing 1024 rows 21 -> 30 where the table has room for 16384).  parts_all: one piece per compute unit, two of the
 // pipelined kernel's (2048 rows of 16384 317 -> 275 us) unless that makes many
 // records of few units (256 rows 61 -> 73).
 struct PrefillPlan {
@@ -2408,14 +2408,17 @@ struct PrefillPlan {
   int64_t groups, slots;   // workgroups of the launch, records
   size_t records, words;   // bytes
 };
-PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv_heads, int cap) {
+// most: not this call's plan but one whose workspace does for any call of at
+// most as many rows (with fewer rows a sequence the kernel may be another).
+PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv_heads, int cap, bool most = false) {
   PrefillPlan d;
   const int64_t rows = (int64_t)n_rows * (n_heads / n_kv_heads);  // of a KV head
   const int64_t u128 = (rows / 128 + 1) * n_kv_heads, u32 = (rows / 32 + 1) * n_kv_heads;
+  const bool far = cap >= 16384 && u128 * cap >= 1 << 20, long_rows = n_rows / 512 >= n_seq;
   if (dtype == BN_F32) {
     d.hw = 1;
     d.kw = u32 <= 2048 ? 4 : 2;
-  } else if (u128 >= 2048 || (cap >= 16384 && u128 * cap >= 1 << 20)) {
+  } else if (far ? u128 < 1024 || long_rows || most : u128 >= 2048 && (long_rows || most)) {
     d.hw = 8;
     d.kw = 1;
   } else if (u128 < 256) {
@@ -2425,7 +2428,7 @@ PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv
     d.hw = 4;
     d.kw = u128 <= 768 ? 2 : 1;
   }
-  d.parts_all = d.hw == 8 && u128 >= 256 ? 512 : 256;
+  d.parts_all = d.hw == 8 && (u128 >= 256 || most) ? 512 : 256;
   const int R = 32 * d.hw;
   const int64_t units = std::min((rows + R - 1) / R + n_seq, rows);  // of a KV head, over the sequences
   // a sequence of U units, the longest of s tiles, counts U * s / 2 tiles at least and is cut
@@ -2441,7 +2444,7 @@ PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv
                                                            : pieces * n_kv_heads;
   d.slots = cut * n_kv_heads;
   d.records = (size_t)d.slots * R * kRec * sizeof(float);
-  d.words = (size_t)d.slots * 16 * d.hw;  // (16 are used; a call of fewer rows, whose records are smaller, needs no more)
+  d.words = (size_t)d.slots * 16 * d.hw;  // (16 are used: the words grow with the records)
   return d;
 }
 
@@ -2627,7 +2630,7 @@ size_t bn_paged_workspace_size(const bn_paged_kv *cache, int n_heads, int n_rows
       check_heads("", n_heads, cache->n_kv_heads, n_rows))
     return 0;
   const DecodePlan d = plan_decode(cache->batch, n_heads, cache->n_kv_heads);
-  const PrefillPlan f = plan_prefill(cache->dtype, cache->batch, n_rows, n_heads, cache->n_kv_heads, c.cap);
+  const PrefillPlan f = plan_prefill(cache->dtype, cache->batch, n_rows, n_heads, cache->n_kv_heads, c.cap, true);
   size_t need = std::max(d.records + d.words, f.records + f.words);
   if (prefix_len > 0) {
     const SharedPlan s = plan_shared(cache->dtype, cache->batch, n_heads, cache->n_kv_heads, std::min(prefix_len, c.cap));
