@@ -856,7 +856,7 @@ __device__ __forceinline__ void part_of(int n, const Piece &w, int &from, int &t
     to = from + q + (w.part < r);
   }
 }
-constexpr int kPartMin = 24;      // tiles of a part at least
+constexpr int kPartMin = 24;      // tiles of a part at least (1024 rows of nothing before them in 8: 30 -> 33 us)
 constexpr int kRow = HD + 4;      // floats of a prefix record's row
 
 // Which piece of work is workgroup L's.  A call's units differ in length (the
@@ -2334,7 +2334,9 @@ unsigned long long next_tag() {
   return (z ^ (z >> 31)) >> 16 | 1;
 }
 
-// The decode kernel's launch: a workgroup per share and column.
+// The decode kernel's launch: a workgroup per share and column, one per compute
+// unit in all (two: 64 caches of 4096 keys 45.8 -> 49.0 us, of 512..4096 34.6 ->
+// 35.7; 256 of 300 21.4 -> 18.8).
 constexpr int kDecGroups = 256;
 struct DecodePlan {
   int hblocks, columns, bins;
@@ -2417,16 +2419,16 @@ PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv
   const bool far = cap >= 16384 && u128 * cap >= 1 << 20, long_rows = n_rows / 512 >= n_seq;
   if (dtype == BN_F32) {
     d.hw = 1;
-    d.kw = u32 <= 2048 ? 4 : 2;
+    d.kw = u32 <= 1024 ? 4 : 2;  // (one prompt of 512 rows 23 us, with 2 waves a unit 30; four of 300 39 and 31)
   } else if (far ? u128 < 1024 || long_rows || most : u128 >= 2048 && (long_rows || most)) {
     d.hw = 8;
     d.kw = 1;
   } else if (u128 < 256) {
-    d.hw = 1;
-    d.kw = u32 <= 256 ? 8 : 4;
+    d.hw = 1;  // (700 rows behind nothing 12.6 us, units of 128 rows 16.3; 256 x 3 behind 8192 93 and 106)
+    d.kw = u32 <= 256 ? 8 : 4;  // (128 rows behind 8000 30 us, with 4 waves 34; 300 rows 43 and 37)
   } else {
     d.hw = 4;
-    d.kw = u128 <= 768 ? 2 : 1;
+    d.kw = u128 <= 768 ? 2 : 1;  // (2000 rows 37 us, with 1 wave a row block 48; 777 x 4 31 and 27)
   }
   d.parts_all = d.hw == 8 && (u128 >= 256 || most) ? 512 : 256;
   const int R = 32 * d.hw;
@@ -2488,7 +2490,11 @@ SharedPlan plan_shared(int dtype, int batch, int n_heads, int n_kv_heads, int pr
   SharedPlan s;
   s.d = plan_decode(batch, n_heads, n_kv_heads);
   const int64_t rows = (int64_t)batch * (n_heads / n_kv_heads);
-  s.hw = dtype == BN_BF16 && rows * n_kv_heads >= 32 * 128 ? 8 : 1;
+  // units of 256 rows (the pipelined kernel) once there is work enough to fill the card with them:
+  // 64 sequences of 32 heads behind 16384 keys 37 us, with units of 32 rows 42; 100 behind 8192 35
+  // and 41; but 64 behind 8192 29 and 27, 16 behind 65536 49 and 44
+  const int64_t work = rows * n_kv_heads * prefix_len;
+  s.hw = dtype == BN_BF16 && rows * n_kv_heads >= 1024 && work >= 3 << 23 ? 8 : 1;
   const int R = 32 * s.hw, steps = (prefix_len + 31) / 32;
   const int64_t units = (rows + R - 1) / R;
   // pieces: one per compute unit, of 8 tiles at least; two of the large kernel's if they keep 32

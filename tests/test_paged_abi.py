@@ -163,6 +163,9 @@ def test_a_workspace_does_for_fewer_rows(dtype):
                        for d in (0, 1)})
         need = [L.bn_paged_workspace_size(C.byref(c), 8 * hkv, n, 0) for n in rows]
         assert need == sorted(need)
+        need = [L.bn_paged_workspace_size(C.byref(c), 8 * hkv, batch, P)
+                for P in (0, 1, 100, 1000, 4000, 5000, 16000, 17000, 30000, 60000, 140000) if P <= pages * 16]
+        assert need == sorted(need)
 
 
 def test_a_workspace_too_small_is_refused():
