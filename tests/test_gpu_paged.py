@@ -501,7 +501,9 @@ def test_shared(case):
 
 
 @pytest.mark.parametrize("case", [("bf16", 2048, 200, 700, 4, 32, 16), ("bf16", 4096, 150, 3000, 8, 8, 32),
-                                  ("bf16", 640, 700, 90, 4, 20, 64), ("f32", 1024, 70, 900, 4, 16, 16)],
+                                  ("bf16", 640, 700, 90, 4, 20, 64), ("f32", 1024, 70, 900, 4, 16, 16),
+                                  ("bf16", 4096, 210, 700, 4, 32, 16), ("bf16", 16384, 100, 300, 1, 16, 32),
+                                  ("bf16", 16384, 100, 100, 4, 20, 64)],
                          ids=lambda c: "-".join(map(str, c)))
 def test_shared_large(case):
     """Large batches (the pipelined kernel) and own keys cut over workgroups; some sequences shorter
@@ -527,6 +529,31 @@ def test_shared_large(case):
     over = (got[0].double() - ref).abs() - tol
     assert (over <= 0).all(), f"{int((over > 0).sum())} past the tolerance, by {float(over.max()):.2e}"
     assert torch.equal(bits(got[0]), bits(got[1])) and torch.equal(bits(got[0]), bits(got[2]))
+
+
+@pytest.mark.parametrize("Bn,P", [(100, 1024), (100, 16384)], ids=["few", "many"])
+def test_shared_prefix_values_that_short_sequences_do_not_see(Bn, P):
+    """Infinite and NaN values of the prefix behind the end of some sequences: these come out as
+    without them, bit for bit, and the others carry them."""
+    H, Hkv, page, dirty = 32, 4, 32, P - 40
+    lens = [P + b % 5 if b % 3 else P - 64 - b for b in range(Bn)]
+    c = Case("bf16", lens, Hkv, page, True, seed=P, nan=False)
+    q = rows_of("bf16", Bn, H, 1).cuda()
+    cache = c.cuda(B)
+    prefix = torch.from_numpy(c.table[1, :P // page].copy()).cuda()
+    ws = B.paged_workspace(cache, H, Bn, P)
+    clean = B.paged_decode_shared(q, cache, prefix, P, scale=0.125, workspace=ws)
+    at = (int(c.table[1, dirty // page]), slice(None), dirty % page)
+    cache.v_pages[at][:, 3] = float("inf")
+    cache.v_pages[at][:, 40] = float("nan")
+    cache.v_pages[at][:, 41] = float("-inf")
+    got = B.paged_decode_shared(q, cache, prefix, P, scale=0.125, workspace=ws)
+    sees = torch.tensor([n > dirty for n in lens]).cuda()
+    assert torch.equal(bits(got[~sees]), bits(clean[~sees])) and torch.isfinite(clean.float()).all()
+    assert (got[sees][..., 3] == float("inf")).all() and (got[sees][..., 41] == float("-inf")).all()
+    assert torch.isnan(got[sees][..., 40]).all()
+    rest = [d for d in range(64) if d not in (3, 40, 41)]
+    assert torch.equal(bits(got[sees][..., rest].contiguous()), bits(clean[sees][..., rest].contiguous()))
 
 
 def test_shared_prefix_page_without_memory():
