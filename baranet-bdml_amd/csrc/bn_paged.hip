@@ -824,6 +824,7 @@ struct PrefillParams {
   unsigned long long tag;
   int slots;      // records that the workspace holds
   int parts_all;  // a part is at least 1 / parts_all of all the call's tiles
+  int pieces;     // of a KV head, at most
   // not 0: the rows are the batch's, the keys those of prefix_pages, and every unit's are
   // cut into so many parts, whose records are left for the launch that adds them
   int prefix_parts;
@@ -927,7 +928,10 @@ __device__ __forceinline__ bool find_piece(const PrefillParams &p, int block, Pi
   count(mine, lane * per < n, all, cut);
   for (int i = 1; i < per; ++i) count(seq(lane * per + i), lane * per + i < n, all, cut);
   int up = wave_scan(all), up_cut = wave_scan(cut);
-  if (idx >= __builtin_amdgcn_readlane(up, 63)) return false;
+  // (row_starts that decrease can count more pieces than the launch has: then none is
+  // done, so that no count of a unit's parts is left unfinished in the workspace)
+  const int total_pieces = __builtin_amdgcn_readlane(up, 63);
+  if (idx >= total_pieces || total_pieces > p.pieces) return false;
   int src, b, k, cuts;  // lane and number of the sequence, piece of it, pieces of cut sequences before it
   if (per == 1) {
     // The longest first over all sequences: from one unit to the one before it
@@ -2407,7 +2411,7 @@ int launch_decode(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
 struct PrefillPlan {
   int hw, kw;  // (hw 8: the pipelined kernel)
   int parts_all;
-  int64_t groups, slots;   // workgroups of the launch, records
+  int64_t pieces, groups, slots;  // pieces of a KV head, workgroups of the launch, records
   size_t records, words;   // bytes
 };
 // most: not this call's plan but one whose workspace does for any call of at
@@ -2439,7 +2443,7 @@ PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv
   const int64_t most_parts = std::max(1, (cap / 32 + 1) / kPartMin);
   const int64_t cut =
       most_parts > 1 ? std::min<int64_t>(units * most_parts, (2 * d.parts_all + d.parts_all / 8) / n_kv_heads + 2) : 0;
-  const int64_t pieces = units + cut;
+  const int64_t pieces = d.pieces = units + cut;
   const int per = n_kv_heads <= 8 && 8 % n_kv_heads == 0 ? 8 / n_kv_heads : 1;
   // (whole rounds of 32 pieces an XCD, which are taken in reverse order every second time)
   d.groups = per > 1 || n_kv_heads == 8 || n_kv_heads == 1 ? ((pieces + per - 1) / per + 31) / 32 * 32 * per * n_kv_heads
@@ -2459,6 +2463,7 @@ int launch_prefill(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
   p.tag = next_tag();
   p.slots = (int)d.slots;
   p.parts_all = d.parts_all;
+  p.pieces = (int)d.pieces;
   p.prefix_parts = 0;
   const dim3 grid((unsigned)d.groups);
   if (dtype == BN_F32) {

@@ -648,6 +648,22 @@ def test_host_memory_is_refused():
     assert s == B.BN_ERR_NOT_DEVICE and "only GPU implementation available" in m
 
 
+def test_a_workspace_after_starts_that_decrease():
+    """A call with row_starts out of order leaves nothing in its workspace that a later one trips over."""
+    for n, H, Hkv in ((600, 16, 2), (40, 8, 1)):
+        c = Case("bf16", [5000] * 40, Hkv, 16, True, seed=n, nan=False, spare=0)
+        q = rows_of("bf16", n, H, 2).cuda()
+        cache = c.cuda(B)
+        good = torch.tensor([0] + [n // 2] * 39 + [n], dtype=torch.int32).cuda()
+        ws = B.paged_workspace(cache, H, n)
+        want = B.paged_prefill(q, cache, good, scale=0.125)
+        for bad in ([0, n] * 20 + [0], [n, 0] * 20 + [n], [0] + [n, n // 2] * 20, list(range(40, -1, -1))):
+            B.paged_prefill(q, cache, torch.tensor(bad, dtype=torch.int32).cuda(), scale=0.125, workspace=ws)
+            for _ in range(2):
+                got = B.paged_prefill(q, cache, good, scale=0.125, workspace=ws)
+                assert torch.equal(bits(got), bits(want))
+
+
 # ------------------------------------------------------------------- together
 @pytest.mark.parametrize("dtype,page,layout", [("f32", 16, True), ("bf16", 8, False), ("bf16", 32, True)])
 def test_a_server_run(dtype, page, layout):
