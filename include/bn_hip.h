@@ -469,7 +469,8 @@ int bn_gqa_decode_noalloc(int dtype, const void *q, const void *k_cache,
  * decreasing), row i of its n at position seq_lens[b] - n + i.  row_starts
  * NULL: one row per sequence (n_rows == batch).  n_rows counts the rows that
  * the tensors have; rows below row_starts[0] and from row_starts[batch] on are
- * padding, left as they are. */
+ * padding, left as they are.  The table, the lengths and row_starts are read
+ * when a call runs and must not change until it has ended. */
 typedef struct bn_paged_kv {
   void *k, *v;               /* pools (device) */
   const int32_t *page_table; /* device [batch, table_stride], max_pages entries a row */
