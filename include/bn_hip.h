@@ -458,7 +458,7 @@ int bn_gqa_decode_noalloc(int dtype, const void *q, const void *k_cache,
  * above max_pages*page_size counts as that many keys.  A page number outside
  * [0, n_pages) has no memory: its keys are not stored and are hidden from every
  * query (a page that was given up, an entry not yet set).  Entries past a
- * sequence's last key are not looked at.  page_size: a power of two, at least 8.
+ * sequence's last key are not looked at.  page_size: a power of two in [8, 2^20].
  * head_dim must be 64, and dtype BN_F32 or BN_BF16 for the pools, the queries
  * and the outputs alike; sums and softmax statistics are fp32.  Any number of
  * query heads per KV head; query head h reads KV head h / (n_heads /

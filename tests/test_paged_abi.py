@@ -58,6 +58,8 @@ CALLS = {"Paged append": append, "Paged decode": decode, "Paged prefill": prefil
     (dict(page_size=4), B.BN_ERR_UNSUPPORTED, "at least 8"),
     (dict(row_stride=(1 << 24) + 8), B.BN_ERR_UNSUPPORTED, "2^24"),
     (dict(page_size=-16), B.BN_ERR_UNSUPPORTED, "power of two"),
+    (dict(page_size=1 << 21, max_pages=1), B.BN_ERR_UNSUPPORTED, "2^20"),
+    (dict(page_size=1 << 25, max_pages=1, n_pages=1), B.BN_ERR_UNSUPPORTED, "2^20"),
     (dict(max_pages=1 << 27), B.BN_ERR_UNSUPPORTED, "2^30"),
     (dict(batch=(1 << 20) + 1), B.BN_ERR_SHAPE | B.BN_ERR_UNSUPPORTED, ""),
     (dict(row_stride=32), B.BN_ERR_INVALID_ARG, "strides"),
