@@ -2232,7 +2232,7 @@ int check_cache(const std::string &op, const bn_paged_kv *kv, Paged *c) {
   if (kv->n_kv_heads <= 0) return fail(BN_ERR_SHAPE, op + ": num_kv_heads must be positive");
   if (kv->head_dim != HD) return fail(BN_ERR_UNSUPPORTED, op + ": head_dim must be 64");
   if (kv->page_size < 8 || kv->page_size > (1 << 20) || (kv->page_size & (kv->page_size - 1)))
-    return fail(BN_ERR_UNSUPPORTED, op + ": page_size must be a power of two in [8, 2^20]");
+    return fail(BN_ERR_UNSUPPORTED, op + ": page_size must be a power of two, at least 8 and at most 2^20");
   const int64_t keys = (int64_t)kv->max_pages * kv->page_size;
   if (keys > (1 << 30))
     return fail(BN_ERR_UNSUPPORTED, op + ": max_pages * page_size must be at most 2^30 keys");
