@@ -257,6 +257,19 @@ def test_decode_offsets_past_32_bits():
         assert (np.abs(got3[b] - (p @ v).numpy()) <= (p @ v.abs()).numpy() * (4 * 2.0 ** -8)).all()
 
 
+def test_append_offsets_past_32_bits():
+    """Rows stored in the last and in a middle page of a pool of more than 2^32 bytes."""
+    n_pages, page, Hkv = 70000, 512, 1
+    pools = [torch.zeros((n_pages, Hkv, page, D), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    table = torch.tensor([[3, n_pages - 1], [69000, 2]], dtype=torch.int32, device="cuda")
+    cache = B.PagedKV(*pools, table, torch.tensor([page + 7, 100], dtype=torch.int32, device="cuda"))
+    k, v = (torch.randn((2, Hkv, D), device="cuda").bfloat16() for _ in range(2))
+    B.paged_append(cache, k, v, theta=0.0)
+    for pool, x in zip(pools, (k, v)):
+        assert torch.equal(pool[n_pages - 1, 0, 6], x[0, 0]) and torch.equal(pool[69000, 0, 99], x[1, 0])
+        assert int(pool.count_nonzero()) == int(x.count_nonzero())
+
+
 # ------------------------------------------------------------------- prefill
 PREFILLS = [
     # dtype, lens (with the new rows), rows, Hkv, H, page, layout, dropped pages, padding rows
@@ -617,6 +630,36 @@ def test_graphs_share_a_workspace(op):
             junk = torch.empty_like(ws)
             if step == 1:
                 ws.copy_(junk.random_(0, 256))
+
+
+def test_a_graph_of_cut_units():
+    """Long sequences, whose units of 256 rows are cut and added up in the launch, replayed from a
+    graph under other lengths, with eager calls of another shape on the same workspace between."""
+    lens, rows = [17000, 6000, 20000], [300, 1, 45]
+    c = Case("bf16", lens, 2, 64, True, seed=3, nan=False)
+    cache = c.cuda(B)
+    q = rows_of("bf16", sum(rows), 32, 6).cuda()
+    st = torch.from_numpy(starts_of(rows)).cuda()
+    ws = B.paged_workspace(cache, 32, sum(rows))
+    o = torch.zeros_like(q)
+    B.paged_prefill(q, cache, st, o=o, scale=0.125, workspace=ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        B.paged_prefill(q, cache, st, o=o, scale=0.125, workspace=ws)
+    for now in (lens, [300, 1, 45], [16999, 0, 9000], lens):
+        cache.seq_lens.copy_(torch.tensor(now, dtype=torch.int32))
+        o.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        got = o.clone()
+        assert torch.equal(bits(got), bits(B.paged_prefill(q, cache, st, scale=0.125)))
+        B.paged_decode(q[:3], cache, scale=0.125, workspace=ws)
+        B.paged_prefill(q[:7], cache, torch.tensor([0, 4, 4, 7], dtype=torch.int32).cuda(), scale=0.125, workspace=ws)
+    c.lens = lens
+    ref, tol = attention64_large(c, q, rows)
+    over = (got.double() - ref).abs() - tol
+    assert (over <= 0).all(), f"{int((over > 0).sum())} past the tolerance, by {float(over.max()):.2e}"
 
 
 def test_calls_on_two_streams():
