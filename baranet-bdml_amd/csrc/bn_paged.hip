@@ -2442,7 +2442,8 @@ PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv
     d.kw = 1;
   } else if (u128 < 256) {
     d.hw = 1;  // (700 rows behind nothing 12.6 us, units of 128 rows 16.3; 256 x 3 behind 8192 93 and 106)
-    d.kw = u32 <= 256 ? 8 : 4;  // (128 rows behind 8000 30 us, with 4 waves 34; 300 rows 43 and 37)
+    // (256 rows behind 4096 29 us, with 4 waves 33; behind nothing 9.7 and 8.5; 300 behind 3700 43 and 37)
+    d.kw = (rows + 31) / 32 * n_kv_heads <= 256 ? 8 : 4;
   } else {
     d.hw = 4;
     d.kw = u128 <= 768 ? 2 : 1;  // (2000 rows 37 us, with 1 wave a row block 48; 777 x 4 31 and 27)
