@@ -1261,12 +1261,24 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
   auto gload = [&](int i) __attribute__((always_inline)) {
     uint32_t o32 = off;
     asm volatile("" : "+v"(o32));  // a scalar base and this offset, not a sum of pointers kept in registers
-    chunks_next = 0;
+    // Four chunks: a lane forms its chunk's offset (in scalars, chunk by chunk, 60 instructions in
+    // the wave's way: 256 rows behind 4096 keys 28.1 us where this takes 26.5).
+    uint64_t mine = 0;
+    if constexpr (NC > 1) {
+      mine = rows.at(entry, key_of(i) + 8 * (NC * hw + (lane & (NC - 1))));
+      chunks_next = (int)__builtin_amdgcn_ballot_w64(rows.there(entry)) & ((1 << NC) - 1);
+    }
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      const int id = __builtin_amdgcn_readlane(entry, j);
-      chunks_next |= rows.there(id) << j;
-      const uint64_t at = rows.at(id, key_of(i) + 8 * (NC * hw + j));
+      uint64_t at;
+      if constexpr (NC > 1) {
+        at = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, j) |
+             (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(mine >> 32), j) << 32;
+      } else {
+        const int id = __builtin_amdgcn_readlane(entry, 0);
+        chunks_next = rows.there(id);
+        at = rows.at(id, key_of(i) + 8 * hw);
+      }
       kr[j] = *(const u32x4 *)(Kg + at + o32);
       vr[j] = *(const u32x4 *)(Vg + at + o32);
     }
