@@ -1186,7 +1186,7 @@ __device__ __forceinline__ void finish_piece(const PrefillParams &p, const Piece
 // reference that moves to the true maximum only when a tile's sum passes 2^16.
 // <4,1>: 7 prompts of 165..1500 tokens 51 us (534 TFLOP/s), VALU 58% and LDS 52%
 // busy, the rest the units' start and end; <1,4>: 256 rows each behind 2697, 5444
-// and 8192 keys 63 us (557), the LDS port 99% busy, but units of 64 rows, with
+// and 8192 keys 61 us (571), the LDS port 99% busy, but units of 64 rows, with
 // half its traffic and two waves a SIMD in place of three, took 6% longer.
 constexpr float kSumLimit = 65536.f, kMoveLog2 = 8.f;
 template <int HW, int KW>
