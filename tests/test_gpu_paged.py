@@ -317,6 +317,20 @@ def test_prefill(case):
         assert torch.equal(bits(o2), bits(o)), "a second call differs"
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("H", [16, 32, 64])
+@pytest.mark.parametrize("lens,rows", [([2 ** 31 - 1, 40], [70, 40]), ([40, 2 ** 31 - 1, 3], [4, 7, 3])], ids=["many", "few"])
+def test_prefill_lengths_past_the_table(dtype, H, lens, rows):
+    """A length past the table, in large groups of heads, leaves the sequences beside it their rows."""
+    print("prefill past the table", dtype, H, lens, rows, flush=True)
+    c = Case(dtype, lens, 1, 16, True, seed=H, max_pages=9)
+    q = rows_of(dtype, sum(rows), H, 11)
+    ref, tol = attention64(c, q, rows)
+    st = torch.from_numpy(starts_of(rows)).cuda()
+    o = torch.full_like(q, 7.0).cuda()
+    check(host(B.paged_prefill(q.cuda(), c.cuda(B), st, o=o, scale=0.125)), ref, tol, "prefill")
+
+
 # many rows, and rows behind long caches: each kernel that the host can pick, whole units and cut ones
 LARGE = [
     ("bf16", [700, 433, 400], [700, 33, 400], 4, 32, 16),
