@@ -146,22 +146,23 @@ __device__ __forceinline__ bool find_piece(const PrefillParams &p, int block, Pi
   float total = lane * per < n ? mine.weight : 0.f;
   for (int i = 1; i < per; ++i) total += lane * per + i < n ? seq(lane * per + i).weight : 0.f;
   total = wave_total(total);
-  const int share = max((int)(total * (float)hkv / (float)p.parts_all), kPartMin);
+  const int share = max((int)min(total * (float)hkv / (float)p.parts_all, 536870912.f), kPartMin);
   // (a division only where it can come to 2 or more)
   auto parts_of = [&](const Seq &s) { return s.steps < 2 * share ? 1 : (int)((uint32_t)s.steps / (uint32_t)share); };
   auto count = [&](const Seq &s, bool in, int &all, int &cut) __attribute__((always_inline)) {
     const int parts = parts_of(s), k = in ? s.units * parts : 0;
-    all += k;
-    cut += parts > 1 ? k : 0;
+    all = min(all + k, p.pieces + 1);
+    cut = min(cut + (parts > 1 ? k : 0), p.pieces + 1);
   };
   int all = 0, cut = 0;
   count(mine, lane * per < n, all, cut);
   for (int i = 1; i < per; ++i) count(seq(lane * per + i), lane * per + i < n, all, cut);
   int up = wave_scan(all), up_cut = wave_scan(cut);
   // (row_starts that decrease can count more pieces than the launch has: then none is
-  // done, so that no count of a unit's parts is left unfinished in the workspace)
-  const int total_pieces = __builtin_amdgcn_readlane(up, 63);
-  if (idx >= total_pieces || total_pieces > p.pieces) return false;
+  // done, so that no count of a unit's parts is left unfinished in the workspace; a lane
+  // counts no further than one too many, and 64 of those are below 2^32)
+  const uint32_t total_pieces = (uint32_t)__builtin_amdgcn_readlane(up, 63);
+  if ((uint32_t)idx >= total_pieces || total_pieces > (uint32_t)p.pieces) return false;
   int src, b, k, cuts;  // lane and number of the sequence, piece of it, pieces of cut sequences before it
   if (per == 1) {
     // The longest first over all sequences: from one unit to the one before it

@@ -1,7 +1,7 @@
 // Runs the paged prefill's plan and every workgroup's search for its piece on
 // the CPU: a wave's 64 lanes are coroutines that meet at each operation across
 // lanes.  Reads one call from stdin -- dtype (0 fp32, 1 bf16), batch, n_rows,
-// n_heads, n_kv_heads, cap, then batch lengths and batch + 1 row starts -- and
+// n_heads, n_kv_heads, cap, workgroups to run at most, then batch lengths and batch + 1 row starts -- and
 // prints the plan (rows of a unit, workgroups, pieces, slots, bytes of records) and a
 // line per piece found: workgroup b g unit part parts row0 rows slot tok0 rem0.
 #include <setjmp.h>
@@ -51,11 +51,11 @@ int wave_scan(int x) {
   const int64_t *v = meet(x);
   int64_t s = 0;
   for (int l = 0; l <= current; ++l) s += v[l];
-  if (s != (int)s) {
+  if (s < INT32_MIN || s > UINT32_MAX) {
     fprintf(stderr, "a scan passes 32 bits: %lld\n", (long long)s);
     exit(2);
   }
-  return (int)s;
+  return (int)(uint32_t)s;
 }
 int wave_min(int x) {
   const int64_t *v = meet(x);
@@ -158,8 +158,8 @@ void run_wave() {
 }  // namespace
 
 int main() {
-  int dtype, batch, n_rows, n_heads, hkv, cap;
-  if (scanf("%d %d %d %d %d %d", &dtype, &batch, &n_rows, &n_heads, &hkv, &cap) != 6) return 1;
+  int dtype, batch, n_rows, n_heads, hkv, cap, most;
+  if (scanf("%d %d %d %d %d %d %d", &dtype, &batch, &n_rows, &n_heads, &hkv, &cap, &most) != 7) return 1;
   std::vector<int32_t> lens(batch), starts(batch + 1);
   for (auto &x : lens)
     if (scanf("%d", &x) != 1) return 1;
@@ -183,7 +183,7 @@ int main() {
   rows_of_unit = 32 * d.hw;
   printf("%d %lld %lld %lld %lld\n", rows_of_unit, (long long)d.groups, (long long)d.pieces, (long long)d.slots,
          (long long)d.records);
-  for (block = 0; block < d.groups; ++block) {
+  for (block = 0; block < std::min<int64_t>(d.groups, most); ++block) {
     run_wave();
     for (int l = 1; l < LANES; ++l)
       if (found[l] != found[0] || (found[0] && __builtin_memcmp(&pieces[l], &pieces[0], sizeof(Piece)))) {

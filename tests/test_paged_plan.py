@@ -19,8 +19,8 @@ def plan(tmp_path_factory):
                     "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(ROOT, "baranet-bdml_amd", "csrc"),
                     os.path.join(ROOT, "tests", "paged_plan.cpp"), "-o", exe], check=True)
 
-    def run(dtype, lens, starts, n_rows, H, Hkv, cap):
-        text = " ".join(map(str, [int(dtype == "bf16"), len(lens), n_rows, H, Hkv, cap, *lens, *starts]))
+    def run(dtype, lens, starts, n_rows, H, Hkv, cap, most=1 << 30):
+        text = " ".join(map(str, [int(dtype == "bf16"), len(lens), n_rows, H, Hkv, cap, most, *lens, *starts]))
         p = subprocess.run([exe], input=text, capture_output=True, text=True, timeout=60)
         assert p.returncode == 0, p.stderr
         first, *rest = ([int(x) for x in line.split()] for line in p.stdout.splitlines())
@@ -108,3 +108,23 @@ def test_drawn_calls(plan):
         lens = [r.choice([n, n + r.randint(0, cap), r.randint(0, cap), INT_MAX, -3]) for n in rows]
         if sum(rows):
             deal(plan, r.choice(["f32", "bf16"]), lens, rows, H, Hkv, cap, r.choice([0, 2]))
+
+
+@pytest.mark.parametrize("batch", [1, 70])
+def test_tiles_past_32_bits(plan, batch):
+    """Many rows of long sequences: the share of a workgroup, in tiles, stays a share."""
+    rows = [(1 << 20) // batch] * batch
+    (R, *_), found = plan("bf16", [1 << 30] * batch, starts_of(rows), sum(rows), 32, 1, 1 << 30, 5)
+    assert len({(b, g, unit, part) for _, b, g, unit, part, *_ in found}) == 5
+    assert all(of == 1 for _, _, _, _, _, of, *_ in found)
+
+
+@pytest.mark.parametrize("dtype,n,H", [("bf16", 1 << 21, 64), ("f32", 1 << 19, 64)])
+def test_starts_that_decrease_count_no_further_than_32_bits(plan, dtype, n, H):
+    """Row starts out of order count the same rows again and again, here 2^32 units and those of 40 rows
+    more: too many, so that no workgroup takes any."""
+    R = 128 if dtype == "bf16" else 32
+    times = (1 << 32) // (n * H // R)
+    starts = [0, n] * times + [n - 40, n]
+    (got, *_), found = plan(dtype, [5] * (len(starts) - 1), starts, n, H, 1, 64, 3)
+    assert got == R and not found
