@@ -2309,6 +2309,22 @@ int launch_shared(const AttnParams &a, int dtype, void *ws, hipStream_t s) {
   return BN_OK;
 }
 
+// The threads of a call's launches, which the runtime counts in 32 bits.
+int check_launch(const std::string &op, int dtype, int batch, const int32_t *starts, int n_rows, int n_heads,
+                 int n_kv_heads, int cap, int prefix_len) {
+  int64_t threads = 0;
+  if (prefix_len > 0) {
+    const SharedPlan m = plan_shared(dtype, batch, n_heads, n_kv_heads, prefix_len);
+    threads = std::max((m.d.bins * m.d.columns + m.n_pre + 16) * 256, (int64_t)batch * n_heads * (HD / 2) + 256);
+  } else if (starts) {
+    const PrefillPlan d = plan_prefill(dtype, batch, n_rows, n_heads, n_kv_heads, cap);
+    threads = d.groups * (d.hw == 8 ? 256 : 64 * d.hw * d.kw);
+  }
+  if (threads >= (int64_t)1 << 32)
+    return fail(BN_ERR_UNSUPPORTED, op + ": too many rows and sequences for one launch (2^32 threads)");
+  return BN_OK;
+}
+
 int attention(const char *name, const bn_paged_kv *kv, const void *q, void *o, const int32_t *starts,
               int n_rows, int n_heads, int64_t q_rs, int64_t o_rs, float scale,
               const int32_t *prefix_pages, int prefix_len, void *workspace, size_t workspace_bytes,
@@ -2330,6 +2346,9 @@ int attention(const char *name, const bn_paged_kv *kv, const void *q, void *o, c
   if (prefix_len > 0 && !prefix_pages) return fail(BN_ERR_INVALID_ARG, op + ": prefix_pages is NULL");
   if ((uintptr_t)prefix_pages & 3u)
     return fail(BN_ERR_UNSUPPORTED, op + ": prefix_pages must be 4-byte aligned");
+  p.prefix_len = std::min(prefix_len, p.c.cap);
+  if ((st = check_launch(op, kv->dtype, kv->batch, starts, n_rows, n_heads, kv->n_kv_heads, p.c.cap, p.prefix_len)))
+    return st;
   const size_t need = bn_paged_workspace_size(kv, n_heads, n_rows, prefix_len);
   if (workspace && workspace_bytes < need)
     return fail(BN_ERR_INVALID_ARG, op + ": workspace of " + std::to_string(workspace_bytes) +
@@ -2343,7 +2362,7 @@ int attention(const char *name, const bn_paged_kv *kv, const void *q, void *o, c
   p.n_rows = n_rows; p.n_heads = n_heads; p.group = n_heads / kv->n_kv_heads;
   p.inv_group = 1.0f / (float)p.group;
   p.cl = scale * kLog2e;
-  p.prefix_pages = prefix_pages; p.prefix_len = std::min(prefix_len, p.c.cap);
+  p.prefix_pages = prefix_pages;
   Workspace ws;
   if ((st = ws.take(workspace, need, stream))) return st;
   hipStream_t s = as_stream(stream);

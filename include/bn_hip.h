@@ -497,7 +497,12 @@ int bn_paged_append(const bn_paged_kv *cache, const void *k, const void *v,
                     int64_t v_row_stride, int64_t q_row_stride,
                     int64_t q_out_row_stride, float theta, void *stream);
 
-/* Workspace of the three attention calls below for up to n_rows query rows
+/* The three attention calls below take n_rows * n_heads up to 2^30 and are
+ * refused where a launch would pass 2^32 threads: never up to 2^23 units,
+ * n_rows * n_heads / 32 + batch * n_kv_heads; with a shared prefix also from
+ * batch * n_heads of 2^27 on.
+ *
+ * Workspace of theirs for up to n_rows query rows
  * (decode: the batch) and prefix_len common keys (0 without): bytes of device
  * memory, 16-byte aligned, any contents.  NULL there: the pool supplies it.
  * Calls in flight at once need workspaces of their own. */

@@ -236,3 +236,28 @@ def test_python_wrappers_refuse_other_devices():
     with pytest.raises(ValueError, match="stream"):
         B._cache_stream(kv, SimpleNamespace(device=torch.device("cuda:1"), cuda_stream=0))
     assert B._cache_stream(kv, SimpleNamespace(device=torch.device("cuda:0"), cuda_stream=7)) == 7
+
+
+@pytest.mark.parametrize("call,c,kw", [
+    (shared, dict(batch=1 << 20, max_pages=16, table_stride=16), dict(H=128, qs=8192, os=8192, P=200)),
+    (shared, dict(batch=1 << 20, max_pages=16, table_stride=16, dtype=B.BN_F32), dict(H=512, qs=32768, os=32768, P=1)),
+    (prefill, dict(batch=1 << 20, n_kv_heads=64), dict(n=1 << 20, H=64, qs=4096, os=4096)),
+    (prefill, dict(batch=1, dtype=B.BN_F32), dict(n=1 << 25, H=32)),
+    (prefill, dict(batch=1 << 20, dtype=B.BN_F32), dict(n=1 << 22, H=240, qs=16384, os=16384)),
+], ids=["shared", "shared_fp32", "many_sequences", "many_rows_fp32", "both_fp32"])
+def test_launches_past_32_bits_are_refused(call, c, kw):
+    s, m = call(cache(**c), **kw)
+    assert s == B.BN_ERR_UNSUPPORTED and "2^32 threads" in m, m
+
+
+@pytest.mark.parametrize("call,c,kw", [
+    (shared, dict(batch=1 << 20, max_pages=16, table_stride=16), dict(H=124, qs=8192, os=8192, P=200)),
+    (prefill, dict(batch=1 << 20, n_kv_heads=4), dict(n=(1 << 22), H=32)),
+    (prefill, dict(batch=1 << 20, n_kv_heads=4, dtype=B.BN_F32), dict(n=(1 << 22), H=32)),
+    (prefill, dict(batch=1), dict(n=1 << 25, H=32)),
+    (prefill, dict(batch=1, dtype=B.BN_F32), dict(n=(1 << 25) - (1 << 16), H=32)),
+    (decode, dict(batch=1 << 20), dict(H=1020, qs=65536, os=65536)),
+], ids=["shared", "many", "many_fp32", "rows", "rows_fp32", "decode"])
+def test_large_calls_below_that_are_not(call, c, kw):
+    s, m = call(cache(**c), **kw)      # past every check of the arguments: no device, or none of its memory
+    assert s in (B.BN_ERR_HIP, B.BN_ERR_NOT_DEVICE), m
