@@ -2048,6 +2048,7 @@ int check_cache(const std::string &op, const bn_paged_kv *kv, Paged *c) {
   if (kv->batch < 0 || kv->n_pages < 0 || kv->max_pages < 0)
     return fail(BN_ERR_SHAPE, op + ": negative batch or number of pages");
   if (kv->n_kv_heads <= 0) return fail(BN_ERR_SHAPE, op + ": num_kv_heads must be positive");
+  if (kv->n_kv_heads > 65535) return fail(BN_ERR_UNSUPPORTED, op + ": more than 65535 KV heads");
   if (kv->head_dim != HD) return fail(BN_ERR_UNSUPPORTED, op + ": head_dim must be 64");
   if (kv->page_size < 8 || kv->page_size > (1 << 20) || (kv->page_size & (kv->page_size - 1)))
     return fail(BN_ERR_UNSUPPORTED, op + ": page_size must be a power of two, at least 8 and at most 2^20");

@@ -461,8 +461,8 @@ int bn_gqa_decode_noalloc(int dtype, const void *q, const void *k_cache,
  * sequence's last key are not looked at.  page_size: a power of two in [8, 2^20].
  * head_dim must be 64, and dtype BN_F32 or BN_BF16 for the pools, the queries
  * and the outputs alike; sums and softmax statistics are fp32.  Any number of
- * query heads per KV head; query head h reads KV head h / (n_heads /
- * n_kv_heads).
+ * query heads per KV head, at most 65535 heads; query head h reads KV head
+ * h / (n_heads / n_kv_heads).
  *
  * New rows of a ragged batch lie one after another: sequence b's are rows
  * row_starts[b] .. row_starts[b+1] - 1 (device int32 [batch + 1], not

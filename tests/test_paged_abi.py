@@ -261,3 +261,10 @@ def test_launches_past_32_bits_are_refused(call, c, kw):
 def test_large_calls_below_that_are_not(call, c, kw):
     s, m = call(cache(**c), **kw)      # past every check of the arguments: no device, or none of its memory
     assert s in (B.BN_ERR_HIP, B.BN_ERR_NOT_DEVICE), m
+
+
+def test_too_many_kv_heads_are_refused():
+    """Also in an append without queries, whose pieces of a row are counted in 32 bits."""
+    for heads in (65536, 1 << 26, 1 << 30):
+        s, m = append(cache(batch=1, n_kv_heads=heads), q=None, qo=None, n=1, ks=heads * 64, vs=heads * 64)
+        assert s == B.BN_ERR_UNSUPPORTED and "65535" in m, m
