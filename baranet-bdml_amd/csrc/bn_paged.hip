@@ -225,6 +225,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 // ----------------------------------------------------- decode, over pages
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -839,6 +840,21 @@ __device__ __forceinline__ int key_limit(const PrefillParams &p, const Piece &w,
   return p.prefix_parts ? min(max(p.a.c.lens[t], 0), p.a.prefix_len)
                         : min(max(w.last - w.rows + t + 1, 0), p.a.c.cap);
 }
+// A tile's row sums come from the matrix cores against a 0/1 selector, which
+// multiplies a lane's row with 1 and the row 16 away with 0: not a row's own sum
+// where that one's probabilities are NaN (its query, or a key that it alone of
+// the two sees).  A sum that is NaN always leads into a fixup, and there the sums
+// are formed from the lane's own probabilities.  (Choosing between the two there
+// cost registers: 200 sequences behind 16387 keys 76 -> 89 us.)
+__device__ __forceinline__ float own_sums(const bf16x8 (&pb)[2]) {
+  float sum = 0.f;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+      sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{pb[u][j], pb[u][j + 1]}, bf16x2{(__bf16)1.f, (__bf16)1.f}, sum, false);
+  return sum + __shfl_xor(sum, 32, 64);
+}
 // Infinite and NaN values of keys that not every row of a workgroup sees: a row
 // that does not see one weighs it with 0, and 0 times it is not 0.  They are
 // staged as zeros (tame), and if there were any, add_odd() puts each, as it
@@ -1131,7 +1147,8 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
     mcv = m_new;
-    return exps(s, mn, pb);
+    exps(s, mn, pb);
+    return own_sums(pb);
   };
 
   if (ni > 0) {
@@ -1490,7 +1507,7 @@ __device__ __forceinline__ void prefill_pipe_body(const PrefillParams &p, PipeLd
       for (int i = 0; i < 16; ++i) o[rt][dt][i] *= alpha;
     mcv[rt] = m_new;
     exps(s, mn, pb);
-    rs = rowsum(pb);
+    rs = own_sums(pb);
   };
   auto step = [&](auto masked_tag, int t, const bf16_t *vs, const bf16_t *ks, f32x16 (&sc)[RT], f32x16 (&sn)[RT],
                   bf16x8 (&pp)[RT][2], bf16x8 (&pc)[RT][2], float (&rsp)[RT], float (&rsc)[RT])

@@ -452,6 +452,68 @@ def test_prefill_hidden_values_large(dtype, Hkv, H, rows):
     c.vd[pg, 1, sl, 5] = old
 
 
+# each prefill kernel: dtype, cached keys, new rows, KV heads, heads, room of the table in pages of 16
+KERNELS = [("f32", 20, 140, 1, 4, 0), ("bf16", 20, 140, 1, 4, 0), ("bf16", 20, 140, 4, 32, 0),
+           ("bf16", 70, 500, 4, 32, 0), ("bf16", 70, 1100, 4, 32, 0), ("bf16", 0, 4096, 4, 32, 0),
+           ("bf16", 70, 1100, 4, 32, 1100), ("f32", 70, 500, 2, 8, 0)]
+
+
+@pytest.mark.parametrize("kernel", KERNELS, ids=lambda k: "-".join(map(str, k)))
+@pytest.mark.parametrize("what", ["key", "query", "inf"])
+def test_prefill_scores_of_other_rows(kernel, what):
+    """A key that is NaN reaches the rows that see it, one of infinite scores no row that does not, and
+    a NaN query none but its own."""
+    dtype, past, n, Hkv, H, spare = kernel
+    c = Case(dtype, [past + n], Hkv, 16, True, seed=8, nan=False, spare=2 + spare)
+    q = rows_of(dtype, n, H, 9).cuda()
+    st = torch.tensor([0, n], dtype=torch.int32).cuda()
+    cache = c.cuda(B)
+    ref, tol = attention64_large(c, q, [n])
+    hit = torch.zeros((n, H), dtype=torch.bool, device="cuda")
+    G = H // Hkv
+    if what == "query":
+        for i, h in ((0, 0), (5, H - 1), (n // 2, G // 2), (n - 1, 0)):
+            q[i, h, 7] = float("nan")
+            hit[i, h] = True
+    else:
+        i = n // 2 + 3
+        pg, sl = c.place(0, past + i)
+        c.kd[pg, Hkv - 1, sl, 11] = float("nan") if what == "key" else float("inf")
+        hit[i:, H - G:] = True
+    got = B.paged_prefill(q, cache, st, scale=0.125)
+    over = (got.double() - ref).abs() - tol
+    assert (over[~hit] <= 0).all(), f"{int((~(over[~hit] <= 0)).sum())} elements of rows that it must not reach"
+    if what == "inf":   # where its score is -inf it weighs nothing, else the row is NaN
+        up = hit & (q[:, :, 11] > 0)
+        assert torch.isnan(got[up]).all() and torch.isfinite(got[hit & (q[:, :, 11] < 0)]).all()
+    else:
+        assert torch.isnan(got[hit]).all()
+
+
+@pytest.mark.parametrize("dtype,Bn,P", [("f32", 40, 304), ("bf16", 40, 304), ("bf16", 100, 16384)])
+def test_shared_scores_of_other_rows(dtype, Bn, P):
+    """The same behind a shared prefix: sequences that end before the key, and a NaN query among the batch."""
+    H, Hkv, page, dirty = 32, 4, 16, P - 40
+    lens = [P + b % 5 if b % 3 else P - 64 - b for b in range(Bn)]
+    c = Case(dtype, lens, Hkv, page, True, seed=P, nan=False)
+    q = rows_of(dtype, Bn, H, 1).cuda()
+    cache = c.cuda(B)
+    prefix = c.table[1, :P // page].copy()
+    own = c.table.copy()
+    c.table[:, :P // page] = prefix     # attention64_large takes the prefix from each table
+    ref, tol = attention64_large(c, q, [1] * Bn)
+    c.table[:] = own
+    cache.k_pages[int(prefix[dirty // page]), 1, dirty % page, 3] = float("nan")
+    q[4, 9] = float("nan")
+    got = B.paged_decode_shared(q, cache, torch.from_numpy(prefix).cuda(), P, scale=0.125)
+    hit = torch.zeros((Bn, H), dtype=torch.bool, device="cuda")
+    hit[torch.tensor([x > dirty for x in lens]), H // Hkv:2 * H // Hkv] = True
+    hit[4, 9] = True
+    assert torch.isnan(got[hit]).all()
+    over = (got.double() - ref).abs() - tol
+    assert (over[~hit] <= 0).all(), f"{int((~(over[~hit] <= 0)).sum())} elements of rows that it must not reach"
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_prefill_extreme_scores(dtype):
     """Growing scores (the running maximum moves at every tile), then huge ones."""
