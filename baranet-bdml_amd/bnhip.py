@@ -178,13 +178,28 @@ def stream_of(torch_stream=None):
     return C.c_void_p(s.cuda_stream)
 
 
+def made_on(stream, make):
+    """A call's output, make(): memory of the stream that writes it (None: the
+    current one).  Its block is free for the next one of that stream only, once
+    what the present stream does with it is done."""
+    if stream is None:
+        return make()
+    import torch
+    with torch.cuda.stream(stream):
+        t = make()
+    now = torch.cuda.current_stream(t.device)
+    if now != stream:
+        t.record_stream(now)
+    return t
+
+
 def gqa_prefill(q, k, v, o=None, scale=None, causal=True, seq_offset=0, stream=None):
     """q [B,Sq,H,D], k/v [B,Skv,Hkv,D] torch (f32 or bf16, rows contiguous)."""
     B, Sq, H, D = q.shape
     _, Skv, Hkv, _ = k.shape
     if o is None:
         import torch
-        o = torch.empty_like(q)
+        o = made_on(stream, lambda: torch.empty_like(q))
     sc = 1.0 / math.sqrt(D) if scale is None else scale
     assert k.stride(1) == v.stride(1) and k.stride(0) == v.stride(0)
     call("bn_gqa_prefill", _torch_dtype_code(q), q.data_ptr(), k.data_ptr(), v.data_ptr(),
@@ -199,7 +214,7 @@ def fused_head_attention(q, k, v, n_heads, n_kv_heads, head_dim=64, o=None, scal
     torch 2-D views -> o [Sq, H*D]."""
     if o is None:
         import torch
-        o = torch.empty((q.shape[0], n_heads * head_dim), device=q.device, dtype=q.dtype)
+        o = made_on(stream, lambda: torch.empty((q.shape[0], n_heads * head_dim), device=q.device, dtype=q.dtype))
     sc = 1.0 / math.sqrt(head_dim) if scale is None else scale
     call("bn_fused_head_attention", C.byref(view(q)), C.byref(view(k)), C.byref(view(v)),
          C.byref(view(o)), n_heads, n_kv_heads, head_dim, sc, int(causal), seq_offset,
@@ -210,8 +225,8 @@ def fused_head_attention(q, k, v, n_heads, n_kv_heads, head_dim=64, o=None, scal
 def add_rmsnorm(x, delta, weight, eps, h=None, y=None, stream=None):
     """(h, y): h = x + delta, y = RMSNorm(h) * weight; h may be x (in place)."""
     import torch
-    h = torch.empty_like(x) if h is None else h
-    y = torch.empty_like(x) if y is None else y
+    h = made_on(stream, lambda: torch.empty_like(x)) if h is None else h
+    y = made_on(stream, lambda: torch.empty_like(x)) if y is None else y
     call("bn_add_rmsnorm", C.byref(view(x)), C.byref(view(delta)), C.byref(view(weight)),
          C.byref(view(h)), C.byref(view(y)), eps, stream_of(stream))
     return h, y
@@ -220,7 +235,7 @@ def add_rmsnorm(x, delta, weight, eps, h=None, y=None, stream=None):
 def silu_mul(gate, up, out=None, stream=None):
     """silu(gate) * up (SwiGLU activation)."""
     import torch
-    out = torch.empty_like(gate) if out is None else out
+    out = made_on(stream, lambda: torch.empty_like(gate)) if out is None else out
     call("bn_silu_mul", C.byref(view(gate)), C.byref(view(up)), C.byref(view(out)), stream_of(stream))
     return out
 
@@ -231,8 +246,9 @@ def gqa_prefill_lse(q, k, v, o=None, lse=None, scale=None, causal=True, seq_offs
     import torch
     B, Sq, H, D = q.shape
     _, Skv, Hkv, _ = k.shape
-    o = torch.empty_like(q) if o is None else o
-    lse = torch.empty((B, H, Sq), device=q.device, dtype=torch.float32) if lse is None else lse
+    o = made_on(stream, lambda: torch.empty_like(q)) if o is None else o
+    if lse is None:
+        lse = made_on(stream, lambda: torch.empty((B, H, Sq), device=q.device, dtype=torch.float32))
     sc = 1.0 / math.sqrt(D) if scale is None else scale
     assert k.stride(1) == v.stride(1) and k.stride(0) == v.stride(0) and lse.is_contiguous()
     call("bn_gqa_prefill_lse", _torch_dtype_code(q), q.data_ptr(), k.data_ptr(), v.data_ptr(),
@@ -249,9 +265,9 @@ def gqa_prefill_backward(q, k, v, o, dout, lse, scale=None, causal=True, seq_off
     import torch
     B, Sq, H, D = q.shape
     _, Skv, Hkv, _ = k.shape
-    dq = torch.empty_like(q) if dq is None else dq
-    dk = torch.empty_like(k) if dk is None else dk
-    dv = torch.empty_like(k) if dv is None else dv
+    dq = made_on(stream, lambda: torch.empty_like(q)) if dq is None else dq
+    dk = made_on(stream, lambda: torch.empty_like(k)) if dk is None else dk
+    dv = made_on(stream, lambda: torch.empty_like(k)) if dv is None else dv
     sc = 1.0 / math.sqrt(D) if scale is None else scale
     assert k.stride()[:2] == v.stride()[:2] == dk.stride()[:2] == dv.stride()[:2]
     assert q.stride()[:2] == dq.stride()[:2] and o.stride()[:2] == dout.stride()[:2]
@@ -268,7 +284,8 @@ def linear_rope(x, w, y=None, rope_cols=0, position_offset=0, head_dim=64, theta
                 workspace=None, stream=None):
     """y = x @ w with RoPE on columns [0, rope_cols) (2-D torch, f32 or bf16)."""
     import torch
-    y = torch.empty((x.shape[0], w.shape[1]), dtype=x.dtype, device=x.device) if y is None else y
+    if y is None:
+        y = made_on(stream, lambda: torch.empty((x.shape[0], w.shape[1]), dtype=x.dtype, device=x.device))
     ws, wsb = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
     call("bn_linear_rope", C.byref(view(x)), C.byref(view(w)), C.byref(view(y)), rope_cols,
          position_offset, head_dim, theta, ws, wsb, stream_of(stream))
@@ -285,7 +302,7 @@ def gqa_decode(q, k_cache, v_cache, seq_lens, o=None, scale=None, workspace=None
     B, H, D = q.shape
     _, Lmax, Hkv, _ = k_cache.shape
     if o is None:
-        o = torch.empty_like(q)
+        o = made_on(stream, lambda: torch.empty_like(q))
     if not (q.is_contiguous() and o.is_contiguous()):
         raise ValueError("gqa_decode: q and o must be contiguous [B, H, D]")
     if tuple(v_cache.shape) != tuple(k_cache.shape) or v_cache.stride() != k_cache.stride():
@@ -319,7 +336,7 @@ def gqa_decode_planned(q, k_cache, v_cache, seq_lens, h_seq_lens, o=None, scale=
     B, H, D = q.shape
     _, Lmax, Hkv, _ = k_cache.shape
     if o is None:
-        o = torch.empty_like(q)
+        o = made_on(stream, lambda: torch.empty_like(q))
     sc = 1.0 / math.sqrt(D) if scale is None else scale
     if not (q.is_contiguous() and o.is_contiguous()):
         raise ValueError("gqa_decode_planned: q and o must be contiguous [B, H, D]")
@@ -470,7 +487,7 @@ def paged_append(cache, k, v, q=None, q_out=None, row_starts=None, theta=10000.0
 def paged_decode(q, cache, o=None, scale=None, workspace=None, stream=None):
     """One query row per sequence over its pages: q, o [B, H, D]."""
     import torch
-    o = torch.empty_like(q) if o is None else o
+    o = made_on(stream, lambda: torch.empty_like(q)) if o is None else o
     qp, qs = _paged_rows("paged_decode: q", q, cache, cache.batch)
     op, os_ = _paged_rows("paged_decode: o", o, cache, cache.batch, q.shape[1])
     call("bn_paged_decode", cache.ref, qp, op, q.shape[1], qs, os_,
@@ -484,7 +501,7 @@ def paged_prefill(q, cache, row_starts=None, o=None, scale=None, workspace=None,
     rows of sequence b row_starts[b] .. row_starts[b+1]-1, the last of them
     at position seq_lens[b] - 1 (rows of no sequence are left as they are)."""
     import torch
-    o = torch.empty_like(q) if o is None else o
+    o = made_on(stream, lambda: torch.empty_like(q)) if o is None else o
     n = q.shape[0]
     qp, qs = _paged_rows("paged_prefill: q", q, cache, None)
     op, os_ = _paged_rows("paged_prefill: o", o, cache, n, q.shape[1])
@@ -498,7 +515,7 @@ def paged_decode_shared(q, cache, prefix_pages, prefix_len, o=None, scale=None, 
     """paged_decode of a batch whose sequences begin with the same prefix_len
     keys, those of prefix_pages (int32, device), read once for all."""
     import torch
-    o = torch.empty_like(q) if o is None else o
+    o = made_on(stream, lambda: torch.empty_like(q)) if o is None else o
     qp, qs = _paged_rows("paged_decode_shared: q", q, cache, cache.batch)
     op, os_ = _paged_rows("paged_decode_shared: o", o, cache, cache.batch, q.shape[1])
     if prefix_pages.dtype != torch.int32 or prefix_pages.dim() != 1 or not prefix_pages.is_contiguous() or \

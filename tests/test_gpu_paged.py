@@ -759,6 +759,51 @@ def test_calls_on_two_streams():
         assert torch.equal(bits(g), bits(w))
 
 
+@pytest.mark.parametrize("op", ["decode", "prefill", "shared"])
+def test_calls_on_a_given_stream(op):
+    """stream=: the output is not memory that the present stream still writes, and once dropped it is not
+    the present stream's while the call's is at work."""
+    c, cache = big_case()
+    q = rows_of("bf16", 4, 16, 6).cuda()
+    st = torch.tensor([0, 1, 2, 3, 4], dtype=torch.int32).cuda()
+    pages = cache.page_table[0, :40].contiguous()
+    ws = B.paged_workspace(cache, 16, 4, 600)
+    work = torch.zeros((8192, 8192), dtype=torch.bfloat16, device="cuda")
+    s = torch.cuda.Stream()
+
+    def call(stream=None):
+        if op == "decode":
+            return B.paged_decode(q, cache, scale=0.125, workspace=ws, stream=stream)
+        if op == "prefill":
+            return B.paged_prefill(q, cache, st, scale=0.125, workspace=ws, stream=stream)
+        return B.paged_decode_shared(q, cache, pages, 600, scale=0.125, workspace=ws, stream=stream)
+
+    def busy():     # some milliseconds
+        for _ in range(4):
+            torch.mm(work, work)
+
+    want = call()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        t = torch.empty_like(q)
+        busy()
+        t.fill_(7.0)
+        at = t.data_ptr()
+        del t       # free for the present stream's next tensor, written when busy() is through
+        o = call(s)
+        assert o.data_ptr() != at
+        torch.cuda.synchronize()
+        assert torch.equal(bits(o), bits(want))
+        with torch.cuda.stream(s):
+            busy()
+        o = call(s)
+        at = o.data_ptr()
+        del o
+        t = torch.empty_like(q)
+        assert t.data_ptr() != at
+        torch.cuda.synchronize()
+
+
 def test_host_memory_is_refused():
     c = Case("bf16", [5, 9], 2, 16, True)
     kv = B.PagedKV(c.k, c.v, torch.from_numpy(c.table.copy()), torch.tensor([5, 9], dtype=torch.int32))

@@ -268,3 +268,62 @@ def test_too_many_kv_heads_are_refused():
     for heads in (65536, 1 << 26, 1 << 30):
         s, m = append(cache(batch=1, n_kv_heads=heads), q=None, qo=None, n=1, ks=heads * 64, vs=heads * 64)
         assert s == B.BN_ERR_UNSUPPORTED and "65535" in m, m
+
+
+def outputs_of(stream):
+    """Every call of the binding that makes its outputs, with the given stream: {name: outputs}."""
+    k = torch.zeros((5, 2, 16, 64), dtype=torch.bfloat16)
+    kv = B.PagedKV(k, k.clone(), torch.zeros((3, 4), dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
+    q3, st = torch.zeros((3, 8, 64), dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int32)
+    q, kc = torch.zeros((2, 6, 8, 64), dtype=torch.bfloat16), torch.zeros((2, 6, 2, 64), dtype=torch.bfloat16)
+    x, w, lens = torch.zeros((3, 512)), torch.zeros((1, 512)), torch.zeros(2, dtype=torch.int32)
+    lse = torch.zeros((2, 8, 6))
+    return {
+        "paged_decode": B.paged_decode(q3, kv, stream=stream),
+        "paged_prefill": B.paged_prefill(q3, kv, st, stream=stream),
+        "paged_decode_shared": B.paged_decode_shared(q3, kv, lens, 20, stream=stream),
+        "gqa_prefill": B.gqa_prefill(q, kc, kc, stream=stream),
+        "gqa_prefill_lse": B.gqa_prefill_lse(q, kc, kc, stream=stream),
+        "gqa_prefill_backward": B.gqa_prefill_backward(q, kc, kc, q, q, lse, stream=stream),
+        "gqa_decode": B.gqa_decode(q[:, 0].contiguous(), kc, kc, lens, stream=stream),
+        "gqa_decode_planned": B.gqa_decode_planned(q[:, 0].contiguous(), kc, kc, lens, [0, 0], stream=stream),
+        "fused_head_attention": B.fused_head_attention(x, x[:, :128], x[:, :128], 8, 2, stream=stream),
+        "add_rmsnorm": B.add_rmsnorm(x, x, w, 1e-5, stream=stream),
+        "silu_mul": B.silu_mul(x, x, stream=stream),
+        "linear_rope": B.linear_rope(x, torch.zeros((512, 64)), stream=stream),
+    }
+
+
+def test_outputs_are_memory_of_the_stream_that_writes_them(monkeypatch):
+    """A block that work of the present stream still uses is not the output of a call on another, and is not
+    handed out again while either works on it."""
+    import contextlib
+    under, made, kept = [None], {}, {}
+
+    @contextlib.contextmanager
+    def on(stream):
+        under.append(stream)
+        yield
+        under.pop()
+
+    def tracked(make):
+        def run(*a, **kw):
+            t = make(*a, **kw)
+            made[t.data_ptr()] = under[-1]
+            return t
+        return run
+
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: "present")
+    monkeypatch.setattr(torch, "empty_like", tracked(torch.empty_like))
+    monkeypatch.setattr(torch, "empty", tracked(torch.empty))
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: kept.__setitem__(t.data_ptr(), s))
+    monkeypatch.setattr(B, "call", lambda *a: None)
+    monkeypatch.setattr(B, "stream_of", lambda s: s)
+    monkeypatch.setattr(B, "_cache_stream", lambda cache, s: s)
+    for stream, keeps in (("other", "present"), ("present", None), (None, None)):
+        kept.clear()
+        for name, out in outputs_of(stream).items():
+            for t in out if isinstance(out, tuple) else (out,):
+                assert made[t.data_ptr()] == stream, name
+                assert kept.get(t.data_ptr()) == keeps, name
