@@ -9,8 +9,9 @@
 //
 // What lies in a page is found through the sequence's table, read on the
 // device: every table entry is checked against n_pages before it is an
-// address, and lengths are clamped to what the table can hold, so that no
-// contents of those arrays lead outside the pools.
+// address, and keys are counted up to what the table can hold, so that no
+// contents of those arrays lead outside the pools.  (Positions are counted from
+// the length as it stands.)
 #include <algorithm>
 #include <atomic>
 
@@ -115,7 +116,7 @@ struct AppendParams {
   void *qo;
   const int32_t *starts;
   int64_t k_rs, v_rs, q_rs, qo_rs;
-  int n_rows, n_heads;  // n_heads: 0 without q
+  int n_heads;          // 0 without q
   int turn;             // rotate
   double f[HD / 2];     // turns per position of each pair: theta^(-2p/64) / (2 pi)
 };
@@ -858,8 +859,10 @@ __device__ __forceinline__ float own_sums(const bf16x8 (&pb)[2]) {
 // Infinite and NaN values of keys that not every row of a workgroup sees: a row
 // that does not see one weighs it with 0, and 0 times it is not 0.  They are
 // staged as zeros (tame), and if there were any, add_odd() puts each, as it
-// is, into the rows that see it when the tiles are through (what a sum with
-// one of them in it comes to, whatever its weight): nothing of this in the loop.
+// is, into the rows that see it when the tiles are through: nothing of this in
+// the loop.  (A sum with one of them in it is infinite or NaN whatever its weight;
+// of a weight of 0 the products of the tiles that all rows see make NaN, this leaves
+// it infinite.)
 template <typename T>
 __device__ __forceinline__ bool tame(u32x4 &x) {  // true: there was one
   bool odd = false;
@@ -2096,7 +2099,7 @@ int check_cache(const std::string &op, const bn_paged_kv *kv, Paged *c) {
   c->k = kv->k; c->v = kv->v; c->table = kv->page_table; c->lens = kv->seq_lens;
   c->page_stride = kv->page_stride; c->head_stride = kv->head_stride; c->row_stride = kv->row_stride;
   c->table_stride = kv->table_stride;
-  c->batch = kv->batch; c->n_pages = kv->n_pages; c->max_pages = kv->max_pages;
+  c->batch = kv->batch; c->n_pages = kv->n_pages;
   c->shift = __builtin_ctz((unsigned)kv->page_size);
   c->n_kv_heads = kv->n_kv_heads;
   c->cap = kv->n_pages > 0 ? (int)keys : 0;  // without a page there is no key
@@ -2421,7 +2424,7 @@ int bn_paged_append(const bn_paged_kv *cache, const void *k, const void *v, cons
   if ((st = scope.enter(op, cache->seq_lens))) return st;
   p.k = k; p.v = v; p.q = q; p.qo = q_out; p.starts = row_starts;
   p.k_rs = k_row_stride; p.v_rs = v_row_stride; p.q_rs = q_row_stride; p.qo_rs = q_out_row_stride;
-  p.n_rows = n_rows; p.n_heads = q ? n_heads : 0;
+  p.n_heads = q ? n_heads : 0;
   p.turn = theta > 0.f;
   for (int i = 0; i < HD / 2; ++i)
     p.f[i] = theta > 0.f ? std::pow((double)theta, -2.0 * i / HD) / (2.0 * M_PI) : 0.0;

@@ -454,13 +454,23 @@ int bn_gqa_decode_noalloc(int dtype, const void *q, const void *k_cache,
  * sequence b are in the cache, the rows of the present call included: a row
  * is appended, and attends to itself, under a length that counts it.  Both
  * arrays are device int32, read on the device by every call (nothing is kept
- * from one call for the next): a length below 1 is an empty sequence, one
- * above max_pages*page_size counts as that many keys.  A page number outside
+ * from one call for the next): a length below 1 is an empty sequence; of one
+ * above max_pages*page_size, positions are counted from the length as it stands,
+ * and the keys are the table's first max_pages*page_size (a row past them is not
+ * stored, and sees them all).  A page number outside
  * [0, n_pages) has no memory: its keys are not stored and are hidden from every
  * query (a page that was given up, an entry not yet set).  Entries past a
- * sequence's last key are not looked at.  page_size: a power of two in [8, 2^20].
+ * sequence's last key are not looked at.  page_size: a power of two in [8, 2^20];
+ * page_stride below 2^30 elements, row_stride at most 2^24; max_pages*page_size at
+ * most 2^30 keys, 2^34 over the batch; at most 2^20 sequences.
  * head_dim must be 64, and dtype BN_F32 or BN_BF16 for the pools, the queries
- * and the outputs alike; sums and softmax statistics are fp32.  Any number of
+ * and the outputs alike; sums and softmax statistics are fp32, and bf16 calls'
+ * probabilities enter the sums as bf16 values, off by at most 2^-8 of themselves (a
+ * prefill's row sums are those of the same values, as far as the matrix cores
+ * form them).  What is infinite or NaN reaches the rows that see it and no other: an
+ * element of such a value makes that element of every row that sees its key
+ * infinite or NaN (infinite, or NaN where its weight is 0 or infinities of both
+ * signs meet), whatever the key's weight.  Any number of
  * query heads per KV head, at most 65535 heads; query head h reads KV head
  * h / (n_heads / n_kv_heads).
  *
@@ -489,8 +499,8 @@ typedef struct bn_paged_kv {
  * tensors); q, q_out: [n_rows, n_heads, 64] or both NULL.  A row whose position
  * lies outside the table, or on a page without memory, is not stored (its q
  * is written all the same); two rows that land on one place leave either's
- * elements there.  k, v, q and q_out must not lie in the pools.  At most 2^23
- * rows. */
+ * elements there.  k, v, q and q_out must not lie in the pools, and q_out not in k, v
+ * or, but for q itself, q.  At most 2^23 rows. */
 int bn_paged_append(const bn_paged_kv *cache, const void *k, const void *v,
                     const void *q, void *q_out, const int32_t *row_starts,
                     int n_rows, int n_heads, int64_t k_row_stride,
@@ -498,14 +508,15 @@ int bn_paged_append(const bn_paged_kv *cache, const void *k, const void *v,
                     int64_t q_out_row_stride, float theta, void *stream);
 
 /* The three attention calls below take n_rows * n_heads up to 2^30 and are
- * refused where a launch would pass 2^32 threads: never up to 2^23 units,
- * n_rows * n_heads / 32 + batch * n_kv_heads; with a shared prefix also from
- * batch * n_heads of 2^27 on.
+ * refused where a launch would pass 2^32 threads: never while
+ * n_rows * n_heads / 32 + batch * n_kv_heads is at most 2^23; behind a shared
+ * prefix also from batch * n_heads of 2^27 on.  o may be q itself (with q's row
+ * stride); it must not overlap q otherwise, nor the pools.
  *
- * Workspace of theirs for up to n_rows query rows
- * (decode: the batch) and prefix_len common keys (0 without): bytes of device
- * memory, 16-byte aligned, any contents.  NULL there: the pool supplies it.
- * Calls in flight at once need workspaces of their own. */
+ * Their workspace for up to n_rows query rows (decode: the batch) and prefix_len
+ * common keys (0 without): bytes of device memory, 16-byte aligned, any
+ * contents.  NULL in a call: the pool supplies it.  Calls in flight at once need
+ * workspaces of their own. */
 size_t bn_paged_workspace_size(const bn_paged_kv *cache, int n_heads, int n_rows,
                                int prefix_len);
 
@@ -530,8 +541,8 @@ int bn_paged_prefill(const bn_paged_kv *cache, const void *q, void *o,
  * are those of prefix_pages (device int32, ceil(prefix_len / page_size)
  * entries) for every sequence, read once for all of them; the others come from
  * the sequence's own table, whose entries for pages wholly below prefix_len
- * are not looked at.  seq_lens counts the prefix; a sequence shorter than it
- * sees its first seq_lens[b] keys of it. */
+ * are not looked at.  seq_lens counts the prefix, and so does max_pages; a
+ * sequence shorter than it sees its first seq_lens[b] keys of it. */
 int bn_paged_decode_shared(const bn_paged_kv *cache, const void *q, void *o,
                            int n_heads, int64_t q_row_stride,
                            int64_t o_row_stride, float scale,

@@ -490,6 +490,32 @@ def test_prefill_scores_of_other_rows(kernel, what):
         assert torch.isnan(got[hit]).all()
 
 
+@pytest.mark.parametrize("kernel", KERNELS, ids=lambda k: "-".join(map(str, k)))
+def test_prefill_values_of_no_weight(kernel):
+    """An infinite element of a key that weighs nothing makes that element of the rows that see it infinite
+    or NaN, in tiles that all rows of a workgroup see and in others."""
+    dtype, past, n, Hkv, H, spare = kernel
+    c = Case(dtype, [past + n], Hkv, 16, True, seed=8, nan=False, spare=2 + spare)
+    q = rows_of(dtype, n, H, 9).cuda().abs()
+    st = torch.tensor([0, n], dtype=torch.int32).cuda()
+    cache = c.cuda(B)
+    hit = torch.zeros((n, D), dtype=torch.bool, device="cuda")
+    for j, d in ((3, 5), (past + n // 2, 8), (past + n - 2, 63)):
+        pg, sl = c.place(0, j)
+        c.kd[pg, :, sl] = -1000.0
+        hit[max(j - past, 0):, d] = True
+    ref, tol = attention64_large(c, q, [n])
+    for j, d in ((3, 5), (past + n // 2, 8), (past + n - 2, 63)):
+        pg, sl = c.place(0, j)
+        c.vd[pg, :, sl, d] = float("inf")
+    hit = hit[:, None].expand(n, H, D)
+    got = B.paged_prefill(q, cache, st, scale=0.125)
+    over = (got.double() - ref).abs() - tol
+    assert not torch.isfinite(got[hit]).any() and (over[~hit] <= 0).all()
+    last = B.paged_decode(q[-1:].contiguous(), cache, scale=0.125)
+    assert torch.equal(torch.isfinite(last)[0], ~hit[-1])
+
+
 @pytest.mark.parametrize("dtype,Bn,P", [("f32", 40, 304), ("bf16", 40, 304), ("bf16", 100, 16384)])
 def test_shared_scores_of_other_rows(dtype, Bn, P):
     """The same behind a shared prefix: sequences that end before the key, and a NaN query among the batch."""
@@ -653,6 +679,27 @@ def test_shared_prefix_page_without_memory():
     ref, tol = attention64(c, q, [1] * 3, prefix=prefix, prefix_len=64)
     got = B.paged_decode_shared(q.cuda(), c.cuda(B), torch.from_numpy(prefix).cuda(), 64, scale=0.125)
     check(host(got), ref, tol, "shared")
+
+
+@pytest.mark.parametrize("dtype,lens,rows,H", [("bf16", [9000, 300, 17], [1, 1, 1], 32), ("f32", [900, 0, 17], [1, 1, 1], 8),
+                                               ("bf16", [3000, 300, 17], [700, 290, 17], 32), ("f32", [900, 300, 17], [70, 290, 17], 8),
+                                               ("bf16", [20000, 6000], [300, 290], 32), ("bf16", [6000] * 2, [4400, 4500], 32)], ids=str)
+def test_outputs_in_the_queries_place(dtype, lens, rows, H):
+    """o may be q itself: decode, prefill and a shared prefix give the same bits."""
+    c = Case(dtype, lens, 4, 16, True, seed=H, nan=False, spare=2)
+    cache = c.cuda(B)
+    q = rows_of(dtype, sum(rows), H, 5).cuda()
+    st = torch.from_numpy(starts_of(rows)).cuda()
+    prefix = cache.page_table[0, :16].contiguous()
+    one = q[:len(lens)]
+    for x, call in ((q, lambda q, o: B.paged_prefill(q, cache, st, o=o, scale=0.125)),
+                    (one, lambda q, o: B.paged_decode(q, cache, o=o, scale=0.125)),
+                    (one, lambda q, o: B.paged_decode_shared(q, cache, prefix, 250, o=o, scale=0.125))):
+        want = call(x, None)
+        for _ in range(3):
+            y = x.clone()
+            assert call(y, y) is y
+            assert torch.equal(bits(y), bits(want))
 
 
 # ------------------------------------------------------------------- graphs, streams
