@@ -200,6 +200,30 @@ def test_decode_many_sequences():
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_thousands_of_sequences(dtype):
+    """More sequences than 64 to a lane of the scans, most of them short, some empty: the three calls."""
+    n = 4500
+    lens = [int(x) for x in np.random.default_rng(1).integers(0, 40, n)]
+    lens[5], lens[4321], lens[n - 1] = 700, 2100, 33
+    rows = [min(x, 1 + b % 2) for b, x in enumerate(lens)]
+    c = Case(dtype, lens, 1, 16, True, seed=2, nan=False)
+    q = rows_of(dtype, sum(rows), 2, 3).cuda()
+    cache = c.cuda(B)
+    ref, tol = attention64_large(c, q, rows)
+    got = B.paged_prefill(q, cache, torch.from_numpy(starts_of(rows)).cuda(), scale=0.125)
+    assert ((got.double() - ref).abs() <= tol).all()
+    one = rows_of(dtype, n, 2, 4).cuda()
+    ref, tol = attention64_large(c, one, [1] * n)
+    assert ((B.paged_decode(one, cache, scale=0.125).double() - ref).abs() <= tol).all()
+    prefix = c.table[4321, :2].copy()
+    for b in range(n):
+        c.table[b, :2] = prefix
+    ref, tol = attention64_large(c, one, [1] * n)
+    got = B.paged_decode_shared(one, cache, torch.from_numpy(prefix).cuda(), 32, scale=0.125)
+    assert ((got.double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_decode_extreme_scores(dtype):
     """Scores far apart, equal, and -inf: a key of -inf weighs nothing, keys of -inf alone give zeros
     (where V is finite, 0 is what their weights of 0 give)."""

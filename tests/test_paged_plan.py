@@ -72,6 +72,7 @@ CASES = [
     ("bf16", [10, -5, 0], [12, 9, 4], 8, 2, 64),      # more rows than keys
     ("bf16", [4000] * 64, [1] * 63 + [200], 24, 3, 4096),
     ("f32", [8192], [1], 7, 7, 8192),
+    ("bf16", [20 + b % 50 for b in range(4300)], [b % 3 // 2 for b in range(4300)], 4, 1, 64),   # runs of a lane past 64
 ]
 
 
