@@ -221,8 +221,6 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   }
 }
 
-// --------------------------------------------------------------- attention
-
 // ----------------------------------------------------- decode, over pages
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -246,7 +244,7 @@ template <> struct DecTile<bf16_t> { static constexpr int TK = 32, LPR = 8, P = 
 template <> struct DecTile<float> { static constexpr int TK = 16, LPR = 16, P = HD + 4; };
 
 constexpr int kMaxRows = 16;   // query heads of a KV head that one workgroup serves
-constexpr int kHold = HD + 4;  // the same in LDS, rows 16-byte aligned
+constexpr int kHold = HD + 4;  // floats of a part's row in LDS: a record's, 16-byte aligned
 constexpr int kHoldRows = 160; // rows of LDS for the waves' parts of sequences
 constexpr int kShareMin = 4;   // tiles of a share at least
 constexpr int kMergeBatch = 16;  // records read at once
@@ -316,7 +314,8 @@ __device__ __forceinline__ float2 get2(const float *p) {
 //
 // Per tile, with the query heads as columns of the products:
 //   S^T[key][head] = K . Q^T,  O^T[d][head] += V^T . P^T
-// on v_mfma_f32_16x16x32_bf16 (bf16 probabilities: half a step of 2^-8 each)
+// on v_mfma_f32_16x16x32_bf16 (bf16 probabilities, the products' operands: off by at most
+// 2^-8 each; outputs 0.0023 off 64 bits in the mean, 0.0017 of it their own rounding)
 // or v_mfma_f32_16x16x4_f32; a lane holds its 8 (4) keys' scores of one head,
 // which are the second product's operand as they stand.  Bound by memory: 64
 // caches of 512..4096 keys (32 and 4 heads) 33 us, 4.6 TB/s; three of 34763 to
@@ -993,12 +992,12 @@ __device__ __forceinline__ void finish_piece(const PrefillParams &p, const Piece
 // piece's tiles in turn; their (m, l, O) meet in LDS.  Per wave and tile
 //   S^T[key][row] = K . Q^T  (v_mfma_f32_32x32x16_bf16: 16 keys of one row a lane)
 //   O^T[d][row] += V^T . P^T, whose operand is P^T as the scores left it
-// (bf16 probabilities: half a step of 2^-8 each, in the row sum too, which the
+// (bf16 probabilities, the matrix cores' operands: off by at most 2^-8 each, in the row sum too, which the
 // matrix cores form against a 0/1 selector).  Weights are taken against a
 // reference that moves to the true maximum only when a tile's sum passes 2^16.
-// <4,1>: 7 prompts of 165..1500 tokens 51 us (534 TFLOP/s), VALU 58% and LDS 52%
+// <4,1>: 7 prompts of 165..1500 tokens 50 us (543 TFLOP/s), VALU 58% and LDS 52%
 // busy, the rest the units' start and end; <1,4>: 256 rows each behind 2697, 5444
-// and 8192 keys 61 us (571), the LDS port 99% busy, but units of 64 rows, with
+// and 8192 keys 62 us (565), the LDS port 99% busy, but units of 64 rows, with
 // half its traffic and two waves a SIMD in place of three, took 6% longer.
 constexpr float kSumLimit = 65536.f, kMoveLog2 = 8.f;
 template <int HW, int KW>
@@ -1294,8 +1293,9 @@ __global__ __launch_bounds__(64 * HW * KW, OCC) void paged_prefill_bf16_kernel(P
 // the matrix cores) are looked at one step later, when they are long there; only
 // if one passes 2^16 does the tile run again from its scores, still at hand,
 // against the true maximum.  Tiles that every row of the workgroup sees whole
-// run a step without mask code.  8192 rows behind 8192 keys 818 us, 1008 TFLOP/s,
-// 79% of what an 8192^3 library product reaches: VALU 61%, matrix cores 55% busy.
+// run a step without mask code.  8192 rows behind 8192 keys 836 us (829 to 855 from
+// card to card), 986 TFLOP/s, 77% of what an 8192^3 library product reaches: VALU
+// 61%, matrix cores 55% busy.
 constexpr int kBK = 64;  // keys of a block
 constexpr int kPipeR = 256;
 struct PipeLds {
