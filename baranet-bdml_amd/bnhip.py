@@ -55,6 +55,16 @@ class BnPagedKV(C.Structure):
                                          "n_kv_heads", "head_dim")]
 
 
+class BnPagedQ8(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "page_table", "seq_lens")] + \
+               [(n, C.c_int64) for n in ("page_stride", "head_stride", "row_stride", "scale_page_stride",
+                                         "scale_head_stride", "table_stride")] + \
+               [(n, C.c_int32) for n in ("batch", "n_pages", "max_pages", "page_size", "n_kv_heads", "head_dim")]
+
+
+BN_Q8_BLOCK = 16
+
+
 class BnError(RuntimeError):
     def __init__(self, status, msg):
         super().__init__(msg)
@@ -81,7 +91,7 @@ def lib():
     except ImportError:
         pass
     L = C.CDLL(LIB_PATH)
-    vp, V, P = C.c_void_p, C.POINTER(BnView), C.POINTER(BnPagedKV)
+    vp, V, P, P8 = C.c_void_p, C.POINTER(BnView), C.POINTER(BnPagedKV), C.POINTER(BnPagedQ8)
     i, f, i64, sz = C.c_int, C.c_float, C.c_int64, C.c_size_t
     sig = {
         "bn_abi_version": ([], i), "bn_last_error": ([], C.c_char_p),
@@ -128,6 +138,14 @@ def lib():
         "bn_paged_decode": ([P, vp, vp, i, i64, i64, f, vp, sz, vp], i),
         "bn_paged_prefill": ([P, vp, vp, vp, i, i, i64, i64, f, vp, sz, vp], i),
         "bn_paged_decode_shared": ([P, vp, vp, i, i64, i64, f, vp, i, vp, sz, vp], i),
+        "bn_qk_norm_rope": ([i] + [vp] * 7 + [i] * 4 + [i64] * 4 + [i, f, f, vp], i),
+        "bn_qk_norm_rope_backward_workspace_size": ([i] * 4, sz),
+        "bn_qk_norm_rope_backward": ([i] + [vp] * 11 + [i] * 4 + [i64] * 6 + [i, f, f, vp, sz, vp], i),
+        "bn_paged_q8_append": ([P8, i, vp, vp, vp, vp, vp, i, i] + [i64] * 4 + [f, vp, vp, f, vp], i),
+        "bn_paged_q8_read": ([P8, i, vp, vp, vp, i, i64, i64, vp], i),
+        "bn_paged_q8_workspace_size": ([P8, i, i], sz),
+        "bn_paged_q8_decode": ([P8, i, vp, vp, i, i64, i64, f, vp, sz, vp], i),
+        "bn_paged_q8_prefill": ([P8, i, vp, vp, vp, i, i, i64, i64, f, vp, sz, vp], i),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -405,16 +423,17 @@ class PagedKV:
             batch, hkv, d
 
 
-def _paged_rows(what, t, cache, rows, heads=None):
+def _paged_rows(what, t, cache, rows, heads=None, dtype=None):
     """(pointer, row stride) of a [rows, heads, D] tensor whose heads are
-    contiguous within a row, of the cache's type."""
+    contiguous within a row, of the cache's type (or dtype)."""
     shape, stride, d = t.shape, t.stride(), cache.head_dim
     if len(shape) != 3 or shape[2] != d or (heads is not None and shape[1] != heads) or \
             (rows is not None and shape[0] != rows):
         raise ValueError(f"{what}: expected [{'rows' if rows is None else rows}, "
                          f"{'heads' if heads is None else heads}, {d}], got {tuple(shape)}")
-    if t.dtype != cache.dtype or t.device != cache.device:
-        raise ValueError(f"{what}: dtype and device must be the cache's")
+    if t.dtype != (cache.dtype if dtype is None else dtype) or t.device != cache.device:
+        raise ValueError(f"{what}: dtype and device must be the cache's" if dtype is None else
+                         f"{what}: must be {dtype}, on the device of the others")
     if stride[2] != 1 or (shape[1] > 1 and stride[1] != d):
         raise ValueError(f"{what}: a row's heads must be contiguous")
     return t.data_ptr(), stride[0] if shape[0] > 1 else shape[1] * d
@@ -527,3 +546,247 @@ def paged_decode_shared(q, cache, prefix_pages, prefix_len, o=None, scale=None, 
          1.0 / math.sqrt(q.shape[2]) if scale is None else scale, prefix_pages.data_ptr(), prefix_len,
          *_workspace(workspace, cache), _cache_stream(cache, stream))
     return o
+
+
+# ------------------------------------------------- paged KV cache in 8 bits
+class PagedQ8:
+    """A paged KV cache in 8 bits as the ``paged_q8_*`` calls take it: k_pages and
+    v_pages [n_pages, Hkv, page_size, D] of e4m3 codes (float8_e4m3fn or uint8; any
+    strides, rows contiguous, both alike), k_scales and v_scales [n_pages, Hkv,
+    page_size / 16] of powers of two (float8_e8m0fnu or uint8; a page's blocks
+    contiguous, both alike), page_table and seq_lens as for ``PagedKV``."""
+
+    def __init__(self, k_pages, v_pages, k_scales, v_scales, page_table, seq_lens):
+        import torch
+        if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride():
+            raise ValueError("PagedQ8: k_pages and v_pages must be [n_pages, Hkv, page_size, D] of the "
+                             "same shape and strides")
+        if k_pages.stride(3) != 1:
+            raise ValueError("PagedQ8: key rows must be contiguous (stride 1 along head_dim)")
+        if k_pages.dtype not in (torch.float8_e4m3fn, torch.uint8) or v_pages.dtype != k_pages.dtype:
+            raise ValueError("PagedQ8: pools must be float8_e4m3fn or uint8, both alike")
+        n_pages, hkv, page_size, d = k_pages.shape
+        if page_size % BN_Q8_BLOCK:
+            raise ValueError(f"PagedQ8: page_size must be a multiple of {BN_Q8_BLOCK}")
+        if tuple(k_scales.shape) != (n_pages, hkv, page_size // BN_Q8_BLOCK) or \
+                v_scales.shape != k_scales.shape or v_scales.stride() != k_scales.stride():
+            raise ValueError("PagedQ8: k_scales and v_scales must be [n_pages, Hkv, page_size / 16] of the same "
+                             "strides")
+        if k_scales.dtype not in (torch.float8_e8m0fnu, torch.uint8) or v_scales.dtype != k_scales.dtype:
+            raise ValueError("PagedQ8: scales must be float8_e8m0fnu or uint8, both alike")
+        if k_scales.shape[2] > 1 and k_scales.stride(2) != 1:
+            raise ValueError("PagedQ8: the scales of a page and head must be contiguous")
+        if page_table.dim() != 2 or seq_lens.shape != page_table.shape[:1]:
+            raise ValueError("PagedQ8: page_table must be [B, max_pages] and seq_lens [B]")
+        if page_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+            raise ValueError("PagedQ8: page_table and seq_lens must be int32")
+        if (page_table.shape[1] > 1 and page_table.stride(1) != 1) or not seq_lens.is_contiguous():
+            raise ValueError("PagedQ8: page_table rows and seq_lens must be contiguous")
+        tensors = (k_pages, v_pages, k_scales, v_scales, page_table, seq_lens)
+        if len({t.device for t in tensors}) != 1:
+            raise ValueError("PagedQ8: tensors on different devices")
+        self.k_pages, self.v_pages, self.k_scales, self.v_scales, self.page_table, self.seq_lens = tensors
+        batch, max_pages = page_table.shape
+        self.view = BnPagedQ8(*(t.data_ptr() for t in tensors), *k_pages.stride()[:3], *k_scales.stride()[:2],
+                              page_table.stride(0), batch, n_pages, max_pages, page_size, hkv, d)
+        self.ref = C.byref(self.view)
+        self.device, self.batch, self.kv_heads, self.head_dim = k_pages.device, batch, hkv, d
+
+
+def _rows_dtype(what, t):
+    import torch
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{what}: must be float32 or bfloat16")
+    return t.dtype
+
+
+def _head_weight(what, w, cache, dtype):
+    if w is None:
+        return None
+    if tuple(w.shape) != (cache.head_dim,) or w.dtype != dtype or w.device != cache.device or not w.is_contiguous():
+        raise ValueError(f"{what}: must be a contiguous [{cache.head_dim}] tensor of the rows' type and device")
+    return w.data_ptr()
+
+
+def paged_q8_append(cache, k, v, q=None, q_out=None, row_starts=None, theta=10000.0, q_weight=None,
+                    k_weight=None, eps=1e-5, stream=None):
+    """``paged_append`` into a cache in 8 bits: the new rows' queries and keys
+    normed head by head (where a weight [D] is given), turned by their positions,
+    keys and values rounded and stored; k, v, q, q_out and the weights float32 or
+    bfloat16, all alike.  Returns q_out (default: in place), or None without q."""
+    n, dt = k.shape[0], _rows_dtype("paged_q8_append: k", k)
+    kp, ks = _paged_rows("paged_q8_append: k", k, cache, n, cache.kv_heads, dt)
+    vp, vs = _paged_rows("paged_q8_append: v", v, cache, n, cache.kv_heads, dt)
+    qp, qs, op, os_, heads = None, 0, None, 0, 0
+    if q is not None:
+        q_out = q if q_out is None else q_out
+        heads = q.shape[1]
+        qp, qs = _paged_rows("paged_q8_append: q", q, cache, n, None, dt)
+        op, os_ = _paged_rows("paged_q8_append: q_out", q_out, cache, n, heads, dt)
+    elif q_out is not None:
+        raise ValueError("paged_q8_append: q_out without q")
+    call("bn_paged_q8_append", cache.ref, _torch_dtype_code(k), kp, vp, qp, op,
+         _row_starts("paged_q8_append", row_starts, cache, n), n, heads, ks, vs, qs, os_, theta,
+         _head_weight("paged_q8_append: q_weight", q_weight, cache, dt),
+         _head_weight("paged_q8_append: k_weight", k_weight, cache, dt), eps, _cache_stream(cache, stream))
+    return q_out
+
+
+def paged_q8_read(cache, row_starts=None, k=None, v=None, n_rows=None, dtype=None, stream=None):
+    """(k, v) [rows, Hkv, D] of the cache's last keys: rows of sequence b are
+    row_starts[b] .. row_starts[b+1]-1, the last of them position seq_lens[b] - 1
+    (None: one row each).  Given k or v alone, that one; given neither, both are made, of
+    n_rows rows (default: the batch's, without row_starts) and dtype (default bfloat16)."""
+    import torch
+    if k is None and v is None:
+        n = cache.batch if n_rows is None and row_starts is None else n_rows
+        if n is None:
+            raise ValueError("paged_q8_read: n_rows, k or v is needed with row_starts")
+        k, v = (made_on(stream, lambda: torch.zeros((n, cache.kv_heads, cache.head_dim), device=cache.device,
+                                                    dtype=torch.bfloat16 if dtype is None else dtype))
+                for _ in range(2))
+    one = k if k is not None else v
+    n, dt = one.shape[0], _rows_dtype("paged_q8_read: k and v", one)
+    (kp, ks), (vp, vs) = ((None, 0) if t is None else _paged_rows(f"paged_q8_read: {name}", t, cache, n,
+                                                                  cache.kv_heads, dt)
+                          for name, t in (("k", k), ("v", v)))
+    call("bn_paged_q8_read", cache.ref, _torch_dtype_code(one), kp, vp,
+         _row_starts("paged_q8_read", row_starts, cache, n), n, ks, vs, _cache_stream(cache, stream))
+    return k, v
+
+
+def paged_q8_workspace(cache, n_heads, n_rows):
+    """A workspace for the attention calls over the cache with up to n_rows
+    query rows; one per call in flight."""
+    import torch
+    n = lib().bn_paged_q8_workspace_size(cache.ref, n_heads, n_rows)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.device)
+
+
+def paged_q8_decode(q, cache, o=None, scale=None, workspace=None, stream=None):
+    """One query row per sequence over its pages: q, o [B, H, D], bfloat16."""
+    import torch
+    o = made_on(stream, lambda: torch.empty_like(q)) if o is None else o
+    qp, qs = _paged_rows("paged_q8_decode: q", q, cache, cache.batch, None, torch.bfloat16)
+    op, os_ = _paged_rows("paged_q8_decode: o", o, cache, cache.batch, q.shape[1], torch.bfloat16)
+    call("bn_paged_q8_decode", cache.ref, BN_BF16, qp, op, q.shape[1], qs, os_,
+         1.0 / math.sqrt(q.shape[2]) if scale is None else scale,
+         *_workspace(workspace, cache), _cache_stream(cache, stream))
+    return o
+
+
+def paged_q8_prefill(q, cache, row_starts=None, o=None, scale=None, workspace=None, stream=None):
+    """The new rows of a ragged batch over the cache, causal: q, o [rows, H, D]
+    bfloat16, rows of sequence b row_starts[b] .. row_starts[b+1]-1, the last of
+    them at position seq_lens[b] - 1 (rows of no sequence are left as they are)."""
+    import torch
+    o = made_on(stream, lambda: torch.empty_like(q)) if o is None else o
+    n = q.shape[0]
+    qp, qs = _paged_rows("paged_q8_prefill: q", q, cache, None, None, torch.bfloat16)
+    op, os_ = _paged_rows("paged_q8_prefill: o", o, cache, n, q.shape[1], torch.bfloat16)
+    call("bn_paged_q8_prefill", cache.ref, BN_BF16, qp, op, _row_starts("paged_q8_prefill", row_starts, cache, n), n,
+         q.shape[1], qs, os_, 1.0 / math.sqrt(q.shape[2]) if scale is None else scale,
+         *_workspace(workspace, cache), _cache_stream(cache, stream))
+    return o
+
+
+# ------------------------------------------------- norms of single heads
+def _qk_rows(what, t, like, heads):
+    """(pointer, row stride) of a [rows, heads, D] tensor of like's type, device, rows and D."""
+    if t.dim() != 3 or t.shape[0] != like.shape[0] or t.shape[1] != heads or t.shape[2] != like.shape[2]:
+        raise ValueError(f"{what}: expected [{like.shape[0]}, {heads}, {like.shape[2]}], got {tuple(t.shape)}")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{what}: dtype and device must be q's")
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError(f"{what}: a row's heads must be contiguous")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _qk_args(what, q, k, q_weight, k_weight, positions, stream):
+    import torch
+    if q.dim() != 3:
+        raise ValueError(f"{what}: q must be [rows, heads, D]")
+    _rows_dtype(f"{what}: q", q)
+    if (k is None) != (k_weight is None):
+        raise ValueError(f"{what}: k and k_weight must be given together")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (tuple(w.shape) != (q.shape[2],) or w.dtype != q.dtype or w.device != q.device or
+                              not w.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be a contiguous [{q.shape[2]}] tensor of q's type and device")
+    if positions is not None and (positions.dtype != torch.int32 or tuple(positions.shape) != (q.shape[0],) or
+                                  not positions.is_contiguous() or positions.device != q.device):
+        raise ValueError(f"{what}: positions must be int32 [rows] on q's device")
+    if q.device.type != "cuda":
+        raise ValueError(f"{what}: its tensors are not on a GPU")
+    if stream is not None and stream.device != q.device:
+        raise ValueError(f"{what}: the stream is another device's")
+    return torch._C._cuda_getCurrentRawStream(q.device.index) if stream is None else stream.cuda_stream
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, eps=1e-5, positions=None, position_offset=0, theta=10000.0,
+                 q_out=None, k_out=None, stream=None):
+    """(q_out, k_out): every head of q [rows, H, D] and k [rows, Hkv, D] normed
+    (RMSNorm over D, weights [D]) and turned by its row's position
+    (positions[row], default the row's number, + position_offset) in one pass.
+    Heads contiguous, row strides of their own; float32 or bfloat16.  k and
+    k_weight may be None.  q_out may be q, k_out k."""
+    import torch
+    s = _qk_args("qk_norm_rope", q, k, q_weight, k_weight, positions, stream)
+    q_out = made_on(stream, lambda: torch.empty(q.shape, dtype=q.dtype, device=q.device)) if q_out is None else q_out
+    (qp, qs), (op, os_) = (_qk_rows(f"qk_norm_rope: {n}", t, q, q.shape[1]) for n, t in (("q", q), ("q_out", q_out)))
+    kp, ks, kop, kos, hkv = None, 0, None, 0, 0
+    if k is not None:
+        hkv = k.shape[1] if k.dim() == 3 else 0
+        k_out = made_on(stream, lambda: torch.empty(k.shape, dtype=k.dtype, device=k.device)) if k_out is None else k_out
+        (kp, ks), (kop, kos) = (_qk_rows(f"qk_norm_rope: {n}", t, q, hkv) for n, t in (("k", k), ("k_out", k_out)))
+    elif k_out is not None:
+        raise ValueError("qk_norm_rope: k_out without k")
+    call("bn_qk_norm_rope", _torch_dtype_code(q), qp, kp, q_weight.data_ptr(),
+         None if k_weight is None else k_weight.data_ptr(), op, kop,
+         None if positions is None else positions.data_ptr(), q.shape[0], q.shape[1], hkv, q.shape[2], qs, ks, os_, kos,
+         position_offset, eps, theta, s)
+    return q_out, k_out
+
+
+def qk_norm_rope_workspace(n_rows, n_heads, n_kv_heads, head_dim=64, device="cuda"):
+    """A workspace for qk_norm_rope_backward; one per call in flight."""
+    import torch
+    n = lib().bn_qk_norm_rope_backward_workspace_size(n_rows, n_heads, n_kv_heads, head_dim)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
+
+
+def qk_norm_rope_backward(q, k, q_weight, k_weight, dq_out, dk_out, eps=1e-5, positions=None, position_offset=0,
+                          theta=10000.0, dq=None, dk=None, workspace=None, stream=None):
+    """(dq, dk, dq_weight, dk_weight) of qk_norm_rope from the gradients of its
+    outputs; the weights' gradients are float32.  dq may be dq_out or q, dk
+    dk_out or k.  Without k (None, and its weight and gradient) dk and dk_weight
+    are None."""
+    import torch
+    what = "qk_norm_rope_backward"
+    s = _qk_args(what, q, k, q_weight, k_weight, positions, stream)
+    if (k is None) != (dk_out is None):
+        raise ValueError(f"{what}: k and dk_out must be given together")
+    new = lambda t: made_on(stream, lambda: torch.empty(t.shape, dtype=t.dtype, device=t.device))  # noqa: E731
+    grad = lambda: made_on(stream, lambda: torch.empty(q.shape[2], dtype=torch.float32, device=q.device))  # noqa: E731
+    dq = new(q) if dq is None else dq
+    (qp, qs), (gp, gs), (dp, ds) = (_qk_rows(f"{what}: {n}", t, q, q.shape[1])
+                                    for n, t in (("q", q), ("dq_out", dq_out), ("dq", dq)))
+    kp, ks, gkp, gks, dkp, dks, hkv, dwk = None, 0, None, 0, None, 0, 0, None
+    if k is not None:
+        hkv = k.shape[1] if k.dim() == 3 else 0
+        dk, dwk = new(k) if dk is None else dk, grad()
+        (kp, ks), (gkp, gks), (dkp, dks) = (_qk_rows(f"{what}: {n}", t, q, hkv)
+                                            for n, t in (("k", k), ("dk_out", dk_out), ("dk", dk)))
+    elif dk is not None:
+        raise ValueError(f"{what}: dk without k")
+    dwq = grad()
+    ws, wsb = None, 0
+    if workspace is not None:
+        if workspace.device != q.device or not workspace.is_contiguous():
+            raise ValueError(f"{what}: the workspace must be contiguous memory of q's device")
+        ws, wsb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    call("bn_qk_norm_rope_backward", _torch_dtype_code(q), qp, kp, q_weight.data_ptr(),
+         None if k_weight is None else k_weight.data_ptr(), gp, gkp, dp, dkp, dwq.data_ptr(),
+         None if dwk is None else dwk.data_ptr(), None if positions is None else positions.data_ptr(), q.shape[0],
+         q.shape[1], hkv, q.shape[2], qs, ks, gs, gks, ds, dks, position_offset, eps, theta, ws, wsb, s)
+    return dq, dk, dwq, dwk

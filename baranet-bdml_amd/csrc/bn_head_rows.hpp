@@ -1,0 +1,81 @@
+// bn_head_rows.hpp -- rows of heads, eight consecutive elements a lane, a head's
+// lanes next to each other: what kernels that norm or turn single heads share.
+#pragma once
+
+#include "bn_paged_device.hpp"
+
+namespace bn {
+namespace {
+
+struct Eight {
+  float x[8];
+};
+template <typename T>
+struct Raw8 {  // as loaded
+  u32x4 r[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r[i] = ((const u32x4 *)p)[i];
+  }
+  __device__ __forceinline__ Eight floats() const {
+    Eight y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        y.x[2 * i] = __uint_as_float(r[0][i] << 16);
+        y.x[2 * i + 1] = __uint_as_float(r[0][i] & 0xffff0000u);
+      } else {
+        y.x[i] = __uint_as_float(r[0][i]);
+        y.x[4 + i] = __uint_as_float(r[sizeof(T) / 2 - 1][i]);
+      }
+    }
+    return y;
+  }
+};
+template <typename T>
+__device__ __forceinline__ void store8(T *p, const Eight &y) {
+  if constexpr (sizeof(T) == 2) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r[i] = (uint32_t)f32_to_bf16(y.x[2 * i]) | ((uint32_t)f32_to_bf16(y.x[2 * i + 1]) << 16);
+    *(u32x4 *)p = r;
+  } else {
+    *(float4 *)p = make_float4(y.x[0], y.x[1], y.x[2], y.x[3]);
+    *(float4 *)(p + 4) = make_float4(y.x[4], y.x[5], y.x[6], y.x[7]);
+  }
+}
+
+// The sum over the LANES lanes of a head (a power of two up to 32), in each of them.
+template <int LANES>
+__device__ __forceinline__ float head_sum(float v) {
+  if constexpr (LANES >= 2) v = dpp_addf<0xB1, 0xf>(v);   // the neighbour's
+  if constexpr (LANES >= 4) v = dpp_addf<0x4E, 0xf>(v);   // the other pair's of four
+  if constexpr (LANES >= 8) v = dpp_addf<0x141, 0xf>(v);  // the other four's of eight
+  if constexpr (LANES >= 16) v = dpp_addf<0x140, 0xf>(v);  // the other eight's of sixteen
+  if constexpr (LANES >= 32) v += __shfl_xor(v, 16, 64);
+  return v;
+}
+
+// 1 / sqrt(mean(x^2) + eps) of a head of 8 LANES elements.
+template <int LANES>
+__device__ __forceinline__ float head_rms(const Eight &v, float eps) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s = fmaf(v.x[i], v.x[i], s);
+  return rsqrtf(fmaf(head_sum<LANES>(s), 1.0f / (8 * LANES), eps));
+}
+
+// The four pairs turned by their angles (back: by the negative ones).
+__device__ __forceinline__ void turn8(Eight &v, const float2 *cs, bool back = false) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = cs[i];
+    const float s = back ? -t.y : t.y, a = v.x[2 * i], b = v.x[2 * i + 1];
+    v.x[2 * i] = a * t.x - b * s;
+    v.x[2 * i + 1] = a * s + b * t.x;
+  }
+}
+
+}  // namespace
+}  // namespace bn

@@ -16,20 +16,19 @@ unsigned long long next_tag();
 
 namespace {
 
-bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+inline bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 
-// Sizes, strides and pointers of a cache; on success *c is the kernels' form.
-int check_cache(const std::string &op, const bn_paged_kv *kv, Paged *c) {
-  if (!kv) return fail(BN_ERR_INVALID_ARG, op + ": cache is NULL");
-  if (kv->dtype != BN_F32 && kv->dtype != BN_BF16)
-    return fail(BN_ERR_UNSUPPORTED, op + ": dtype must be F32 or BF16");
+// Sizes, strides and pointers of a cache whose elements have `bytes` bytes and whose
+// pages hold at least `least` keys; on success *c is the kernels' form.
+inline int check_pool(const std::string &op, const bn_paged_kv *kv, int bytes, int least, Paged *c) {
   if (kv->batch < 0 || kv->n_pages < 0 || kv->max_pages < 0)
     return fail(BN_ERR_SHAPE, op + ": negative batch or number of pages");
   if (kv->n_kv_heads <= 0) return fail(BN_ERR_SHAPE, op + ": num_kv_heads must be positive");
   if (kv->n_kv_heads > 65535) return fail(BN_ERR_UNSUPPORTED, op + ": more than 65535 KV heads");
   if (kv->head_dim != HD) return fail(BN_ERR_UNSUPPORTED, op + ": head_dim must be 64");
-  if (kv->page_size < 8 || kv->page_size > (1 << 20) || (kv->page_size & (kv->page_size - 1)))
-    return fail(BN_ERR_UNSUPPORTED, op + ": page_size must be a power of two, at least 8 and at most 2^20");
+  if (kv->page_size < least || kv->page_size > (1 << 20) || (kv->page_size & (kv->page_size - 1)))
+    return fail(BN_ERR_UNSUPPORTED, op + ": page_size must be a power of two, at least " + std::to_string(least) +
+                                        " and at most 2^20");
   const int64_t keys = (int64_t)kv->max_pages * kv->page_size;
   if (keys > (1 << 30))
     return fail(BN_ERR_UNSUPPORTED, op + ": max_pages * page_size must be at most 2^30 keys");
@@ -41,7 +40,7 @@ int check_cache(const std::string &op, const bn_paged_kv *kv, Paged *c) {
   if (kv->row_stride > (1 << 24) || kv->page_stride >= (1 << 30))
     return fail(BN_ERR_UNSUPPORTED,
                 op + ": cache row stride must be at most 2^24 elements, page stride below 2^30");
-  const int64_t vec = kv->dtype == BN_BF16 ? 8 : 4, most = (int64_t)1 << 40;
+  const int64_t vec = 16 / bytes, most = (int64_t)1 << 40;
   for (int64_t s : {kv->page_stride, kv->head_stride, kv->row_stride})
     if (s < HD || s % vec || s > most)
       return fail(BN_ERR_INVALID_ARG, op + ": cache strides must be multiples of " + std::to_string(vec) +
@@ -63,13 +62,19 @@ int check_cache(const std::string &op, const bn_paged_kv *kv, Paged *c) {
   c->cap = kv->n_pages > 0 ? (int)keys : 0;  // without a page there is no key
   return BN_OK;
 }
+inline int check_cache(const std::string &op, const bn_paged_kv *kv, Paged *c) {
+  if (!kv) return fail(BN_ERR_INVALID_ARG, op + ": cache is NULL");
+  if (kv->dtype != BN_F32 && kv->dtype != BN_BF16)
+    return fail(BN_ERR_UNSUPPORTED, op + ": dtype must be F32 or BF16");
+  return check_pool(op, kv, kv->dtype == BN_BF16 ? 2 : 4, 8, c);
+}
 
-// A [n_rows, heads, 64] tensor with a row stride.
-int check_rows(const std::string &op, const char *name, const void *t, int n_rows, int64_t heads,
-               int64_t row_stride, int dtype) {
+// A [n_rows, heads, head_dim] tensor with a row stride.
+inline int check_rows(const std::string &op, const char *name, const void *t, int n_rows, int64_t heads,
+                      int64_t row_stride, int dtype, int head_dim = HD) {
   if (n_rows == 0) return BN_OK;
   if (!t) return fail(BN_ERR_INVALID_ARG, op + ": " + name + " is NULL");
-  if (row_stride < heads * HD)
+  if (row_stride < heads * head_dim)
     return fail(BN_ERR_SHAPE, op + ": " + name + " row stride smaller than heads*head_dim");
   if (!aligned16(t) || row_stride % (dtype == BN_BF16 ? 8 : 4) || row_stride > ((int64_t)1 << 40))
     return fail(BN_ERR_UNSUPPORTED, op + ": " + name +
@@ -77,7 +82,7 @@ int check_rows(const std::string &op, const char *name, const void *t, int n_row
   return BN_OK;
 }
 
-int check_starts(const std::string &op, const int32_t *row_starts, int n_rows, int batch) {
+inline int check_starts(const std::string &op, const int32_t *row_starts, int n_rows, int batch) {
   if (n_rows < 0) return fail(BN_ERR_SHAPE, op + ": negative number of rows");
   if (!row_starts && n_rows != batch)
     return fail(BN_ERR_SHAPE, op + ": without row_starts there is one row per sequence");
@@ -85,7 +90,7 @@ int check_starts(const std::string &op, const int32_t *row_starts, int n_rows, i
   return BN_OK;
 }
 
-int check_heads(const std::string &op, int n_heads, int n_kv_heads, int n_rows) {
+inline int check_heads(const std::string &op, int n_heads, int n_kv_heads, int n_rows) {
   if (n_heads <= 0 || n_heads % n_kv_heads != 0)
     return fail(BN_ERR_SHAPE, op + ": num_heads must be a positive multiple of num_kv_heads");
   if (n_heads > 65535) return fail(BN_ERR_UNSUPPORTED, op + ": more than 65535 heads");
@@ -100,7 +105,7 @@ class DeviceScope {
   int before_ = -1;
 
  public:
-  int enter(const std::string &op, const void *memory) {
+  int enter(const std::string &op, const void *memory, const char *what = "the cache") {
     int st = ensure_device();
     if (st) return st;
     const int lib = library_device();
@@ -116,7 +121,7 @@ class DeviceScope {
       return fail(BN_ERR_NOT_DEVICE, op + ": only GPU implementation available");
     }
     if (a.type == hipMemoryTypeDevice && a.device != lib)
-      return fail(BN_ERR_INVALID_ARG, op + ": the cache is on device " + std::to_string(a.device) +
+      return fail(BN_ERR_INVALID_ARG, op + ": " + what + " is on device " + std::to_string(a.device) +
                                           ", the library on device " + std::to_string(lib));
     return BN_OK;
   }

@@ -251,7 +251,7 @@ struct PrefillPlan {
 };
 // most: not this call's plan but one whose workspace does for any call of at
 // most as many rows (with fewer rows a sequence the kernel may be another).
-PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv_heads, int cap, bool most = false) {
+inline PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv_heads, int cap, bool most = false) {
   PrefillPlan d;
   const int64_t rows = (int64_t)n_rows * (n_heads / n_kv_heads);  // of a KV head
   const int64_t u128 = (rows / 128 + 1) * n_kv_heads, u32 = (rows / 32 + 1) * n_kv_heads;

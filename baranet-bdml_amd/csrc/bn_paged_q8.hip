@@ -1,0 +1,485 @@
+// bn_paged_q8.hip -- the paged KV cache in 8 bits: e4m3 codes under a power of
+// two for every 16 keys of a page and KV head.  Appending (norms, rotation,
+// rounding), reading back, and the attention over the pages.
+//
+// A float's e4m3 code has its relative precision, 2^-4, wherever the scale puts
+// it above 2^-6, so nothing is gained by a finer scale than a power of two; and
+// with that every value is a bf16 number, a scale that grows leaves older codes'
+// values as they are (but for those that become subnormal), and the attention's
+// kernels are those of the bf16 cache behind the conversion.
+#include "bn_head_rows.hpp"
+#include "bn_paged_host.hpp"
+
+namespace bn {
+namespace {
+
+constexpr int kBlock = BN_Q8_BLOCK;
+constexpr int kLow = 10, kHigh = 247;  // scale bytes
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// The cache as the kernels see it.
+struct Q8 {
+  Paged c;  // strides of the codes, in bytes
+  uint8_t *ks, *vs;
+  int64_t scale_page, scale_head;
+};
+
+// 2^(byte - 127)
+__device__ __forceinline__ float scale_of(int byte) { return __uint_as_float((uint32_t)min(max(byte, kLow), kHigh) << 23); }
+// Codes 2 HALF and 2 HALF + 1 of four, as values.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+template <bool HALF>
+__device__ __forceinline__ f32x2 two_values(uint32_t codes, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, scale, HALF);
+}
+__device__ __forceinline__ Eight values(u32x2 codes, float scale) {
+  Eight y;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const f32x2 a = two_values<false>(codes[i], scale), b = two_values<true>(codes[i], scale);
+    y.x[4 * i] = a[0]; y.x[4 * i + 1] = a[1]; y.x[4 * i + 2] = b[0]; y.x[4 * i + 3] = b[1];
+  }
+  return y;
+}
+// The smallest scale byte with which |x| up to amax (finite) is at most 448.
+__device__ __forceinline__ int byte_of(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  // amax = 1.m 2^(E - 127) <= 1.75 2^8 2^n: n = E - 127 - 8, one more where 1.m is above 1.75
+  const int e = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u);
+  return min(max(e, kLow), kHigh);
+}
+__device__ __forceinline__ float finite_size(float x) { return fabsf(x) < INFINITY ? fabsf(x) : 0.f; }
+// Eight codes of x under the scale of a byte.
+__device__ __forceinline__ u32x2 codes_of(const Eight &x, int byte) {
+  const float inverse = __uint_as_float((uint32_t)(254 - byte) << 23), most = byte == kHigh ? 240.f : 448.f;
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float s = fminf(fmaxf(x.x[i] * inverse, -most), most);
+    y[i] = fabsf(x.x[i]) < INFINITY ? s : NAN;
+  }
+  u32x2 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
+    r[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], w, true);
+  }
+  return r;
+}
+
+// ------------------------------------------------------ a call's units of work
+// A unit: the rows of a call that fall into one block of a sequence, so that one
+// workgroup sees all of a block that the call writes.
+struct Unit {
+  int row0, rows;  // of the tensors; rows <= 16
+  int b;
+  int64_t pos0;    // position of row0
+};
+// Sequence b's units have numbers from (starts[b] - starts[0]) / 16 + 2 b on, of
+// which n rows never need more than n / 16 + 2: the sequence is found by a search
+// among 64 at a time, and numbers without a unit are left out.  False: none.
+__device__ __forceinline__ bool find_unit(const Paged &c, const int32_t *starts, int n_rows, int number, Unit &u) {
+  if (!starts) {
+    u.b = u.row0 = number;
+    u.rows = 1;
+    u.pos0 = (int64_t)max(c.lens[number], 0) - 1;
+    return true;
+  }
+  const int lane = threadIdx.x & 63;
+  auto start = [&](int b) { return min(max(starts[b], 0), n_rows); };
+  const int s0 = start(0);
+  auto first_of = [&](int b) { return ((start(b) - s0) >> 4) + 2 * b; };
+  int lo = 0, hi = c.batch;  // first_of(lo) <= number, and number < first_of(hi) unless it is past all
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) >> 6, at = lo + step * lane;
+    const unsigned long long below =
+        __builtin_amdgcn_ballot_w64(at < hi && first_of(min(at, c.batch)) <= number);
+    const int n = __builtin_popcountll(below);
+    if (n == 0) return false;  // (starts that decrease)
+    lo = lo + step * (n - 1);
+    hi = min(hi, lo + step);
+  }
+  const int j = number - first_of(lo);
+  const int from = start(lo), to = start(lo + 1);
+  if (j < 0 || to <= from) return false;
+  // (starts[lo + 1] may lie past the tensors' rows)
+  const int64_t p0 = (int64_t)max(c.lens[lo], 0) - starts[lo + 1] + from, end = p0 + (to - from);
+  const int64_t block0 = ((p0 >> 4) + j) * kBlock;
+  if (block0 >= end) return false;
+  const int64_t p = block0 > p0 ? block0 : p0, q = block0 + kBlock < end ? block0 + kBlock : end;
+  u.b = lo;
+  u.row0 = from + (int)(p - p0);
+  u.rows = (int)(q - p);
+  u.pos0 = p;
+  return true;
+}
+int64_t count_units(const int32_t *starts, int n_rows, int batch) {
+  return starts ? (int64_t)n_rows / kBlock + 2 * (int64_t)batch : batch;
+}
+
+// Where a unit's rows lie: byte offsets of its first slot and of its block's scale
+// in KV head 0 (-1: the block has no memory).
+struct Place {
+  int64_t codes, scale;
+  int slot;  // of the first row in its block
+};
+__device__ __forceinline__ Place place_of(const Q8 &q, const Unit &u) {
+  Place p{-1, -1, (int)(u.pos0 & (kBlock - 1))};
+  // (a block lies within the table or outside it as a whole)
+  if (u.pos0 < 0 || u.pos0 >= q.c.cap) return p;
+  const int pos = (int)u.pos0, page = q.c.table[u.b * q.c.table_stride + (pos >> q.c.shift)];
+  if ((unsigned)page >= (unsigned)q.c.n_pages) return p;
+  const int in_page = pos & ((1 << q.c.shift) - 1);
+  p.codes = page * q.c.page_stride + in_page * q.c.row_stride;
+  p.scale = page * q.scale_page + (in_page >> 4);
+  return p;
+}
+
+// ------------------------------------------------------------------ append
+struct Q8AppendParams {
+  Q8 s;
+  const void *k, *v, *q, *wq, *wk;
+  void *qo;
+  const int32_t *starts;
+  int64_t k_rs, v_rs, q_rs, qo_rs;
+  int n_rows, n_heads, turn;  // n_heads: 0 without q
+  float eps;
+  double f[HD / 2];  // turns per position of each pair
+};
+
+// A unit a workgroup.  The angles of its rows once; then its waves take the
+// block's KV heads, K and V, in turn, 16 rows of 64 elements in two pieces of eight
+// a lane: norm, rotation, the block's largest element, the scale, the codes.  The
+// queries' pieces go to all threads.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_q8_append_kernel(Q8AppendParams p) {
+  __shared__ float2 cs[kBlock][HD / 2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Paged &c = p.s.c;
+  Unit u;
+  if (!find_unit(c, p.starts, p.n_rows, blockIdx.x, u)) return;
+  if (p.turn) {
+    for (int i = tid; i < u.rows * (HD / 2); i += 256)
+      cs[i / (HD / 2)][i % (HD / 2)] = cos_sin((double)(u.pos0 + i / (HD / 2)) * p.f[i % (HD / 2)]);
+    __syncthreads();
+  }
+  const int e = lane % 8 * 8;
+  auto normed = [&](Eight &x, const void *w) __attribute__((always_inline)) {
+    const float r = head_rms<8>(x, p.eps);
+    Raw8<T> wr;
+    wr.load((const T *)w + e);
+    const Eight y = wr.floats();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x.x[j] *= r * y.x[j];
+  };
+  const Place at = place_of(p.s, u);
+  if (at.codes >= 0) {
+    for (int task = wave; task < 2 * c.n_kv_heads; task += 4) {
+      const bool is_v = task >= c.n_kv_heads;
+      const int g = is_v ? task - c.n_kv_heads : task;
+      Eight x[2];
+      float amax = 0.f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int row = lane / 8 + 8 * n;
+        if (row < u.rows) {
+          Raw8<T> raw;
+          raw.load((is_v ? (const T *)p.v + (int64_t)(u.row0 + row) * p.v_rs
+                         : (const T *)p.k + (int64_t)(u.row0 + row) * p.k_rs) + g * HD + e);
+          x[n] = raw.floats();
+          if (!is_v) {
+            if (p.wk) normed(x[n], p.wk);
+            if (p.turn) turn8(x[n], &cs[row][e / 2]);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_size(x[n].x[j]));
+        }
+      }
+      amax = wave_max(amax);
+      uint8_t *const codes = (uint8_t *)(is_v ? c.v : c.k) + at.codes + g * c.head_stride;
+      uint8_t *const scale = (is_v ? p.s.vs : p.s.ks) + at.scale + g * p.s.scale_head;
+      int byte = byte_of(amax);
+      if (at.slot > 0) {  // older rows in the block
+        const int before = min(max((int)*scale, kLow), kHigh);
+        if (byte > before) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int back = lane / 8 + 8 * n - at.slot;  // rows before the first: negative
+            if (back >= 0) continue;
+            u32x2 *const row = (u32x2 *)(codes + back * c.row_stride + e);
+            *row = codes_of(values(*row, scale_of(before)), byte);
+          }
+        }
+        byte = max(byte, before);
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int row = lane / 8 + 8 * n;
+        if (row < u.rows) *(u32x2 *)(codes + row * c.row_stride + e) = codes_of(x[n], byte);
+      }
+      if (lane == 0) *scale = (uint8_t)byte;
+    }
+  }
+  const int per = p.n_heads * 8, total = u.rows * per;
+  for (int i = tid; i < total; i += 256) {
+    const int row = (int)((uint32_t)i / (uint32_t)per), h = (i - row * per) / 8;
+    Raw8<T> raw;
+    raw.load((const T *)p.q + (int64_t)(u.row0 + row) * p.q_rs + h * HD + e);
+    Eight x = raw.floats();
+    if (p.wq) normed(x, p.wq);
+    if (p.turn) turn8(x, &cs[row][e / 2]);
+    store8((T *)p.qo + (int64_t)(u.row0 + row) * p.qo_rs + h * HD + e, x);
+  }
+}
+
+// -------------------------------------------------------------------- read
+struct Q8ReadParams {
+  Q8 s;
+  void *k, *v;
+  const int32_t *starts;
+  int64_t k_rs, v_rs;
+  int n_rows;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void paged_q8_read_kernel(Q8ReadParams p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Paged &c = p.s.c;
+  Unit u;
+  if (!find_unit(c, p.starts, p.n_rows, blockIdx.x, u)) return;
+  const Place at = place_of(p.s, u);
+  const int e = lane % 8 * 8;
+  for (int task = wave; task < 2 * c.n_kv_heads; task += 4) {
+    const bool is_v = task >= c.n_kv_heads;
+    const int g = is_v ? task - c.n_kv_heads : task;
+    T *const out = (T *)(is_v ? p.v : p.k);
+    if (!out) continue;
+    const uint8_t *const codes = (const uint8_t *)(is_v ? c.v : c.k) + at.codes + g * c.head_stride;
+    const float scale = at.codes < 0 ? 0.f : scale_of((is_v ? p.s.vs : p.s.ks)[at.scale + g * p.s.scale_head]);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int row = lane / 8 + 8 * n;
+      if (row >= u.rows) continue;
+      Eight x{};
+      if (at.codes >= 0) x = values(*(const u32x2 *)(codes + row * c.row_stride + e), scale);
+      store8(out + (int64_t)(u.row0 + row) * (is_v ? p.v_rs : p.k_rs) + g * HD + e, x);
+    }
+  }
+}
+
+// --------------------------------------------------------------- attention
+struct Q8AttnParams {
+  Q8 s;
+  const void *q;
+  void *o;
+  const int32_t *starts;
+  int64_t q_rs, o_rs;
+  int n_rows, n_heads, group;
+  float cl;  // scale * log2(e)
+};
+// A wave per row and head: 64 keys at a time, a key's score a lane, then an element
+// of the output a lane.
+__global__ __launch_bounds__(64) void paged_q8_attention_kernel(Q8AttnParams p) {
+  __shared__ float q[HD];
+  const Paged &c = p.s.c;
+  const int lane = threadIdx.x, row = blockIdx.x, h = blockIdx.y, g = h / p.group;
+  const int b = sequence_of(p.starts, c.batch, row);
+  if (b < 0) return;
+  const int64_t pos = p.starts ? (int64_t)max(c.lens[b], 0) - p.starts[b + 1] + row : (int64_t)max(c.lens[b], 0) - 1;
+  const int seen = pos < 0 ? 0 : pos >= c.cap ? c.cap : (int)pos + 1;
+  q[lane] = bf16_to_f32(((const bf16_t *)p.q + row * p.q_rs + h * HD)[lane]);
+  __syncthreads();
+  float m = -INFINITY, l = 0.f, o = 0.f;
+  const int32_t *const table = c.table + b * c.table_stride;
+  auto page_of = [&](int key) { return table[key >> c.shift]; };
+  auto in_page = [&](int key) { return key & ((1 << c.shift) - 1); };
+  for (int k0 = 0; k0 < seen; k0 += 64) {
+    const int key = k0 + lane;
+    float s = -INFINITY;
+    if (key < seen) {
+      const int page = page_of(key);
+      if ((unsigned)page < (unsigned)c.n_pages) {
+        const u32x2 *const at = (const u32x2 *)((const uint8_t *)c.k + page * c.page_stride + g * c.head_stride +
+                                                in_page(key) * c.row_stride);
+        const float scale = scale_of(p.s.ks[page * p.s.scale_page + g * p.s.scale_head + (in_page(key) >> 4)]);
+        s = 0.f;
+        for (int i = 0; i < 8; ++i) {
+          const Eight x = values(at[i], scale);
+          for (int j = 0; j < 8; ++j) s = fmaf(x.x[j], q[8 * i + j], s);
+        }
+        s *= p.cl;
+      }
+    }
+    const float mt = fmaxf(m, wave_max(s)), ref = mt == -INFINITY ? 0.f : mt;
+    const float e = __builtin_amdgcn_exp2f(s - ref), alpha = __builtin_amdgcn_exp2f(m - ref);
+    m = mt;
+    l = l * alpha + wave_sum(e);
+    o *= alpha;
+    for (int j = 0; j < min(64, seen - k0); ++j) {
+      const int page = __builtin_amdgcn_readfirstlane(page_of(k0 + j));
+      if ((unsigned)page >= (unsigned)c.n_pages) continue;
+      const float scale = scale_of(p.s.vs[page * p.s.scale_page + g * p.s.scale_head + (in_page(k0 + j) >> 4)]);
+      const uint8_t code = ((const uint8_t *)c.v + page * c.page_stride + g * c.head_stride +
+                            in_page(k0 + j) * c.row_stride)[lane];
+      o = fmaf(__shfl(e, j, 64), two_values<false>(code, scale)[0], o);
+    }
+  }
+  ((bf16_t *)p.o + row * p.o_rs + h * HD)[lane] = f32_to_bf16(o * (l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l));
+}
+
+// ---------------------------------------------------------------- the host
+int check_q8(const std::string &op, const bn_paged_q8 *kv, Q8 *s) {
+  if (!kv) return fail(BN_ERR_INVALID_ARG, op + ": cache is NULL");
+  const bn_paged_kv codes{kv->k, kv->v, kv->page_table, kv->seq_lens, kv->page_stride, kv->head_stride,
+                          kv->row_stride, kv->table_stride, BN_BF16, kv->batch, kv->n_pages, kv->max_pages,
+                          kv->page_size, kv->n_kv_heads, kv->head_dim};
+  const int st = check_pool(op, &codes, 1, kBlock, &s->c);
+  if (st || kv->batch == 0) return st;
+  const int64_t most = (int64_t)1 << 40, blocks = kv->page_size / kBlock;
+  if (kv->n_pages > 0 && (!kv->k_scale || !kv->v_scale))
+    return fail(BN_ERR_INVALID_ARG, op + ": NULL pointer to scales in the cache");
+  if ((kv->n_pages > 1 && kv->scale_page_stride < blocks) || (kv->n_kv_heads > 1 && kv->scale_head_stride < blocks) ||
+      kv->scale_page_stride < 0 || kv->scale_head_stride < 0 || kv->scale_page_stride > most ||
+      kv->scale_head_stride > most)
+    return fail(BN_ERR_INVALID_ARG, op + ": scale strides must be at least a page's blocks");
+  s->ks = (uint8_t *)kv->k_scale;
+  s->vs = (uint8_t *)kv->v_scale;
+  s->scale_page = kv->scale_page_stride;
+  s->scale_head = kv->scale_head_stride;
+  return BN_OK;
+}
+
+int attention_q8(const char *name, const bn_paged_q8 *kv, int dtype, const void *q, void *o, const int32_t *starts,
+                 int n_rows, int n_heads, int64_t q_rs, int64_t o_rs, float scale, void *workspace,
+                 size_t workspace_bytes, void *stream) {
+  const std::string op = name;
+  Q8AttnParams p;
+  int st = check_q8(op, kv, &p.s);
+  if (st || (st = check_heads(op, n_heads, kv->n_kv_heads, n_rows)) ||
+      (st = check_starts(op, starts, n_rows, kv->batch)))
+    return st;
+  if (dtype != BN_BF16) return fail(BN_ERR_UNSUPPORTED, op + ": dtype must be BF16");
+  if (!(scale > 0.f) || !std::isfinite(scale))
+    return fail(BN_ERR_INVALID_ARG, op + ": scale must be positive and finite");
+  if (n_rows == 0 || kv->batch == 0) return BN_OK;
+  if ((st = check_rows(op, "q", q, n_rows, n_heads, q_rs, dtype)) ||
+      (st = check_rows(op, "o", o, n_rows, n_heads, o_rs, dtype)))
+    return st;
+  const size_t need = bn_paged_q8_workspace_size(kv, n_heads, n_rows);
+  if (workspace && workspace_bytes < need)
+    return fail(BN_ERR_INVALID_ARG, op + ": workspace of " + std::to_string(workspace_bytes) +
+                                        " bytes, need " + std::to_string(need));
+  if (workspace && !aligned16(workspace))
+    return fail(BN_ERR_UNSUPPORTED, op + ": workspace must be 16-byte aligned");
+  DeviceScope scope;
+  if ((st = scope.enter(op, kv->seq_lens))) return st;
+  p.q = q; p.o = o; p.starts = starts;
+  p.q_rs = q_rs; p.o_rs = o_rs;
+  p.n_rows = n_rows; p.n_heads = n_heads; p.group = n_heads / kv->n_kv_heads;
+  p.cl = scale * kLog2e;
+  hipLaunchKernelGGL(paged_q8_attention_kernel, dim3((unsigned)n_rows, (unsigned)n_heads), dim3(64), 0,
+                     as_stream(stream), p);
+  BN_LAUNCH_CHECK();
+  return BN_OK;
+}
+
+}  // namespace
+}  // namespace bn
+
+using namespace bn;
+
+extern "C" {
+
+int bn_paged_q8_append(const bn_paged_q8 *cache, int dtype, const void *k, const void *v, const void *q,
+                       void *q_out, const int32_t *row_starts, int n_rows, int n_heads, int64_t k_row_stride,
+                       int64_t v_row_stride, int64_t q_row_stride, int64_t q_out_row_stride, float theta,
+                       const void *q_weight, const void *k_weight, float eps, void *stream) {
+  const std::string op = "Paged Q8 append";
+  Q8AppendParams p;
+  int st = check_q8(op, cache, &p.s);
+  if (st || (st = check_starts(op, row_starts, n_rows, cache->batch))) return st;
+  if (dtype != BN_F32 && dtype != BN_BF16) return fail(BN_ERR_UNSUPPORTED, op + ": dtype must be F32 or BF16");
+  if (!q != !q_out) return fail(BN_ERR_INVALID_ARG, op + ": q and q_out must be given together");
+  if (q_weight && !q) return fail(BN_ERR_INVALID_ARG, op + ": q_weight without q");
+  if (q && (st = check_heads(op, n_heads, cache->n_kv_heads, n_rows))) return st;
+  if (n_rows > (1 << 23)) return fail(BN_ERR_UNSUPPORTED, op + ": more than 2^23 rows");
+  if (!(theta >= 0.f) || !std::isfinite(theta))
+    return fail(BN_ERR_INVALID_ARG, op + ": theta must be positive and finite, or 0 for no rotation");
+  if ((q_weight || k_weight) && (!(eps >= 0.f) || !std::isfinite(eps)))
+    return fail(BN_ERR_INVALID_ARG, op + ": eps must be finite and not negative");
+  if (!aligned16(q_weight) || !aligned16(k_weight))
+    return fail(BN_ERR_UNSUPPORTED, op + ": weights must be 16-byte aligned");
+  if (n_rows == 0 || cache->batch == 0) return BN_OK;
+  if ((st = check_rows(op, "k", k, n_rows, cache->n_kv_heads, k_row_stride, dtype)) ||
+      (st = check_rows(op, "v", v, n_rows, cache->n_kv_heads, v_row_stride, dtype)) ||
+      (q && ((st = check_rows(op, "q", q, n_rows, n_heads, q_row_stride, dtype)) ||
+             (st = check_rows(op, "q_out", q_out, n_rows, n_heads, q_out_row_stride, dtype)))))
+    return st;
+  if (q == q_out && q && q_row_stride != q_out_row_stride)
+    return fail(BN_ERR_INVALID_ARG, op + ": q_out in q's place must have its row stride");
+  DeviceScope scope;
+  if ((st = scope.enter(op, cache->seq_lens))) return st;
+  p.k = k; p.v = v; p.q = q; p.qo = q_out; p.wq = q_weight; p.wk = k_weight; p.starts = row_starts;
+  p.k_rs = k_row_stride; p.v_rs = v_row_stride; p.q_rs = q_row_stride; p.qo_rs = q_out_row_stride;
+  p.n_rows = n_rows;
+  p.n_heads = q ? n_heads : 0;
+  p.turn = theta > 0.f;
+  p.eps = eps;
+  for (int i = 0; i < HD / 2; ++i)
+    p.f[i] = theta > 0.f ? std::pow((double)theta, -2.0 * i / HD) / (2.0 * M_PI) : 0.0;
+  hipStream_t s = as_stream(stream);
+  const dim3 grid((unsigned)count_units(row_starts, n_rows, cache->batch)), block(256);
+  if (dtype == BN_BF16) hipLaunchKernelGGL(paged_q8_append_kernel<bf16_t>, grid, block, 0, s, p);
+  else hipLaunchKernelGGL(paged_q8_append_kernel<float>, grid, block, 0, s, p);
+  BN_LAUNCH_CHECK();
+  return BN_OK;
+}
+
+int bn_paged_q8_read(const bn_paged_q8 *cache, int dtype, void *k, void *v, const int32_t *row_starts, int n_rows,
+                     int64_t k_row_stride, int64_t v_row_stride, void *stream) {
+  const std::string op = "Paged Q8 read";
+  Q8ReadParams p;
+  int st = check_q8(op, cache, &p.s);
+  if (st || (st = check_starts(op, row_starts, n_rows, cache->batch))) return st;
+  if (dtype != BN_F32 && dtype != BN_BF16) return fail(BN_ERR_UNSUPPORTED, op + ": dtype must be F32 or BF16");
+  if (n_rows > (1 << 23)) return fail(BN_ERR_UNSUPPORTED, op + ": more than 2^23 rows");
+  if (n_rows == 0 || cache->batch == 0) return BN_OK;
+  if (!k && !v) return fail(BN_ERR_INVALID_ARG, op + ": k and v are NULL");
+  if ((k && (st = check_rows(op, "k", k, n_rows, cache->n_kv_heads, k_row_stride, dtype))) ||
+      (v && (st = check_rows(op, "v", v, n_rows, cache->n_kv_heads, v_row_stride, dtype))))
+    return st;
+  DeviceScope scope;
+  if ((st = scope.enter(op, cache->seq_lens))) return st;
+  p.k = k; p.v = v; p.starts = row_starts;
+  p.k_rs = k_row_stride; p.v_rs = v_row_stride;
+  p.n_rows = n_rows;
+  hipStream_t s = as_stream(stream);
+  const dim3 grid((unsigned)count_units(row_starts, n_rows, cache->batch)), block(256);
+  if (dtype == BN_BF16) hipLaunchKernelGGL(paged_q8_read_kernel<bf16_t>, grid, block, 0, s, p);
+  else hipLaunchKernelGGL(paged_q8_read_kernel<float>, grid, block, 0, s, p);
+  BN_LAUNCH_CHECK();
+  return BN_OK;
+}
+
+size_t bn_paged_q8_workspace_size(const bn_paged_q8 *cache, int n_heads, int n_rows) {
+  Q8 s;
+  if (n_rows <= 0 || !cache || check_q8("", cache, &s) || cache->batch == 0 ||
+      check_heads("", n_heads, cache->n_kv_heads, n_rows))
+    return 0;
+  return 0;
+}
+
+int bn_paged_q8_decode(const bn_paged_q8 *cache, int dtype, const void *q, void *o, int n_heads,
+                       int64_t q_row_stride, int64_t o_row_stride, float scale, void *workspace,
+                       size_t workspace_bytes, void *stream) {
+  return attention_q8("Paged Q8 decode", cache, dtype, q, o, nullptr, cache ? cache->batch : 0, n_heads, q_row_stride,
+                      o_row_stride, scale, workspace, workspace_bytes, stream);
+}
+
+int bn_paged_q8_prefill(const bn_paged_q8 *cache, int dtype, const void *q, void *o, const int32_t *row_starts,
+                        int n_rows, int n_heads, int64_t q_row_stride, int64_t o_row_stride, float scale,
+                        void *workspace, size_t workspace_bytes, void *stream) {
+  return attention_q8("Paged Q8 prefill", cache, dtype, q, o, row_starts, n_rows, n_heads, q_row_stride, o_row_stride,
+                      scale, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,339 @@
+// bn_qk_norm.hip -- RMSNorm of every head of queries and keys with the rotation
+// by the row's position in the same pass, and its backward pass.
+//
+// The reference norms whole rows (op_rmsnorm.cuh:8-53) and turns heads
+// (op_rope.cuh:55-99); here the norm is a head's own.  With r = 1 / sqrt(mean(x^2)
+// + eps) and R the rotation by the row's position:
+//   y = R (w * x r)
+//   g = R^T dy,  dx = r (w g) - x r^3 / D * sum_d(w g x),  dw = sum_{rows, heads} g x r.
+// Everything between load and store is fp32; a head's sums are formed by its 2 to
+// 32 lanes, the weights' gradients per lane, then per workgroup, then over the
+// workgroups in the order of their numbers.
+#include <algorithm>
+
+#include "bn_head_rows.hpp"
+#include "bn_paged_host.hpp"
+
+namespace bn {
+namespace {
+
+constexpr int kMaxHeadDim = 256, kMostRows = 8;  // rows of a workgroup at once
+struct QkParams {
+  const void *q, *k, *wq, *wk, *gq, *gk;  // gq, gk: gradients of the outputs (backward)
+  void *qo, *ko;                          // outputs (backward: gradients of q and k)
+  const int32_t *positions;
+  int64_t q_rs, k_rs, gq_rs, gk_rs, qo_rs, ko_rs;
+  int n_rows, n_heads, n_kv_heads, rows, turn;  // rows: of a workgroup at once
+  int64_t offset;
+  float eps;
+  float *parts;                   // backward: [workgroups][2][D] sums
+  double f[kMaxHeadDim / 2];      // turns per position of each pair
+};
+
+// The pairs' cosines and sines of the rows that a workgroup has at once.
+template <int D>
+__device__ __forceinline__ void angles(const QkParams &p, float2 (*cs)[D / 2], int row0, int rows) {
+  if (!p.turn) return;
+  for (int i = threadIdx.x; i < rows * (D / 2); i += blockDim.x) {
+    const int r = i / (D / 2), row = row0 + r;
+    const int64_t pos = (p.positions ? (int64_t)p.positions[row] : (int64_t)row) + p.offset;
+    cs[r][i % (D / 2)] = cos_sin((double)pos * p.f[i % (D / 2)]);
+  }
+}
+
+// `rows` rows a workgroup: their angles once, then their heads' pieces of eight
+// elements, four of a thread on their way at once, the first of them while the
+// angles are formed.
+constexpr int kPieces = 4;
+template <typename T, int D>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkParams p) {
+  constexpr int LANES = D / 8;
+  __shared__ float2 cs[kMostRows][D / 2];
+  const int tid = threadIdx.x, row0 = blockIdx.x * p.rows, rows = min(p.rows, p.n_rows - row0);
+  const int heads = p.n_heads + p.n_kv_heads, per = heads * LANES, total = rows * per;
+  struct At {
+    int row, head, e;  // row of the workgroup, head (keys' behind the queries'), element
+  };
+  auto place = [&](int i) __attribute__((always_inline)) {
+    const int row = (int)((uint32_t)i / (uint32_t)per), rest = i - row * per;
+    return At{row, rest / LANES, rest % LANES * 8};
+  };
+  Raw8<T> raw[kPieces];
+  auto load = [&](int first) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      const int i = first + 256 * n;
+      if (i >= total) break;
+      const At a = place(i);
+      raw[n].load(a.head < p.n_heads
+                      ? (const T *)p.q + (int64_t)(row0 + a.row) * p.q_rs + a.head * D + a.e
+                      : (const T *)p.k + (int64_t)(row0 + a.row) * p.k_rs + (a.head - p.n_heads) * D + a.e);
+    }
+  };
+  load(tid);
+  angles<D>(p, cs, row0, rows);
+  __syncthreads();
+  for (int first = tid; first < total; first += 256 * kPieces) {
+    if (first != tid) load(first);
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      const int i = first + 256 * n;
+      if (i >= total) break;
+      const At a = place(i);
+      const bool is_q = a.head < p.n_heads;
+      Eight v = raw[n].floats();
+      const float r = head_rms<LANES>(v, p.eps);
+      Raw8<T> wr;
+      wr.load((const T *)(is_q ? p.wq : p.wk) + a.e);
+      const Eight w = wr.floats();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v.x[j] *= r * w.x[j];
+      if (p.turn) turn8(v, &cs[a.row][a.e / 2]);
+      store8(is_q ? (T *)p.qo + (int64_t)(row0 + a.row) * p.qo_rs + a.head * D + a.e
+                  : (T *)p.ko + (int64_t)(row0 + a.row) * p.ko_rs + (a.head - p.n_heads) * D + a.e,
+             v);
+    }
+  }
+}
+
+// A workgroup takes every gridDim.x-th group of `rows` rows.  A thread's pieces lie at
+// one place of their heads, so it adds up eight elements of each weight's
+// gradient in registers; a workgroup's sums go to the workspace.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void qk_norm_rope_backward_kernel(QkParams p) {
+  constexpr int LANES = D / 8;
+  __shared__ float2 cs[kMostRows][D / 2];
+  __shared__ float sums[4][2][D];
+  const int tid = threadIdx.x, lane = tid & 63, e = tid % LANES * 8;
+  Eight dw[2] = {};
+  for (int64_t at = (int64_t)blockIdx.x * p.rows; at < p.n_rows; at += (int64_t)gridDim.x * p.rows) {
+    const int row0 = (int)at, rows = min(p.rows, p.n_rows - row0);
+    __syncthreads();  // the angles before are no longer read
+    angles<D>(p, cs, row0, rows);
+    __syncthreads();
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const int heads = side ? p.n_kv_heads : p.n_heads, per = heads * LANES, total = rows * per;
+      const T *const x = (const T *)(side ? p.k : p.q), *const dy = (const T *)(side ? p.gk : p.gq);
+      T *const dx = (T *)(side ? p.ko : p.qo);
+      const int64_t x_rs = side ? p.k_rs : p.q_rs, dy_rs = side ? p.gk_rs : p.gq_rs, dx_rs = side ? p.ko_rs : p.qo_rs;
+      if (total == 0) continue;
+      Raw8<T> wr;
+      wr.load((const T *)(side ? p.wk : p.wq) + e);
+      const Eight w = wr.floats();
+      for (int i = tid; i < total; i += 256) {
+        const int row = (int)((uint32_t)i / (uint32_t)per), h = (i - row * per) / LANES;
+        Raw8<T> xr, gr;
+        xr.load(x + (row0 + row) * x_rs + h * D + e);
+        gr.load(dy + (row0 + row) * dy_rs + h * D + e);
+        const Eight v = xr.floats();
+        Eight g = gr.floats();
+        if (p.turn) turn8(g, &cs[row][e / 2], true);
+        const float r = head_rms<LANES>(v, p.eps);
+        float dot = 0.f;
+        Eight y;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float u = v.x[j] * r;  // the normed element
+          dw[side].x[j] = fmaf(g.x[j], u, dw[side].x[j]);
+          g.x[j] *= w.x[j];
+          dot = fmaf(g.x[j], u, dot);
+          y.x[j] = u;
+        }
+        dot = head_sum<LANES>(dot) * (1.0f / D);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y.x[j] = r * (g.x[j] - y.x[j] * dot);
+        store8(dx + (row0 + row) * dx_rs + h * D + e, y);
+      }
+    }
+  }
+#pragma unroll
+  for (int side = 0; side < 2; ++side)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float s = dw[side].x[j];
+#pragma unroll
+      for (int m = LANES; m < 64; m <<= 1) s += __shfl_xor(s, m, 64);
+      if (lane < LANES) sums[tid >> 6][side][e + j] = s;
+    }
+  __syncthreads();
+  for (int i = tid; i < 2 * D; i += 256)
+    p.parts[(int64_t)blockIdx.x * 2 * D + i] =
+        (sums[0][i / D][i % D] + sums[1][i / D][i % D]) + (sums[2][i / D][i % D] + sums[3][i / D][i % D]);
+}
+
+// The workgroups' sums, added: 32 lanes an element.
+__global__ __launch_bounds__(256) void qk_norm_rope_weights_kernel(const float *parts, int n, int d, float *dwq,
+                                                                   float *dwk) {
+  const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  float s = 0.f;
+  for (int i = lane; i < n; i += 32) s += parts[(int64_t)i * 2 * d + e];
+#pragma unroll
+  for (int m = 16; m; m >>= 1) s += __shfl_xor(s, m, 64);
+  if (lane == 0) {
+    if (e < d) dwq[e] = s;
+    else if (dwk) dwk[e - d] = s;
+  }
+}
+
+constexpr int kBackGroups = 1024;
+int rows_at_once(int n_rows) { return n_rows >= 8192 ? 8 : n_rows >= 2048 ? 4 : 1; }
+int back_groups(int n_rows) { return std::min((n_rows + rows_at_once(n_rows) - 1) / rows_at_once(n_rows), kBackGroups); }
+
+int check_qk(const std::string &op, int dtype, const void *q, const void *k, const void *wq, const void *wk,
+             int n_rows, int n_heads, int n_kv_heads, int head_dim, float eps, float theta) {
+  if (dtype != BN_F32 && dtype != BN_BF16) return fail(BN_ERR_UNSUPPORTED, op + ": dtype must be F32 or BF16");
+  if (n_rows < 0) return fail(BN_ERR_SHAPE, op + ": negative number of rows");
+  if (n_rows > (1 << 23)) return fail(BN_ERR_UNSUPPORTED, op + ": more than 2^23 rows");
+  if (n_heads <= 0) return fail(BN_ERR_SHAPE, op + ": num_heads must be positive");
+  if (n_kv_heads < 0) return fail(BN_ERR_SHAPE, op + ": negative num_kv_heads");
+  if (n_heads > 65535 || n_kv_heads > 65535) return fail(BN_ERR_UNSUPPORTED, op + ": more than 65535 heads");
+  if (head_dim < 16 || head_dim > kMaxHeadDim || (head_dim & (head_dim - 1)))
+    return fail(BN_ERR_UNSUPPORTED, op + ": head_dim must be 16, 32, 64, 128 or 256");
+  if (!(eps >= 0.f) || !std::isfinite(eps))
+    return fail(BN_ERR_INVALID_ARG, op + ": eps must be finite and not negative");
+  if (!(theta >= 0.f) || !std::isfinite(theta))
+    return fail(BN_ERR_INVALID_ARG, op + ": theta must be positive and finite, or 0 for no rotation");
+  if (n_rows > 0 && ((n_kv_heads > 0) != (k != nullptr)))
+    return fail(BN_ERR_INVALID_ARG, op + ": k and num_kv_heads must be given together");
+  if (!wq || (n_kv_heads > 0 && !wk)) return fail(BN_ERR_INVALID_ARG, op + ": weight is NULL");
+  if (!aligned16(wq) || !aligned16(wk)) return fail(BN_ERR_UNSUPPORTED, op + ": weights must be 16-byte aligned");
+  return BN_OK;
+}
+
+void fill_turns(double *f, int head_dim, float theta) {
+  for (int i = 0; i < head_dim / 2; ++i)
+    f[i] = theta > 0.f ? std::pow((double)theta, -2.0 * i / head_dim) / (2.0 * M_PI) : 0.0;
+}
+
+// K<T, D> for the dtype and head dimension
+#define BN_QK_LAUNCH(K, grid, s, p)                                                             \
+  do {                                                                                          \
+    if (dtype == BN_BF16) {                                                                     \
+      if (head_dim == 16) hipLaunchKernelGGL((K<bf16_t, 16>), grid, dim3(256), 0, s, p);        \
+      else if (head_dim == 32) hipLaunchKernelGGL((K<bf16_t, 32>), grid, dim3(256), 0, s, p);   \
+      else if (head_dim == 64) hipLaunchKernelGGL((K<bf16_t, 64>), grid, dim3(256), 0, s, p);   \
+      else if (head_dim == 128) hipLaunchKernelGGL((K<bf16_t, 128>), grid, dim3(256), 0, s, p); \
+      else hipLaunchKernelGGL((K<bf16_t, 256>), grid, dim3(256), 0, s, p);                      \
+    } else {                                                                                    \
+      if (head_dim == 16) hipLaunchKernelGGL((K<float, 16>), grid, dim3(256), 0, s, p);         \
+      else if (head_dim == 32) hipLaunchKernelGGL((K<float, 32>), grid, dim3(256), 0, s, p);    \
+      else if (head_dim == 64) hipLaunchKernelGGL((K<float, 64>), grid, dim3(256), 0, s, p);    \
+      else if (head_dim == 128) hipLaunchKernelGGL((K<float, 128>), grid, dim3(256), 0, s, p);  \
+      else hipLaunchKernelGGL((K<float, 256>), grid, dim3(256), 0, s, p);                       \
+    }                                                                                           \
+  } while (0)
+
+}  // namespace
+}  // namespace bn
+
+using namespace bn;
+
+extern "C" {
+
+int bn_qk_norm_rope(int dtype, const void *q, const void *k, const void *q_weight, const void *k_weight,
+                    void *q_out, void *k_out, const int32_t *positions, int n_rows, int n_heads, int n_kv_heads,
+                    int head_dim, int64_t q_row_stride, int64_t k_row_stride, int64_t q_out_row_stride,
+                    int64_t k_out_row_stride, int position_offset, float eps, float theta, void *stream) {
+  const std::string op = "QK norm";
+  int st = check_qk(op, dtype, q, k, q_weight, k_weight, n_rows, n_heads, n_kv_heads, head_dim, eps, theta);
+  if (st) return st;
+  if (n_rows == 0) return BN_OK;
+  if ((st = check_rows(op, "q", q, n_rows, n_heads, q_row_stride, dtype, head_dim)) ||
+      (st = check_rows(op, "q_out", q_out, n_rows, n_heads, q_out_row_stride, dtype, head_dim)) ||
+      (k && ((st = check_rows(op, "k", k, n_rows, n_kv_heads, k_row_stride, dtype, head_dim)) ||
+             (st = check_rows(op, "k_out", k_out, n_rows, n_kv_heads, k_out_row_stride, dtype, head_dim)))))
+    return st;
+  if ((q == q_out && q_row_stride != q_out_row_stride) || (k && k == k_out && k_row_stride != k_out_row_stride))
+    return fail(BN_ERR_INVALID_ARG, op + ": an output in its input's place must have its row stride");
+  if ((uintptr_t)positions & 3u) return fail(BN_ERR_UNSUPPORTED, op + ": positions must be 4-byte aligned");
+  DeviceScope scope;
+  if ((st = scope.enter(op, q, "q"))) return st;
+  QkParams p{};
+  p.q = q; p.k = k; p.wq = q_weight; p.wk = k_weight; p.qo = q_out; p.ko = k_out;
+  p.positions = positions;
+  p.q_rs = q_row_stride; p.k_rs = k_row_stride; p.qo_rs = q_out_row_stride; p.ko_rs = k_out_row_stride;
+  p.n_rows = n_rows; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads;
+  p.rows = rows_at_once(n_rows);
+  p.turn = theta > 0.f;
+  p.offset = position_offset;
+  p.eps = eps;
+  fill_turns(p.f, head_dim, theta);
+  const dim3 grid((unsigned)((n_rows + p.rows - 1) / p.rows));
+  BN_QK_LAUNCH(qk_norm_rope_kernel, grid, as_stream(stream), p);
+  BN_LAUNCH_CHECK();
+  return BN_OK;
+}
+
+size_t bn_qk_norm_rope_backward_workspace_size(int n_rows, int n_heads, int n_kv_heads, int head_dim) {
+  const float w = 0.f;
+  if (check_qk("", BN_F32, &w, n_kv_heads > 0 ? &w : nullptr, (const void *)16, (const void *)16, n_rows, n_heads, n_kv_heads,
+               head_dim, 0.f, 0.f))
+    return 0;
+  return (size_t)back_groups(n_rows) * 2 * head_dim * sizeof(float);
+}
+
+int bn_qk_norm_rope_backward(int dtype, const void *q, const void *k, const void *q_weight, const void *k_weight,
+                             const void *dq_out, const void *dk_out, void *dq, void *dk, float *dq_weight,
+                             float *dk_weight, const int32_t *positions, int n_rows, int n_heads, int n_kv_heads,
+                             int head_dim, int64_t q_row_stride, int64_t k_row_stride, int64_t dq_out_row_stride,
+                             int64_t dk_out_row_stride, int64_t dq_row_stride, int64_t dk_row_stride,
+                             int position_offset, float eps, float theta, void *workspace, size_t workspace_bytes,
+                             void *stream) {
+  const std::string op = "QK norm backward";
+  int st = check_qk(op, dtype, q, k, q_weight, k_weight, n_rows, n_heads, n_kv_heads, head_dim, eps, theta);
+  if (st) return st;
+  if (!dq_weight || (n_kv_heads > 0 && !dk_weight))
+    return fail(BN_ERR_INVALID_ARG, op + ": gradient of a weight is NULL");
+  if (((uintptr_t)dq_weight | (uintptr_t)dk_weight) & 3u)
+    return fail(BN_ERR_UNSUPPORTED, op + ": gradients of the weights must be 4-byte aligned");
+  if (n_rows > 0 &&
+      ((st = check_rows(op, "q", q, n_rows, n_heads, q_row_stride, dtype, head_dim)) ||
+       (st = check_rows(op, "dq_out", dq_out, n_rows, n_heads, dq_out_row_stride, dtype, head_dim)) ||
+       (st = check_rows(op, "dq", dq, n_rows, n_heads, dq_row_stride, dtype, head_dim)) ||
+       (k && ((st = check_rows(op, "k", k, n_rows, n_kv_heads, k_row_stride, dtype, head_dim)) ||
+              (st = check_rows(op, "dk_out", dk_out, n_rows, n_kv_heads, dk_out_row_stride, dtype, head_dim)) ||
+              (st = check_rows(op, "dk", dk, n_rows, n_kv_heads, dk_row_stride, dtype, head_dim))))))
+    return st;
+  if (n_rows > 0 && ((dq == q && dq_row_stride != q_row_stride) || (dq == dq_out && dq_row_stride != dq_out_row_stride) ||
+                     (k && ((dk == k && dk_row_stride != k_row_stride) || (dk == dk_out && dk_row_stride != dk_out_row_stride)))))
+    return fail(BN_ERR_INVALID_ARG, op + ": an output in an input's place must have its row stride");
+  if ((uintptr_t)positions & 3u) return fail(BN_ERR_UNSUPPORTED, op + ": positions must be 4-byte aligned");
+  const size_t need = bn_qk_norm_rope_backward_workspace_size(n_rows, n_heads, n_kv_heads, head_dim);
+  if (workspace && workspace_bytes < need)
+    return fail(BN_ERR_INVALID_ARG, op + ": workspace of " + std::to_string(workspace_bytes) + " bytes, need " +
+                                        std::to_string(need));
+  if (workspace && !aligned16(workspace))
+    return fail(BN_ERR_UNSUPPORTED, op + ": workspace must be 16-byte aligned");
+  DeviceScope scope;
+  if ((st = scope.enter(op, q_weight, "q_weight"))) return st;
+  QkParams p{};
+  p.q = q; p.k = k; p.wq = q_weight; p.wk = k_weight; p.gq = dq_out; p.gk = dk_out; p.qo = dq; p.ko = dk;
+  p.positions = positions;
+  p.q_rs = q_row_stride; p.k_rs = k_row_stride; p.gq_rs = dq_out_row_stride; p.gk_rs = dk_out_row_stride;
+  p.qo_rs = dq_row_stride; p.ko_rs = dk_row_stride;
+  p.n_rows = n_rows; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads;
+  p.rows = rows_at_once(n_rows);
+  p.turn = theta > 0.f;
+  p.offset = position_offset;
+  p.eps = eps;
+  fill_turns(p.f, head_dim, theta);
+  Workspace ws;
+  if ((st = ws.take(workspace, need, stream))) return st;
+  p.parts = (float *)ws.p;
+  hipStream_t s = as_stream(stream);
+  const int groups = back_groups(n_rows);
+  auto launch = [&]() -> int {
+    if (groups > 0) {
+      BN_QK_LAUNCH(qk_norm_rope_backward_kernel, dim3((unsigned)groups), s, p);
+      BN_LAUNCH_CHECK();
+    }
+    hipLaunchKernelGGL(qk_norm_rope_weights_kernel, dim3((unsigned)(2 * head_dim / 8)), dim3(256), 0, s, p.parts, groups,
+                       head_dim, dq_weight, n_kv_heads > 0 ? dk_weight : nullptr);
+    BN_LAUNCH_CHECK();
+    return BN_OK;
+  };
+  return ws.release(launch());
+}
+
+}  // extern "C"

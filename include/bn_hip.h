@@ -549,6 +549,119 @@ int bn_paged_decode_shared(const bn_paged_kv *cache, const void *q, void *o,
                            const int32_t *prefix_pages, int prefix_len,
                            void *workspace, size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------- norms of single heads, with RoPE
+ * No counterpart in the reference (its norms are of whole rows): RMSNorm of
+ * every head of q and k over its head_dim elements, and the rotation by the
+ * row's position, in one pass:
+ *   y = R(pos) (w * x / sqrt(mean(x^2) + eps)),
+ * pair p of the head turned by pos * theta^(-2p/head_dim) as bn_paged_append
+ * turns it (the angle in 64 bits; theta 0: nothing is turned), with one
+ * rounding at the end.  q, q_out: [n_rows, n_heads, head_dim] with row strides of
+ * their own (column ranges of a QKV projection's output are such tensors), k and
+ * k_out: [n_rows, n_kv_heads, head_dim]; k, k_out and k_weight NULL with
+ * n_kv_heads 0: q alone.  Weights: head_dim elements.  dtype BN_F32 or BN_BF16 for
+ * all of them; everything between is fp32.  positions: device int32 [n_rows]
+ * (NULL: row r is at r), position_offset is added; positions at or past 2^31
+ * or below -2^31 are not represented.  q_out may be q and k_out k (with the
+ * same row stride); no other overlap.  head_dim: 16, 32, 64, 128 or 256; at most
+ * 2^23 rows and 65535 heads; pointers and row strides multiples of 16 bytes. */
+int bn_qk_norm_rope(int dtype, const void *q, const void *k, const void *q_weight,
+                    const void *k_weight, void *q_out, void *k_out,
+                    const int32_t *positions, int n_rows, int n_heads,
+                    int n_kv_heads, int head_dim, int64_t q_row_stride,
+                    int64_t k_row_stride, int64_t q_out_row_stride,
+                    int64_t k_out_row_stride, int position_offset, float eps,
+                    float theta, void *stream);
+
+/* Its backward pass: from the gradients dq_out and dk_out of its outputs, with
+ * the q and k that it was given, dq and dk (of dtype) and the weights' gradients
+ * dq_weight and dk_weight (always fp32, head_dim elements, sums over all rows and
+ * heads, the same bits in every run).  dq may be dq_out or q in their place, with
+ * their row stride, dk dk_out or k.  n_rows 0: the weights' gradients are zeros.
+ * workspace: device memory of bn_qk_norm_rope_backward_workspace_size() bytes,
+ * 16-byte aligned, any contents (NULL: taken from the pool); calls in flight at once
+ * need workspaces of their own. */
+size_t bn_qk_norm_rope_backward_workspace_size(int n_rows, int n_heads, int n_kv_heads,
+                                               int head_dim);
+int bn_qk_norm_rope_backward(int dtype, const void *q, const void *k,
+                             const void *q_weight, const void *k_weight,
+                             const void *dq_out, const void *dk_out, void *dq, void *dk,
+                             float *dq_weight, float *dk_weight, const int32_t *positions,
+                             int n_rows, int n_heads, int n_kv_heads, int head_dim,
+                             int64_t q_row_stride, int64_t k_row_stride,
+                             int64_t dq_out_row_stride, int64_t dk_out_row_stride,
+                             int64_t dq_row_stride, int64_t dk_row_stride,
+                             int position_offset, float eps, float theta,
+                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------ paged KV cache in 8 bits
+ * bn_paged_kv's cache in half of bf16's memory: every element is an e4m3
+ * number (OCP: no infinities, 0x7f and 0xff are NaN, largest value 448) times a
+ * power of two that BN_Q8_BLOCK consecutive keys of a page have in common, one
+ * for each KV head and for K and V:
+ *   value = code * 2^(byte - 127)
+ * with code at k[page*page_stride + g*head_stride + s*row_stride + d] and byte at
+ * k_scale[page*scale_page_stride + g*scale_head_stride + s / BN_Q8_BLOCK]
+ * (strides in bytes; those of the codes multiples of 16; K and V share them).  A byte
+ * outside [10, 247], which no append writes, counts as the nearest of them: so
+ * every code's value is zero or a normal bf16 number (but for 256 to 448 times
+ * 2^120, which no append writes either and which are infinite).  Page table, lengths, pages without
+ * memory, rows of a ragged batch and the limits are bn_paged_kv's, but for
+ * page_size: a power of two in [BN_Q8_BLOCK, 2^20]. */
+#define BN_Q8_BLOCK 16
+typedef struct bn_paged_q8 {
+  void *k, *v;               /* codes (device) */
+  void *k_scale, *v_scale;   /* scales' bytes (device) */
+  const int32_t *page_table; /* device [batch, table_stride], max_pages entries a row */
+  const int32_t *seq_lens;   /* device [batch] */
+  int64_t page_stride, head_stride, row_stride;   /* of the codes */
+  int64_t scale_page_stride, scale_head_stride;   /* of the scales */
+  int64_t table_stride;                           /* elements */
+  int32_t batch, n_pages, max_pages, page_size, n_kv_heads, head_dim;
+} bn_paged_q8;
+
+/* bn_paged_append into such a cache: norms (where weights are given), rotation,
+ * and K and V rounded to nearest, ties to even, once, from fp32.  dtype: that of k, v,
+ * q, q_out and the weights (BN_F32 or BN_BF16).  q_weight, k_weight: 64 elements,
+ * or NULL for no norm of q, of k; as bn_qk_norm_rope norms a head, with eps.
+ * The scale of a block is the smallest power of two 2^n, n in [-117, 120], with
+ * which its largest element is at most 448; a call whose first row in a block comes
+ * behind older rows of it takes their scale if that is larger, and else rounds
+ * the older rows again under its own (a power of two only moves the window of
+ * exponents: they change where they fall below 2^-6 of it).  A block is written anew
+ * by a call that has its first row, whatever was there.  An infinite or NaN
+ * element is stored as NaN and has no part in the scale; at scale 2^120 codes go up to 240.
+ * Rows of two sequences that land in one block leave either's there, under
+ * either's scale.  Otherwise as bn_paged_append. */
+int bn_paged_q8_append(const bn_paged_q8 *cache, int dtype, const void *k,
+                       const void *v, const void *q, void *q_out,
+                       const int32_t *row_starts, int n_rows, int n_heads,
+                       int64_t k_row_stride, int64_t v_row_stride,
+                       int64_t q_row_stride, int64_t q_out_row_stride, float theta,
+                       const void *q_weight, const void *k_weight, float eps,
+                       void *stream);
+
+/* The cache's rows back: row i of sequence b's n rows (row_starts as for the
+ * append) is the key and the value at position seq_lens[b] - n + i, to k and v
+ * [n_rows, n_kv_heads, 64] of dtype BN_F32 or BN_BF16, exactly (either may be
+ * NULL).  A position outside the table or on a page without memory gives zeros.
+ * k and v must not lie in the cache.  At most 2^23 rows. */
+int bn_paged_q8_read(const bn_paged_q8 *cache, int dtype, void *k, void *v,
+                     const int32_t *row_starts, int n_rows, int64_t k_row_stride,
+                     int64_t v_row_stride, void *stream);
+
+/* bn_paged_workspace_size, bn_paged_decode and bn_paged_prefill over such a
+ * cache.  dtype: that of q and o, BN_BF16. */
+size_t bn_paged_q8_workspace_size(const bn_paged_q8 *cache, int n_heads, int n_rows);
+int bn_paged_q8_decode(const bn_paged_q8 *cache, int dtype, const void *q, void *o,
+                       int n_heads, int64_t q_row_stride, int64_t o_row_stride,
+                       float scale, void *workspace, size_t workspace_bytes,
+                       void *stream);
+int bn_paged_q8_prefill(const bn_paged_q8 *cache, int dtype, const void *q, void *o,
+                        const int32_t *row_starts, int n_rows, int n_heads,
+                        int64_t q_row_stride, int64_t o_row_stride, float scale,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
