@@ -697,7 +697,7 @@ def _qk_rows(what, t, like, heads):
         raise ValueError(f"{what}: expected [{like.shape[0]}, {heads}, {like.shape[2]}], got {tuple(t.shape)}")
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{what}: dtype and device must be q's")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    if t.shape[0] and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
         raise ValueError(f"{what}: a row's heads must be contiguous")
     return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
 
