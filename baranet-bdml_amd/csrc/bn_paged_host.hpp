@@ -7,7 +7,7 @@
 #include <string>
 
 #include "bn_common.hpp"
-#include "bn_paged_plan.hpp"
+#include "bn_paged_device.hpp"
 
 namespace bn {
 
@@ -153,6 +153,29 @@ class Workspace {
   }
 };
 
+// The decode kernel's launch: a workgroup per share and column, one per compute
+// unit in all (two: 64 caches of 4096 keys 45.8 -> 49.0 us, of 512..4096 34.6 ->
+// 35.7; 256 of 300 21.4 -> 18.8).
+constexpr int kDecGroups = 256;
+struct DecodePlan {
+  int hblocks, columns, bins;
+  size_t records, words;  // bytes
+};
+inline DecodePlan plan_decode(int batch, int n_heads, int n_kv_heads) {
+  DecodePlan d;
+  d.hblocks = (n_heads / n_kv_heads + kMaxRows - 1) / kMaxRows;
+  d.columns = d.hblocks * n_kv_heads;
+  d.bins = std::max(1, kDecGroups / d.columns);
+  d.records = d.bins == 1 ? 0 : (size_t)d.bins * 2 * d.columns * kMaxRows * kRec * sizeof(float);
+  d.words = d.bins == 1 ? 0 : (size_t)batch * d.columns * 16;
+  return d;
+}
+
+// The threads of a prefill's launch, which the runtime counts in 32 bits.
+inline int64_t prefill_threads(int dtype, int batch, int n_rows, int n_heads, int n_kv_heads, int cap) {
+  const PrefillPlan d = plan_prefill(dtype, batch, n_rows, n_heads, n_kv_heads, cap);
+  return d.groups * (d.hw == 8 ? 256 : 64 * d.hw * d.kw);
+}
 
 }  // namespace
 }  // namespace bn

@@ -15,7 +15,6 @@ namespace {
 
 constexpr int kBlock = BN_Q8_BLOCK;
 constexpr int kLow = 10, kHigh = 247;  // scale bytes
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // The cache as the kernels see it.
 struct Q8 {
@@ -267,63 +266,47 @@ __global__ __launch_bounds__(256) void paged_q8_read_kernel(Q8ReadParams p) {
 }
 
 // --------------------------------------------------------------- attention
-struct Q8AttnParams {
-  Q8 s;
-  const void *q;
-  void *o;
-  const int32_t *starts;
-  int64_t q_rs, o_rs;
-  int n_rows, n_heads, group;
-  float cl;  // scale * log2(e)
-};
-// A wave per row and head: 64 keys at a time, a key's score a lane, then an element
-// of the output a lane.
-__global__ __launch_bounds__(64) void paged_q8_attention_kernel(Q8AttnParams p) {
-  __shared__ float q[HD];
-  const Paged &c = p.s.c;
-  const int lane = threadIdx.x, row = blockIdx.x, h = blockIdx.y, g = h / p.group;
-  const int b = sequence_of(p.starts, c.batch, row);
-  if (b < 0) return;
-  const int64_t pos = p.starts ? (int64_t)max(c.lens[b], 0) - p.starts[b + 1] + row : (int64_t)max(c.lens[b], 0) - 1;
-  const int seen = pos < 0 ? 0 : pos >= c.cap ? c.cap : (int)pos + 1;
-  q[lane] = bf16_to_f32(((const bf16_t *)p.q + row * p.q_rs + h * HD)[lane]);
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  const int32_t *const table = c.table + b * c.table_stride;
-  auto page_of = [&](int key) { return table[key >> c.shift]; };
-  auto in_page = [&](int key) { return key & ((1 << c.shift) - 1); };
-  for (int k0 = 0; k0 < seen; k0 += 64) {
-    const int key = k0 + lane;
-    float s = -INFINITY;
-    if (key < seen) {
-      const int page = page_of(key);
-      if ((unsigned)page < (unsigned)c.n_pages) {
-        const u32x2 *const at = (const u32x2 *)((const uint8_t *)c.k + page * c.page_stride + g * c.head_stride +
-                                                in_page(key) * c.row_stride);
-        const float scale = scale_of(p.s.ks[page * p.s.scale_page + g * p.s.scale_head + (in_page(key) >> 4)]);
-        s = 0.f;
-        for (int i = 0; i < 8; ++i) {
-          const Eight x = values(at[i], scale);
-          for (int j = 0; j < 8; ++j) s = fmaf(x.x[j], q[8 * i + j], s);
-        }
-        s *= p.cl;
-      }
-    }
-    const float mt = fmaxf(m, wave_max(s)), ref = mt == -INFINITY ? 0.f : mt;
-    const float e = __builtin_amdgcn_exp2f(s - ref), alpha = __builtin_amdgcn_exp2f(m - ref);
-    m = mt;
-    l = l * alpha + wave_sum(e);
-    o *= alpha;
-    for (int j = 0; j < min(64, seen - k0); ++j) {
-      const int page = __builtin_amdgcn_readfirstlane(page_of(k0 + j));
-      if ((unsigned)page >= (unsigned)c.n_pages) continue;
-      const float scale = scale_of(p.s.vs[page * p.s.scale_page + g * p.s.scale_head + (in_page(k0 + j) >> 4)]);
-      const uint8_t code = ((const uint8_t *)c.v + page * c.page_stride + g * c.head_stride +
-                            in_page(k0 + j) * c.row_stride)[lane];
-      o = fmaf(__shfl(e, j, 64), two_values<false>(code, scale)[0], o);
-    }
+// The bf16 cache's kernels over codes: eight elements become bf16 in four
+// instructions, their scale an operand, where the bf16 cache's are stored to LDS
+// (prefill) or where the products' operands are read from it (decode).
+struct E4m3Pages {
+  typedef uint8_t T;
+  typedef u32x2 Raw;
+  static constexpr bool kScaled = true;
+  const uint8_t *ks, *vs;
+  int64_t page, head;
+  __device__ __forceinline__ const uint8_t *scales(int g, bool values) const { return (values ? vs : ks) + g * head; }
+  // the byte of the block of key k of page id (no page: page 0's)
+  __device__ __forceinline__ int scale(const uint8_t *base, const PageRows &rows, int id, int k) const {
+    return base[(rows.there(id) ? id : 0) * page + ((k & rows.slot_mask) >> 4)];
   }
-  ((bf16_t *)p.o + row * p.o_rs + h * HD)[lane] = f32_to_bf16(o * (l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l));
+  __device__ __forceinline__ int scale_bits(int byte) const { return min(max(byte, kLow), kHigh) << 23; }
+  __device__ __forceinline__ u32x4 bf16(uint32_t lo, uint32_t hi, float scale) const {
+    u32x4 y;
+    y[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+    y[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+    y[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+    y[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+    return y;
+  }
+  __device__ __forceinline__ u32x4 bf16(Raw x, int bits) const { return bf16(x[0], x[1], __builtin_bit_cast(float, bits)); }
+  __device__ __forceinline__ float value(const PageRows &rows, const char *Vg, int g, int id, int k, int lane) const {
+    const uint8_t code = ((const uint8_t *)Vg + rows.at(id, k))[lane];
+    return two_values<false>(code, scale_of(scale(scales(g, true), rows, id, k)))[0];
+  }
+};
+__global__ __launch_bounds__(256) void paged_q8_decode_kernel(DecodeParams p, E4m3Pages src) {
+  __shared__ __attribute__((aligned(16))) DecodeLds<uint8_t> lds;
+  decode_body<uint8_t>(p, lds, blockIdx.x, src);
+}
+template <int HW, int KW, int OCC>
+__global__ __launch_bounds__(64 * HW * KW, OCC) void paged_q8_prefill_kernel(PrefillParams p, E4m3Pages src) {
+  __shared__ __attribute__((aligned(16))) PrefillLds<HW, KW> lds;
+  prefill_bf16_body<HW, KW>(p, lds, blockIdx.x, src);
+}
+__global__ __launch_bounds__(256, 2) void paged_q8_prefill_pipe_kernel(PrefillParams p, E4m3Pages src) {
+  __shared__ __attribute__((aligned(16))) PipeLds lds;
+  prefill_pipe_body(p, lds, blockIdx.x, src);
 }
 
 // ---------------------------------------------------------------- the host
@@ -348,12 +331,55 @@ int check_q8(const std::string &op, const bn_paged_q8 *kv, Q8 *s) {
   return BN_OK;
 }
 
+int launch_decode(const AttnParams &a, const E4m3Pages &src, void *ws, hipStream_t s) {
+  const DecodePlan d = plan_decode(a.c.batch, a.n_heads, a.c.n_kv_heads);
+  DecodeParams p;
+  p.a = a;
+  p.ws = (float *)ws;
+  p.arrive_end = (unsigned long long *)((char *)ws + d.records + d.words);
+  p.tag = next_tag();
+  p.bins = d.bins; p.hblocks = d.hblocks; p.columns = d.columns;
+  p.k0 = 0;
+  p.parts = nullptr;
+  p.cuts = nullptr;
+  hipLaunchKernelGGL(paged_q8_decode_kernel, dim3((unsigned)(d.bins * d.columns)), dim3(256), 0, s, p, src);
+  BN_LAUNCH_CHECK();
+  return BN_OK;
+}
+
+int launch_prefill(const AttnParams &a, const E4m3Pages &src, void *ws, hipStream_t s) {
+  const PrefillPlan d = plan_prefill(BN_BF16, a.c.batch, a.n_rows, a.n_heads, a.c.n_kv_heads, a.c.cap);
+  PrefillParams p;
+  p.a = a;
+  p.ws = (float *)ws;
+  p.arrive_end = (unsigned long long *)((char *)ws + d.records + d.words);
+  p.tag = next_tag();
+  p.slots = (int)d.slots;
+  p.parts_all = d.parts_all;
+  p.pieces = (int)d.pieces;
+  p.prefix_parts = 0;
+  const dim3 grid((unsigned)d.groups);
+  if (d.hw == 8) {
+    hipLaunchKernelGGL(paged_q8_prefill_pipe_kernel, grid, dim3(256), 0, s, p, src);
+  } else if (d.hw == 4) {
+    if (d.kw == 2) hipLaunchKernelGGL((paged_q8_prefill_kernel<4, 2, 4>), grid, dim3(512), 0, s, p, src);
+    else hipLaunchKernelGGL((paged_q8_prefill_kernel<4, 1, 4>), grid, dim3(256), 0, s, p, src);
+  } else if (d.kw == 8) {
+    hipLaunchKernelGGL((paged_q8_prefill_kernel<1, 8, 2>), grid, dim3(512), 0, s, p, src);
+  } else {
+    hipLaunchKernelGGL((paged_q8_prefill_kernel<1, 4, 3>), grid, dim3(256), 0, s, p, src);
+  }
+  BN_LAUNCH_CHECK();
+  return BN_OK;
+}
+
 int attention_q8(const char *name, const bn_paged_q8 *kv, int dtype, const void *q, void *o, const int32_t *starts,
                  int n_rows, int n_heads, int64_t q_rs, int64_t o_rs, float scale, void *workspace,
                  size_t workspace_bytes, void *stream) {
   const std::string op = name;
-  Q8AttnParams p;
-  int st = check_q8(op, kv, &p.s);
+  Q8 c;
+  AttnParams p;
+  int st = check_q8(op, kv, &c);
   if (st || (st = check_heads(op, n_heads, kv->n_kv_heads, n_rows)) ||
       (st = check_starts(op, starts, n_rows, kv->batch)))
     return st;
@@ -364,6 +390,8 @@ int attention_q8(const char *name, const bn_paged_q8 *kv, int dtype, const void 
   if ((st = check_rows(op, "q", q, n_rows, n_heads, q_rs, dtype)) ||
       (st = check_rows(op, "o", o, n_rows, n_heads, o_rs, dtype)))
     return st;
+  if (starts && prefill_threads(BN_BF16, kv->batch, n_rows, n_heads, kv->n_kv_heads, c.c.cap) >= (int64_t)1 << 32)
+    return fail(BN_ERR_UNSUPPORTED, op + ": too many rows and sequences for one launch (2^32 threads)");
   const size_t need = bn_paged_q8_workspace_size(kv, n_heads, n_rows);
   if (workspace && workspace_bytes < need)
     return fail(BN_ERR_INVALID_ARG, op + ": workspace of " + std::to_string(workspace_bytes) +
@@ -372,14 +400,19 @@ int attention_q8(const char *name, const bn_paged_q8 *kv, int dtype, const void 
     return fail(BN_ERR_UNSUPPORTED, op + ": workspace must be 16-byte aligned");
   DeviceScope scope;
   if ((st = scope.enter(op, kv->seq_lens))) return st;
+  p.c = c.c;
   p.q = q; p.o = o; p.starts = starts;
   p.q_rs = q_rs; p.o_rs = o_rs;
   p.n_rows = n_rows; p.n_heads = n_heads; p.group = n_heads / kv->n_kv_heads;
+  p.inv_group = 1.0f / (float)p.group;
   p.cl = scale * kLog2e;
-  hipLaunchKernelGGL(paged_q8_attention_kernel, dim3((unsigned)n_rows, (unsigned)n_heads), dim3(64), 0,
-                     as_stream(stream), p);
-  BN_LAUNCH_CHECK();
-  return BN_OK;
+  p.prefix_pages = nullptr;
+  p.prefix_len = 0;
+  const E4m3Pages src{c.ks, c.vs, c.scale_page, c.scale_head};
+  Workspace ws;
+  if ((st = ws.take(workspace, need, stream))) return st;
+  hipStream_t s = as_stream(stream);
+  return ws.release(starts ? launch_prefill(p, src, ws.p, s) : launch_decode(p, src, ws.p, s));
 }
 
 }  // namespace
@@ -465,7 +498,9 @@ size_t bn_paged_q8_workspace_size(const bn_paged_q8 *cache, int n_heads, int n_r
   if (n_rows <= 0 || !cache || check_q8("", cache, &s) || cache->batch == 0 ||
       check_heads("", n_heads, cache->n_kv_heads, n_rows))
     return 0;
-  return 0;
+  const DecodePlan d = plan_decode(cache->batch, n_heads, cache->n_kv_heads);
+  const PrefillPlan f = plan_prefill(BN_BF16, cache->batch, n_rows, n_heads, cache->n_kv_heads, s.c.cap, true);
+  return std::max(d.records + d.words, f.records + f.words);
 }
 
 int bn_paged_q8_decode(const bn_paged_q8 *cache, int dtype, const void *q, void *o, int n_heads,
