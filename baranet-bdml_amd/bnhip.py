@@ -594,16 +594,17 @@ class PagedQ8:
 
 
 def _rows_dtype(what, t):
-    import torch
-    if t.dtype not in (torch.float32, torch.bfloat16):
+    """(type, the library's code) of rows."""
+    code = _row_type(t)
+    if code is None:
         raise ValueError(f"{what}: must be float32 or bfloat16")
-    return t.dtype
+    return t.dtype, code
 
 
 def _head_weight(what, w, cache, dtype):
     if w is None:
         return None
-    if tuple(w.shape) != (cache.head_dim,) or w.dtype != dtype or w.device != cache.device or not w.is_contiguous():
+    if w.shape != (cache.head_dim,) or w.dtype != dtype or w.device != cache.device or not w.is_contiguous():
         raise ValueError(f"{what}: must be a contiguous [{cache.head_dim}] tensor of the rows' type and device")
     return w.data_ptr()
 
@@ -614,7 +615,7 @@ def paged_q8_append(cache, k, v, q=None, q_out=None, row_starts=None, theta=1000
     normed head by head (where a weight [D] is given), turned by their positions,
     keys and values rounded and stored; k, v, q, q_out and the weights float32 or
     bfloat16, all alike.  Returns q_out (default: in place), or None without q."""
-    n, dt = k.shape[0], _rows_dtype("paged_q8_append: k", k)
+    n, (dt, code) = k.shape[0], _rows_dtype("paged_q8_append: k", k)
     kp, ks = _paged_rows("paged_q8_append: k", k, cache, n, cache.kv_heads, dt)
     vp, vs = _paged_rows("paged_q8_append: v", v, cache, n, cache.kv_heads, dt)
     qp, qs, op, os_, heads = None, 0, None, 0, 0
@@ -625,7 +626,7 @@ def paged_q8_append(cache, k, v, q=None, q_out=None, row_starts=None, theta=1000
         op, os_ = _paged_rows("paged_q8_append: q_out", q_out, cache, n, heads, dt)
     elif q_out is not None:
         raise ValueError("paged_q8_append: q_out without q")
-    call("bn_paged_q8_append", cache.ref, _torch_dtype_code(k), kp, vp, qp, op,
+    call("bn_paged_q8_append", cache.ref, code, kp, vp, qp, op,
          _row_starts("paged_q8_append", row_starts, cache, n), n, heads, ks, vs, qs, os_, theta,
          _head_weight("paged_q8_append: q_weight", q_weight, cache, dt),
          _head_weight("paged_q8_append: k_weight", k_weight, cache, dt), eps, _cache_stream(cache, stream))
@@ -637,8 +638,8 @@ def paged_q8_read(cache, row_starts=None, k=None, v=None, n_rows=None, dtype=Non
     row_starts[b] .. row_starts[b+1]-1, the last of them position seq_lens[b] - 1
     (None: one row each).  Given k or v alone, that one; given neither, both are made, of
     n_rows rows (default: the batch's, without row_starts) and dtype (default bfloat16)."""
-    import torch
     if k is None and v is None:
+        import torch
         n = cache.batch if n_rows is None and row_starts is None else n_rows
         if n is None:
             raise ValueError("paged_q8_read: n_rows, k or v is needed with row_starts")
@@ -646,12 +647,14 @@ def paged_q8_read(cache, row_starts=None, k=None, v=None, n_rows=None, dtype=Non
                                                     dtype=torch.bfloat16 if dtype is None else dtype))
                 for _ in range(2))
     one = k if k is not None else v
-    n, dt = one.shape[0], _rows_dtype("paged_q8_read: k and v", one)
-    (kp, ks), (vp, vs) = ((None, 0) if t is None else _paged_rows(f"paged_q8_read: {name}", t, cache, n,
-                                                                  cache.kv_heads, dt)
-                          for name, t in (("k", k), ("v", v)))
-    call("bn_paged_q8_read", cache.ref, _torch_dtype_code(one), kp, vp,
-         _row_starts("paged_q8_read", row_starts, cache, n), n, ks, vs, _cache_stream(cache, stream))
+    n, (dt, code) = one.shape[0], _rows_dtype("paged_q8_read: k and v", one)
+    kp, ks, vp, vs = None, 0, None, 0
+    if k is not None:
+        kp, ks = _paged_rows("paged_q8_read: k", k, cache, n, cache.kv_heads, dt)
+    if v is not None:
+        vp, vs = _paged_rows("paged_q8_read: v", v, cache, n, cache.kv_heads, dt)
+    call("bn_paged_q8_read", cache.ref, code, kp, vp, _row_starts("paged_q8_read", row_starts, cache, n), n, ks, vs,
+         _cache_stream(cache, stream))
     return k, v
 
 
@@ -691,36 +694,66 @@ def paged_q8_prefill(q, cache, row_starts=None, o=None, scale=None, workspace=No
 
 
 # ------------------------------------------------- norms of single heads
-def _qk_rows(what, t, like, heads):
-    """(pointer, row stride) of a [rows, heads, D] tensor of like's type, device, rows and D."""
-    if t.dim() != 3 or t.shape[0] != like.shape[0] or t.shape[1] != heads or t.shape[2] != like.shape[2]:
-        raise ValueError(f"{what}: expected [{like.shape[0]}, {heads}, {like.shape[2]}], got {tuple(t.shape)}")
-    if t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{what}: dtype and device must be q's")
-    if t.shape[0] and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
-        raise ValueError(f"{what}: a row's heads must be contiguous")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+_ROW_TYPES = {}  # torch types of rows -> the library's; filled by the first call
 
 
-def _qk_args(what, q, k, q_weight, k_weight, positions, stream):
-    import torch
-    if q.dim() != 3:
-        raise ValueError(f"{what}: q must be [rows, heads, D]")
-    _rows_dtype(f"{what}: q", q)
+def _row_type(t):
+    """The library's code of float32 or bfloat16, None of other types (without an import or a dict a call)."""
+    if not _ROW_TYPES:
+        import torch
+        _ROW_TYPES.update({torch.float32: BN_F32, torch.bfloat16: BN_BF16})
+    return _ROW_TYPES.get(t.dtype)
+
+
+def _qk_rows(op, name, t, rows, heads, like):
+    """(pointer, row stride) of a [rows, heads, D] tensor of like's type, device and D."""
+    shape, stride = t.shape, t.stride()
+    d = like.shape[2]
+    if shape != (rows, heads, d):
+        raise ValueError(f"{op}: {name}: expected [{rows}, {heads}, {d}], got {tuple(shape)}")
+    if t is not like and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{op}: {name}: dtype and device must be q's")
+    if rows and (stride[2] != 1 or (heads > 1 and stride[1] != d)):
+        raise ValueError(f"{op}: {name}: a row's heads must be contiguous")
+    return t.data_ptr(), stride[0] if rows > 1 else heads * d
+
+
+def _qk_args(op, q, k, q_weight, k_weight, positions, stream):
+    """What both directions check alike: (type, stream, pointer of the positions)."""
+    if q.dim() != 3 or (k is not None and k.dim() != 3):
+        raise ValueError(f"{op}: q and k must be [rows, heads, D]")
+    code, device = _row_type(q), q.device
+    if code is None:
+        raise ValueError(f"{op}: q must be float32 or bfloat16")
     if (k is None) != (k_weight is None):
-        raise ValueError(f"{what}: k and k_weight must be given together")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (tuple(w.shape) != (q.shape[2],) or w.dtype != q.dtype or w.device != q.device or
+        raise ValueError(f"{op}: k and k_weight must be given together")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != q.shape[2:] or w.dtype != q.dtype or w.device != device or
                               not w.is_contiguous()):
-            raise ValueError(f"{what}: {name} must be a contiguous [{q.shape[2]}] tensor of q's type and device")
-    if positions is not None and (positions.dtype != torch.int32 or tuple(positions.shape) != (q.shape[0],) or
-                                  not positions.is_contiguous() or positions.device != q.device):
-        raise ValueError(f"{what}: positions must be int32 [rows] on q's device")
-    if q.device.type != "cuda":
-        raise ValueError(f"{what}: its tensors are not on a GPU")
-    if stream is not None and stream.device != q.device:
-        raise ValueError(f"{what}: the stream is another device's")
-    return torch._C._cuda_getCurrentRawStream(q.device.index) if stream is None else stream.cuda_stream
+            raise ValueError(f"{op}: {'q_weight' if w is q_weight else 'k_weight'} must be a contiguous "
+                             f"[{q.shape[2]}] tensor of q's type and device")
+    if positions is None:
+        pp = None
+    else:
+        import torch
+        if positions.dtype != torch.int32 or positions.shape != q.shape[:1] or not positions.is_contiguous() or \
+                positions.device != device:
+            raise ValueError(f"{op}: positions must be int32 [rows] on q's device")
+        pp = positions.data_ptr()
+    if device.type != "cuda":
+        raise ValueError(f"{op}: its tensors are not on a GPU")
+    if stream is None:
+        import torch
+        return code, torch._C._cuda_getCurrentRawStream(device.index), pp
+    if stream.device != device:
+        raise ValueError(f"{op}: the stream is another device's")
+    return code, stream.cuda_stream, pp
+
+
+def _like(t, stream):
+    """A contiguous tensor of t's shape and type, memory of the stream."""
+    import torch
+    return made_on(stream, lambda: torch.empty(t.shape, dtype=t.dtype, device=t.device))
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, eps=1e-5, positions=None, position_offset=0, theta=10000.0,
@@ -730,21 +763,24 @@ def qk_norm_rope(q, k, q_weight, k_weight, eps=1e-5, positions=None, position_of
     (positions[row], default the row's number, + position_offset) in one pass.
     Heads contiguous, row strides of their own; float32 or bfloat16.  k and
     k_weight may be None.  q_out may be q, k_out k."""
-    import torch
-    s = _qk_args("qk_norm_rope", q, k, q_weight, k_weight, positions, stream)
-    q_out = made_on(stream, lambda: torch.empty(q.shape, dtype=q.dtype, device=q.device)) if q_out is None else q_out
-    (qp, qs), (op, os_) = (_qk_rows(f"qk_norm_rope: {n}", t, q, q.shape[1]) for n, t in (("q", q), ("q_out", q_out)))
-    kp, ks, kop, kos, hkv = None, 0, None, 0, 0
-    if k is not None:
-        hkv = k.shape[1] if k.dim() == 3 else 0
-        k_out = made_on(stream, lambda: torch.empty(k.shape, dtype=k.dtype, device=k.device)) if k_out is None else k_out
-        (kp, ks), (kop, kos) = (_qk_rows(f"qk_norm_rope: {n}", t, q, hkv) for n, t in (("k", k), ("k_out", k_out)))
-    elif k_out is not None:
-        raise ValueError("qk_norm_rope: k_out without k")
-    call("bn_qk_norm_rope", _torch_dtype_code(q), qp, kp, q_weight.data_ptr(),
-         None if k_weight is None else k_weight.data_ptr(), op, kop,
-         None if positions is None else positions.data_ptr(), q.shape[0], q.shape[1], hkv, q.shape[2], qs, ks, os_, kos,
-         position_offset, eps, theta, s)
+    op = "qk_norm_rope"
+    code, s, pp = _qk_args(op, q, k, q_weight, k_weight, positions, stream)
+    rows, heads, d = q.shape
+    qp, qs = _qk_rows(op, "q", q, rows, heads, q)
+    q_out = _like(q, stream) if q_out is None else q_out
+    op_, os_ = _qk_rows(op, "q_out", q_out, rows, heads, q)
+    if k is None:
+        if k_out is not None:
+            raise ValueError(f"{op}: k_out without k")
+        call("bn_qk_norm_rope", code, qp, None, q_weight.data_ptr(), None, op_, None, pp, rows, heads, 0, d, qs, 0, os_, 0,
+             position_offset, eps, theta, s)
+        return q_out, None
+    hkv = k.shape[1]
+    kp, ks = _qk_rows(op, "k", k, rows, hkv, q)
+    k_out = _like(k, stream) if k_out is None else k_out
+    kop, kos = _qk_rows(op, "k_out", k_out, rows, hkv, q)
+    call("bn_qk_norm_rope", code, qp, kp, q_weight.data_ptr(), k_weight.data_ptr(), op_, kop, pp, rows, heads, hkv, d, qs,
+         ks, os_, kos, position_offset, eps, theta, s)
     return q_out, k_out
 
 
@@ -762,31 +798,33 @@ def qk_norm_rope_backward(q, k, q_weight, k_weight, dq_out, dk_out, eps=1e-5, po
     dk_out or k.  Without k (None, and its weight and gradient) dk and dk_weight
     are None."""
     import torch
-    what = "qk_norm_rope_backward"
-    s = _qk_args(what, q, k, q_weight, k_weight, positions, stream)
+    op = "qk_norm_rope_backward"
+    code, s, pp = _qk_args(op, q, k, q_weight, k_weight, positions, stream)
     if (k is None) != (dk_out is None):
-        raise ValueError(f"{what}: k and dk_out must be given together")
-    new = lambda t: made_on(stream, lambda: torch.empty(t.shape, dtype=t.dtype, device=t.device))  # noqa: E731
-    grad = lambda: made_on(stream, lambda: torch.empty(q.shape[2], dtype=torch.float32, device=q.device))  # noqa: E731
-    dq = new(q) if dq is None else dq
-    (qp, qs), (gp, gs), (dp, ds) = (_qk_rows(f"{what}: {n}", t, q, q.shape[1])
-                                    for n, t in (("q", q), ("dq_out", dq_out), ("dq", dq)))
-    kp, ks, gkp, gks, dkp, dks, hkv, dwk = None, 0, None, 0, None, 0, 0, None
+        raise ValueError(f"{op}: k and dk_out must be given together")
+    rows, heads, d = q.shape
+    qp, qs = _qk_rows(op, "q", q, rows, heads, q)
+    gp, gs = _qk_rows(op, "dq_out", dq_out, rows, heads, q)
+    dq = _like(q, stream) if dq is None else dq
+    dp, ds = _qk_rows(op, "dq", dq, rows, heads, q)
+    kp, ks, gkp, gks, dkp, dks, hkv = None, 0, None, 0, None, 0, 0
     if k is not None:
-        hkv = k.shape[1] if k.dim() == 3 else 0
-        dk, dwk = new(k) if dk is None else dk, grad()
-        (kp, ks), (gkp, gks), (dkp, dks) = (_qk_rows(f"{what}: {n}", t, q, hkv)
-                                            for n, t in (("k", k), ("dk_out", dk_out), ("dk", dk)))
+        hkv = k.shape[1]
+        kp, ks = _qk_rows(op, "k", k, rows, hkv, q)
+        gkp, gks = _qk_rows(op, "dk_out", dk_out, rows, hkv, q)
+        dk = _like(k, stream) if dk is None else dk
+        dkp, dks = _qk_rows(op, "dk", dk, rows, hkv, q)
     elif dk is not None:
-        raise ValueError(f"{what}: dk without k")
-    dwq = grad()
+        raise ValueError(f"{op}: dk without k")
     ws, wsb = None, 0
     if workspace is not None:
         if workspace.device != q.device or not workspace.is_contiguous():
-            raise ValueError(f"{what}: the workspace must be contiguous memory of q's device")
+            raise ValueError(f"{op}: the workspace must be contiguous memory of q's device")
         ws, wsb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    call("bn_qk_norm_rope_backward", _torch_dtype_code(q), qp, kp, q_weight.data_ptr(),
-         None if k_weight is None else k_weight.data_ptr(), gp, gkp, dp, dkp, dwq.data_ptr(),
-         None if dwk is None else dwk.data_ptr(), None if positions is None else positions.data_ptr(), q.shape[0],
-         q.shape[1], hkv, q.shape[2], qs, ks, gs, gks, ds, dks, position_offset, eps, theta, ws, wsb, s)
-    return dq, dk, dwq, dwk
+    dw = made_on(stream, lambda: torch.empty((2, d), dtype=torch.float32, device=q.device))
+    dwq, dwk = dw.unbind()
+    at = dw.data_ptr()
+    call("bn_qk_norm_rope_backward", code, qp, kp, q_weight.data_ptr(), None if k is None else k_weight.data_ptr(), gp, gkp,
+         dp, dkp, at, None if k is None else at + 4 * d, pp, rows, heads, hkv, d, qs, ks, gs, gks, ds, dks,
+         position_offset, eps, theta, ws, wsb, s)
+    return dq, dk, dwq, None if k is None else dwk

@@ -295,9 +295,470 @@ struct E4m3Pages {
     return two_values<false>(code, scale_of(scale(scales(g, true), rows, id, k)))[0];
   }
 };
-__global__ __launch_bounds__(256) void paged_q8_decode_kernel(DecodeParams p, E4m3Pages src) {
-  __shared__ __attribute__((aligned(16))) DecodeLds<uint8_t> lds;
-  decode_body<uint8_t>(p, lds, blockIdx.x, src);
+// ------------------------------------------------------------------ decode
+// The batch's tiles of 64 keys, sequences in order, are dealt in equal shares to the
+// workgroups of a column (a KV head, or up to 16 of its query heads).  A
+// workgroup finds the sequences of its share by a scan of the lengths, one thread a
+// run of them, and lists them in LDS; its eight waves take the listed tiles in turn,
+// each with the next one's rows on their way, leave their parts of each sequence
+// (reference, sum, accumulator) in LDS and add them up; then the next list, if the
+// share has more sequences than LDS holds parts of.  What lies where -- page
+// offsets, scales -- a wave looks up for 64 of its tiles at once, a tile a lane, so
+// that a step has only to read it from there: the loop's instructions, not the
+// bytes, are what bounds this kernel when they are many (650 a tile, with eight
+// waves a compute unit: 2.6 us a tile).
+//
+// Per tile, with the query heads as columns of the products, as the bf16 cache's:
+//   S^T[key][head] = K . Q^T,  O^T[d][head] += V^T . P^T   (v_mfma_f32_16x16x32_bf16)
+// K's operand is sixteen codes of a row and V's a transposing read's column of
+// eight rows, both converted (exactly) where they are used, the scale an operand.  A
+// score tile's rows are keys 4 (u % 2) + 8 (row / 4) + row % 4 of its 32, so that a
+// lane's scores of two tiles are those of eight keys in a row, V's operand's order.
+constexpr int kWaves = 8, kTile = 64;
+constexpr int kListed = 32;                  // sequences of a list
+constexpr int kHoldParts = 256;              // rows of LDS for the waves' parts of sequences
+constexpr int kPitch = HD + 16;              // bytes of a row in LDS: b128 reads of 16 rows spread over the banks
+constexpr int kRows16 = 16 * kPitch + 64;    // sixteen rows, and 64 bytes so that rows 16 apart do too
+constexpr int kHoldRow = HD + 4;             // floats of a part's row: a record's, 16-byte aligned
+constexpr int kShareLeast = 8;               // tiles of a share at least: one a wave
+constexpr int kMerged = 16;                  // records read at once
+struct Q8DecodeLds {
+  uint8_t k[kWaves][4 * kRows16], v[kWaves][4 * kRows16];
+  float hold[kHoldParts * kHoldRow];
+  int list_b[kListed], list_first[kListed], list_len[kListed];  // sequence, position of its first tile, keys
+  int sums[2][kWaves], rank0, last_in[2];
+};
+
+__global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodeParams p, E4m3Pages src) {
+  __shared__ __attribute__((aligned(16))) Q8DecodeLds lds;
+  const Paged &c = p.a.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, grp = lane >> 4;
+  const int bin = blockIdx.x / p.columns, col = blockIdx.x - bin * p.columns;
+  const int g = col / p.hblocks, hb = col - g * p.hblocks;
+  const int rows = min(kMaxRows, p.a.group - kMaxRows * hb), head0 = g * p.a.group + kMaxRows * hb;
+
+  // ---- the share
+  auto keys_of = [&](int b) { return max(min(c.lens[b], c.cap), 0); };
+  auto tiles_of = [](int len) { return (int)((uint32_t)(len + kTile - 1) / kTile); };
+  const int per = (c.batch + 64 * kWaves - 1) / (64 * kWaves), from = min(tid * per, c.batch), to = min(from + per, c.batch);
+  int own = 0, some = 0;  // tiles of the thread's run of sequences; sequences of it that have any
+#pragma unroll 8
+  for (int b = from; b < to; ++b) {
+    const int t = tiles_of(keys_of(b));
+    own += t;
+    some += t > 0;
+  }
+  int upto = wave_scan(own), rank = wave_scan(some);
+  if (lane == 63) {
+    lds.sums[0][wave] = upto;
+    lds.sums[1][wave] = rank;
+  }
+  if (tid == 0) lds.rank0 = 0;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) {
+    const int t = lds.sums[0][v], r = lds.sums[1][v];
+    total += t;
+    upto += v < wave ? t : 0;
+    rank += v < wave ? r : 0;
+  }
+  upto -= own;
+  rank -= some;  // before the thread's run
+  const int share =
+      __builtin_amdgcn_readfirstlane(max((int)((uint32_t)(total + p.bins - 1) / (uint32_t)p.bins), kShareLeast));
+  const int pos0 = (int)min((int64_t)bin * share, (int64_t)total), end = min(pos0 + share, total);
+
+  // what a piece of work leaves: two or four elements of a head's row
+  auto write4 = [&](int b, int h, int d, const f32x4 &x, float sum) __attribute__((always_inline)) {
+    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+    bf16_t *const op = (bf16_t *)p.a.o + b * p.a.o_rs + (head0 + h) * HD + d;
+    const uint32_t lo = (uint32_t)f32_to_bf16(x[0] * inv) | ((uint32_t)f32_to_bf16(x[1] * inv) << 16);
+    const uint32_t hi = (uint32_t)f32_to_bf16(x[2] * inv) | ((uint32_t)f32_to_bf16(x[3] * inv) << 16);
+    *(uint2 *)op = make_uint2(lo, hi);
+  };
+  // row h of the record of a sequence's piece in bin `at` (a bin has two: the end
+  // of a sequence begun before it, and the start of one, begun in bin0, that goes on)
+  auto record = [&](int at, int bin0, int h) __attribute__((always_inline)) {
+    return p.ws + ((((int64_t)at * 2 + (at == bin0)) * p.columns + col) * kMaxRows + h) * kRec;
+  };
+  const int quads = (rows + 3) >> 2;  // a wave adds up four rows at a time, four elements a lane
+  auto place_of_unit = [&](int u) { return quads == 1 ? u : quads == 2 ? u >> 1 : quads == 4 ? u >> 2 : u * 0x5556 >> 16; };
+  struct Cut {  // a sequence that is cut between shares: its first bin and its number of pieces, one a bin
+    int b, bin0, pieces;
+  };
+  Cut cuts[2] = {{0, 0, 0}, {0, 0, 0}};  // one that began before the share, one that goes on
+
+  if (pos0 < end) {
+    // the first sequence's number among those that have tiles
+    if (upto <= pos0 && pos0 < upto + own) {
+      int at = upto, r = rank;
+      for (int b = from; b < to; ++b) {
+        const int t = tiles_of(keys_of(b));
+        if (at + t > pos0) break;
+        at += t;
+        r += t > 0;
+      }
+      lds.rank0 = r;
+    }
+    const uint32_t off = (uint32_t)((lane >> 2) * c.row_stride + (lane & 3) * 16);
+    const char *const Kg = (const char *)c.k + g * c.head_stride, *const Vg = (const char *)c.v + g * c.head_stride;
+    const uint8_t *const ksg = src.scales(g, false), *const vsg = src.scales(g, true);
+    const PageRows pages = PageRows::of<uint8_t>(c);
+    uint8_t *const kt = lds.k[wave], *const vt = lds.v[wave];
+    const float cl = p.a.cl;
+
+    int at = pos0, listed = 0;                // the share's tiles and sequences that are through
+    int wb = from, wfirst = upto, wrank = rank;  // the thread's first sequence that is not
+    for (;;) {
+      // ---- the list: the next sequences of the share
+      if (tid < kListed) lds.list_b[tid] = -1;
+      __syncthreads();
+      if (upto < end && upto + own > at) {
+        for (int t; wb < to && wfirst + (t = tiles_of(keys_of(wb))) <= at; ++wb) {
+          wfirst += t;
+          wrank += t > 0;
+        }
+        int first = wfirst, r = wrank - lds.rank0 - listed;
+        for (int b = wb; b < to && first < end && r < kListed; ++b) {
+          const int len = keys_of(b), t = tiles_of(len);
+          if (t > 0) {
+            lds.list_b[r] = b;
+            lds.list_first[r] = first;
+            lds.list_len[r] = len;
+          }
+          first += t;
+          r += t > 0;
+        }
+      }
+      __syncthreads();
+      // lane l: the list's l-th sequence
+      const int lb = lds.list_b[lane & (kListed - 1)], lfirst = lds.list_first[lane & (kListed - 1)],
+                llen = lds.list_len[lane & (kListed - 1)];
+      bool there = lane < kListed && lb >= 0;
+      const int lend = there ? lfirst + tiles_of(llen) : 0;
+      const int lstop = min(lend, end), lcount = there ? lstop - max(lfirst, at) : 0;
+      const int lparts = min(lcount, kWaves), lupto = wave_scan(lparts), lbefore = lupto - lparts;
+      there = there && lupto * rows <= kHoldParts;
+      const int n_list = __builtin_popcountll(__builtin_amdgcn_ballot_w64(there));
+      const int stop = __builtin_amdgcn_readlane(lstop, n_list - 1);
+
+      // ---- the wave's tiles, at + wave + 8 i, looked up 64 at a time
+      const int n = stop - at > wave ? (stop - at - wave + kWaves - 1) / kWaves : 0;
+      uint32_t at_lo[4], at_hi[4];  // byte offset of rows 16 r ..
+      uint32_t kscales, vscales;    // bytes of rows 16 r ..
+      int info, first_keys;         // place in the list | bits 8 ..: rows 16 r .. have memory; keys of the tile
+      auto look_up = [&](int i0) __attribute__((always_inline)) {
+        const int pos = min(at + wave + kWaves * (i0 + lane), stop - 1);
+        int place = 0;
+        for (int l = 0; l < n_list - 1; ++l) place += pos >= __builtin_amdgcn_readlane(lstop, l);
+        const int b = lds.list_b[place], len = lds.list_len[place], key0 = kTile * (pos - lds.list_first[place]);
+        const int32_t *const table = c.table + b * c.table_stride;
+        info = place;
+        first_keys = min(len - key0, kTile);
+        int id[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) id[r] = table[(uint32_t)min(key0 + 16 * r, len - 1) >> c.shift];
+        kscales = vscales = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          info |= pages.there(id[r]) << (8 + r);
+          const uint64_t x = pages.at(id[r], key0 + 16 * r);
+          at_lo[r] = (uint32_t)x;
+          at_hi[r] = (uint32_t)(x >> 32);
+          kscales |= (uint32_t)min(max(src.scale(ksg, pages, id[r], key0 + 16 * r), kLow), kHigh) << (8 * r);
+          vscales |= (uint32_t)min(max(src.scale(vsg, pages, id[r], key0 + 16 * r), kLow), kHigh) << (8 * r);
+        }
+      };
+      struct Tile {  // in flight: its rows' pieces, 16 rows an instruction
+        u32x4 k[4], v[4];
+        int info, keys;
+        uint32_t ks, vs;
+      } x;
+      auto load = [&](int i) __attribute__((always_inline)) {
+        const int j = i & 63;
+        x.info = __builtin_amdgcn_readlane(info, j);
+        x.keys = __builtin_amdgcn_readlane(first_keys, j);
+        x.ks = __builtin_amdgcn_readlane(kscales, j);
+        x.vs = __builtin_amdgcn_readlane(vscales, j);
+        uint32_t o32 = off;
+        asm volatile("" : "+v"(o32));  // a scalar base and this offset, not a sum of pointers kept in registers
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {  // streamed once: non-temporal
+          const uint64_t to_row = (uint32_t)__builtin_amdgcn_readlane(at_lo[r], j) |
+                                  (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi[r], j) << 32;
+          x.k[r] = __builtin_nontemporal_load((const u32x4 *)(Kg + to_row + o32));
+          x.v[r] = __builtin_nontemporal_load((const u32x4 *)(Vg + to_row + o32));
+        }
+      };
+      u32x4 q[2], qn[2];  // head l16's elements 16 grp .. + 15
+      auto load_q = [&](int place) __attribute__((always_inline)) {
+        const bf16_t *const qp = (const bf16_t *)p.a.q + (int64_t)__builtin_amdgcn_readlane(lb, place) * p.a.q_rs +
+                                 (head0 + min(l16, rows - 1)) * HD + 16 * grp;
+        qn[0] = *(const u32x4 *)qp;
+        qn[1] = *(const u32x4 *)(qp + 8);
+      };
+      float mc = -INFINITY, sum = 0.f;  // of head l16: reference, log2 units; this lane's keys' sum
+      f32x4 o[4];
+      bool fresh = true;
+      if (n > 0) {
+        look_up(0);
+        load(0);
+        load_q(x.info & 255);
+      }
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const int place = x.info & 255, have = x.info >> 8 & 15, keys = x.keys;
+        const uint32_t ks = x.ks, vs = x.vs;
+        // a wave's LDS instructions execute in order, so its tile needs no
+        // barrier; wave_barrier keeps the compiler from moving them across
+        __builtin_amdgcn_wave_barrier();
+        if (keys < kTile || have != 15) {  // no key: zeros, whatever lies there
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if ((lane >> 2) + 16 * r >= keys || !(have >> r & 1)) x.k[r] = x.v[r] = u32x4{0, 0, 0, 0};
+        }
+        {
+          uint8_t *const kd = kt + (lane >> 2) * kPitch + (lane & 3) * 16, *const vd = vt + (lane >> 2) * kPitch + (lane & 3) * 16;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) *(u32x4 *)(kd + r * kRows16) = x.k[r];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) *(u32x4 *)(vd + r * kRows16) = x.v[r];
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (fresh) {
+          q[0] = qn[0];
+          q[1] = qn[1];
+          mc = -INFINITY;
+          sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = f32x4{};
+        }
+        bool ends = i + 1 == n;
+        if (!ends) {
+          if (((i + 1) & 63) == 0) look_up(i + 1);
+          load(i + 1);
+          ends = (x.info & 255) != place;
+          if (ends) load_q(x.info & 255);
+        }
+        fresh = ends;
+        // scores: s[u][j] of key 32 (u / 2) + 8 grp + 4 (u % 2) + j
+        f32x4 s[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int row = 8 * (l16 >> 2) + 4 * (u & 1) + (l16 & 3);  // of its 32; its sixteen: l16 / 8
+          const u32x4 y = *(const u32x4 *)(kt + (u >> 1) * 2 * kRows16 + row * kPitch + (l16 >> 3) * 64 + 16 * grp);
+          const float scale = __uint_as_float((ks >> (16 * (u >> 1) + (l16 & 8)) & 255u) << 23);
+          s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, src.bf16(y[0], y[1], scale)),
+                                                         __builtin_bit_cast(bf16x8, q[0]), f32x4{}, 0, 0, 0);
+          s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, src.bf16(y[2], y[3], scale)),
+                                                         __builtin_bit_cast(bf16x8, q[1]), s[u], 0, 0, 0);
+        }
+        if (keys < kTile || have != 15) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int key = 32 * (u >> 1) + 8 * grp + 4 * (u & 1) + j;
+              if (key >= keys || !(have >> (key >> 4) & 1)) s[u][j] = -INFINITY;
+            }
+        }
+        // The probabilities are taken against a reference that is the true running maximum only when it was
+        // last moved: it moves when a lane's weights against it pass 2^16 in sum (or are NaN).  They are
+        // rounded to bf16, the products' operands, off by at most 2^-8 each; the sum is of the same values.
+        bf16x8 pb[2];
+        float rs;
+        auto weigh = [&](float ref) __attribute__((always_inline)) {
+          rs = 0.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              pb[h][j] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * h + (j >> 2)][j & 3], cl, -ref));
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+              rs = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{pb[h][j], pb[h][j + 1]}, bf16x2{(__bf16)1.f, (__bf16)1.f}, rs, false);
+          }
+        };
+        weigh(mc);  // (no key yet: mc is -inf, and the sum +inf or NaN)
+        if (__builtin_amdgcn_ballot_w64(!(rs <= 65536.f)) != 0) {
+          float mx = s[0][0];
+#pragma unroll
+          for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j >> 2][j & 3]);
+          mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+          const float m_new = fmaxf(mc, mx * cl);
+          const float ref = m_new == -INFINITY ? 0.f : m_new;  // no key above -inf yet: weights 0
+          const float alpha = __builtin_amdgcn_exp2f(mc - ref);
+          mc = m_new;
+          sum *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
+          weigh(ref);
+        }
+        sum += rs;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // V^T: slot j of lane (grp, l16) is V[key 32 h + 8 grp + j][16 dt + l16]
+          const uint8_t *const vp = vt + h * 2 * kRows16 + (8 * grp + (l16 >> 1)) * kPitch + (grp >> 1) * 64 + 8 * (l16 & 1);
+          const float scale = __uint_as_float((vs >> (16 * h + 8 * (grp >> 1)) & 255u) << 23);
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) {
+            const u32x2 y = lds_tr8(vp + 16 * dt);
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, src.bf16(y[0], y[1], scale)), pb[h],
+                                                            o[dt], 0, 0, 0);
+          }
+        }
+        if (ends) {
+          sum += __shfl_xor(sum, 16, 64);
+          sum += __shfl_xor(sum, 32, 64);
+          const int begin = max(__builtin_amdgcn_readlane(lfirst, place), at) - at;
+          const int parts0 = __builtin_amdgcn_readlane(lbefore, place);
+          if (l16 < rows) {
+            float *const h = lds.hold + ((parts0 + ((wave - begin) & (kWaves - 1))) * rows + l16) * kHoldRow;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *(f32x4 *)(h + 16 * j + 4 * grp) = o[j];
+            if (grp == 0) *(float2 *)(h + HD) = make_float2(mc, sum);
+          }
+        }
+      }
+      __syncthreads();
+
+      // ---- the listed sequences' parts, added up
+#pragma unroll 1
+      for (int u = wave; u < n_list * quads; u += kWaves) {
+        const int place = place_of_unit(u), h = 4 * (u - place * quads) + (lane >> 4), d = 4 * (lane & 15);
+        const int b = __builtin_amdgcn_readlane(lb, place), parts = __builtin_amdgcn_readlane(lparts, place);
+        const int first = __builtin_amdgcn_readlane(lfirst, place), last = __builtin_amdgcn_readlane(lend, place);
+        const int parts0 = __builtin_amdgcn_readlane(lbefore, place);
+        if (h >= rows) continue;
+        const float *const r = lds.hold + (parts0 * rows + h) * kHoldRow;
+        float2 ml[kWaves];
+        f32x4 y[kWaves];
+        float M = -INFINITY, L = 0.f;
+        f32x4 A{};
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) {
+          const float *const e = r + min(v, parts - 1) * rows * kHoldRow;
+          ml[v] = *(const float2 *)(e + HD);
+          y[v] = *(const f32x4 *)(e + d);
+        }
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) M = fmaxf(M, ml[v].x);
+        const float Mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) {
+          const float f = __builtin_amdgcn_exp2f(ml[v].x - Mu);
+          L = v < parts ? fmaf(ml[v].y, f, L) : L;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) A[j] = v < parts ? fmaf(y[v][j], f, A[j]) : A[j];
+        }
+        if (first >= pos0 && last <= end) {
+          write4(b, h, d, A, L);
+        } else {  // (cut: the only piece of it in this share)
+          float *const to_rec = record(bin, first >= pos0 ? bin : -1, h);
+          put2(to_rec + d, A[0], A[1]);
+          put2(to_rec + d + 2, A[2], A[3]);
+          if (d == 0) put2(to_rec + HD, M, L);
+        }
+      }
+      auto cut_of = [&](int place, Cut &u) __attribute__((always_inline)) {
+        const int first = __builtin_amdgcn_readlane(lfirst, place), last = __builtin_amdgcn_readlane(lend, place);
+        u.b = __builtin_amdgcn_readlane(lb, place);
+        u.bin0 = (int)((uint32_t)first / (uint32_t)share);
+        u.pieces = (int)((uint32_t)(last - 1) / (uint32_t)share) - u.bin0 + 1;
+      };
+      if (__builtin_amdgcn_readlane(lfirst, 0) < pos0 && at == pos0) cut_of(0, cuts[0]);
+      if (__builtin_amdgcn_readlane(lend, n_list - 1) > end && __builtin_amdgcn_readlane(lfirst, n_list - 1) >= pos0)
+        cut_of(n_list - 1, cuts[1]);
+      if (stop >= end) break;
+      __syncthreads();  // the list and the places are free again
+      at = stop;
+      listed += n_list;
+    }
+
+    // ---- cut sequences: the last of their pieces to arrive adds their records, in the order of the keys
+    if (cuts[0].pieces | cuts[1].pieces) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the records' stores have reached memory
+      __syncthreads();
+      if (tid < 2) {
+        const Cut u = tid ? cuts[1] : cuts[0];
+        lds.last_in[tid] =
+            u.pieces && arrive_last(p.arrive_end - 2 * ((int64_t)u.b * p.columns + col + 1), u.pieces, p.tag);
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int side = 0; side < 2; ++side) {
+        if (!lds.last_in[side]) continue;
+        const Cut u = side ? cuts[1] : cuts[0];
+        // Two rows a wave, two elements a lane; every groups-th record a group of waves, then the
+        // groups' sums.  Only records that are there are asked for: past the caches a compute unit
+        // gets some 64 bytes a few ns (16 a lane always, 8 us behind the last arrival).
+        const int pairs = (rows + 1) >> 1, groups = pairs <= 4 ? pairs == 3 ? 2 : kWaves / pairs : 1;
+        const int part = pairs == 1 ? wave : pairs == 2 ? wave >> 1 : pairs == 3 ? wave * 0x5556 >> 16 : pairs == 4 ? wave >> 2 : 0;
+        const int h = 2 * (wave - part * pairs) + (lane >> 5), d = 2 * (lane & 31);
+        if (part < groups && h < rows) {
+          float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
+#pragma unroll 1
+          for (int n0 = part; n0 < u.pieces; n0 += kMerged * groups) {
+            float2 ml[kMerged], y[kMerged];
+#pragma unroll
+            for (int v = 0; v < kMerged; ++v) {
+              ml[v] = make_float2(-INFINITY, 0.f);
+              y[v] = make_float2(0.f, 0.f);
+              if (n0 + v * groups < u.pieces) {
+                const float *const r = record(u.bin0 + n0 + v * groups, u.bin0, h);
+                ml[v] = get2(r + HD);
+                y[v] = get2(r + d);
+              }
+            }
+            float mx = M;
+#pragma unroll
+            for (int v = 0; v < kMerged; ++v) mx = fmaxf(mx, ml[v].x);
+            const float mu = mx == -INFINITY ? 0.f : mx, fo = __builtin_amdgcn_exp2f(M - mu);
+            L *= fo;
+            A0 *= fo;
+            A1 *= fo;
+#pragma unroll
+            for (int v = 0; v < kMerged; ++v) {
+              const float f = __builtin_amdgcn_exp2f(ml[v].x - mu);
+              L = fmaf(ml[v].y, f, L);
+              A0 = fmaf(y[v].x, f, A0);
+              A1 = fmaf(y[v].y, f, A1);
+            }
+            M = mx;
+          }
+          float *const r = lds.hold + (part * rows + h) * kHoldRow;
+          *(float2 *)(r + d) = make_float2(A0, A1);
+          if (d == 0) *(float2 *)(r + HD) = make_float2(M, L);
+        }
+        __syncthreads();
+        if (part == 0 && h < rows) {
+          float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
+#pragma unroll 1
+          for (int v = 0; v < groups; ++v) {
+            const float *const r = lds.hold + (v * rows + h) * kHoldRow;
+            const float2 ml = *(const float2 *)(r + HD), y = *(const float2 *)(r + d);
+            const float mn = fmaxf(M, ml.x), mu = mn == -INFINITY ? 0.f : mn;
+            const float fo = __builtin_amdgcn_exp2f(M - mu), fn = __builtin_amdgcn_exp2f(ml.x - mu);
+            L = fmaf(ml.y, fn, L * fo);
+            A0 = fmaf(y.x, fn, A0 * fo);
+            A1 = fmaf(y.y, fn, A1 * fo);
+            M = mn;
+          }
+          const float inv = L > 0.f ? 1.0f / L : 0.f;
+          *(uint32_t *)((bf16_t *)p.a.o + u.b * p.a.o_rs + (head0 + h) * HD + d) =
+              (uint32_t)f32_to_bf16(A0 * inv) | ((uint32_t)f32_to_bf16(A1 * inv) << 16);
+        }
+        __syncthreads();
+      }
+    }
+  }
+  // sequences without a key
+  for (int b = bin; b < c.batch; b += p.bins)
+    if (c.lens[b] <= 0 || c.cap == 0)
+      for (int k = tid; k < rows * (HD / 4); k += 64 * kWaves) write4(b, k / (HD / 4), 4 * (k % (HD / 4)), f32x4{}, 0.f);
 }
 template <int HW, int KW, int OCC>
 __global__ __launch_bounds__(64 * HW * KW, OCC) void paged_q8_prefill_kernel(PrefillParams p, E4m3Pages src) {
@@ -342,7 +803,8 @@ int launch_decode(const AttnParams &a, const E4m3Pages &src, void *ws, hipStream
   p.k0 = 0;
   p.parts = nullptr;
   p.cuts = nullptr;
-  hipLaunchKernelGGL(paged_q8_decode_kernel, dim3((unsigned)(d.bins * d.columns)), dim3(256), 0, s, p, src);
+  hipLaunchKernelGGL(paged_q8_decode_kernel, dim3((unsigned)(d.bins * d.columns)),
+                     dim3(64 * kWaves), 0, s, p, src);
   BN_LAUNCH_CHECK();
   return BN_OK;
 }

@@ -272,14 +272,14 @@ def test_outputs_are_memory_of_the_stream_that_writes_them(monkeypatch):
     monkeypatch.setattr(B, "made_on", lambda stream, make: made.append(stream) or make())
     monkeypatch.setattr(B, "call", lambda *a: None)
     monkeypatch.setattr(B, "_cache_stream", lambda cache, stream: 0)
-    monkeypatch.setattr(B, "_qk_args", lambda *a: 0)
+    monkeypatch.setattr(B, "_qk_args", lambda *a: (B.BN_BF16, 0, None))
     kv, st, q = q8(), object(), torch.zeros((3, 8, 64), dtype=torch.bfloat16)
     starts = torch.zeros(4, dtype=torch.int32)
     for call, n in ((lambda: B.paged_q8_decode(q, kv, stream=st), 1),
                     (lambda: B.paged_q8_prefill(q, kv, starts, stream=st), 1),
                     (lambda: B.paged_q8_read(kv, starts, n_rows=3, stream=st), 2),
                     (lambda: B.qk_norm_rope(q, q, q[0, 0], q[0, 0], stream=st), 2),
-                    (lambda: B.qk_norm_rope_backward(q, q, q[0, 0], q[0, 0], q, q, stream=st), 4)):
+                    (lambda: B.qk_norm_rope_backward(q, q, q[0, 0], q[0, 0], q, q, stream=st), 3)):
         made.clear()
         call()
         assert made == [st] * n
