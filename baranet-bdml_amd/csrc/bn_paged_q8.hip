@@ -339,9 +339,10 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
   const int rows = min(kMaxRows, p.a.group - kMaxRows * hb), head0 = g * p.a.group + kMaxRows * hb;
 
   // ---- the share
-  auto keys_of = [&](int b) { return max(min(c.lens[b], c.cap), 0); };
   auto tiles_of = [](int len) { return (int)((uint32_t)(len + kTile - 1) / kTile); };
   const int per = (c.batch + 64 * kWaves - 1) / (64 * kWaves), from = min(tid * per, c.batch), to = min(from + per, c.batch);
+  const int len0 = from < to ? c.lens[from] : 0;  // (the only one up to 512 sequences)
+  auto keys_of = [&](int b) __attribute__((always_inline)) { return max(min(b == from ? len0 : c.lens[b], c.cap), 0); };
   int own = 0, some = 0;  // tiles of the thread's run of sequences; sequences of it that have any
 #pragma unroll 8
   for (int b = from; b < to; ++b) {
@@ -370,21 +371,20 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
       __builtin_amdgcn_readfirstlane(max((int)((uint32_t)(total + p.bins - 1) / (uint32_t)p.bins), kShareLeast));
   const int pos0 = (int)min((int64_t)bin * share, (int64_t)total), end = min(pos0 + share, total);
 
-  // what a piece of work leaves: two or four elements of a head's row
-  auto write4 = [&](int b, int h, int d, const f32x4 &x, float sum) __attribute__((always_inline)) {
+  auto write2 = [&](int b, int h, int d, float x, float y, float sum) __attribute__((always_inline)) {
     const float inv = sum > 0.f ? 1.0f / sum : 0.f;
-    bf16_t *const op = (bf16_t *)p.a.o + b * p.a.o_rs + (head0 + h) * HD + d;
-    const uint32_t lo = (uint32_t)f32_to_bf16(x[0] * inv) | ((uint32_t)f32_to_bf16(x[1] * inv) << 16);
-    const uint32_t hi = (uint32_t)f32_to_bf16(x[2] * inv) | ((uint32_t)f32_to_bf16(x[3] * inv) << 16);
-    *(uint2 *)op = make_uint2(lo, hi);
+    *(uint32_t *)((bf16_t *)p.a.o + b * p.a.o_rs + (head0 + h) * HD + d) =
+        (uint32_t)f32_to_bf16(x * inv) | ((uint32_t)f32_to_bf16(y * inv) << 16);
   };
   // row h of the record of a sequence's piece in bin `at` (a bin has two: the end
   // of a sequence begun before it, and the start of one, begun in bin0, that goes on)
   auto record = [&](int at, int bin0, int h) __attribute__((always_inline)) {
     return p.ws + ((((int64_t)at * 2 + (at == bin0)) * p.columns + col) * kMaxRows + h) * kRec;
   };
-  const int quads = (rows + 3) >> 2;  // a wave adds up four rows at a time, four elements a lane
-  auto place_of_unit = [&](int u) { return quads == 1 ? u : quads == 2 ? u >> 1 : quads == 4 ? u >> 2 : u * 0x5556 >> 16; };
+  const int pairs = (rows + 1) >> 1;  // results are formed two rows a wave
+  auto by_pairs = [&](int u) __attribute__((always_inline)) {  // u / pairs (u up to 32 * 8, pairs up to 8)
+    return (int)(((uint32_t)u * (uint32_t)(65536 / pairs + 1)) >> 16);
+  };
   struct Cut {  // a sequence that is cut between shares: its first bin and its number of pieces, one a bin
     int b, bin0, pieces;
   };
@@ -474,14 +474,11 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
       struct Tile {  // in flight: its rows' pieces, 16 rows an instruction
         u32x4 k[4], v[4];
         int info, keys;
-        uint32_t ks, vs;
       } x;
       auto load = [&](int i) __attribute__((always_inline)) {
         const int j = i & 63;
         x.info = __builtin_amdgcn_readlane(info, j);
         x.keys = __builtin_amdgcn_readlane(first_keys, j);
-        x.ks = __builtin_amdgcn_readlane(kscales, j);
-        x.vs = __builtin_amdgcn_readlane(vscales, j);
         uint32_t o32 = off;
         asm volatile("" : "+v"(o32));  // a scalar base and this offset, not a sum of pointers kept in registers
 #pragma unroll
@@ -510,7 +507,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
 #pragma unroll 1
       for (int i = 0; i < n; ++i) {
         const int place = x.info & 255, have = x.info >> 8 & 15, keys = x.keys;
-        const uint32_t ks = x.ks, vs = x.vs;
+        const uint32_t ks = __builtin_amdgcn_readlane(kscales, i & 63), vs = __builtin_amdgcn_readlane(vscales, i & 63);
         // a wave's LDS instructions execute in order, so its tile needs no
         // barrier; wave_barrier keeps the compiler from moving them across
         __builtin_amdgcn_wave_barrier();
@@ -625,24 +622,22 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
       }
       __syncthreads();
 
-      // ---- the listed sequences' parts, added up
+      // ---- the listed sequences' parts, added up: two rows a wave, two elements a lane
 #pragma unroll 1
-      for (int u = wave; u < n_list * quads; u += kWaves) {
-        const int place = place_of_unit(u), h = 4 * (u - place * quads) + (lane >> 4), d = 4 * (lane & 15);
+      for (int u = wave; u < n_list * pairs; u += kWaves) {
+        const int place = by_pairs(u), h = 2 * (u - place * pairs) + (lane >> 5), d = 2 * (lane & 31);
         const int b = __builtin_amdgcn_readlane(lb, place), parts = __builtin_amdgcn_readlane(lparts, place);
         const int first = __builtin_amdgcn_readlane(lfirst, place), last = __builtin_amdgcn_readlane(lend, place);
         const int parts0 = __builtin_amdgcn_readlane(lbefore, place);
         if (h >= rows) continue;
         const float *const r = lds.hold + (parts0 * rows + h) * kHoldRow;
-        float2 ml[kWaves];
-        f32x4 y[kWaves];
-        float M = -INFINITY, L = 0.f;
-        f32x4 A{};
+        float2 ml[kWaves], y[kWaves];
+        float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
 #pragma unroll
         for (int v = 0; v < kWaves; ++v) {
           const float *const e = r + min(v, parts - 1) * rows * kHoldRow;
           ml[v] = *(const float2 *)(e + HD);
-          y[v] = *(const f32x4 *)(e + d);
+          y[v] = *(const float2 *)(e + d);
         }
 #pragma unroll
         for (int v = 0; v < kWaves; ++v) M = fmaxf(M, ml[v].x);
@@ -651,15 +646,14 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
         for (int v = 0; v < kWaves; ++v) {
           const float f = __builtin_amdgcn_exp2f(ml[v].x - Mu);
           L = v < parts ? fmaf(ml[v].y, f, L) : L;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) A[j] = v < parts ? fmaf(y[v][j], f, A[j]) : A[j];
+          A0 = v < parts ? fmaf(y[v].x, f, A0) : A0;
+          A1 = v < parts ? fmaf(y[v].y, f, A1) : A1;
         }
         if (first >= pos0 && last <= end) {
-          write4(b, h, d, A, L);
+          write2(b, h, d, A0, A1, L);
         } else {  // (cut: the only piece of it in this share)
           float *const to_rec = record(bin, first >= pos0 ? bin : -1, h);
-          put2(to_rec + d, A[0], A[1]);
-          put2(to_rec + d + 2, A[2], A[3]);
+          put2(to_rec + d, A0, A1);
           if (d == 0) put2(to_rec + HD, M, L);
         }
       }
@@ -695,8 +689,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
         // Two rows a wave, two elements a lane; every groups-th record a group of waves, then the
         // groups' sums.  Only records that are there are asked for: past the caches a compute unit
         // gets some 64 bytes a few ns (16 a lane always, 8 us behind the last arrival).
-        const int pairs = (rows + 1) >> 1, groups = pairs <= 4 ? pairs == 3 ? 2 : kWaves / pairs : 1;
-        const int part = pairs == 1 ? wave : pairs == 2 ? wave >> 1 : pairs == 3 ? wave * 0x5556 >> 16 : pairs == 4 ? wave >> 2 : 0;
+        const int part = by_pairs(wave), groups = by_pairs(kWaves);
         const int h = 2 * (wave - part * pairs) + (lane >> 5), d = 2 * (lane & 31);
         if (part < groups && h < rows) {
           float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
@@ -747,9 +740,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
             A1 = fmaf(y.y, fn, A1 * fo);
             M = mn;
           }
-          const float inv = L > 0.f ? 1.0f / L : 0.f;
-          *(uint32_t *)((bf16_t *)p.a.o + u.b * p.a.o_rs + (head0 + h) * HD + d) =
-              (uint32_t)f32_to_bf16(A0 * inv) | ((uint32_t)f32_to_bf16(A1 * inv) << 16);
+          write2(u.b, h, d, A0, A1, L);
         }
         __syncthreads();
       }
@@ -758,7 +749,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
   // sequences without a key
   for (int b = bin; b < c.batch; b += p.bins)
     if (c.lens[b] <= 0 || c.cap == 0)
-      for (int k = tid; k < rows * (HD / 4); k += 64 * kWaves) write4(b, k / (HD / 4), 4 * (k % (HD / 4)), f32x4{}, 0.f);
+      for (int k = tid; k < rows * (HD / 2); k += 64 * kWaves) write2(b, k / (HD / 2), 2 * (k % (HD / 2)), 0.f, 0.f, 0.f);
 }
 template <int HW, int KW, int OCC>
 __global__ __launch_bounds__(64 * HW * KW, OCC) void paged_q8_prefill_kernel(PrefillParams p, E4m3Pages src) {
