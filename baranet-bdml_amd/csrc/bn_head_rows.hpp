@@ -77,5 +77,35 @@ __device__ __forceinline__ void turn8(Eight &v, const float2 *cs, bool back = fa
   }
 }
 
+// Thread tid's way through rows of `per` pieces each, every `by`-th piece, without a division a piece.
+struct Walk {
+  int row, rest, per, rows_by, rest_by;
+  __device__ __forceinline__ Walk(int tid, int by, int per_) : per(per_) {
+    row = (int)((uint32_t)tid / (uint32_t)per);
+    rest = tid - row * per;
+    rows_by = __builtin_amdgcn_readfirstlane((int)((uint32_t)by / (uint32_t)per));
+    rest_by = by - rows_by * per;
+  }
+  __device__ __forceinline__ void step() {
+    row += rows_by;
+    rest += rest_by;
+    if (rest >= per) {
+      rest -= per;
+      ++row;
+    }
+  }
+};
+
+// f[i] = theta^(-2i/head_dim) / (2 pi): turns per position of each pair (theta 0: none).
+inline void fill_turns(double *f, int head_dim, float theta) {
+  const int n = head_dim / 2;
+  double low[8];  // (a power of eight pairs and one within: a few roundings instead of a pow a pair)
+  for (int i = 0; i < 8 && i < n; ++i) low[i] = theta > 0.f ? std::pow((double)theta, -2.0 * i / head_dim) : 0.0;
+  for (int i = 0; i < n; i += 8) {
+    const double high = theta > 0.f ? std::pow((double)theta, -2.0 * i / head_dim) / (2.0 * M_PI) : 0.0;
+    for (int j = 0; j < 8; ++j) f[i + j] = high * low[j];
+  }
+}
+
 }  // namespace
 }  // namespace bn

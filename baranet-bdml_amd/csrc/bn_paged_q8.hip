@@ -146,23 +146,49 @@ struct Q8AppendParams {
   double f[HD / 2];  // turns per position of each pair
 };
 
-// A unit a workgroup.  The angles of its rows once; then its waves take the
-// block's KV heads, K and V, in turn, 16 rows of 64 elements in two pieces of eight
-// a lane: norm, rotation, the block's largest element, the scale, the codes.  The
-// queries' pieces go to all threads.
+// A unit a workgroup.  Its rows' angles once, while the first pieces of queries and
+// the first task's rows are on their way; then its waves take the block's KV heads, K
+// and V, in turn, 16 rows of 64 elements in two pieces of eight a lane: norm,
+// rotation, the block's largest element, the scale, the codes.  The queries' pieces go
+// to all threads.
+constexpr int kAppendThreads = 512, kPieces = 4;
 template <typename T>
-__global__ __launch_bounds__(256) void paged_q8_append_kernel(Q8AppendParams p) {
+__global__ __launch_bounds__(kAppendThreads) void paged_q8_append_kernel(Q8AppendParams p) {
   __shared__ float2 cs[kBlock][HD / 2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Paged &c = p.s.c;
   Unit u;
   if (!find_unit(c, p.starts, p.n_rows, blockIdx.x, u)) return;
+  const int e = lane % 8 * 8, per = p.n_heads * 8, total = u.rows * per, tasks = 2 * c.n_kv_heads;
+  Walk at_q(tid, kAppendThreads, max(per, 1));
+  Raw8<T> qx[kPieces];
+  int q_row[kPieces], q_at[kPieces];
+  auto load_q = [&](int first) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      if (first + kAppendThreads * n >= total) break;
+      q_row[n] = at_q.row;
+      q_at[n] = at_q.rest * 8;
+      at_q.step();
+      qx[n].load((const T *)p.q + (int64_t)(u.row0 + q_row[n]) * p.q_rs + q_at[n]);
+    }
+  };
+  Raw8<T> kx[2];
+  auto load_kv = [&](int task) __attribute__((always_inline)) {
+    const bool is_v = task >= c.n_kv_heads;
+    const T *const x = (is_v ? (const T *)p.v : (const T *)p.k) + (task - (is_v ? c.n_kv_heads : 0)) * HD + e;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+      if (lane / 8 + 8 * n < u.rows) kx[n].load(x + (int64_t)(u.row0 + lane / 8 + 8 * n) * (is_v ? p.v_rs : p.k_rs));
+  };
+  if (wave < tasks) load_kv(wave);
+  load_q(tid);
+  const Place at = place_of(p.s, u);
   if (p.turn) {
-    for (int i = tid; i < u.rows * (HD / 2); i += 256)
+    for (int i = tid; i < u.rows * (HD / 2); i += kAppendThreads)
       cs[i / (HD / 2)][i % (HD / 2)] = cos_sin((double)(u.pos0 + i / (HD / 2)) * p.f[i % (HD / 2)]);
     __syncthreads();
   }
-  const int e = lane % 8 * 8;
   auto normed = [&](Eight &x, const void *w) __attribute__((always_inline)) {
     const float r = head_rms<8>(x, p.eps);
     Raw8<T> wr;
@@ -171,21 +197,21 @@ __global__ __launch_bounds__(256) void paged_q8_append_kernel(Q8AppendParams p) 
 #pragma unroll
     for (int j = 0; j < 8; ++j) x.x[j] *= r * y.x[j];
   };
-  const Place at = place_of(p.s, u);
   if (at.codes >= 0) {
-    for (int task = wave; task < 2 * c.n_kv_heads; task += 4) {
+    for (int task = wave; task < tasks; task += kAppendThreads / 64) {
+      if (task != wave) load_kv(task);
       const bool is_v = task >= c.n_kv_heads;
       const int g = is_v ? task - c.n_kv_heads : task;
+      uint8_t *const codes = (uint8_t *)(is_v ? c.v : c.k) + at.codes + g * c.head_stride;
+      uint8_t *const scale = (is_v ? p.s.vs : p.s.ks) + at.scale + g * p.s.scale_head;
+      const int before = at.slot > 0 ? min(max((int)*scale, kLow), kHigh) : 0;  // of older rows in the block
       Eight x[2];
       float amax = 0.f;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const int row = lane / 8 + 8 * n;
         if (row < u.rows) {
-          Raw8<T> raw;
-          raw.load((is_v ? (const T *)p.v + (int64_t)(u.row0 + row) * p.v_rs
-                         : (const T *)p.k + (int64_t)(u.row0 + row) * p.k_rs) + g * HD + e);
-          x[n] = raw.floats();
+          x[n] = kx[n].floats();
           if (!is_v) {
             if (p.wk) normed(x[n], p.wk);
             if (p.turn) turn8(x[n], &cs[row][e / 2]);
@@ -194,23 +220,17 @@ __global__ __launch_bounds__(256) void paged_q8_append_kernel(Q8AppendParams p) 
           for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_size(x[n].x[j]));
         }
       }
-      amax = wave_max(amax);
-      uint8_t *const codes = (uint8_t *)(is_v ? c.v : c.k) + at.codes + g * c.head_stride;
-      uint8_t *const scale = (is_v ? p.s.vs : p.s.ks) + at.scale + g * p.s.scale_head;
-      int byte = byte_of(amax);
-      if (at.slot > 0) {  // older rows in the block
-        const int before = min(max((int)*scale, kLow), kHigh);
-        if (byte > before) {
+      int byte = byte_of(wave_max(amax));
+      if (at.slot > 0 && byte > before) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const int back = lane / 8 + 8 * n - at.slot;  // rows before the first: negative
-            if (back >= 0) continue;
-            u32x2 *const row = (u32x2 *)(codes + back * c.row_stride + e);
-            *row = codes_of(values(*row, scale_of(before)), byte);
-          }
+        for (int n = 0; n < 2; ++n) {
+          const int back = lane / 8 + 8 * n - at.slot;  // rows before the first: negative
+          if (back >= 0) continue;
+          u32x2 *const row = (u32x2 *)(codes + back * c.row_stride + e);
+          *row = codes_of(values(*row, scale_of(before)), byte);
         }
-        byte = max(byte, before);
       }
+      byte = max(byte, before);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const int row = lane / 8 + 8 * n;
@@ -219,15 +239,16 @@ __global__ __launch_bounds__(256) void paged_q8_append_kernel(Q8AppendParams p) 
       if (lane == 0) *scale = (uint8_t)byte;
     }
   }
-  const int per = p.n_heads * 8, total = u.rows * per;
-  for (int i = tid; i < total; i += 256) {
-    const int row = (int)((uint32_t)i / (uint32_t)per), h = (i - row * per) / 8;
-    Raw8<T> raw;
-    raw.load((const T *)p.q + (int64_t)(u.row0 + row) * p.q_rs + h * HD + e);
-    Eight x = raw.floats();
-    if (p.wq) normed(x, p.wq);
-    if (p.turn) turn8(x, &cs[row][e / 2]);
-    store8((T *)p.qo + (int64_t)(u.row0 + row) * p.qo_rs + h * HD + e, x);
+  for (int first = tid; first < total; first += kAppendThreads * kPieces) {
+    if (first != tid) load_q(first);
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+      if (first + kAppendThreads * n >= total) break;
+      Eight x = qx[n].floats();
+      if (p.wq) normed(x, p.wq);
+      if (p.turn) turn8(x, &cs[q_row[n]][e / 2]);
+      store8((T *)p.qo + (int64_t)(u.row0 + q_row[n]) * p.qo_rs + q_at[n], x);
+    }
   }
 }
 
@@ -910,10 +931,9 @@ int bn_paged_q8_append(const bn_paged_q8 *cache, int dtype, const void *k, const
   p.n_heads = q ? n_heads : 0;
   p.turn = theta > 0.f;
   p.eps = eps;
-  for (int i = 0; i < HD / 2; ++i)
-    p.f[i] = theta > 0.f ? std::pow((double)theta, -2.0 * i / HD) / (2.0 * M_PI) : 0.0;
+  fill_turns(p.f, HD, theta);
   hipStream_t s = as_stream(stream);
-  const dim3 grid((unsigned)count_units(row_starts, n_rows, cache->batch)), block(256);
+  const dim3 grid((unsigned)count_units(row_starts, n_rows, cache->batch)), block(kAppendThreads);
   if (dtype == BN_BF16) hipLaunchKernelGGL(paged_q8_append_kernel<bf16_t>, grid, block, 0, s, p);
   else hipLaunchKernelGGL(paged_q8_append_kernel<float>, grid, block, 0, s, p);
   BN_LAUNCH_CHECK();

@@ -50,24 +50,23 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkParams p) {
   constexpr int LANES = D / 8;
   __shared__ float2 cs[kMostRows][D / 2];
   const int tid = threadIdx.x, row0 = blockIdx.x * p.rows, rows = min(p.rows, p.n_rows - row0);
-  const int heads = p.n_heads + p.n_kv_heads, per = heads * LANES, total = rows * per;
-  struct At {
+  const int per = (p.n_heads + p.n_kv_heads) * LANES, total = rows * per;
+  Walk at(tid, 256, per);
+  struct Piece8 {
     int row, head, e;  // row of the workgroup, head (keys' behind the queries'), element
-  };
-  auto place = [&](int i) __attribute__((always_inline)) {
-    const int row = (int)((uint32_t)i / (uint32_t)per), rest = i - row * per;
-    return At{row, rest / LANES, rest % LANES * 8};
-  };
-  Raw8<T> raw[kPieces];
+    Raw8<T> raw;
+  } x[kPieces];
   auto load = [&](int first) __attribute__((always_inline)) {
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) {
-      const int i = first + 256 * n;
-      if (i >= total) break;
-      const At a = place(i);
-      raw[n].load(a.head < p.n_heads
-                      ? (const T *)p.q + (int64_t)(row0 + a.row) * p.q_rs + a.head * D + a.e
-                      : (const T *)p.k + (int64_t)(row0 + a.row) * p.k_rs + (a.head - p.n_heads) * D + a.e);
+      if (first + 256 * n >= total) break;
+      x[n].row = at.row;
+      x[n].head = at.rest / LANES;
+      x[n].e = at.rest % LANES * 8;
+      at.step();
+      const int64_t row = row0 + x[n].row;
+      x[n].raw.load(x[n].head < p.n_heads ? (const T *)p.q + row * p.q_rs + x[n].head * D + x[n].e
+                                          : (const T *)p.k + row * p.k_rs + (x[n].head - p.n_heads) * D + x[n].e);
     }
   };
   load(tid);
@@ -77,25 +76,25 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkParams p) {
     if (first != tid) load(first);
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) {
-      const int i = first + 256 * n;
-      if (i >= total) break;
-      const At a = place(i);
-      const bool is_q = a.head < p.n_heads;
-      Eight v = raw[n].floats();
+      if (first + 256 * n >= total) break;
+      const bool is_q = x[n].head < p.n_heads;
+      Eight v = x[n].raw.floats();
       const float r = head_rms<LANES>(v, p.eps);
       Raw8<T> wr;
-      wr.load((const T *)(is_q ? p.wq : p.wk) + a.e);
+      wr.load((const T *)(is_q ? p.wq : p.wk) + x[n].e);
       const Eight w = wr.floats();
 #pragma unroll
       for (int j = 0; j < 8; ++j) v.x[j] *= r * w.x[j];
-      if (p.turn) turn8(v, &cs[a.row][a.e / 2]);
-      store8(is_q ? (T *)p.qo + (int64_t)(row0 + a.row) * p.qo_rs + a.head * D + a.e
-                  : (T *)p.ko + (int64_t)(row0 + a.row) * p.ko_rs + (a.head - p.n_heads) * D + a.e,
+      if (p.turn) turn8(v, &cs[x[n].row][x[n].e / 2]);
+      const int64_t row = row0 + x[n].row;
+      store8(is_q ? (T *)p.qo + row * p.qo_rs + x[n].head * D + x[n].e
+                  : (T *)p.ko + row * p.ko_rs + (x[n].head - p.n_heads) * D + x[n].e,
              v);
     }
   }
 }
 
+constexpr int kPairs = 2;  // pieces of rows and gradients of a thread on their way at once
 // A workgroup takes every gridDim.x-th group of `rows` rows.  A thread's pieces lie at
 // one place of their heads, so it adds up eight elements of each weight's
 // gradient in registers; a workgroup's sums go to the workspace.
@@ -121,29 +120,41 @@ __global__ __launch_bounds__(256) void qk_norm_rope_backward_kernel(QkParams p) 
       Raw8<T> wr;
       wr.load((const T *)(side ? p.wk : p.wq) + e);
       const Eight w = wr.floats();
-      for (int i = tid; i < total; i += 256) {
-        const int row = (int)((uint32_t)i / (uint32_t)per), h = (i - row * per) / LANES;
-        Raw8<T> xr, gr;
-        xr.load(x + (row0 + row) * x_rs + h * D + e);
-        gr.load(dy + (row0 + row) * dy_rs + h * D + e);
-        const Eight v = xr.floats();
-        Eight g = gr.floats();
-        if (p.turn) turn8(g, &cs[row][e / 2], true);
-        const float r = head_rms<LANES>(v, p.eps);
-        float dot = 0.f;
-        Eight y;
+      Walk at(tid, 256, per);
+      for (int first = tid; first < total; first += 256 * kPairs) {
+        Raw8<T> xr[kPairs], gr[kPairs];
+        int row[kPairs], to[kPairs];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float u = v.x[j] * r;  // the normed element
-          dw[side].x[j] = fmaf(g.x[j], u, dw[side].x[j]);
-          g.x[j] *= w.x[j];
-          dot = fmaf(g.x[j], u, dot);
-          y.x[j] = u;
+        for (int n = 0; n < kPairs; ++n) {
+          if (first + 256 * n >= total) break;
+          row[n] = at.row;
+          to[n] = at.rest / LANES * D + e;
+          at.step();
+          xr[n].load(x + (row0 + row[n]) * x_rs + to[n]);
+          gr[n].load(dy + (row0 + row[n]) * dy_rs + to[n]);
         }
-        dot = head_sum<LANES>(dot) * (1.0f / D);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y.x[j] = r * (g.x[j] - y.x[j] * dot);
-        store8(dx + (row0 + row) * dx_rs + h * D + e, y);
+        for (int n = 0; n < kPairs; ++n) {
+          if (first + 256 * n >= total) break;
+          const Eight v = xr[n].floats();
+          Eight g = gr[n].floats();
+          if (p.turn) turn8(g, &cs[row[n]][e / 2], true);
+          const float r = head_rms<LANES>(v, p.eps);
+          float dot = 0.f;
+          Eight y;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float u = v.x[j] * r;  // the normed element
+            dw[side].x[j] = fmaf(g.x[j], u, dw[side].x[j]);
+            g.x[j] *= w.x[j];
+            dot = fmaf(g.x[j], u, dot);
+            y.x[j] = u;
+          }
+          dot = head_sum<LANES>(dot) * (1.0f / D);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y.x[j] = r * (g.x[j] - y.x[j] * dot);
+          store8(dx + (row0 + row[n]) * dx_rs + to[n], y);
+        }
       }
     }
   }
@@ -162,23 +173,35 @@ __global__ __launch_bounds__(256) void qk_norm_rope_backward_kernel(QkParams p) 
         (sums[0][i / D][i % D] + sums[1][i / D][i % D]) + (sums[2][i / D][i % D] + sums[3][i / D][i % D]);
 }
 
-// The workgroups' sums, added: 32 lanes an element.
+// The workgroups' sums, added: eight elements a workgroup, 32 threads an element.
 __global__ __launch_bounds__(256) void qk_norm_rope_weights_kernel(const float *parts, int n, int d, float *dwq,
                                                                    float *dwk) {
-  const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  constexpr int N = 16;  // on their way at once
+  __shared__ float sums[4][8];
+  const int tid = threadIdx.x, e = blockIdx.x * 8 + (tid & 7);
   float s = 0.f;
-  for (int i = lane; i < n; i += 32) s += parts[(int64_t)i * 2 * d + e];
+  for (int i0 = tid >> 3; i0 < n; i0 += 32 * N) {
+    float x[N];
 #pragma unroll
-  for (int m = 16; m; m >>= 1) s += __shfl_xor(s, m, 64);
-  if (lane == 0) {
-    if (e < d) dwq[e] = s;
-    else if (dwk) dwk[e - d] = s;
+    for (int j = 0; j < N; ++j) x[j] = i0 + 32 * j < n ? parts[(int64_t)(i0 + 32 * j) * 2 * d + e] : 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) s += x[j];
   }
+#pragma unroll
+  for (int m = 8; m < 64; m <<= 1) s += __shfl_xor(s, m, 64);
+  if ((tid & 63) < 8) sums[tid >> 6][tid & 7] = s;
+  __syncthreads();
+  if (tid >= 8) return;
+  s = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
+  if (e < d) dwq[e] = s;
+  else if (dwk) dwk[e - d] = s;
 }
 
 constexpr int kBackGroups = 1024;
 int rows_at_once(int n_rows) { return n_rows >= 8192 ? 8 : n_rows >= 2048 ? 4 : 1; }
-int back_groups(int n_rows) { return std::min((n_rows + rows_at_once(n_rows) - 1) / rows_at_once(n_rows), kBackGroups); }
+// Backward: more rows a workgroup, so that there are few sums to add (1000 rows 19.8 us with a row each).
+int rows_back(int n_rows) { return std::max(1, std::min(n_rows / 256, kMostRows)); }
+int back_groups(int n_rows) { return std::min((n_rows + rows_back(n_rows) - 1) / rows_back(n_rows), kBackGroups); }
 
 int check_qk(const std::string &op, int dtype, const void *q, const void *k, const void *wq, const void *wk,
              int n_rows, int n_heads, int n_kv_heads, int head_dim, float eps, float theta) {
@@ -199,11 +222,6 @@ int check_qk(const std::string &op, int dtype, const void *q, const void *k, con
   if (!wq || (n_kv_heads > 0 && !wk)) return fail(BN_ERR_INVALID_ARG, op + ": weight is NULL");
   if (!aligned16(wq) || !aligned16(wk)) return fail(BN_ERR_UNSUPPORTED, op + ": weights must be 16-byte aligned");
   return BN_OK;
-}
-
-void fill_turns(double *f, int head_dim, float theta) {
-  for (int i = 0; i < head_dim / 2; ++i)
-    f[i] = theta > 0.f ? std::pow((double)theta, -2.0 * i / head_dim) / (2.0 * M_PI) : 0.0;
 }
 
 // K<T, D> for the dtype and head dimension
@@ -313,7 +331,7 @@ int bn_qk_norm_rope_backward(int dtype, const void *q, const void *k, const void
   p.q_rs = q_row_stride; p.k_rs = k_row_stride; p.gq_rs = dq_out_row_stride; p.gk_rs = dk_out_row_stride;
   p.qo_rs = dq_row_stride; p.ko_rs = dk_row_stride;
   p.n_rows = n_rows; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads;
-  p.rows = rows_at_once(n_rows);
+  p.rows = rows_back(n_rows);
   p.turn = theta > 0.f;
   p.offset = position_offset;
   p.eps = eps;
