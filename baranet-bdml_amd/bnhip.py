@@ -705,49 +705,52 @@ def _row_type(t):
     return _ROW_TYPES.get(t.dtype)
 
 
-def _qk_rows(op, name, t, rows, heads, like):
-    """(pointer, row stride) of a [rows, heads, D] tensor of like's type, device and D."""
-    shape, stride = t.shape, t.stride()
-    d = like.shape[2]
-    if shape != (rows, heads, d):
-        raise ValueError(f"{op}: {name}: expected [{rows}, {heads}, {d}], got {tuple(shape)}")
-    if t is not like and (t.dtype != like.dtype or t.device != like.device):
+def _qk_rows(op, name, t, rows, heads, d, dtype, device):
+    """(pointer, row stride) of a [rows, heads, d] tensor of a type and device."""
+    stride = t.stride()
+    if t.shape != (rows, heads, d):
+        raise ValueError(f"{op}: {name}: expected [{rows}, {heads}, {d}], got {tuple(t.shape)}")
+    if t.dtype != dtype or t.device != device:
         raise ValueError(f"{op}: {name}: dtype and device must be q's")
     if rows and (stride[2] != 1 or (heads > 1 and stride[1] != d)):
         raise ValueError(f"{op}: {name}: a row's heads must be contiguous")
     return t.data_ptr(), stride[0] if rows > 1 else heads * d
 
 
+def _qk_weight(op, name, w, d, dtype, device):
+    if w.shape != (d,) or w.dtype != dtype or w.device != device or not w.is_contiguous():
+        raise ValueError(f"{op}: {name} must be a contiguous [{d}] tensor of q's type and device")
+    return w.data_ptr()
+
+
 def _qk_args(op, q, k, q_weight, k_weight, positions, stream):
-    """What both directions check alike: (type, stream, pointer of the positions)."""
+    """What both directions check alike: (type's code, stream, pointers of the positions and of the
+    weights, what _qk_rows wants of q's shape)."""
     if q.dim() != 3 or (k is not None and k.dim() != 3):
         raise ValueError(f"{op}: q and k must be [rows, heads, D]")
-    code, device = _row_type(q), q.device
+    code, (rows, heads, d), dtype, device = _row_type(q), q.shape, q.dtype, q.device
     if code is None:
         raise ValueError(f"{op}: q must be float32 or bfloat16")
     if (k is None) != (k_weight is None):
         raise ValueError(f"{op}: k and k_weight must be given together")
-    for w in (q_weight, k_weight):
-        if w is not None and (w.shape != q.shape[2:] or w.dtype != q.dtype or w.device != device or
-                              not w.is_contiguous()):
-            raise ValueError(f"{op}: {'q_weight' if w is q_weight else 'k_weight'} must be a contiguous "
-                             f"[{q.shape[2]}] tensor of q's type and device")
-    if positions is None:
-        pp = None
-    else:
-        import torch
-        if positions.dtype != torch.int32 or positions.shape != q.shape[:1] or not positions.is_contiguous() or \
+    wq = _qk_weight(op, "q_weight", q_weight, d, dtype, device)
+    wk = None if k is None else _qk_weight(op, "k_weight", k_weight, d, dtype, device)
+    import torch
+    pp = None
+    if positions is not None:
+        if positions.dtype != torch.int32 or positions.shape != (rows,) or not positions.is_contiguous() or \
                 positions.device != device:
             raise ValueError(f"{op}: positions must be int32 [rows] on q's device")
         pp = positions.data_ptr()
     if device.type != "cuda":
         raise ValueError(f"{op}: its tensors are not on a GPU")
     if stream is None:
-        import torch
-        return code, torch._C._cuda_getCurrentRawStream(device.index), pp
-    if stream.device != device:
+        s = torch._C._cuda_getCurrentRawStream(device.index)
+    elif stream.device != device:
         raise ValueError(f"{op}: the stream is another device's")
-    return code, stream.cuda_stream, pp
+    else:
+        s = stream.cuda_stream
+    return code, s, pp, wq, wk, rows, heads, (d, dtype, device)
 
 
 def _like(t, stream):
@@ -764,23 +767,20 @@ def qk_norm_rope(q, k, q_weight, k_weight, eps=1e-5, positions=None, position_of
     Heads contiguous, row strides of their own; float32 or bfloat16.  k and
     k_weight may be None.  q_out may be q, k_out k."""
     op = "qk_norm_rope"
-    code, s, pp = _qk_args(op, q, k, q_weight, k_weight, positions, stream)
-    rows, heads, d = q.shape
-    qp, qs = _qk_rows(op, "q", q, rows, heads, q)
+    code, s, pp, wq, wk, rows, heads, kind = _qk_args(op, q, k, q_weight, k_weight, positions, stream)
     q_out = _like(q, stream) if q_out is None else q_out
-    op_, os_ = _qk_rows(op, "q_out", q_out, rows, heads, q)
-    if k is None:
-        if k_out is not None:
-            raise ValueError(f"{op}: k_out without k")
-        call("bn_qk_norm_rope", code, qp, None, q_weight.data_ptr(), None, op_, None, pp, rows, heads, 0, d, qs, 0, os_, 0,
-             position_offset, eps, theta, s)
-        return q_out, None
-    hkv = k.shape[1]
-    kp, ks = _qk_rows(op, "k", k, rows, hkv, q)
-    k_out = _like(k, stream) if k_out is None else k_out
-    kop, kos = _qk_rows(op, "k_out", k_out, rows, hkv, q)
-    call("bn_qk_norm_rope", code, qp, kp, q_weight.data_ptr(), k_weight.data_ptr(), op_, kop, pp, rows, heads, hkv, d, qs,
-         ks, os_, kos, position_offset, eps, theta, s)
+    qp, qs = _qk_rows(op, "q", q, rows, heads, *kind)
+    op_, os_ = _qk_rows(op, "q_out", q_out, rows, heads, *kind)
+    kp, ks, kop, kos, hkv = None, 0, None, 0, 0
+    if k is not None:
+        hkv = k.shape[1]
+        k_out = _like(k, stream) if k_out is None else k_out
+        kp, ks = _qk_rows(op, "k", k, rows, hkv, *kind)
+        kop, kos = _qk_rows(op, "k_out", k_out, rows, hkv, *kind)
+    elif k_out is not None:
+        raise ValueError(f"{op}: k_out without k")
+    call("bn_qk_norm_rope", code, qp, kp, wq, wk, op_, kop, pp, rows, heads, hkv, kind[0], qs, ks, os_, kos,
+         position_offset, eps, theta, s)
     return q_out, k_out
 
 
@@ -799,21 +799,21 @@ def qk_norm_rope_backward(q, k, q_weight, k_weight, dq_out, dk_out, eps=1e-5, po
     are None."""
     import torch
     op = "qk_norm_rope_backward"
-    code, s, pp = _qk_args(op, q, k, q_weight, k_weight, positions, stream)
+    code, s, pp, wq, wk, rows, heads, kind = _qk_args(op, q, k, q_weight, k_weight, positions, stream)
     if (k is None) != (dk_out is None):
         raise ValueError(f"{op}: k and dk_out must be given together")
-    rows, heads, d = q.shape
-    qp, qs = _qk_rows(op, "q", q, rows, heads, q)
-    gp, gs = _qk_rows(op, "dq_out", dq_out, rows, heads, q)
+    d = kind[0]
     dq = _like(q, stream) if dq is None else dq
-    dp, ds = _qk_rows(op, "dq", dq, rows, heads, q)
+    qp, qs = _qk_rows(op, "q", q, rows, heads, *kind)
+    gp, gs = _qk_rows(op, "dq_out", dq_out, rows, heads, *kind)
+    dp, ds = _qk_rows(op, "dq", dq, rows, heads, *kind)
     kp, ks, gkp, gks, dkp, dks, hkv = None, 0, None, 0, None, 0, 0
     if k is not None:
         hkv = k.shape[1]
-        kp, ks = _qk_rows(op, "k", k, rows, hkv, q)
-        gkp, gks = _qk_rows(op, "dk_out", dk_out, rows, hkv, q)
         dk = _like(k, stream) if dk is None else dk
-        dkp, dks = _qk_rows(op, "dk", dk, rows, hkv, q)
+        kp, ks = _qk_rows(op, "k", k, rows, hkv, *kind)
+        gkp, gks = _qk_rows(op, "dk_out", dk_out, rows, hkv, *kind)
+        dkp, dks = _qk_rows(op, "dk", dk, rows, hkv, *kind)
     elif dk is not None:
         raise ValueError(f"{op}: dk without k")
     ws, wsb = None, 0
@@ -824,7 +824,6 @@ def qk_norm_rope_backward(q, k, q_weight, k_weight, dq_out, dk_out, eps=1e-5, po
     dw = made_on(stream, lambda: torch.empty((2, d), dtype=torch.float32, device=q.device))
     dwq, dwk = dw.unbind()
     at = dw.data_ptr()
-    call("bn_qk_norm_rope_backward", code, qp, kp, q_weight.data_ptr(), None if k is None else k_weight.data_ptr(), gp, gkp,
-         dp, dkp, at, None if k is None else at + 4 * d, pp, rows, heads, hkv, d, qs, ks, gs, gks, ds, dks,
-         position_offset, eps, theta, ws, wsb, s)
+    call("bn_qk_norm_rope_backward", code, qp, kp, wq, wk, gp, gkp, dp, dkp, at, None if k is None else at + 4 * d, pp,
+         rows, heads, hkv, d, qs, ks, gs, gks, ds, dks, position_offset, eps, theta, ws, wsb, s)
     return dq, dk, dwq, None if k is None else dwk

@@ -272,7 +272,7 @@ def test_outputs_are_memory_of_the_stream_that_writes_them(monkeypatch):
     monkeypatch.setattr(B, "made_on", lambda stream, make: made.append(stream) or make())
     monkeypatch.setattr(B, "call", lambda *a: None)
     monkeypatch.setattr(B, "_cache_stream", lambda cache, stream: 0)
-    monkeypatch.setattr(B, "_qk_args", lambda *a: (B.BN_BF16, 0, None))
+    monkeypatch.setattr(B, "_qk_args", lambda op, q, *a: (B.BN_BF16, 0, None, 0, 0, *q.shape[:2], (q.shape[2], q.dtype, q.device)))
     kv, st, q = q8(), object(), torch.zeros((3, 8, 64), dtype=torch.bfloat16)
     starts = torch.zeros(4, dtype=torch.int32)
     for call, n in ((lambda: B.paged_q8_decode(q, kv, stream=st), 1),
