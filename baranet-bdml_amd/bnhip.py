@@ -667,12 +667,14 @@ def paged_q8_workspace(cache, n_heads, n_rows):
 
 
 def paged_q8_decode(q, cache, o=None, scale=None, workspace=None, stream=None):
-    """One query row per sequence over its pages: q, o [B, H, D], bfloat16."""
-    import torch
-    o = made_on(stream, lambda: torch.empty_like(q)) if o is None else o
-    qp, qs = _paged_rows("paged_q8_decode: q", q, cache, cache.batch, None, torch.bfloat16)
-    op, os_ = _paged_rows("paged_q8_decode: o", o, cache, cache.batch, q.shape[1], torch.bfloat16)
-    call("bn_paged_q8_decode", cache.ref, BN_BF16, qp, op, q.shape[1], qs, os_,
+    """One query row per sequence over its pages: q, o [B, H, D], float32 or bfloat16."""
+    dt, code = _rows_dtype("paged_q8_decode: q", q)
+    if o is None:
+        import torch
+        o = made_on(stream, lambda: torch.empty_like(q))
+    qp, qs = _paged_rows("paged_q8_decode: q", q, cache, cache.batch, None, dt)
+    op, os_ = _paged_rows("paged_q8_decode: o", o, cache, cache.batch, q.shape[1], dt)
+    call("bn_paged_q8_decode", cache.ref, code, qp, op, q.shape[1], qs, os_,
          1.0 / math.sqrt(q.shape[2]) if scale is None else scale,
          *_workspace(workspace, cache), _cache_stream(cache, stream))
     return o
@@ -680,14 +682,16 @@ def paged_q8_decode(q, cache, o=None, scale=None, workspace=None, stream=None):
 
 def paged_q8_prefill(q, cache, row_starts=None, o=None, scale=None, workspace=None, stream=None):
     """The new rows of a ragged batch over the cache, causal: q, o [rows, H, D]
-    bfloat16, rows of sequence b row_starts[b] .. row_starts[b+1]-1, the last of
-    them at position seq_lens[b] - 1 (rows of no sequence are left as they are)."""
-    import torch
-    o = made_on(stream, lambda: torch.empty_like(q)) if o is None else o
+    float32 or bfloat16, rows of sequence b row_starts[b] .. row_starts[b+1]-1, the
+    last of them at position seq_lens[b] - 1 (rows of no sequence are left as they are)."""
+    dt, code = _rows_dtype("paged_q8_prefill: q", q)
+    if o is None:
+        import torch
+        o = made_on(stream, lambda: torch.empty_like(q))
     n = q.shape[0]
-    qp, qs = _paged_rows("paged_q8_prefill: q", q, cache, None, None, torch.bfloat16)
-    op, os_ = _paged_rows("paged_q8_prefill: o", o, cache, n, q.shape[1], torch.bfloat16)
-    call("bn_paged_q8_prefill", cache.ref, BN_BF16, qp, op, _row_starts("paged_q8_prefill", row_starts, cache, n), n,
+    qp, qs = _paged_rows("paged_q8_prefill: q", q, cache, None, None, dt)
+    op, os_ = _paged_rows("paged_q8_prefill: o", o, cache, n, q.shape[1], dt)
+    call("bn_paged_q8_prefill", cache.ref, code, qp, op, _row_starts("paged_q8_prefill", row_starts, cache, n), n,
          q.shape[1], qs, os_, 1.0 / math.sqrt(q.shape[2]) if scale is None else scale,
          *_workspace(workspace, cache), _cache_stream(cache, stream))
     return o

@@ -96,21 +96,24 @@ struct PageRows {
     return (uint64_t)(there(id) ? (uint32_t)id : 0u) * page_bytes + (uint64_t)((uint32_t)key & slot_mask) * row_bytes;
   }
 };
-// How a pool holds its rows, for the kernels whose products are bf16: eight elements
-// as loaded (Raw), and as bf16.  Bf16Pages: as they stand.
+// How a pool holds its rows: a lane's 16 bytes of products' operands (piece) and two
+// elements (pair) as they are loaded, and as they are used.  PlainPages: as they stand.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-struct Bf16Pages {
-  typedef bf16_t T;
+template <typename E>
+struct PlainPages {
+  typedef E T;
   typedef u32x4 Raw;
+  typedef float2 Pair;  // (fp32)
   static constexpr bool kScaled = false;
   // (kScaled: where the scales of KV head g's keys, or values, lie, and what a lane loads of them)
   __device__ __forceinline__ const uint8_t *scales(int, bool) const { return nullptr; }
   __device__ __forceinline__ int scale(const uint8_t *, const PageRows &, int, int) const { return 0; }
   __device__ __forceinline__ int scale_bits(int) const { return 0; }
-  __device__ __forceinline__ u32x4 bf16(Raw x, int) const { return x; }
+  __device__ __forceinline__ u32x4 piece(Raw x, int) const { return x; }
+  __device__ __forceinline__ float2 pair(Pair x, int) const { return x; }
   // element `lane` of a value's row, key k of page id
   __device__ __forceinline__ float value(const PageRows &rows, const char *Vg, int, int id, int k, int lane) const {
-    return Elem<bf16_t>::load((const bf16_t *)(Vg + rows.at(id, k)) + lane);
+    return Elem<E>::load((const E *)(Vg + rows.at(id, k)) + lane);
   }
 };
 // table entries are read as scalars
@@ -231,6 +234,519 @@ struct DecodeParams {
   int *cuts;
 };
 
+// A tile of keys as a wave loads it: four 16-byte loads per lane of K and four
+// of V, LPR lanes a row: whole rows, 1 KB of a head-major page an instruction
+// (loads straight into the products' operands, 16 rows of 64 bytes an
+// instruction, streamed a third slower).  P: pitch of a row in LDS, elements
+// (144 and 272 bytes: the fragment reads below spread over the banks).
+template <typename T> struct DecTile;
+template <> struct DecTile<bf16_t> { static constexpr int TK = 32, LPR = 8, P = HD + 8; };
+template <> struct DecTile<float> { static constexpr int TK = 16, LPR = 16, P = HD + 4; };
+
+// The batch's tiles, sequences in order, are dealt in equal shares to the
+// workgroups of a column (a KV head, or up to 16 of its query heads), so that
+// any mix of lengths keeps every compute unit streaming to the end.  A
+// workgroup's four waves take its share's tiles in turn, across the borders of
+// sequences, with the loads of the next tiles and the table entries of the one
+// after them in flight; no barrier between them.  A wave leaves its part of
+// each sequence (running maximum, sum, accumulator) in LDS; when the share, or
+// as many sequences as LDS has room for, are through, the workgroup adds the
+// waves' parts.  A sequence that lies in one share is then written; of one cut
+// between shares each workgroup leaves a record in the workspace and counts
+// itself in, and the last to arrive adds the records, in the order of the keys,
+// and writes the output: one launch, and the same bits whoever arrives last.
+//
+// Per tile, with the query heads as columns of the products:
+//   S^T[key][head] = K . Q^T,  O^T[d][head] += V^T . P^T
+// on v_mfma_f32_16x16x32_bf16 (bf16 probabilities, the products' operands: off by at most
+// 2^-8 each; outputs 0.0023 off 64 bits in the mean, 0.0017 of it their own rounding)
+// or v_mfma_f32_16x16x4_f32; a lane holds its 8 (4) keys' scores of one head,
+// which are the second product's operand as they stand.  Bound by memory: 64
+// caches of 512..4096 keys (32 and 4 heads) 33 us, 4.6 TB/s; three of 34763 to
+// 131072 49 us, 5.1 TB/s, a copy's rate.  One of 640 fp32 keys 8.3 us: launch,
+// lengths, table, keys and the merge's round trip, one after another.
+template <typename T>
+struct DecodeLds {
+  T k[4][DecTile<T>::TK * DecTile<T>::P];
+  T v[4][DecTile<T>::TK * DecTile<T>::P];
+  float hold[kHoldRows * kHold];
+  int last_in[2];
+};
+template <typename T, class Src = PlainPages<T>>
+__device__ __forceinline__ void decode_body(const DecodeParams &p, DecodeLds<T> &lds, int block,
+                                            const Src &src = Src{}) {
+  using Ti = DecTile<T>;
+  using E = typename Src::T;  // the pools' elements
+  constexpr bool BF = sizeof(T) == 2;
+  constexpr int TK = Ti::TK, LPR = Ti::LPR, RPI = 64 / LPR, VEC = HD / LPR, P = Ti::P;
+  constexpr int NS = TK / 16;  // 16-key score tiles
+  constexpr int NQ = BF ? 2 : 4;
+  float *const hold = lds.hold;
+
+  const Paged &c = p.a.c;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, grp = lane >> 4;
+  const int bin = block / p.columns, col = block - bin * p.columns;
+  const int g = col / p.hblocks, hb = col - g * p.hblocks;
+  const int rows = min(kMaxRows, p.a.group - kMaxRows * hb), head0 = g * p.a.group + kMaxRows * hb;
+  const int room = kHoldRows / (4 * rows);  // sequences that LDS has room for
+  // the first tile begins at a multiple of the smallest page, so that eight rows
+  // of a tile from a multiple of eight on lie in one page
+  const int k0 = p.k0 & -8;
+  auto clamp_len = [&](int n) { return max(min(n, c.cap), 0); };
+  auto tiles_of = [&](int len) { return len > p.k0 ? (int)((uint32_t)(len - k0 + TK - 1) / TK) : 0; };
+
+  // ---- the share: every wave scans the lengths for itself, a run of
+  // `per` sequences a lane
+  const int per = (c.batch + 63) >> 6;
+  int own, some = 0;
+  auto length_of = [&](int b) __attribute__((always_inline)) {
+    const int n = c.lens[min(b, c.batch - 1)];
+    return b < c.batch ? clamp_len(n) : 0;
+  };
+  if (per == 1) {
+    some = length_of(lane);
+    own = tiles_of(some);
+  } else {
+    own = 0;
+    for (int i = 0; i < per; i += 8) {
+      int n[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) n[j] = c.lens[min(lane * per + i + j, c.batch - 1)];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        own += i + j < per && lane * per + i + j < c.batch ? tiles_of(clamp_len(n[j])) : 0;
+    }
+  }
+  const int upto = wave_scan(own);
+  const int total = __builtin_amdgcn_readlane(upto, 63);
+  const int share =
+      __builtin_amdgcn_readfirstlane(max((int)((uint32_t)(total + p.bins - 1) / (uint32_t)p.bins), kShareMin));
+  const int pos0 = (int)min((int64_t)bin * share, (int64_t)total), n_wg = min(share, total - pos0);
+
+  struct Window {  // 64 lengths from sequence b0 on, one a lane
+    int b0, len;
+  };
+  auto window = [&](int b) __attribute__((always_inline)) { return Window{b, length_of(b + lane)}; };
+  struct Tile {
+    int b, t, len, ord;  // tile t of sequence b of len keys, the share's ord-th sequence
+  };
+  // the sequence behind x's that has a tile (there is one)
+  auto next_seq = [&](Tile x, Window &w) __attribute__((always_inline)) {
+    int b = x.b + 1;
+    for (;;) {
+      if (b - w.b0 >= 64) w = window(b);
+      const unsigned long long there = __builtin_amdgcn_ballot_w64(tiles_of(w.len) > 0) >> (b - w.b0);
+      if (there) {
+        b += __builtin_ctzll(there);
+        return Tile{b, 0, __builtin_amdgcn_readlane(w.len, b - w.b0), x.ord + 1};
+      }
+      b = w.b0 + 64;
+    }
+  };
+  auto skip = [&](Tile x, int by, Window &w) __attribute__((always_inline)) {
+    x.t += by;
+    for (int nt; x.t >= (nt = tiles_of(x.len));) {
+      const int t = x.t - nt;
+      x = next_seq(x, w);
+      x.t = t;
+    }
+    return x;
+  };
+
+  // ---- loads: the RPI rows of a load instruction lie in one page, so that its
+  // table entry and address are scalars and a lane's offset to them is fixed
+  const int crow = lane / LPR, ccol = (lane % LPR) * VEC;
+  const uint32_t off = (uint32_t)((crow * c.row_stride + ccol) * sizeof(E));
+  const char *const Kg = (const char *)((const E *)c.k + g * c.head_stride);
+  const char *const Vg = (const char *)((const E *)c.v + g * c.head_stride);
+  const PageRows page_rows = PageRows::of<E>(c);
+  const uint8_t *const sg = src.scales(g, lane & 1);  // (scaled: even lanes K's, odd ones V's; a tile lies in one block)
+  // A tile's table entries are read as scalars: they come in their own order,
+  // not behind the rows requested before them (as vector loads they held up
+  // the next rows: 64 caches of 4096 keys 51 us).
+  int ids[4];  // of rows RPI r .. of the tile to load next
+  struct Rows {
+    typename Src::Raw k[4], v[4];  // the lane's pieces of a tile
+    int scale;                     // scaled: the byte of the tile's keys, or values
+    int lo, hi;        // keys lo .. hi - 1 of the tile are the sequence's
+    int pages;         // bit r: rows RPI r .. have memory (else page 0 is read)
+  };
+  auto load_ids = [&](const Tile &x) __attribute__((always_inline)) {
+    const int b = __builtin_amdgcn_readfirstlane(x.b), key0 = k0 + TK * __builtin_amdgcn_readfirstlane(x.t);
+    const int last = __builtin_amdgcn_readfirstlane(x.len) - 1;
+    const scalar_bytes row = (scalar_bytes)(c.table + b * c.table_stride);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) ids[r] = *(scalar_ints)(row + ((uint32_t)(min(key0 + RPI * r, last) >> c.shift) << 2));
+  };
+  uint64_t at[4];  // byte offsets of the rows
+  int at_pages;   // bit r: those rows have memory (else page 0's are read)
+  auto locate_rows = [&](const Tile &x) __attribute__((always_inline)) {
+    const int key0 = k0 + TK * __builtin_amdgcn_readfirstlane(x.t);
+    at_pages = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      at_pages |= page_rows.there(ids[r]) << r;
+      at[r] = page_rows.at(ids[r], key0 + RPI * r);
+    }
+  };
+  auto load_rows = [&](Rows &y, const Tile &x) __attribute__((always_inline)) {
+    const int key0 = k0 + TK * x.t;
+    y.lo = p.k0 - key0;
+    y.hi = x.len - key0;
+    y.pages = at_pages;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {  // streamed once: non-temporal
+      y.k[r] = __builtin_nontemporal_load((const typename Src::Raw *)(Kg + at[r] + off));
+      y.v[r] = __builtin_nontemporal_load((const typename Src::Raw *)(Vg + at[r] + off));
+    }
+    if constexpr (Src::kScaled) y.scale = src.scale(sg, page_rows, ids[0], key0);
+  };
+  T *const kt = lds.k[wave], *const vt = lds.v[wave];
+  auto store_rows = [&](const Rows &x, bool masked) __attribute__((always_inline)) {
+    int bits = 0;
+    if constexpr (Src::kScaled) bits = src.scale_bits(x.scale);
+    struct {
+      u32x4 k[4], v[4];
+    } y;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      y.k[r] = src.piece(x.k[r], __builtin_amdgcn_readlane(bits, 0));
+      y.v[r] = src.piece(x.v[r], __builtin_amdgcn_readlane(bits, 1));
+    }
+    if (masked) {  // no key: zeros, whatever lies there (0 times an infinite value is none)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = crow + RPI * r;
+        if (row < x.lo || row >= x.hi || !(x.pages >> r & 1)) y.k[r] = y.v[r] = u32x4{0, 0, 0, 0};
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) *(u32x4 *)(kt + (crow + RPI * r) * P + ccol) = y.k[r];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) *(u32x4 *)(vt + (crow + RPI * r) * P + ccol) = y.v[r];
+  };
+  // queries: lane holds head l16's elements 8 grp + 32 t .. +7 (bf16), 16 grp .. +15 (fp32)
+  u32x4 q[NQ], qn[NQ];
+  auto load_q = [&](int b) __attribute__((always_inline)) {
+    const T *const qp = (const T *)p.a.q + b * p.a.q_rs + (head0 + min(l16, rows - 1)) * HD;
+#pragma unroll
+    for (int t = 0; t < NQ; ++t) qn[t] = *(const u32x4 *)(qp + (BF ? 8 * grp + 32 * t : 16 * grp + 4 * t));
+  };
+
+  // ---- a tile's arithmetic.  The probabilities are taken against a reference
+  // that is the true running maximum only when it was last moved: it moves when
+  // a key's weight against it passes 2^16 (or is NaN), which saves the maximum
+  // over the lanes and the rescaling of the accumulator for most tiles.
+  float mc = -INFINITY, l = 0.f;  // of head l16: reference, log2 units; this lane's keys' sum
+  f32x4 o[4];
+  const float cl = p.a.cl;
+  auto compute = [&](bool masked, int lo, int hi, int pages) __attribute__((always_inline)) {
+    f32x4 s[NS];
+    if constexpr (BF) {
+#pragma unroll
+      for (int u = 0; u < NS; ++u) {
+        const bf16_t *kp = kt + 8 * grp + (16 * u + l16) * P;
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8 *)kp, __builtin_bit_cast(bf16x8, q[0]),
+                                                       f32x4{}, 0, 0, 0);
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8 *)(kp + 32),
+                                                       __builtin_bit_cast(bf16x8, q[1]), s[u], 0, 0, 0);
+      }
+    } else {
+      const float *kp = kt + 16 * grp + l16 * P;
+      f32x4 s2[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {  // four chains
+        const f32x4 a = *(const f32x4 *)(kp + 4 * t), b = __builtin_bit_cast(f32x4, q[t]);
+        s2[t] = f32x4{};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s2[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], s2[t], 0, 0, 0);
+      }
+      s[0] = (s2[0] + s2[1]) + (s2[2] + s2[3]);
+    }
+    // s[u][i]: key 16u + 4grp + i of the tile, head l16
+    if (masked) {
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 16 * u + 4 * grp + i;
+          if (row < lo || row >= hi || !(pages >> (row / RPI) & 1)) s[u][i] = -INFINITY;
+        }
+    }
+    float e[4 * NS], rs;
+    auto weigh = [&](float ref) __attribute__((always_inline)) {
+      rs = 0.f;
+#pragma unroll
+      for (int u = 0; u < NS; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[4 * u + i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], cl, -ref));
+          rs += e[4 * u + i];
+        }
+    };
+    weigh(mc);  // (no key yet: mc is -inf, and the sum +inf or NaN)
+    if (__builtin_amdgcn_ballot_w64(!(rs <= 65536.f)) != 0) {
+      float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+      if constexpr (NS > 1) mx = fmaxf(mx, fmaxf(fmaxf(s[NS - 1][0], s[NS - 1][1]), fmaxf(s[NS - 1][2], s[NS - 1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float m_new = fmaxf(mc, mx * cl);
+      const float ref = m_new == -INFINITY ? 0.f : m_new;  // no key above -inf yet: weights 0
+      const float alpha = __builtin_amdgcn_exp2f(mc - ref);
+      mc = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
+      weigh(ref);
+    }
+    l += rs;
+    if constexpr (BF) {
+      bf16x8 pb;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pb[i] = (__bf16)e[i];
+      // V^T: slot j of lane (grp, l16) is V[key 16(j/4) + 4grp + j%4][16dt + l16]
+      const bf16_t *vp = vt + (4 * grp + (l16 >> 2)) * P + 4 * (l16 & 3);
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) {
+        const bf16x4 x = lds_tr16(vp + 16 * dt), y = lds_tr16(vp + 16 * P + 16 * dt);
+        const bf16x8 a = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pb, o[dt], 0, 0, 0);
+      }
+    } else {
+      // k slot grp of step i is key 4grp + i; row r of product dt is d = 4r + dt
+      f32x4 a[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = *(const f32x4 *)(vt + (4 * grp + i) * P + 4 * l16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][dt], e[i], o[dt], 0, 0, 0);
+    }
+  };
+
+  // ---- results: two elements of a head's row a thread
+  auto write2 = [&](int b, int h, int d, float x, float y, float ref, float sum) __attribute__((always_inline)) {
+    if (p.parts) {  // one part of the row: left for the launch that adds them
+      float *const r = p.parts + ((int64_t)b * p.a.n_heads + head0 + h) * kRec;
+      *(float2 *)(r + d) = make_float2(x, y);
+      if (d == 0) *(float2 *)(r + HD) = make_float2(ref, sum);
+      return;
+    }
+    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+    T *const op = (T *)p.a.o + b * p.a.o_rs + (head0 + h) * HD + d;
+    if constexpr (BF)
+      *(uint32_t *)op = (uint32_t)f32_to_bf16(x * inv) | ((uint32_t)f32_to_bf16(y * inv) << 16);
+    else
+      *(float2 *)op = make_float2(x * inv, y * inv);
+  };
+  // row h of the record of a sequence's piece in bin `at` (a bin has two: the end
+  // of a sequence begun before it, and the start of one, begun in bin0, that goes on)
+  auto record = [&](int at, int bin0, int h) __attribute__((always_inline)) {
+    return p.ws + ((((int64_t)at * 2 + (at == bin0)) * p.columns + col) * kMaxRows + h) * kRec;
+  };
+  // a cut sequence: its first bin and the number of its pieces, one a bin
+  struct Cut {
+    int b, bin0, pieces;
+  };
+  Cut cuts[2] = {{0, 0, 0}, {0, 0, 0}};  // one that began before the share, one that goes on
+
+  if (n_wg > 0) {
+    Tile x;       // the wave's tile (its loads are in flight)
+    Window w;     // of the tiles to come
+    Tile seg;     // the next sequence whose parts are to be added (its t: 0), ...
+    Window sw;
+    int first;    // ... and the position of its first tile
+    {
+      const int src = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > pos0));
+      first = __builtin_amdgcn_readlane(upto - own, src);
+      if (per == 1) {
+        w = Window{0, some};
+        seg = Tile{src, 0, __builtin_amdgcn_readlane(some, src), 0};
+      } else {
+        w = window(src * per);
+        for (;;) {  // (one round unless a lane's run is longer than a window)
+          const int t = tiles_of(w.len), up = wave_scan(t);
+          const unsigned long long hit = __builtin_amdgcn_ballot_w64(first + up > pos0);
+          if (hit) {
+            const int i = __builtin_ctzll(hit);
+            first += __builtin_amdgcn_readlane(up - t, i);
+            seg = Tile{w.b0 + i, 0, __builtin_amdgcn_readlane(w.len, i), 0};
+            break;
+          }
+          first += __builtin_amdgcn_readlane(up, 63);
+          w = window(w.b0 + 64);
+        }
+      }
+      sw = w;
+    }
+    const int n = n_wg > wave ? (n_wg - wave + 3) / 4 : 0;  // the wave's tiles
+    Rows buf;
+    Tile ahead[3];  // the wave's tiles i .. i + 2 (the last one again past the end)
+    bool fresh = true;
+    if (n > 0) {
+      x = seg;
+      x.t = pos0 - first;
+      if (wave) x = skip(x, wave, w);
+      load_q(x.b);
+      load_ids(x);
+      ahead[0] = x;
+      ahead[1] = 1 < n ? skip(x, 4, w) : x;
+      locate_rows(x);
+      load_rows(buf, x);
+      load_ids(ahead[1]);
+      ahead[2] = 2 < n ? skip(ahead[1], 4, w) : ahead[1];
+    }
+    int i = 0, base = 0;  // base: the sequence in the first place of LDS
+    auto step = [&]() __attribute__((always_inline)) {
+      locate_rows(ahead[1]);
+      const int lo = buf.lo, hi = buf.hi, pages = buf.pages;
+      const bool masked = lo > 0 || hi < TK || pages != 15;
+      // a wave's LDS instructions execute in order, so its tile needs no
+      // barrier; wave_barrier keeps the compiler from moving them across
+      __builtin_amdgcn_wave_barrier();
+      store_rows(buf, masked);
+      __builtin_amdgcn_wave_barrier();
+      if (fresh) {
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) q[t] = qn[t];
+        mc = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = f32x4{};
+      }
+      x = ahead[0];
+      const bool ends = i + 1 == n || ahead[1].b != x.b;
+      if (i + 1 < n) {
+        load_rows(buf, ahead[1]);
+        if (ends) load_q(ahead[1].b);
+        load_ids(ahead[2]);
+        ahead[0] = ahead[1];
+        ahead[1] = ahead[2];
+        if (i + 3 < n) ahead[2] = skip(ahead[2], 4, w);
+      }
+      compute(masked, lo, hi, pages);
+      if (ends) {
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (l16 < rows) {
+          float *const h = hold + (((x.ord - base) * 4 + wave) * rows + l16) * kHold;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // bf16: o[j] is d = 16j + 4grp ..; fp32: o[0..3][j] is d = 16grp + 4j ..
+            *(f32x4 *)(h + (BF ? 16 * j + 4 * grp : 16 * grp + 4 * j)) =
+                BF ? o[j] : f32x4{o[0][j], o[1][j], o[2][j], o[3][j]};
+          if (grp == 0) *(float2 *)(h + HD) = make_float2(mc, l);
+        }
+      }
+      fresh = ends;
+      ++i;
+    };
+    for (;;) {
+      while (i < n && ahead[0].ord < base + room) step();
+      __syncthreads();
+      bool more = true;
+      for (int place = 0; more && place < room; ++place) {
+        const int nt = tiles_of(seg.len), i0 = max(first - pos0, 0), i1 = min(first + nt - pos0, n_wg);
+        const int bin0 = (int)((uint32_t)first / (uint32_t)share);
+        const int pieces = (int)((uint32_t)(first + nt - 1) / (uint32_t)share) - bin0 + 1;
+        if (p.parts) {
+          if (tid == 0 && bin0 == bin) p.cuts[seg.b * p.columns + col] = pieces << 16 | bin0;
+        } else if (pieces > 1) {
+          cuts[bin0 == bin] = Cut{seg.b, bin0, pieces};
+        }
+        for (int k = tid; k < rows * (HD / 2); k += 256) {
+          const int h = k / (HD / 2), d = 2 * (k % (HD / 2));
+          const float *r = hold + (place * 4 * rows + h) * kHold;
+          float2 ml[4];
+          float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            ml[v] = make_float2(-INFINITY, 0.f);  // no tile of it
+            if (((v - i0) & 3) < i1 - i0) ml[v] = *(const float2 *)(r + v * rows * kHold + HD);
+            M = fmaxf(M, ml[v].x);
+          }
+          const float Mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            if (((v - i0) & 3) >= i1 - i0) continue;
+            const float f = __builtin_amdgcn_exp2f(ml[v].x - Mu);
+            const float2 a = *(const float2 *)(r + v * rows * kHold + d);
+            L = fmaf(ml[v].y, f, L);
+            A0 = fmaf(a.x, f, A0);
+            A1 = fmaf(a.y, f, A1);
+          }
+          if (pieces == 1) {
+            write2(seg.b, h, d, A0, A1, M, L);
+          } else {
+            float *const to = record(bin, bin0, h);
+            put2(to + d, A0, A1);
+            if (d == 0) put2(to + HD, M, L);
+          }
+        }
+        first += nt;
+        more = first < pos0 + n_wg;
+        if (more) seg = next_seq(seg, sw);
+      }
+      if (!more) break;
+      __syncthreads();  // the places are free again
+      base += room;
+    }
+    if (cuts[0].pieces | cuts[1].pieces) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the records' stores have reached memory
+      __syncthreads();
+      if (tid < 2) {
+        const Cut u = tid ? cuts[1] : cuts[0];
+        lds.last_in[tid] =
+            u.pieces && arrive_last(p.arrive_end - 2 * ((int64_t)u.b * p.columns + col + 1), u.pieces, p.tag);
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int side = 0; side < 2; ++side) {
+        if (!lds.last_in[side]) continue;
+        const Cut u = side ? cuts[1] : cuts[0];
+        for (int k = tid; k < rows * (HD / 2); k += 256) {
+          const int h = k / (HD / 2), d = 2 * (k % (HD / 2));
+          float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
+          for (int n0 = 0; n0 < u.pieces; n0 += kMergeBatch) {
+            float2 ml[kMergeBatch], a[kMergeBatch];
+#pragma unroll
+            for (int v = 0; v < kMergeBatch; ++v) {
+              const float *const r = record(u.bin0 + min(n0 + v, u.pieces - 1), u.bin0, h);
+              ml[v] = get2(r + HD);
+              a[v] = get2(r + d);
+            }
+            float mx = M;
+#pragma unroll
+            for (int v = 0; v < kMergeBatch; ++v) mx = n0 + v < u.pieces ? fmaxf(mx, ml[v].x) : mx;
+            const float mu = mx == -INFINITY ? 0.f : mx, fo = __builtin_amdgcn_exp2f(M - mu);
+            L *= fo;
+            A0 *= fo;
+            A1 *= fo;
+#pragma unroll
+            for (int v = 0; v < kMergeBatch; ++v) {
+              const bool in = n0 + v < u.pieces;  // (a record past the end is never multiplied: it may hold anything)
+              const float f = __builtin_amdgcn_exp2f(ml[v].x - mu);
+              L = in ? fmaf(ml[v].y, f, L) : L;
+              A0 = in ? fmaf(a[v].x, f, A0) : A0;
+              A1 = in ? fmaf(a[v].y, f, A1) : A1;
+            }
+            M = mx;
+          }
+          write2(u.b, h, d, A0, A1, M, L);
+        }
+      }
+    }
+  }
+  // sequences without a key
+  for (int b = bin; b < c.batch; b += p.bins)
+    if (tiles_of(clamp_len(c.lens[b])) == 0)
+      for (int k = tid; k < rows * (HD / 2); k += 256) {
+        write2(b, k / (HD / 2), 2 * (k % (HD / 2)), 0.f, 0.f, -INFINITY, 0.f);
+        if (k == 0 && p.parts) p.cuts[b * p.columns + col] = 1 << 16;
+      }
+}
 // ------------------------------------------------- prefill, over pages
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -454,7 +970,7 @@ struct PrefillLds {
   Piece piece;  // kept here across the tiles, not in scalar registers
   int last_in;
 };
-template <int HW, int KW, class Src = Bf16Pages>
+template <int HW, int KW, class Src = PlainPages<bf16_t>>
 __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, PrefillLds<HW, KW> &lds, int block,
                                                   const Src &src = Src{}) {
   typedef typename Src::T T;
@@ -545,7 +1061,7 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
     const int bits = src.scale_bits(sc);
     u32x4 vb[NC];
 #pragma unroll
-    for (int j = 0; j < NC; ++j) vb[j] = src.bf16(vr[j], __builtin_amdgcn_readlane(bits, NC + j));
+    for (int j = 0; j < NC; ++j) vb[j] = src.piece(vr[j], __builtin_amdgcn_readlane(bits, NC + j));
     if (key0 + 32 > keys.end || chunks_next != (1 << NC) - 1) {  // no key: zeros, whatever lies there
 #pragma unroll
       for (int j = 0; j < NC; ++j)
@@ -559,7 +1075,7 @@ __device__ __forceinline__ void prefill_bf16_body(const PrefillParams &p, Prefil
     }
 #pragma unroll
     for (int j = 0; j < NC; ++j)
-      *(u32x4 *)(kd + (8 * (NC * hw + j) + crow) * KP + ccol) = src.bf16(kr[j], __builtin_amdgcn_readlane(bits, j));
+      *(u32x4 *)(kd + (8 * (NC * hw + j) + crow) * KP + ccol) = src.piece(kr[j], __builtin_amdgcn_readlane(bits, j));
 #pragma unroll
     for (int j = 0; j < NC; ++j) *(u32x4 *)(vd + (8 * (NC * hw + j) + crow) * VP + ccol) = vb[j];
     if (HW > 1 && lane == 0) lds.chunk_ok[kw][b][hw] = (unsigned char)chunks_next;
@@ -753,7 +1269,7 @@ struct PipeLds {
   Piece piece;
   int odd[4], last_in;
 };
-template <class Src = Bf16Pages>
+template <class Src = PlainPages<bf16_t>>
 __device__ __forceinline__ void prefill_pipe_body(const PrefillParams &p, PipeLds &lds, int block,
                                                   const Src &src = Src{}) {
   typedef typename Src::T T;
@@ -851,14 +1367,14 @@ __device__ __forceinline__ void prefill_pipe_body(const PrefillParams &p, PipeLd
   auto lstore_k = [&](int blk) __attribute__((always_inline)) {
     bf16_t *ks = kring + (blk & 1) * KBUF;
     const int bits = src.scale_bits(sk);
-    *(u32x4 *)(ks + crow * KP + ccol) = src.bf16(k0, __builtin_amdgcn_readlane(bits, 0));
-    *(u32x4 *)(ks + (crow + 32) * KP + ccol) = src.bf16(k1, __builtin_amdgcn_readlane(bits, 1));
+    *(u32x4 *)(ks + crow * KP + ccol) = src.piece(k0, __builtin_amdgcn_readlane(bits, 0));
+    *(u32x4 *)(ks + (crow + 32) * KP + ccol) = src.piece(k1, __builtin_amdgcn_readlane(bits, 1));
     if (lane < 2) lds.chunk_ok[blk & 3][wave + 4 * lane] = (unsigned char)(k_ok >> lane & 1);
   };
   auto lstore_v = [&](int blk) __attribute__((always_inline)) {
     bf16_t *vs = vring + (blk & 1) * VBUF;
     const int bits = src.scale_bits(sv);
-    u32x4 x0 = src.bf16(v0, __builtin_amdgcn_readlane(bits, 0)), x1 = src.bf16(v1, __builtin_amdgcn_readlane(bits, 1));
+    u32x4 x0 = src.piece(v0, __builtin_amdgcn_readlane(bits, 0)), x1 = src.piece(v1, __builtin_amdgcn_readlane(bits, 1));
     if (first + kBK * (blk + 1) > end || v_ok != 3) {  // no key: zeros, whatever lies there
       const int key = first + kBK * blk + crow;
       if (!(v_ok & 1) || key >= end) x0 = u32x4{0, 0, 0, 0};
@@ -1178,6 +1694,219 @@ __device__ __forceinline__ void prefill_pipe_body(const PrefillParams &p, PipeLd
     }
     write(t, h, rt, L);
   }
+}
+
+// fp32, v_mfma_f32_32x32x2f32: matrix-core time is all that counts.  32 rows a
+// unit, its tiles dealt to KW waves, no barrier before the merge: a wave
+// stages its own K tile in LDS one tile ahead (rows of 272 B) and reads V
+// straight from the pages as the second product's operand (two adjacent d of
+// one key row a lane), requested before the scores' products, which cover it.
+// 1636 and 1492 rows behind 435 and 539 (20 heads) 212 us, 96 TFLOP/s; 512 rows
+// 20.6 us (52), matrix cores 39% busy: units of unequal length, 6 us of start.
+template <int KW>
+struct PrefillLdsF32 {
+  float smem[KW * 32 * (HD + 4)];
+  float red_m[KW][32], red_l[KW][32];
+  int odd[KW];
+  Piece piece;
+  int last_in;
+};
+template <int KW, class Src = PlainPages<float>>
+__device__ __forceinline__ void prefill_f32_body(const PrefillParams &p, PrefillLdsF32<KW> &lds, int block,
+                                                 const Src &src = Src{}) {
+  typedef typename Src::T T;
+  constexpr int R = 32, KP = HD + 4;  // K row and O row pitch, floats
+  constexpr int TILE = 32 * KP;
+  float *const smem = lds.smem;
+  auto &red_m = lds.red_m, &red_l = lds.red_l;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int kw = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, hf = lane >> 5;
+  Piece w;
+  if (!find_piece<R>(p, block, w)) return;
+  if (tid == 0) lds.piece = w;
+  const Paged &c = p.a.c;
+  const PieceKeys keys = piece_keys<R>(p, w);
+  const float cl = p.a.cl;
+  float *const kl = smem + kw * TILE;
+  int head;
+  const int tok = token_of(w, p.a.inv_group, p.a.group, r32, head);
+  const bool there = tok < w.rows;
+  const int limit = there ? key_limit(p, w, tok) : keys.end;
+
+  const PageRows rows = PageRows::of<T>(c);
+  const uint32_t row_bytes = rows.row_bytes;
+  const uint32_t koff = (lane >> 4) * row_bytes + (lane & 15) * (4 * sizeof(T));  // 4 rows a load
+  const uint32_t voff = 4 * hf * row_bytes + r32 * (2 * sizeof(T));
+  const char *const Kg = (const char *)((const T *)c.k + w.g * c.head_stride);
+  const char *const Vg = (const char *)((const T *)c.v + w.g * c.head_stride);
+  typename Src::Raw kr[8];
+  // scaled: lanes r and 4 + r (mod 8): the byte of rows 8r .. of K, of V, of the tile to load next
+  int sc = 0;
+  const uint8_t *const sg = src.scales(w.g, lane & 4);
+  int entry = 0;  // lane r (mod 4): of rows 8r .. of the tile to load next
+  uint64_t at[4], vat[4];  // byte offsets of rows 8r .. of the tile to load next, of this tile
+  int pages = 0, pages_next = 0;
+  auto load_ids = [&](int t) __attribute__((always_inline)) { entry = keys.entry(32 * t + 8 * (lane & 3)); };
+  auto gload_k = [&](int t) __attribute__((always_inline)) {
+    pages_next = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int id = __builtin_amdgcn_readlane(entry, r);
+      pages_next |= rows.there(id) << r;
+      at[r] = rows.at(id, 32 * t + 8 * r);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        kr[2 * r + j] = *(const typename Src::Raw *)(Kg + at[r] + (uint64_t)(j * 4u) * row_bytes + koff);
+    }
+    if constexpr (Src::kScaled) sc = src.scale(sg, rows, entry, 32 * t + 8 * (lane & 3));
+  };
+  float qreg[32];  // k slot (hf, t) of the score product is d = 32 hf + t
+  {
+    const float *const qp = (const float *)p.a.q + (int64_t)(w.row0 + (there ? tok : 0)) * p.a.q_rs +
+                            (w.g * p.a.group + (there ? head : 0)) * HD + 32 * hf;
+#pragma unroll
+    for (int t = 0; t < 32; t += 4) {
+      const float4 x = *(const float4 *)(qp + t);
+      qreg[t] = x.x; qreg[t + 1] = x.y; qreg[t + 2] = x.z; qreg[t + 3] = x.w;
+    }
+  }
+  float mc = -INFINITY, l = 0.f;
+  f32x16 ow[1][2] = {{f32x16{}, f32x16{}}};  // ow[0][j] row i is d = 2i + j
+  f32x16 (&o)[2] = ow[0];
+  bool any_odd = false;
+  int t = keys.t0 + kw;
+  if (t < keys.t1) {
+    load_ids(t);
+    gload_k(t);
+    load_ids(t + KW);
+  }
+  for (; t < keys.t1; t += KW) {
+    pages = pages_next;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) vat[r] = at[r];
+    const int bits = src.scale_bits(sc);
+    // the wave's own tile: its LDS instructions execute in order
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      *(u32x4 *)(kl + (4 * j + (lane >> 4)) * KP + (lane & 15) * 4) =
+          src.piece(kr[j], __builtin_amdgcn_readlane(bits, j >> 1));
+    __builtin_amdgcn_wave_barrier();
+    // this tile's V: key slot (hf, i) of the second product is key 8(i/4) + 4hf + i%4
+    typename Src::Pair vp[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      vp[i] = *(const typename Src::Pair *)(Vg + vat[i >> 2] + (uint64_t)(i & 3u) * row_bytes + voff);
+    gload_k(t + KW);  // past the range: the last key's page again, not used
+    load_ids(t + 2 * KW);
+    f32x16 s = f32x16{};
+    const float *krow = kl + r32 * KP + 32 * hf;
+#pragma unroll
+    for (int u = 0; u < 32; u += 4) {
+      const float4 a = *(const float4 *)(krow + u);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x, qreg[u], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.y, qreg[u + 1], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.z, qreg[u + 2], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(a.w, qreg[u + 3], s, 0, 0, 0);
+    }
+    float2 vr[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) vr[i] = src.pair(vp[i], __builtin_amdgcn_readlane(bits, 4 + (i >> 2)));
+    const int kb = 32 * t;
+    if (kb + 32 > keys.whole || pages != 15) {
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int k = (i >> 2) * 8 + hf * 4 + (i & 3);
+        const bool page = pages >> (i >> 2) & 1;
+        if (kb + k >= limit || !page) s[i] = -INFINITY;
+        if (kb + k >= keys.end || !page) vr[i] = make_float2(0.f, 0.f);  // no key: whatever lies there
+        const bool bx = !(fabsf(vr[i].x) < INFINITY), by = !(fabsf(vr[i].y) < INFINITY);
+        vr[i] = make_float2(bx ? 0.f : vr[i].x, by ? 0.f : vr[i].y);
+        odd |= bx || by;
+      }
+      any_odd |= __builtin_amdgcn_ballot_w64(odd) != 0;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float m_new = fmaxf(mc, mx * cl);
+    const float ref = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(mc - ref);
+    float rs = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], cl, -ref));
+      rs += s[i];
+    }
+    l = l * alpha + rs;  // per half-wave; the halves are summed at the end
+    mc = m_new;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[j][i] *= alpha;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[i].x, s[i], o[0], 0, 0, 0);
+      o[1] = __builtin_amdgcn_mfma_f32_32x32x2f32(vr[i].y, s[i], o[1], 0, 0, 0);
+    }
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if (hf == 0) {
+    red_m[kw][r32] = mc;
+    red_l[kw][r32] = l;
+  }
+  if (lane == 0) lds.odd[kw] = any_odd;
+  __syncthreads();
+  any_odd = false;
+#pragma unroll
+  for (int v = 0; v < KW; ++v) any_odd |= lds.odd[v] != 0;
+  float M = red_m[0][r32];
+#pragma unroll
+  for (int v = 1; v < KW; ++v) M = fmaxf(M, red_m[v][r32]);
+  const float f = mc == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - M);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[j][i] *= f;
+  if (any_odd && kw == 0) {
+    const int limits[1] = {limit};
+    const int g = lds.piece.g;
+    add_odd(keys, rows, [&](int id, int k, int i) { return src.value(rows, Vg, g, id, k, i); },
+            max(32 * keys.t0, keys.whole & -32), min(32 * keys.t1, keys.end), ow, limits,
+            [&](int i) { return 2 * (8 * (i >> 2 & 3) + 4 * hf + (i & 3)) + (i >> 4); });
+  }
+#pragma unroll
+  for (int gi = 0; gi < 4; ++gi) {
+    float *dst = kl + r32 * KP + 2 * (8 * gi + 4 * hf);
+    *(float4 *)dst = make_float4(o[0][4 * gi], o[1][4 * gi], o[0][4 * gi + 1], o[1][4 * gi + 1]);
+    *(float4 *)(dst + 4) = make_float4(o[0][4 * gi + 2], o[1][4 * gi + 2], o[0][4 * gi + 3], o[1][4 * gi + 3]);
+  }
+  __syncthreads();
+  constexpr int NV = HD / (2 * KW);
+  finish_piece<float, R, 64 * KW>(p, lds.piece, &lds.last_in, [&](int row, int d0, float (&acc)[NV]) __attribute__((always_inline)) {
+    float Mr = red_m[0][row];
+#pragma unroll
+    for (int v = 1; v < KW; ++v) Mr = fmaxf(Mr, red_m[v][row]);
+    const float Mu = Mr == -INFINITY ? 0.f : Mr;
+    float L = 0.f;
+#pragma unroll
+    for (int v = 0; v < KW; ++v) L += red_l[v][row] * __builtin_amdgcn_exp2f(red_m[v][row] - Mu);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; i += 4)
+#pragma unroll
+      for (int v = 0; v < KW; ++v) {
+        const float4 x = *(const float4 *)(smem + v * TILE + row * KP + d0 + i);
+        acc[i] += x.x; acc[i + 1] += x.y; acc[i + 2] += x.z; acc[i + 3] += x.w;
+      }
+    return make_float2(Mr, L);
+  });
 }
 
 }  // namespace

@@ -287,12 +287,12 @@ __global__ __launch_bounds__(256) void paged_q8_read_kernel(Q8ReadParams p) {
 }
 
 // --------------------------------------------------------------- attention
-// The bf16 cache's kernels over codes: eight elements become bf16 in four
+// The other caches' kernels over codes: eight elements become bf16 in four
 // instructions, their scale an operand, where the bf16 cache's are stored to LDS
-// (prefill) or where the products' operands are read from it (decode).
-struct E4m3Pages {
+// (prefill) or where the products' operands are read from it (decode); and four
+// elements fp32 in two for queries in fp32.
+struct E4m3Scales {
   typedef uint8_t T;
-  typedef u32x2 Raw;
   static constexpr bool kScaled = true;
   const uint8_t *ks, *vs;
   int64_t page, head;
@@ -302,6 +302,13 @@ struct E4m3Pages {
     return base[(rows.there(id) ? id : 0) * page + ((k & rows.slot_mask) >> 4)];
   }
   __device__ __forceinline__ int scale_bits(int byte) const { return min(max(byte, kLow), kHigh) << 23; }
+  __device__ __forceinline__ float value(const PageRows &rows, const char *Vg, int g, int id, int k, int lane) const {
+    const uint8_t code = ((const uint8_t *)Vg + rows.at(id, k))[lane];
+    return two_values<false>(code, scale_of(scale(scales(g, true), rows, id, k)))[0];
+  }
+};
+struct E4m3Pages : E4m3Scales {  // as bf16
+  typedef u32x2 Raw;
   __device__ __forceinline__ u32x4 bf16(uint32_t lo, uint32_t hi, float scale) const {
     u32x4 y;
     y[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
@@ -310,12 +317,22 @@ struct E4m3Pages {
     y[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
     return y;
   }
-  __device__ __forceinline__ u32x4 bf16(Raw x, int bits) const { return bf16(x[0], x[1], __builtin_bit_cast(float, bits)); }
-  __device__ __forceinline__ float value(const PageRows &rows, const char *Vg, int g, int id, int k, int lane) const {
-    const uint8_t code = ((const uint8_t *)Vg + rows.at(id, k))[lane];
-    return two_values<false>(code, scale_of(scale(scales(g, true), rows, id, k)))[0];
+  __device__ __forceinline__ u32x4 piece(Raw x, int bits) const { return bf16(x[0], x[1], __builtin_bit_cast(float, bits)); }
+};
+struct E4m3PagesF32 : E4m3Scales {  // as fp32
+  typedef uint32_t Raw;
+  typedef uint16_t Pair;
+  __device__ __forceinline__ u32x4 piece(Raw x, int bits) const {
+    const float scale = __builtin_bit_cast(float, bits);
+    const f32x2 a = two_values<false>(x, scale), b = two_values<true>(x, scale);
+    return u32x4{__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(b[0]), __float_as_uint(b[1])};
+  }
+  __device__ __forceinline__ float2 pair(Pair x, int bits) const {
+    const f32x2 a = two_values<false>(x, __builtin_bit_cast(float, bits));
+    return make_float2(a[0], a[1]);
   }
 };
+
 // ------------------------------------------------------------------ decode
 // The batch's tiles of 64 keys, sequences in order, are dealt in equal shares to the
 // workgroups of a column (a KV head, or up to 16 of its query heads).  A
@@ -777,6 +794,16 @@ __global__ __launch_bounds__(64 * HW * KW, OCC) void paged_q8_prefill_kernel(Pre
   __shared__ __attribute__((aligned(16))) PrefillLds<HW, KW> lds;
   prefill_bf16_body<HW, KW>(p, lds, blockIdx.x, src);
 }
+// Queries in fp32: the fp32 cache's kernels, whose time the matrix cores' fp32 rate sets.
+__global__ __launch_bounds__(256) void paged_q8_decode_f32_kernel(DecodeParams p, E4m3PagesF32 src) {
+  __shared__ __attribute__((aligned(16))) DecodeLds<float> lds;
+  decode_body<float>(p, lds, blockIdx.x, src);
+}
+template <int KW>
+__global__ __launch_bounds__(64 * KW, 2) void paged_q8_prefill_f32_kernel(PrefillParams p, E4m3PagesF32 src) {
+  __shared__ __attribute__((aligned(16))) PrefillLdsF32<KW> lds;
+  prefill_f32_body<KW>(p, lds, blockIdx.x, src);
+}
 __global__ __launch_bounds__(256, 2) void paged_q8_prefill_pipe_kernel(PrefillParams p, E4m3Pages src) {
   __shared__ __attribute__((aligned(16))) PipeLds lds;
   prefill_pipe_body(p, lds, blockIdx.x, src);
@@ -804,7 +831,7 @@ int check_q8(const std::string &op, const bn_paged_q8 *kv, Q8 *s) {
   return BN_OK;
 }
 
-int launch_decode(const AttnParams &a, const E4m3Pages &src, void *ws, hipStream_t s) {
+int launch_decode(const AttnParams &a, int dtype, const E4m3Scales &scales, void *ws, hipStream_t s) {
   const DecodePlan d = plan_decode(a.c.batch, a.n_heads, a.c.n_kv_heads);
   DecodeParams p;
   p.a = a;
@@ -815,14 +842,15 @@ int launch_decode(const AttnParams &a, const E4m3Pages &src, void *ws, hipStream
   p.k0 = 0;
   p.parts = nullptr;
   p.cuts = nullptr;
-  hipLaunchKernelGGL(paged_q8_decode_kernel, dim3((unsigned)(d.bins * d.columns)),
-                     dim3(64 * kWaves), 0, s, p, src);
+  const dim3 grid((unsigned)(d.bins * d.columns));
+  if (dtype == BN_F32) hipLaunchKernelGGL(paged_q8_decode_f32_kernel, grid, dim3(256), 0, s, p, E4m3PagesF32{scales});
+  else hipLaunchKernelGGL(paged_q8_decode_kernel, grid, dim3(64 * kWaves), 0, s, p, E4m3Pages{scales});
   BN_LAUNCH_CHECK();
   return BN_OK;
 }
 
-int launch_prefill(const AttnParams &a, const E4m3Pages &src, void *ws, hipStream_t s) {
-  const PrefillPlan d = plan_prefill(BN_BF16, a.c.batch, a.n_rows, a.n_heads, a.c.n_kv_heads, a.c.cap);
+int launch_prefill(const AttnParams &a, int dtype, const E4m3Scales &scales, void *ws, hipStream_t s) {
+  const PrefillPlan d = plan_prefill(dtype, a.c.batch, a.n_rows, a.n_heads, a.c.n_kv_heads, a.c.cap);
   PrefillParams p;
   p.a = a;
   p.ws = (float *)ws;
@@ -833,7 +861,12 @@ int launch_prefill(const AttnParams &a, const E4m3Pages &src, void *ws, hipStrea
   p.pieces = (int)d.pieces;
   p.prefix_parts = 0;
   const dim3 grid((unsigned)d.groups);
-  if (d.hw == 8) {
+  const E4m3Pages src{scales};
+  const E4m3PagesF32 src32{scales};
+  if (dtype == BN_F32) {
+    if (d.kw == 4) hipLaunchKernelGGL(paged_q8_prefill_f32_kernel<4>, grid, dim3(256), 0, s, p, src32);
+    else hipLaunchKernelGGL(paged_q8_prefill_f32_kernel<2>, grid, dim3(128), 0, s, p, src32);
+  } else if (d.hw == 8) {
     hipLaunchKernelGGL(paged_q8_prefill_pipe_kernel, grid, dim3(256), 0, s, p, src);
   } else if (d.hw == 4) {
     if (d.kw == 2) hipLaunchKernelGGL((paged_q8_prefill_kernel<4, 2, 4>), grid, dim3(512), 0, s, p, src);
@@ -857,14 +890,14 @@ int attention_q8(const char *name, const bn_paged_q8 *kv, int dtype, const void 
   if (st || (st = check_heads(op, n_heads, kv->n_kv_heads, n_rows)) ||
       (st = check_starts(op, starts, n_rows, kv->batch)))
     return st;
-  if (dtype != BN_BF16) return fail(BN_ERR_UNSUPPORTED, op + ": dtype must be BF16");
+  if (dtype != BN_F32 && dtype != BN_BF16) return fail(BN_ERR_UNSUPPORTED, op + ": dtype must be F32 or BF16");
   if (!(scale > 0.f) || !std::isfinite(scale))
     return fail(BN_ERR_INVALID_ARG, op + ": scale must be positive and finite");
   if (n_rows == 0 || kv->batch == 0) return BN_OK;
   if ((st = check_rows(op, "q", q, n_rows, n_heads, q_rs, dtype)) ||
       (st = check_rows(op, "o", o, n_rows, n_heads, o_rs, dtype)))
     return st;
-  if (starts && prefill_threads(BN_BF16, kv->batch, n_rows, n_heads, kv->n_kv_heads, c.c.cap) >= (int64_t)1 << 32)
+  if (starts && prefill_threads(dtype, kv->batch, n_rows, n_heads, kv->n_kv_heads, c.c.cap) >= (int64_t)1 << 32)
     return fail(BN_ERR_UNSUPPORTED, op + ": too many rows and sequences for one launch (2^32 threads)");
   const size_t need = bn_paged_q8_workspace_size(kv, n_heads, n_rows);
   if (workspace && workspace_bytes < need)
@@ -882,11 +915,11 @@ int attention_q8(const char *name, const bn_paged_q8 *kv, int dtype, const void 
   p.cl = scale * kLog2e;
   p.prefix_pages = nullptr;
   p.prefix_len = 0;
-  const E4m3Pages src{c.ks, c.vs, c.scale_page, c.scale_head};
+  const E4m3Scales scales{c.ks, c.vs, c.scale_page, c.scale_head};
   Workspace ws;
   if ((st = ws.take(workspace, need, stream))) return st;
   hipStream_t s = as_stream(stream);
-  return ws.release(starts ? launch_prefill(p, src, ws.p, s) : launch_decode(p, src, ws.p, s));
+  return ws.release(starts ? launch_prefill(p, dtype, scales, ws.p, s) : launch_decode(p, dtype, scales, ws.p, s));
 }
 
 }  // namespace
@@ -972,8 +1005,12 @@ size_t bn_paged_q8_workspace_size(const bn_paged_q8 *cache, int n_heads, int n_r
       check_heads("", n_heads, cache->n_kv_heads, n_rows))
     return 0;
   const DecodePlan d = plan_decode(cache->batch, n_heads, cache->n_kv_heads);
-  const PrefillPlan f = plan_prefill(BN_BF16, cache->batch, n_rows, n_heads, cache->n_kv_heads, s.c.cap, true);
-  return std::max(d.records + d.words, f.records + f.words);
+  size_t need = d.records + d.words;  // (for either type)
+  for (int dtype : {BN_F32, BN_BF16}) {
+    const PrefillPlan f = plan_prefill(dtype, cache->batch, n_rows, n_heads, cache->n_kv_heads, s.c.cap, true);
+    need = std::max(need, f.records + f.words);
+  }
+  return need;
 }
 
 int bn_paged_q8_decode(const bn_paged_q8 *cache, int dtype, const void *q, void *o, int n_heads,

@@ -650,8 +650,10 @@ int bn_paged_q8_read(const bn_paged_q8 *cache, int dtype, void *k, void *v,
                      const int32_t *row_starts, int n_rows, int64_t k_row_stride,
                      int64_t v_row_stride, void *stream);
 
-/* bn_paged_workspace_size, bn_paged_decode and bn_paged_prefill over such a
- * cache.  dtype: that of q and o, BN_BF16. */
+/* bn_paged_workspace_size (its workspace does for either dtype), bn_paged_decode and
+ * bn_paged_prefill over such a cache.  dtype: that of q and o, BN_F32 or BN_BF16; products
+ * and probabilities are of that type too, sums and softmax statistics fp32, and
+ * everything that is said there of bf16 and fp32 calls holds. */
 size_t bn_paged_q8_workspace_size(const bn_paged_q8 *cache, int n_heads, int n_rows);
 int bn_paged_q8_decode(const bn_paged_q8 *cache, int dtype, const void *q, void *o,
                        int n_heads, int64_t q_row_stride, int64_t o_row_stride,

@@ -1,6 +1,6 @@
 """Inputs and the plain 64-bit form of the 8-bit paged cache's operators, for their tests.
 
-Attention: the cache's values are bf16 numbers, so paged_util's tolerances for bf16 caches are these.
+Attention: the cache's values are bf16 numbers, so paged_util's tolerances hold, those of the queries' type.
 Rounding to the cache: a value is off by at most half a step of e4m3 (2^-4 of itself, 2^-10 of the
 scale below 2^-6 of it) and by what the 32-bit arithmetic before it was off.
 """
@@ -64,8 +64,9 @@ class Case8(Case):
     """A case whose cache is in 8 bits: k, v are its values (bf16 exactly); places that no visible key
     has hold NaN codes, and blocks without one scales of any byte."""
 
-    def __init__(self, lens, Hkv=2, page=16, layout=True, seed=0, nan=True, spread=1.0, **kw):
+    def __init__(self, lens, Hkv=2, page=16, layout=True, seed=0, nan=True, spread=1.0, dtype="bf16", **kw):
         super().__init__("bf16", lens, Hkv, page, layout, seed=seed, nan=False, **kw)
+        self.dtype = dtype                                # that of queries and outputs
         r = np.random.default_rng(seed + 1000)
         blocks = page // BLOCK
         seen = np.zeros((self.n_pages, page), bool)

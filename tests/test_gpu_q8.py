@@ -348,13 +348,18 @@ DECODES = [
 ]
 
 
+DTYPES = pytest.mark.parametrize("dtype", ["bf16", "f32"])
+
+
+@DTYPES
 @pytest.mark.parametrize("case", DECODES, ids=lambda c: f"{len(c[0])}x{max(c[0])}-{c[1]}-{c[2]}-p{c[3]}-{c[4]}-d{len(c[5])}")
-def test_decode(case):
+def test_decode(case, dtype):
     lens, Hkv, H, page, layout, drop = case
-    print("decode", case, flush=True)
+    print("decode", case, dtype, flush=True)
     big = max(lens) > 10 ** 6
-    c = Case8(lens, Hkv, page, layout, drop=drop, seed=H, max_pages=4 if big else None, junk=2 ** 31 - 1, pad_table=5)
-    q = rows_of("bf16", len(lens), H, 1)
+    c = Case8(lens, Hkv, page, layout, drop=drop, seed=H, max_pages=4 if big else None, junk=2 ** 31 - 1, pad_table=5,
+              dtype=dtype)
+    q = rows_of(dtype, len(lens), H, 1)
     ref, tol = attention64(c, q, [1] * len(lens))
     cache = c.cuda(B)
     qd, _ = wide(q.cuda(), 32)
@@ -369,35 +374,40 @@ def test_decode(case):
         assert torch.equal(bits(o2), bits(o)), "a second call differs"
 
 
-@pytest.mark.parametrize("lens", [[20011], [9000, 1, 0, 33], [5000, 40, 7000, 1234, 4000]],
-                         ids=lambda x: "-".join(map(str, x)))
-def test_decode_long(lens):
+@DTYPES
+@pytest.mark.parametrize("lens,Hkv,H", [([20011], 2, 8), ([9000, 1, 0, 33], 2, 8), ([5000, 40, 7000, 1234, 4000], 2, 8),
+                                        ([12000, 700], 1, 1), ([12000, 700, 3000], 1, 5), ([7000, 9000], 1, 12),
+                                        ([5000] * 3, 3, 45)], ids=str)
+def test_decode_long(lens, Hkv, H, dtype):
     """Caches cut over many workgroups."""
-    print("decode long", lens, flush=True)
-    c = Case8(lens, 2, 64, True, drop=[(0, 17)], seed=3)
-    q = rows_of("bf16", len(lens), 8, 5)
+    print("decode long", lens, Hkv, H, dtype, flush=True)
+    c = Case8(lens, Hkv, 64, True, drop=[(0, 17)], seed=3, dtype=dtype)
+    q = rows_of(dtype, len(lens), H, 5)
     ref, tol = attention64(c, q, [1] * len(lens))
     cache = c.cuda(B)
-    ws = B.paged_q8_workspace(cache, 8, len(lens))
+    ws = B.paged_q8_workspace(cache, H, len(lens))
     for _ in range(2):
         check(host(B.paged_q8_decode(q.cuda(), cache, scale=0.125, workspace=ws)), ref, tol, "decode")
 
 
-def test_decode_many_sequences():
-    lens = [int(x) for x in np.random.default_rng(0).integers(0, 90, 1300)]
-    lens[700] = 3000
-    c = Case8(lens, 2, 16, True, seed=1)
-    q = rows_of("bf16", len(lens), 4, 2)
+@pytest.mark.parametrize("n,H,dtype", [(1300, 4, "bf16"), (1300, 4, "f32"), (4000, 1, "bf16"), (2500, 32, "bf16")])
+def test_decode_many_sequences(n, H, dtype):
+    """More sequences than threads, and more in a share than its list and its places hold."""
+    lens = [int(x) for x in np.random.default_rng(0).integers(0, 90, n)]
+    lens[700], lens[900:1000] = 3000, [0] * 100
+    c = Case8(lens, 2 if H > 1 else 1, 16, True, seed=1, dtype=dtype)
+    q = rows_of(dtype, len(lens), H, 2)
     ref, tol = attention64(c, q, [1] * len(lens))
     check(host(B.paged_q8_decode(q.cuda(), c.cuda(B), scale=0.125)), ref, tol, "decode")
 
 
+@DTYPES
 @pytest.mark.parametrize("call", ["decode", "prefill"])
-def test_extreme_scores(call):
+def test_extreme_scores(call, dtype):
     """Scores far apart, so that the largest arrives late, and scales at both ends of their range."""
     lens = [200, 131, 97]
-    c = Case8(lens, 1, 32, True, seed=8, spread=6.0)
-    q = (40 * rows_of("bf16", 3, 4, 1).float()).to(torch.bfloat16)
+    c = Case8(lens, 1, 32, True, seed=8, spread=6.0, dtype=dtype)
+    q = (40 * rows_of(dtype, 3, 4, 1).float()).to(TD[dtype])
     ref, tol = attention64(c, q, [1] * 3)
     cache = c.cuda(B)
     st = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda")
@@ -405,7 +415,7 @@ def test_extreme_scores(call):
         B.paged_q8_prefill(q.cuda(), cache, st, scale=0.125)
     check(host(o), ref, tol, call)
     for byte, x in ((LOW, 2.0 ** -117), (HIGH - 20, 2.0 ** 100)):
-        c = Case8([70], 1, 32, True, seed=9, nan=False, spread=0.0)
+        c = Case8([70], 1, 32, True, seed=9, nan=False, spread=0.0, dtype=dtype)
         c.bytes["v"][:] = byte
         c.v = torch.from_numpy(TABLE[c.codes["v"]] * x)
         ref, tol = attention64(c, q[:1], [1])
@@ -429,14 +439,15 @@ PREFILLS = [
 ]
 
 
+@DTYPES
 @pytest.mark.parametrize("case", PREFILLS, ids=lambda c: f"{len(c[0])}x{max(c[0])}-{max(c[1])}-{c[2]}-{c[3]}-p{c[4]}-{c[5]}-d{len(c[6])}")
-def test_prefill(case):
+def test_prefill(case, dtype):
     lens, rows, Hkv, H, page, layout, drop, pad = case
-    print("prefill", case, flush=True)
+    print("prefill", case, dtype, flush=True)
     big = max(lens) > 10 ** 6
-    c = Case8(lens, Hkv, page, layout, drop=drop, seed=H, max_pages=4 if big else None, junk=-5, pad_table=2)
+    c = Case8(lens, Hkv, page, layout, drop=drop, seed=H, max_pages=4 if big else None, junk=-5, pad_table=2, dtype=dtype)
     n = sum(rows) + 2 * pad
-    q = rows_of("bf16", n, H, 1)
+    q = rows_of(dtype, n, H, 1)
     ref, tol = attention64(c, q, rows, pad)
     cache = c.cuda(B)
     qd, _ = wide(q.cuda(), 32)
@@ -467,12 +478,13 @@ LARGE = [
 ]
 
 
+@DTYPES
 @pytest.mark.parametrize("case", LARGE, ids=lambda c: f"{'-'.join(map(str, c[0]))}-{'-'.join(map(str, c[1]))}-{c[2]}-{c[3]}-p{c[4]}-{c[5]}")
-def test_prefill_large(case):
+def test_prefill_large(case, dtype):
     lens, rows, Hkv, H, page, layout = case
-    print("prefill large", case, flush=True)
-    c = Case8(lens, Hkv, page, layout, seed=1, drop=[(0, 20)])
-    q = rows_of("bf16", sum(rows), H, 4).cuda()
+    print("prefill large", case, dtype, flush=True)
+    c = Case8(lens, Hkv, page, layout, seed=1, drop=[(0, 20)], dtype=dtype)
+    q = rows_of(dtype, sum(rows), H, 4).cuda()
     cache = c.cuda(B)
     ref, tol = attention64_large(c, q, rows)
     st = torch.from_numpy(starts_of(rows)).cuda()
@@ -484,14 +496,15 @@ def test_prefill_large(case):
         assert torch.isfinite(o).all() and (off <= 0).all(), f"{int((off > 0).sum())} past the tolerance, by {off.max():.2e}"
 
 
+@DTYPES
 @pytest.mark.parametrize("rows,lens", [([50], [70]), ([3, 3, 3], [40, 100, 20]), ([700], [900]), ([2100], [2200]),
                                        ([4200], [17000])], ids=str)
-def test_a_hidden_nan_stays_hidden(rows, lens):
+def test_a_hidden_nan_stays_hidden(rows, lens, dtype):
     """NaN values and keys of later positions reach the rows that see them and no other."""
     Hkv, H = 1, 8
-    c = Case8(lens, Hkv, 64, True, seed=6)
+    c = Case8(lens, Hkv, 64, True, seed=6, dtype=dtype)
     cache = c.cuda(B)
-    q = rows_of("bf16", sum(rows), H, 4).cuda()
+    q = rows_of(dtype, sum(rows), H, 4).cuda()
     st = torch.from_numpy(starts_of(rows)).cuda()
     ref, tol = attention64_large(c, q, rows)
     j = lens[0] - rows[0] // 2                       # a key that half of the first sequence's rows see
@@ -646,7 +659,7 @@ def test_a_server_run(dtype, page, layout):
     attention call against 64 bits over what the cache held, and the cache's values against the rows."""
     Hkv, H, prompts, steps = 2, 8, [37, 5, 130], 21
     r = np.random.default_rng(1)
-    c = Case8([n + steps for n in prompts], Hkv, page, layout, seed=7)
+    c = Case8([n + steps for n in prompts], Hkv, page, layout, seed=7, dtype=dtype)
     for x in c.codes.values():
         x[:] = 127                                   # nothing is there yet
     for x in c.bytes.values():
@@ -672,7 +685,7 @@ def test_a_server_run(dtype, page, layout):
                 kk = rotate64(normed64(k[at + i].double().numpy(), w[1].double().numpy(), 1e-5), lens[b] - m + i, 1e4)
                 kept[b].append((kk, v[at + i].double().numpy()))
             at += m
-        qb = q_rot.to(torch.bfloat16)
+        qb = q_rot
         o = B.paged_q8_prefill(qb, cache, st, scale=0.125, workspace=ws) if turn == 0 else \
             B.paged_q8_decode(qb, cache, scale=0.125, workspace=ws)
         # what the cache holds now, read back, is what the attention is measured by

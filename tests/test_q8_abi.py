@@ -241,8 +241,9 @@ def test_python_wrappers_refuse():
     kn = q[:, :2].contiguous()
     for call, match in (
             (lambda: B.paged_q8_decode(q[:2], kv), "paged_q8_decode: q"),
-            (lambda: B.paged_q8_decode(q.float(), kv), "bfloat16"),
+            (lambda: B.paged_q8_decode(q.half(), kv), "float32 or bfloat16"),
             (lambda: B.paged_q8_decode(q, kv, o=q[:, :4]), "paged_q8_decode: o"),
+            (lambda: B.paged_q8_decode(q, kv, o=q.float()), "paged_q8_decode: o"),
             (lambda: B.paged_q8_prefill(torch.zeros((7, 8, 64), dtype=torch.bfloat16), kv), "one row per sequence"),
             (lambda: B.paged_q8_prefill(q, kv, torch.zeros(3, dtype=torch.int32)), "row_starts"),
             (lambda: B.paged_q8_append(kv, q, kn), "paged_q8_append: k"),
