@@ -404,28 +404,32 @@ __device__ __forceinline__ void decode_body(const DecodeParams &p, DecodeLds<T> 
     if constexpr (Src::kScaled) y.scale = src.scale(sg, page_rows, ids[0], key0);
   };
   T *const kt = lds.k[wave], *const vt = lds.v[wave];
-  auto store_rows = [&](const Rows &x, bool masked) __attribute__((always_inline)) {
-    int bits = 0;
-    if constexpr (Src::kScaled) bits = src.scale_bits(x.scale);
-    struct {
-      u32x4 k[4], v[4];
-    } y;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      y.k[r] = src.piece(x.k[r], __builtin_amdgcn_readlane(bits, 0));
-      y.v[r] = src.piece(x.v[r], __builtin_amdgcn_readlane(bits, 1));
-    }
+  auto put_rows = [&](u32x4 (&k)[4], u32x4 (&v)[4], const Rows &y, bool masked) __attribute__((always_inline)) {
     if (masked) {  // no key: zeros, whatever lies there (0 times an infinite value is none)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = crow + RPI * r;
-        if (row < x.lo || row >= x.hi || !(x.pages >> r & 1)) y.k[r] = y.v[r] = u32x4{0, 0, 0, 0};
+        if (row < y.lo || row >= y.hi || !(y.pages >> r & 1)) k[r] = v[r] = u32x4{0, 0, 0, 0};
       }
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) *(u32x4 *)(kt + (crow + RPI * r) * P + ccol) = y.k[r];
+    for (int r = 0; r < 4; ++r) *(u32x4 *)(kt + (crow + RPI * r) * P + ccol) = k[r];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) *(u32x4 *)(vt + (crow + RPI * r) * P + ccol) = y.v[r];
+    for (int r = 0; r < 4; ++r) *(u32x4 *)(vt + (crow + RPI * r) * P + ccol) = v[r];
+  };
+  auto store_rows = [&](Rows &y, bool masked) __attribute__((always_inline)) {
+    if constexpr (Src::kScaled) {
+      const int bits = src.scale_bits(y.scale);
+      u32x4 k[4], v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        k[r] = src.piece(y.k[r], __builtin_amdgcn_readlane(bits, 0));
+        v[r] = src.piece(y.v[r], __builtin_amdgcn_readlane(bits, 1));
+      }
+      put_rows(k, v, y, masked);
+    } else {
+      put_rows(y.k, y.v, y, masked);
+    }
   };
   // queries: lane holds head l16's elements 8 grp + 32 t .. +7 (bf16), 16 grp .. +15 (fp32)
   u32x4 q[NQ], qn[NQ];
