@@ -32,17 +32,22 @@ struct Raw8 {  // as loaded
     return y;
   }
 };
-template <typename T>
+template <typename T, bool NT = false>  // NT: past the caches' keeping
 __device__ __forceinline__ void store8(T *p, const Eight &y) {
-  if constexpr (sizeof(T) == 2) {
-    u32x4 r;
+  u32x4 r[sizeof(T) / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r[i] = (uint32_t)f32_to_bf16(y.x[2 * i]) | ((uint32_t)f32_to_bf16(y.x[2 * i + 1]) << 16);
-    *(u32x4 *)p = r;
-  } else {
-    *(float4 *)p = make_float4(y.x[0], y.x[1], y.x[2], y.x[3]);
-    *(float4 *)(p + 4) = make_float4(y.x[4], y.x[5], y.x[6], y.x[7]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      r[0][i] = (uint32_t)f32_to_bf16(y.x[2 * i]) | ((uint32_t)f32_to_bf16(y.x[2 * i + 1]) << 16);
+    } else {
+      r[0][i] = __float_as_uint(y.x[i]);
+      r[sizeof(T) / 2 - 1][i] = __float_as_uint(y.x[4 + i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) {
+    if constexpr (NT) __builtin_nontemporal_store(r[i], (u32x4 *)p + i);
+    else ((u32x4 *)p)[i] = r[i];
   }
 }
 

@@ -260,7 +260,12 @@ struct Q8ReadParams {
   int64_t k_rs, v_rs;
   int n_rows;
 };
-template <typename T>
+// A unit a workgroup, its waves the block's KV heads, K and V, in turn.  Bound by memory: 2 x 40000..65536
+// keys of 4 heads 38 us, 4.9 TB/s read and written, a copy's rate.  NT: codes and rows past the caches'
+// keeping, for rows that the memory-side cache (256 MB) would not hold long: 131 MB of them 44.3 -> 40.0
+// us, and a sum of keys and values behind it 73.1 -> 72.0 with them; of 65 MB 23.4 -> 22.4, but with that
+// sum 37.8 -> 39.9.
+template <typename T, bool NT>
 __global__ __launch_bounds__(256) void paged_q8_read_kernel(Q8ReadParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Paged &c = p.s.c;
@@ -280,8 +285,9 @@ __global__ __launch_bounds__(256) void paged_q8_read_kernel(Q8ReadParams p) {
       const int row = lane / 8 + 8 * n;
       if (row >= u.rows) continue;
       Eight x{};
-      if (at.codes >= 0) x = values(*(const u32x2 *)(codes + row * c.row_stride + e), scale);
-      store8(out + (int64_t)(u.row0 + row) * (is_v ? p.v_rs : p.k_rs) + g * HD + e, x);
+      const u32x2 *const from = (const u32x2 *)(codes + row * c.row_stride + e);
+      if (at.codes >= 0) x = values(NT ? __builtin_nontemporal_load(from) : *from, scale);
+      store8<T, NT>(out + (int64_t)(u.row0 + row) * (is_v ? p.v_rs : p.k_rs) + g * HD + e, x);
     }
   }
 }
@@ -993,8 +999,14 @@ int bn_paged_q8_read(const bn_paged_q8 *cache, int dtype, void *k, void *v, cons
   p.n_rows = n_rows;
   hipStream_t s = as_stream(stream);
   const dim3 grid((unsigned)count_units(row_starts, n_rows, cache->batch)), block(256);
-  if (dtype == BN_BF16) hipLaunchKernelGGL(paged_q8_read_kernel<bf16_t>, grid, block, 0, s, p);
-  else hipLaunchKernelGGL(paged_q8_read_kernel<float>, grid, block, 0, s, p);
+  const int64_t bytes = (int64_t)n_rows * cache->n_kv_heads * HD * (dtype == BN_BF16 ? 2 : 4) * (!!k + !!v);
+  if (bytes > (3 << 25)) {
+    if (dtype == BN_BF16) hipLaunchKernelGGL((paged_q8_read_kernel<bf16_t, true>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((paged_q8_read_kernel<float, true>), grid, block, 0, s, p);
+  } else {
+    if (dtype == BN_BF16) hipLaunchKernelGGL((paged_q8_read_kernel<bf16_t, false>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((paged_q8_read_kernel<float, false>), grid, block, 0, s, p);
+  }
   BN_LAUNCH_CHECK();
   return BN_OK;
 }
