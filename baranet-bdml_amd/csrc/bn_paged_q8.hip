@@ -373,12 +373,26 @@ struct Q8DecodeLds {
   int sums[2][kWaves], rank0, last_in[2];
 };
 
+// ONCE: rows past the caches' keeping, where no other workgroup reads their lines: pages whose rows of a
+// KV head lie one behind the other (64 caches of 4096 keys 27.9 us, else 31.5); of token-major pages two
+// heads' rows share a line (64 caches of 512..4096 23.9 us, else 26.1; 33.4 on XCDs of their own).
+template <bool ONCE>
 __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodeParams p, E4m3Pages src) {
   __shared__ __attribute__((aligned(16))) Q8DecodeLds lds;
   const Paged &c = p.a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, grp = lane >> 4;
-  const int bin = blockIdx.x / p.columns, col = blockIdx.x - bin * p.columns;
+  // A share's columns go to one XCD (workgroups are dealt to the eight in turn): they read the same
+  // table entries, and of token-major pages the same 128-byte lines.
+  int bin, col;
+  if ((p.bins & 7) == 0) {
+    const int j = blockIdx.x >> 3, r = (int)((uint32_t)j / (uint32_t)p.columns);
+    col = j - r * p.columns;
+    bin = 8 * r + (blockIdx.x & 7);
+  } else {
+    bin = blockIdx.x / p.columns;
+    col = blockIdx.x - bin * p.columns;
+  }
   const int g = col / p.hblocks, hb = col - g * p.hblocks;
   const int rows = min(kMaxRows, p.a.group - kMaxRows * hb), head0 = g * p.a.group + kMaxRows * hb;
 
@@ -526,11 +540,12 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
         uint32_t o32 = off;
         asm volatile("" : "+v"(o32));  // a scalar base and this offset, not a sum of pointers kept in registers
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {  // streamed once: non-temporal
+        for (int r = 0; r < 4; ++r) {
           const uint64_t to_row = (uint32_t)__builtin_amdgcn_readlane(at_lo[r], j) |
                                   (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi[r], j) << 32;
-          x.k[r] = __builtin_nontemporal_load((const u32x4 *)(Kg + to_row + o32));
-          x.v[r] = __builtin_nontemporal_load((const u32x4 *)(Vg + to_row + o32));
+          const u32x4 *const kp = (const u32x4 *)(Kg + to_row + o32), *const vp = (const u32x4 *)(Vg + to_row + o32);
+          x.k[r] = ONCE ? __builtin_nontemporal_load(kp) : *kp;
+          x.v[r] = ONCE ? __builtin_nontemporal_load(vp) : *vp;
         }
       };
       u32x4 q[2], qn[2];  // head l16's elements 16 grp .. + 15
@@ -850,7 +865,8 @@ int launch_decode(const AttnParams &a, int dtype, const E4m3Scales &scales, void
   p.cuts = nullptr;
   const dim3 grid((unsigned)(d.bins * d.columns));
   if (dtype == BN_F32) hipLaunchKernelGGL(paged_q8_decode_f32_kernel, grid, dim3(256), 0, s, p, E4m3PagesF32{scales});
-  else hipLaunchKernelGGL(paged_q8_decode_kernel, grid, dim3(64 * kWaves), 0, s, p, E4m3Pages{scales});
+  else if (a.c.row_stride == HD) hipLaunchKernelGGL(paged_q8_decode_kernel<true>, grid, dim3(64 * kWaves), 0, s, p, E4m3Pages{scales});
+  else hipLaunchKernelGGL(paged_q8_decode_kernel<false>, grid, dim3(64 * kWaves), 0, s, p, E4m3Pages{scales});
   BN_LAUNCH_CHECK();
   return BN_OK;
 }

@@ -80,6 +80,35 @@ def test_read(dtype, page, layout, pad):
             assert (host(got)[b] == (getattr(c, name)[place[0], :, place[1]].numpy() if place else 0.0)).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_read_many_rows(dtype):
+    """More bytes than the caches keep (another kernel), ragged, with padding around."""
+    Hkv, page, n = 4, 64, 130000 if dtype == "bf16" else 70000
+    lens = [n - 3000, 2500, 777]
+    r = torch.Generator(device="cuda").manual_seed(3)
+    need = [-(-x // page) for x in lens]
+    order = torch.randperm(sum(need) + 3, generator=r, device="cuda").int()
+    table = torch.full((3, max(need)), -1, dtype=torch.int32, device="cuda")
+    for b, m in enumerate(need):
+        table[b, :m] = order[sum(need[:b]):sum(need[:b + 1])]
+    codes = [torch.randint(0, 127, (sum(need) + 3, Hkv, page, D), generator=r, device="cuda", dtype=torch.uint8) for _ in "kv"]
+    sc = [torch.randint(110, 140, (sum(need) + 3, Hkv, page // BLOCK), generator=r, device="cuda", dtype=torch.uint8) for _ in "kv"]
+    cache = B.PagedQ8(*codes, *sc, table, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    st = torch.from_numpy(starts_of(lens, 5)).cuda()
+    outs = [torch.full((sum(lens) + 12, Hkv, D), 7.0, dtype=TD[dtype], device="cuda") for _ in "kv"]
+    B.paged_q8_read(cache, st, k=outs[0], v=outs[1])
+    values = torch.from_numpy(TABLE).float().cuda()
+    for o, c, s in zip(outs, codes, sc):
+        at = 5
+        assert (o[:5] == 7.0).all() and (o[-7:] == 7.0).all()
+        for b, m in enumerate(lens):
+            j = torch.arange(m, device="cuda")
+            pg, sl = table[b, j // page].long(), j % page
+            want = torch.ldexp(values[c[pg, :, sl].long()], s[pg, :, sl // BLOCK].int()[..., None] - 127)
+            assert torch.equal(o[at:at + m].float(), want)
+            at += m
+
+
 # ------------------------------------------------------------------- append
 APPENDS = [
     # dtype, lens (after), new rows, Hkv, H, page, layout, theta, q: None / "out" / "in place", norms
