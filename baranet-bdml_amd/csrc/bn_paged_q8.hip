@@ -494,21 +494,23 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
       // lane l: the list's l-th sequence
       const int lb = lds.list_b[lane & (kListed - 1)], lfirst = lds.list_first[lane & (kListed - 1)],
                 llen = lds.list_len[lane & (kListed - 1)];
-      bool there = lane < kListed && lb >= 0;
-      const int lend = there ? lfirst + tiles_of(llen) : 0;
-      const int lstop = min(lend, end), lcount = there ? lstop - max(lfirst, at) : 0;
-      const int lparts = min(lcount, kWaves), lupto = wave_scan(lparts), lbefore = lupto - lparts;
-      there = there && lupto * rows <= kHoldParts;
+      // A wave takes a run of the list's tiles, so that sequence l and wave w meet in a staircase: each of
+      // their parts has place l + w, and LDS holds the parts of kHoldParts / rows - 7 sequences.
+      const bool there = lane < min(kListed, kHoldParts / rows - (kWaves - 1)) && lb >= 0;
+      const int lend = there ? lfirst + tiles_of(llen) : 0, lstop = min(lend, end);
       const int n_list = __builtin_popcountll(__builtin_amdgcn_ballot_w64(there));
       const int stop = __builtin_amdgcn_readlane(lstop, n_list - 1);
+      const int run = (int)((uint32_t)(stop - at + kWaves - 1) / kWaves);
+      const int lw0 = there ? (int)((uint32_t)(max(lfirst, at) - at) / (uint32_t)run) : 0;  // its first and last wave
+      const int lw1 = there ? (int)((uint32_t)(lstop - 1 - at) / (uint32_t)run) : 0;
 
-      // ---- the wave's tiles, at + wave + 8 i, looked up 64 at a time
-      const int n = stop - at > wave ? (stop - at - wave + kWaves - 1) / kWaves : 0;
+      // ---- the wave's tiles, looked up 64 at a time
+      const int mine = at + wave * run, n = max(min(run, stop - mine), 0);
       uint32_t at_lo[4], at_hi[4];  // byte offset of rows 16 r ..
       uint32_t kscales, vscales;    // bytes of rows 16 r ..
       int info, first_keys;         // place in the list | bits 8 ..: rows 16 r .. have memory; keys of the tile
       auto look_up = [&](int i0) __attribute__((always_inline)) {
-        const int pos = min(at + wave + kWaves * (i0 + lane), stop - 1);
+        const int pos = min(mine + i0 + lane, stop - 1);
         int place = 0;
         for (int l = 0; l < n_list - 1; ++l) place += pos >= __builtin_amdgcn_readlane(lstop, l);
         const int b = lds.list_b[place], len = lds.list_len[place], key0 = kTile * (pos - lds.list_first[place]);
@@ -669,10 +671,8 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
         if (ends) {
           sum += __shfl_xor(sum, 16, 64);
           sum += __shfl_xor(sum, 32, 64);
-          const int begin = max(__builtin_amdgcn_readlane(lfirst, place), at) - at;
-          const int parts0 = __builtin_amdgcn_readlane(lbefore, place);
           if (l16 < rows) {
-            float *const h = lds.hold + ((parts0 + ((wave - begin) & (kWaves - 1))) * rows + l16) * kHoldRow;
+            float *const h = lds.hold + ((place + wave) * rows + l16) * kHoldRow;
 #pragma unroll
             for (int j = 0; j < 4; ++j) *(f32x4 *)(h + 16 * j + 4 * grp) = o[j];
             if (grp == 0) *(float2 *)(h + HD) = make_float2(mc, sum);
@@ -685,11 +685,11 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
 #pragma unroll 1
       for (int u = wave; u < n_list * pairs; u += kWaves) {
         const int place = by_pairs(u), h = 2 * (u - place * pairs) + (lane >> 5), d = 2 * (lane & 31);
-        const int b = __builtin_amdgcn_readlane(lb, place), parts = __builtin_amdgcn_readlane(lparts, place);
+        const int b = __builtin_amdgcn_readlane(lb, place), w0 = __builtin_amdgcn_readlane(lw0, place);
+        const int parts = __builtin_amdgcn_readlane(lw1, place) - w0 + 1;
         const int first = __builtin_amdgcn_readlane(lfirst, place), last = __builtin_amdgcn_readlane(lend, place);
-        const int parts0 = __builtin_amdgcn_readlane(lbefore, place);
         if (h >= rows) continue;
-        const float *const r = lds.hold + (parts0 * rows + h) * kHoldRow;
+        const float *const r = lds.hold + ((place + w0) * rows + h) * kHoldRow;
         float2 ml[kWaves], y[kWaves];
         float M = -INFINITY, L = 0.f, A0 = 0.f, A1 = 0.f;
 #pragma unroll
