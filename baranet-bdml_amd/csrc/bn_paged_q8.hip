@@ -623,20 +623,16 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
             }
         }
         // The probabilities are taken against a reference that is the true running maximum only when it was
-        // last moved: it moves when a lane's weights against it pass 2^16 in sum (or are NaN).  They are
-        // rounded to bf16, the products' operands, off by at most 2^-8 each; the sum is of the same values.
-        bf16x8 pb[2];
-        float rs;
+        // last moved: it moves when a lane's weights against it pass 2^16 in sum (or are NaN).  They enter the
+        // products as two bf16 values each, the upper 16 bits and what is left of them (off by at most 2^-17
+        // together; rounded to one, 3 caches of up to 131072 keys were 0.0024 off 64 bits, not 0.0017).
+        float e[16], rs;
         auto weigh = [&](float ref) __attribute__((always_inline)) {
           rs = 0.f;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              pb[h][j] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * h + (j >> 2)][j & 3], cl, -ref));
-#pragma unroll
-            for (int j = 0; j < 8; j += 2)
-              rs = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{pb[h][j], pb[h][j + 1]}, bf16x2{(__bf16)1.f, (__bf16)1.f}, rs, false);
+          for (int j = 0; j < 16; ++j) {
+            e[j] = __builtin_amdgcn_exp2f(fmaf(s[j >> 2][j & 3], cl, -ref));
+            rs += e[j];
           }
         };
         weigh(mc);  // (no key yet: mc is -inf, and the sum +inf or NaN)
@@ -658,14 +654,24 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
         sum += rs;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          u32x4 hi;
+          bf16x8 lo;
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const uint32_t x = __float_as_uint(e[8 * h + j]), y = __float_as_uint(e[8 * h + j + 1]);
+            hi[j >> 1] = __builtin_amdgcn_perm(y, x, 0x07060302);
+            lo[j] = (__bf16)(e[8 * h + j] - __uint_as_float(x & 0xffff0000u));
+            lo[j + 1] = (__bf16)(e[8 * h + j + 1] - __uint_as_float(y & 0xffff0000u));
+          }
           // V^T: slot j of lane (grp, l16) is V[key 32 h + 8 grp + j][16 dt + l16]
           const uint8_t *const vp = vt + h * 2 * kRows16 + (8 * grp + (l16 >> 1)) * kPitch + (grp >> 1) * 64 + 8 * (l16 & 1);
           const float scale = __uint_as_float((vs >> (16 * h + 8 * (grp >> 1)) & 255u) << 23);
 #pragma unroll
           for (int dt = 0; dt < 4; ++dt) {
             const u32x2 y = lds_tr8(vp + 16 * dt);
-            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, src.bf16(y[0], y[1], scale)), pb[h],
-                                                            o[dt], 0, 0, 0);
+            const bf16x8 v = __builtin_bit_cast(bf16x8, src.bf16(y[0], y[1], scale));
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8, hi), o[dt], 0, 0, 0);
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo, o[dt], 0, 0, 0);
           }
         }
         if (ends) {
