@@ -150,7 +150,9 @@ struct Q8AppendParams {
 // the first task's rows are on their way; then its waves take the block's KV heads, K
 // and V, in turn, 16 rows of 64 elements in two pieces of eight a lane: norm,
 // rotation, the block's largest element, the scale, the codes.  The queries' pieces go
-// to all threads.
+// to all threads.  Bound by memory, VALU 68% busy: 4 x 2048 rows of 32 and 4 heads 19.4 us
+// under the profiler, 4.1 TB/s; 64 rows 5.2, launch and the chain row -> length -> table ->
+// scale.  (Four waves, every row loaded when its turn comes: 24 and 6.)
 constexpr int kAppendThreads = 512, kPieces = 4;
 template <typename T>
 __global__ __launch_bounds__(kAppendThreads) void paged_q8_append_kernel(Q8AppendParams p) {
@@ -343,14 +345,15 @@ struct E4m3PagesF32 : E4m3Scales {  // as fp32
 // The batch's tiles of 64 keys, sequences in order, are dealt in equal shares to the
 // workgroups of a column (a KV head, or up to 16 of its query heads).  A
 // workgroup finds the sequences of its share by a scan of the lengths, one thread a
-// run of them, and lists them in LDS; its eight waves take the listed tiles in turn,
-// each with the next one's rows on their way, leave their parts of each sequence
+// run of them, and lists them in LDS; its eight waves take a run of the listed tiles
+// each, with the next tile's rows on their way, leave their parts of each sequence
 // (reference, sum, accumulator) in LDS and add them up; then the next list, if the
-// share has more sequences than LDS holds parts of.  What lies where -- page
-// offsets, scales -- a wave looks up for 64 of its tiles at once, a tile a lane, so
-// that a step has only to read it from there: the loop's instructions, not the
-// bytes, are what bounds this kernel when they are many (650 a tile, with eight
-// waves a compute unit: 2.6 us a tile).
+// share has more sequences than LDS holds parts of.  A sequence cut between shares
+// leaves records, which the last of its pieces to arrive adds, in the order of the keys.
+// What lies where -- page offsets, scales -- a wave looks up for 64 of its tiles at
+// once, a tile a lane, so that a step has only to read it from there: with lookups and
+// the walk over sequences in every step (650 instructions a tile, four waves) the
+// instructions bounded the kernel, 31.9 us for 64 caches of 512..4096 keys.
 //
 // Per tile, with the query heads as columns of the products, as the bf16 cache's:
 //   S^T[key][head] = K . Q^T,  O^T[d][head] += V^T . P^T   (v_mfma_f32_16x16x32_bf16)
@@ -358,13 +361,19 @@ struct E4m3PagesF32 : E4m3Scales {  // as fp32
 // eight rows, both converted (exactly) where they are used, the scale an operand.  A
 // score tile's rows are keys 4 (u % 2) + 8 (row / 4) + row % 4 of its 32, so that a
 // lane's scores of two tiles are those of eight keys in a row, V's operand's order.
+//
+// Bound by memory, and for small calls by the chain lengths -> list -> table -> rows ->
+// parts -> records: 64 caches of 4096 keys (32 and 4 heads) 29 us, 4.6 TB/s; of 512..4096
+// 22.5, 3.5 TB/s, of which 6 are that chain and 3 the records; three of 34763 to 131072 31.5,
+// 4.0 TB/s; one of 640 9.4.  Four waves and two tiles each in flight: 31.5 and 41.8 us for the
+// second and third.  (Per tile the matrix cores are 6%, VALU 31%, LDS 26% busy.)
 constexpr int kWaves = 8, kTile = 64;
 constexpr int kListed = 32;                  // sequences of a list
 constexpr int kHoldParts = 256;              // rows of LDS for the waves' parts of sequences
 constexpr int kPitch = HD + 16;              // bytes of a row in LDS: b128 reads of 16 rows spread over the banks
 constexpr int kRows16 = 16 * kPitch + 64;    // sixteen rows, and 64 bytes so that rows 16 apart do too
 constexpr int kHoldRow = HD + 4;             // floats of a part's row: a record's, 16-byte aligned
-constexpr int kShareLeast = 8;               // tiles of a share at least: one a wave
+constexpr int kShareLeast = 8;               // tiles of a share at least: one a wave (1 cache of 16384 keys 13.8 us, with 4 tiles 17.6)
 constexpr int kMerged = 16;                  // records read at once
 struct Q8DecodeLds {
   uint8_t k[kWaves][4 * kRows16], v[kWaves][4 * kRows16];
