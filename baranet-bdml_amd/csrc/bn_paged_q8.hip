@@ -262,7 +262,7 @@ struct Q8ReadParams {
   int64_t k_rs, v_rs;
   int n_rows;
 };
-// A unit a workgroup, its waves the block's KV heads, K and V, in turn.  Bound by memory: 2 x 40000..65536
+// A unit a workgroup, its waves the block's KV heads, K and V, in turn.  Bound by memory: 55782 and 65536
 // keys of 4 heads 38 us, 4.9 TB/s read and written, a copy's rate.  NT: codes and rows past the caches'
 // keeping, for rows that the memory-side cache (256 MB) would not hold long: 131 MB of them 44.3 -> 40.0
 // us, and a sum of keys and values behind it 73.1 -> 72.0 with them; of 65 MB 23.4 -> 22.4, but with that

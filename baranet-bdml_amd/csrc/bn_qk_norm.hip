@@ -104,7 +104,7 @@ constexpr int kPairs = 2;  // pieces of rows and gradients of a thread on their 
 // one place of their heads, so it adds up eight elements of each weight's
 // gradient in registers; a workgroup's sums go to the workspace.  Bound by memory: 16384
 // bf16 rows of 32 and 4 heads 46 us, 4.9 TB/s (59 with one piece at once), and 4 for the sums'
-// launch; 1114 fp32 rows 12 and 2.
+// launch; 1504 fp32 rows 12 and 2.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void qk_norm_rope_backward_kernel(QkParams p, Turns<D> t) {
   constexpr int LANES = D / 8;
