@@ -561,8 +561,7 @@ int bn_paged_decode_shared(const bn_paged_kv *cache, const void *q, void *o,
  * k_out: [n_rows, n_kv_heads, head_dim]; k, k_out and k_weight NULL with
  * n_kv_heads 0: q alone.  Weights: head_dim elements.  dtype BN_F32 or BN_BF16 for
  * all of them; everything between is fp32.  positions: device int32 [n_rows]
- * (NULL: row r is at r), position_offset is added; positions at or past 2^31
- * or below -2^31 are not represented.  q_out may be q and k_out k (with the
+ * (NULL: row r is at r), position_offset is added (in 64 bits).  q_out may be q and k_out k (with the
  * same row stride); no other overlap.  head_dim: 16, 32, 64, 128 or 256; at most
  * 2^23 rows and 65535 heads; pointers and row strides multiples of 16 bytes. */
 int bn_qk_norm_rope(int dtype, const void *q, const void *k, const void *q_weight,
@@ -631,8 +630,9 @@ typedef struct bn_paged_q8 {
  * exponents: they change where they fall below 2^-6 of it).  A block is written anew
  * by a call that has its first row, whatever was there.  An infinite or NaN
  * element is stored as NaN and has no part in the scale; at scale 2^120 codes go up to 240.
- * Rows of two sequences that land in one block leave either's there, under
- * either's scale.  Otherwise as bn_paged_append. */
+ * Where one call writes a block twice (for two sequences, or because a page stands
+ * twice in a table) either's rows stay there, under either's scale.  Otherwise as
+ * bn_paged_append. */
 int bn_paged_q8_append(const bn_paged_q8 *cache, int dtype, const void *k,
                        const void *v, const void *q, void *q_out,
                        const int32_t *row_starts, int n_rows, int n_heads,
