@@ -384,7 +384,7 @@ int check_launch(const std::string &op, int dtype, int batch, const int32_t *sta
     const SharedPlan m = plan_shared(dtype, batch, n_heads, n_kv_heads, prefix_len);
     threads = std::max((m.d.bins * m.d.columns + m.n_pre + 16) * 256, (int64_t)batch * n_heads * (HD / 2) + 256);
   } else if (starts) {
-    threads = prefill_threads(dtype, batch, n_rows, n_heads, n_kv_heads, cap);
+    threads = prefill_threads(plan_prefill(dtype, batch, n_rows, n_heads, n_kv_heads, cap));
   }
   if (threads >= (int64_t)1 << 32)
     return fail(BN_ERR_UNSUPPORTED, op + ": too many rows and sequences for one launch (2^32 threads)");

@@ -172,8 +172,7 @@ inline DecodePlan plan_decode(int batch, int n_heads, int n_kv_heads) {
 }
 
 // The threads of a prefill's launch, which the runtime counts in 32 bits.
-inline int64_t prefill_threads(int dtype, int batch, int n_rows, int n_heads, int n_kv_heads, int cap) {
-  const PrefillPlan d = plan_prefill(dtype, batch, n_rows, n_heads, n_kv_heads, cap);
+inline int64_t prefill_threads(const PrefillPlan &d) {
   return d.groups * (d.hw == 8 ? 256 : 64 * d.hw * d.kw);
 }
 

@@ -251,7 +251,9 @@ struct PrefillPlan {
 };
 // most: not this call's plan but one whose workspace does for any call of at
 // most as many rows (with fewer rows a sequence the kernel may be another).
-inline PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv_heads, int cap, bool most = false) {
+// pipe_from: the units of 128 rows from which the pipelined kernel is taken.
+inline PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, int n_kv_heads, int cap, bool most = false,
+                                int pipe_from = 2048) {
   PrefillPlan d;
   const int64_t rows = (int64_t)n_rows * (n_heads / n_kv_heads);  // of a KV head
   const int64_t u128 = (rows / 128 + 1) * n_kv_heads, u32 = (rows / 32 + 1) * n_kv_heads;
@@ -259,7 +261,7 @@ inline PrefillPlan plan_prefill(int dtype, int n_seq, int n_rows, int n_heads, i
   if (dtype == BN_F32) {
     d.hw = 1;
     d.kw = u32 <= 1024 ? 4 : 2;  // (one prompt of 512 rows 23 us, with 2 waves a unit 30; four of 300 39 and 31)
-  } else if (far ? u128 < 1024 || long_rows || most : u128 >= 2048 && (long_rows || most)) {
+  } else if (far ? u128 < 1024 || long_rows || most : u128 >= pipe_from && (long_rows || most)) {
     d.hw = 8;
     d.kw = 1;
   } else if (u128 < 256) {

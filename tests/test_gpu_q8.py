@@ -504,6 +504,7 @@ LARGE = [
     ([6000], [4500], 4, 32, 64, True),
     ([20000], [300], 4, 32, 128, True),
     ([17000, 600], [1500, 600], 2, 16, 64, False),
+    ([900, 3300, 1100], [620, 3200, 1001], 4, 32, 16, False),  # just enough rows for units of 256
 ]
 
 

@@ -151,6 +151,15 @@ def test_a_workspace_too_small_is_refused():
     assert B.lib().bn_paged_q8_workspace_size(C.byref(cache(page_size=8)), 32, 3) == 0
 
 
+@pytest.mark.parametrize("batch,hkv,heads,keys", [(1, 4, 32, 4096), (7, 4, 32, 4096), (7, 4, 32, 40000), (64, 8, 64, 1 << 20),
+                                                  (2, 1, 4, 16384), (300, 3, 15, 500)])
+def test_a_workspace_does_for_fewer_rows(batch, hkv, heads, keys):
+    c = cache(batch=batch, n_kv_heads=hkv, max_pages=-(-keys // 16), table_stride=-(-keys // 16), n_pages=1 << 21)
+    rows = sorted({*range(1, 400), *range(400, 40000, 97), *range(1100 * 128 // heads, 1300 * 128 // heads)})
+    need = [B.lib().bn_paged_q8_workspace_size(C.byref(c), heads, n) for n in rows]
+    assert need[0] > 0 and all(a <= b for a, b in zip(need, need[1:]))
+
+
 # ------------------------------------------------- norms of single heads
 def norm(dtype=B.BN_BF16, q=0x1000, k=0x2000, wq=0x3000, wk=0x4000, qo=0x5000, ko=0x6000, pos=0x7000, n=5, H=8, Hkv=2, D=64,
          qs=512, ks=512, qos=512, kos=128, offset=0, eps=1e-5, theta=1e4):
