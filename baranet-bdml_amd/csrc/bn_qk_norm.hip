@@ -351,7 +351,7 @@ int bn_qk_norm_rope_backward(int dtype, const void *q, const void *k, const void
       BN_LAUNCH_CHECK();
     }
     hipLaunchKernelGGL(qk_norm_rope_weights_kernel, dim3((unsigned)(2 * head_dim / 8)), dim3(256), 0, s, p.parts, groups,
-                       head_dim, dq_weight, n_kv_heads > 0 ? dk_weight : nullptr);
+                       head_dim, dq_weight, dk_weight);
     BN_LAUNCH_CHECK();
     return BN_OK;
   };

@@ -576,7 +576,8 @@ int bn_qk_norm_rope(int dtype, const void *q, const void *k, const void *q_weigh
  * the q and k that it was given, dq and dk (of dtype) and the weights' gradients
  * dq_weight and dk_weight (always fp32, head_dim elements, sums over all rows and
  * heads, the same bits in every run).  dq may be dq_out or q in their place, with
- * their row stride, dk dk_out or k.  n_rows 0: the weights' gradients are zeros.
+ * their row stride, dk dk_out or k.  n_rows 0: the weights' gradients are zeros, and
+ * without k dk_weight's, if it is given.
  * workspace: device memory of bn_qk_norm_rope_backward_workspace_size() bytes,
  * 16-byte aligned, any contents (NULL: taken from the pool); calls in flight at once
  * need workspaces of their own. */

@@ -243,6 +243,19 @@ def test_a_graph_of_both_directions():
             assert torch.equal(a, b), i
 
 
+def test_no_key_heads_give_a_key_weight_no_gradient():
+    x = made("f32", 40, 8, 2, 64)
+    a = {t: x[t].cuda() for t in x}
+    none = a["k"][:, :0]
+    q, k = B.qk_norm_rope(a["q"], none, a["wq"], a["wk"])
+    torch.full((2, 64), 7.0, device="cuda")  # what the gradients' memory held before
+    dq, dk, dwq, dwk = B.qk_norm_rope_backward(a["q"], none, a["wq"], a["wk"], a["gq"], none)
+    alone = B.qk_norm_rope_backward(a["q"], None, a["wq"], None, a["gq"], None)
+    assert k.shape == dk.shape == (40, 0, 64) and (dwk == 0).all()
+    assert torch.equal(dq, alone[0]) and torch.equal(dwq, alone[2]) and alone[3] is None
+    assert torch.equal(q, B.qk_norm_rope(a["q"], None, a["wq"], None)[0])
+
+
 def test_on_a_given_stream():
     x = made("f32", 500, 8, 2, 64)
     a = [x[t].cuda() for t in ("q", "k", "wq", "wk", "gq", "gk")]
