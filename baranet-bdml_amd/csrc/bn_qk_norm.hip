@@ -17,7 +17,8 @@
 namespace bn {
 namespace {
 
-constexpr int kMaxHeadDim = 256, kMostRows = 8;  // rows of a workgroup at once
+constexpr int kMaxHeadDim = 256;
+constexpr int kMostRows = 8, kJoinedRows = 16;  // rows of a workgroup at once; of backward's where one adds all sums
 struct QkParams {
   const void *q, *k, *wq, *wk, *gq, *gk;  // gq, gk: gradients of the outputs (backward)
   void *qo, *ko;                          // outputs (backward: gradients of q and k)
@@ -27,6 +28,8 @@ struct QkParams {
   int64_t offset;
   float eps;
   float *parts;                           // backward: [workgroups][2][D] sums
+  float *dwq, *dwk;                       // the weights' gradients
+  unsigned long long *arrive, tag;
 };
 template <int D>
 struct Turns {  // per position, of each pair (a launch takes 0.35 us less with D = 64's 256 bytes than with D = 256's)
@@ -102,14 +105,19 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkParams p, Turns<D> 
 constexpr int kPairs = 2;  // pieces of rows and gradients of a thread on their way at once
 // A workgroup takes every gridDim.x-th group of `rows` rows.  A thread's pieces lie at
 // one place of their heads, so it adds up eight elements of each weight's
-// gradient in registers; a workgroup's sums go to the workspace.  Bound by memory: 16384
-// bf16 rows of 32 and 4 heads 46 us, 4.9 TB/s (59 with one piece at once), and 4 for the sums'
-// launch; 1504 fp32 rows 12 and 2.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void qk_norm_rope_backward_kernel(QkParams p, Turns<D> t) {
+// gradient in registers; a workgroup's sums go to the workspace, and the last workgroup to
+// arrive (JOINS), or another launch, adds them.  Bound by memory: 16384 bf16 rows of 32 and 4 heads
+// 46 us, 4.9 TB/s (59 with one piece at once), and 4 for the sums' launch; 1504 fp32 rows 14.7
+// with their sums.
+template <typename T, int D, int THREADS, bool JOINS>
+__global__ __launch_bounds__(THREADS) void qk_norm_rope_backward_kernel(QkParams p, Turns<D> t) {
   constexpr int LANES = D / 8;
-  __shared__ float2 cs[kMostRows][D / 2];
-  __shared__ float sums[4][2][D];
+  __shared__ float2 cs[JOINS ? kJoinedRows : kMostRows][D / 2];
+  constexpr int STEP = THREADS / D, N = 16;  // (of the sums behind the rows)
+  __shared__ union {
+    float of_wave[THREADS / 64][2][D], of_groups[STEP][2 * D];
+  } sums;
+  __shared__ bool last;
   const int tid = threadIdx.x, lane = tid & 63, e = tid % LANES * 8;
   Eight dw[2] = {};
   for (int64_t at = (int64_t)blockIdx.x * p.rows; at < p.n_rows; at += (int64_t)gridDim.x * p.rows) {
@@ -127,13 +135,13 @@ __global__ __launch_bounds__(256) void qk_norm_rope_backward_kernel(QkParams p, 
       Raw8<T> wr;
       wr.load((const T *)(side ? p.wk : p.wq) + e);
       const Eight w = wr.floats();
-      Walk at(tid, 256, per);
-      for (int first = tid; first < total; first += 256 * kPairs) {
+      Walk at(tid, THREADS, per);
+      for (int first = tid; first < total; first += THREADS * kPairs) {
         Raw8<T> xr[kPairs], gr[kPairs];
         int row[kPairs], to[kPairs];
 #pragma unroll
         for (int n = 0; n < kPairs; ++n) {
-          if (first + 256 * n >= total) break;
+          if (first + THREADS * n >= total) break;
           row[n] = at.row;
           to[n] = at.rest / LANES * D + e;
           at.step();
@@ -142,7 +150,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_backward_kernel(QkParams p, 
         }
 #pragma unroll
         for (int n = 0; n < kPairs; ++n) {
-          if (first + 256 * n >= total) break;
+          if (first + THREADS * n >= total) break;
           const Eight v = xr[n].floats();
           Eight g = gr[n].floats();
           if (p.turn) turn8(g, &cs[row[n]][e / 2], true);
@@ -172,12 +180,48 @@ __global__ __launch_bounds__(256) void qk_norm_rope_backward_kernel(QkParams p, 
       float s = dw[side].x[j];
 #pragma unroll
       for (int m = LANES; m < 64; m <<= 1) s += __shfl_xor(s, m, 64);
-      if (lane < LANES) sums[tid >> 6][side][e + j] = s;
+      if (lane < LANES) sums.of_wave[tid >> 6][side][e + j] = s;
     }
   __syncthreads();
-  for (int i = tid; i < 2 * D; i += 256)
-    p.parts[(int64_t)blockIdx.x * 2 * D + i] =
-        (sums[0][i / D][i % D] + sums[1][i / D][i % D]) + (sums[2][i / D][i % D] + sums[3][i / D][i % D]);
+  float *const part = p.parts + (int64_t)blockIdx.x * 2 * D;
+  for (int i = 2 * tid; i < 2 * D; i += 2 * THREADS) {
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+      s.x += sums.of_wave[w][i / D][i % D];
+      s.y += sums.of_wave[w][i / D][i % D + 1];
+    }
+    if (JOINS) put2(part + i, s.x, s.y);
+    else *(float2 *)(part + i) = s;
+  }
+  if constexpr (!JOINS) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the sums' stores have reached memory
+  __syncthreads();
+  if (tid == 0) last = arrive_last(p.arrive, (int)gridDim.x, p.tag);
+  __syncthreads();
+  if (!last) return;
+  // The last workgroup to arrive: two elements a thread, of every STEP-th workgroup's sums.
+  const int at2 = tid % D * 2, n = (int)gridDim.x;
+  float2 s = make_float2(0.f, 0.f);
+  for (int i0 = tid / D; i0 < n; i0 += STEP * N) {
+    float2 x[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = i0 + STEP * j < n ? get2(p.parts + (int64_t)(i0 + STEP * j) * 2 * D + at2) : make_float2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      s.x += x[j].x;
+      s.y += x[j].y;
+    }
+  }
+  *(float2 *)&sums.of_groups[tid / D][at2] = s;
+  __syncthreads();
+  for (int i = tid; i < 2 * D; i += THREADS) {
+    float y = 0.f;
+#pragma unroll
+    for (int j = 0; j < STEP; ++j) y += sums.of_groups[j][i];
+    if (i < D) p.dwq[i] = y;
+    else if (p.dwk) p.dwk[i - D] = y;
+  }
 }
 
 // The workgroups' sums, added: eight elements a workgroup, 32 threads an element.
@@ -204,11 +248,29 @@ __global__ __launch_bounds__(256) void qk_norm_rope_weights_kernel(const float *
   else if (dwk) dwk[e - d] = s;
 }
 
-constexpr int kBackGroups = 1024;
 int rows_at_once(int n_rows) { return n_rows >= 8192 ? 8 : n_rows >= 2048 ? 4 : 1; }
-// Backward: more rows a workgroup, so that there are few sums to add (1000 rows 19.8 us with a row each).
-int rows_back(int n_rows) { return std::max(1, std::min(n_rows / 256, kMostRows)); }
-int back_groups(int n_rows) { return std::min((n_rows + rows_back(n_rows) - 1) / rows_back(n_rows), kBackGroups); }
+
+// Backward's launch: its workgroups, their rows at once, whether the last of them adds their sums.
+// It does for small calls, to which a second launch adds more on the host than they take (300 fp32
+// rows of 32 and 4 heads of 64 called one behind the other 15.0 -> 12.1 us; in a graph, where it
+// costs little, 8.1 -> 9.0).  Arrivals are counted one by one and one compute unit reads the sums,
+// so there are at most 128 workgroups and 64 KB of sums (512 bf16 rows in a graph 9.6 us, with 256
+// workgroups 11.8), and a workgroup has at most kJoinedWork elements (777 fp32 rows of heads of
+// 128, which have more, 18.6, now 14.8).
+constexpr size_t kArriveBytes = 256;  // (16 are used: the sums keep their lines: 16384 bf16 rows 51.2 -> 50.1 us)
+constexpr int kBackGroups = 1024, kJoinedGroups = 128, kJoinedWork = 32768;
+struct BackPlan {
+  int rows, groups;
+  bool joins;
+};
+BackPlan plan_back(int n_rows, int heads, int head_dim) {
+  BackPlan d;
+  const int most = std::min(kJoinedGroups, 8192 / head_dim);
+  d.joins = n_rows > 0 && n_rows <= most * kJoinedRows && (int64_t)n_rows * heads * head_dim <= (int64_t)most * kJoinedWork;
+  d.rows = d.joins ? (n_rows + most - 1) / most : std::max(1, std::min(n_rows / 256, kMostRows));
+  d.groups = std::min((n_rows + d.rows - 1) / d.rows, kBackGroups);
+  return d;
+}
 
 int check_qk(const std::string &op, int dtype, const void *q, const void *k, const void *wq, const void *wk,
              int n_rows, int n_heads, int n_kv_heads, int head_dim, float eps, float theta) {
@@ -231,21 +293,21 @@ int check_qk(const std::string &op, int dtype, const void *q, const void *k, con
   return BN_OK;
 }
 
-// K<T, D> for the dtype and head dimension
-#define BN_QK_LAUNCH_D(K, D, grid, s, p)                                                       \
-  do {                                                                                         \
-    Turns<D> t;                                                                                \
-    fill_turns(t.f, D, theta);                                                                 \
-    if (dtype == BN_BF16) hipLaunchKernelGGL((K<bf16_t, D>), grid, dim3(256), 0, s, p, t);     \
-    else hipLaunchKernelGGL((K<float, D>), grid, dim3(256), 0, s, p, t);                       \
+// K<T, D, ...> for the dtype and head dimension
+#define BN_QK_LAUNCH_D(K, D, grid, block, s, p, ...)                                                 \
+  do {                                                                                               \
+    Turns<D> t;                                                                                      \
+    fill_turns(t.f, D, theta);                                                                       \
+    if (dtype == BN_BF16) hipLaunchKernelGGL((K<bf16_t, D, ##__VA_ARGS__>), grid, dim3(block), 0, s, p, t); \
+    else hipLaunchKernelGGL((K<float, D, ##__VA_ARGS__>), grid, dim3(block), 0, s, p, t);            \
   } while (0)
-#define BN_QK_LAUNCH(K, grid, s, p)                            \
-  do {                                                         \
-    if (head_dim == 16) BN_QK_LAUNCH_D(K, 16, grid, s, p);     \
-    else if (head_dim == 32) BN_QK_LAUNCH_D(K, 32, grid, s, p); \
-    else if (head_dim == 64) BN_QK_LAUNCH_D(K, 64, grid, s, p); \
-    else if (head_dim == 128) BN_QK_LAUNCH_D(K, 128, grid, s, p); \
-    else BN_QK_LAUNCH_D(K, 256, grid, s, p);                   \
+#define BN_QK_LAUNCH(K, grid, block, s, p, ...)                                          \
+  do {                                                                                   \
+    if (head_dim == 16) BN_QK_LAUNCH_D(K, 16, grid, block, s, p, ##__VA_ARGS__);         \
+    else if (head_dim == 32) BN_QK_LAUNCH_D(K, 32, grid, block, s, p, ##__VA_ARGS__);    \
+    else if (head_dim == 64) BN_QK_LAUNCH_D(K, 64, grid, block, s, p, ##__VA_ARGS__);    \
+    else if (head_dim == 128) BN_QK_LAUNCH_D(K, 128, grid, block, s, p, ##__VA_ARGS__);  \
+    else BN_QK_LAUNCH_D(K, 256, grid, block, s, p, ##__VA_ARGS__);                       \
   } while (0)
 
 }  // namespace
@@ -283,7 +345,7 @@ int bn_qk_norm_rope(int dtype, const void *q, const void *k, const void *q_weigh
   p.offset = position_offset;
   p.eps = eps;
   const dim3 grid((unsigned)((n_rows + p.rows - 1) / p.rows));
-  BN_QK_LAUNCH(qk_norm_rope_kernel, grid, as_stream(stream), p);
+  BN_QK_LAUNCH(qk_norm_rope_kernel, grid, 256, as_stream(stream), p);
   BN_LAUNCH_CHECK();
   return BN_OK;
 }
@@ -293,7 +355,7 @@ size_t bn_qk_norm_rope_backward_workspace_size(int n_rows, int n_heads, int n_kv
   if (check_qk("", BN_F32, &w, n_kv_heads > 0 ? &w : nullptr, (const void *)16, (const void *)16, n_rows, n_heads, n_kv_heads,
                head_dim, 0.f, 0.f))
     return 0;
-  return (size_t)back_groups(n_rows) * 2 * head_dim * sizeof(float);
+  return kArriveBytes + (size_t)std::min(n_rows, kBackGroups) * 2 * head_dim * sizeof(float);  // (does for fewer rows)
 }
 
 int bn_qk_norm_rope_backward(int dtype, const void *q, const void *k, const void *q_weight, const void *k_weight,
@@ -336,21 +398,30 @@ int bn_qk_norm_rope_backward(int dtype, const void *q, const void *k, const void
   p.q_rs = q_row_stride; p.k_rs = k_row_stride; p.gq_rs = dq_out_row_stride; p.gk_rs = dk_out_row_stride;
   p.qo_rs = dq_row_stride; p.ko_rs = dk_row_stride;
   p.n_rows = n_rows; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads;
-  p.rows = rows_back(n_rows);
+  const BackPlan d = plan_back(n_rows, n_heads + n_kv_heads, head_dim);
+  p.rows = d.rows;
   p.turn = theta > 0.f;
   p.offset = position_offset;
   p.eps = eps;
   Workspace ws;
   if ((st = ws.take(workspace, need, stream))) return st;
-  p.parts = (float *)ws.p;
+  p.arrive = (unsigned long long *)ws.p;
+  p.parts = (float *)((char *)ws.p + kArriveBytes);
+  p.dwq = dq_weight; p.dwk = dk_weight;
+  p.tag = next_tag();
   hipStream_t s = as_stream(stream);
-  const int groups = back_groups(n_rows);
   auto launch = [&]() -> int {
-    if (groups > 0) {
-      BN_QK_LAUNCH(qk_norm_rope_backward_kernel, dim3((unsigned)groups), s, p);
+    if (d.groups > 0) {
+      // (512 threads for bf16 in few workgroups for a compute unit: 2048 rows 13.9 -> 12.6 us, of heads
+      // of 256 38.4 -> 29.1; 16384 rows 49.6 -> 52.4; 777 of heads of 256 in fp32 24.3 -> 27.3)
+      const dim3 grid((unsigned)d.groups);
+      if (d.joins) BN_QK_LAUNCH(qk_norm_rope_backward_kernel, grid, 512, s, p, 512, true);
+      else if (dtype == BN_BF16 && d.groups <= kBackGroups / 2) BN_QK_LAUNCH(qk_norm_rope_backward_kernel, grid, 512, s, p, 512, false);
+      else BN_QK_LAUNCH(qk_norm_rope_backward_kernel, grid, 256, s, p, 256, false);
       BN_LAUNCH_CHECK();
     }
-    hipLaunchKernelGGL(qk_norm_rope_weights_kernel, dim3((unsigned)(2 * head_dim / 8)), dim3(256), 0, s, p.parts, groups,
+    if (d.joins) return BN_OK;
+    hipLaunchKernelGGL(qk_norm_rope_weights_kernel, dim3((unsigned)(2 * head_dim / 8)), dim3(256), 0, s, p.parts, d.groups,
                        head_dim, dq_weight, dk_weight);
     BN_LAUNCH_CHECK();
     return BN_OK;

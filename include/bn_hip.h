@@ -578,9 +578,9 @@ int bn_qk_norm_rope(int dtype, const void *q, const void *k, const void *q_weigh
  * heads, the same bits in every run).  dq may be dq_out or q in their place, with
  * their row stride, dk dk_out or k.  n_rows 0: the weights' gradients are zeros, and
  * without k dk_weight's, if it is given.
- * workspace: device memory of bn_qk_norm_rope_backward_workspace_size() bytes,
- * 16-byte aligned, any contents (NULL: taken from the pool); calls in flight at once
- * need workspaces of their own. */
+ * workspace: device memory of bn_qk_norm_rope_backward_workspace_size() bytes (which
+ * does for fewer rows too), 16-byte aligned, any contents (NULL: taken from the pool);
+ * calls in flight at once need workspaces of their own. */
 size_t bn_qk_norm_rope_backward_workspace_size(int n_rows, int n_heads, int n_kv_heads,
                                                int head_dim);
 int bn_qk_norm_rope_backward(int dtype, const void *q, const void *k,

@@ -198,6 +198,33 @@ def test_weights_gradients_are_the_same_every_time(n):
         assert (first[2] == 0).all() and (first[3] == 0).all()
 
 
+@pytest.mark.parametrize("D,H,Hkv,sizes", [
+    (64, 32, 4, [1, 1820, 129, 5000, 128, 1821, 700, 300]),  # sums added by the last workgroup and by another launch
+    (256, 3, 1, [700, 3, 512, 9000, 513, 32, 33]),
+    (16, 40, 1, [2048, 100, 2049, 8193, 5, 2000]),
+])
+def test_a_workspace_goes_from_call_to_call(D, H, Hkv, sizes):
+    """One workspace, never cleared, for calls of other sizes behind each other: every call's gradients are
+    those of a fresh workspace, and the weights' those of 64 bits."""
+    ws = B.qk_norm_rope_workspace(max(sizes), H, Hkv, D)
+    ws.fill_(0x5b)
+    x = made("bf16", max(sizes), H, Hkv, D, 4)
+    a = {t: x[t].cuda() for t in x}
+    for n in sizes:
+        print("workspace", D, n, flush=True)
+        args = a["q"][:n], a["k"][:n], a["wq"], a["wk"], a["gq"][:n], a["gk"][:n]
+        got = [B.qk_norm_rope_backward(*args, workspace=ws) for _ in range(3)]
+        fresh = B.qk_norm_rope_backward(*args)
+        for g in got:
+            for u, v in zip(g, fresh):
+                assert torch.equal(u, v), n
+        for t, dw, heads in (("q", fresh[2], H), ("k", fresh[3], Hkv)):
+            _, want, _, size = backward64(x[t][:n].double().numpy(), x["w" + t].double().numpy(), x["g" + t][:n].double().numpy(), np.arange(n),
+                                          1e-5, 1e4)
+            depth = n * heads / (256 / (D / 8)) + 1024 / 32 + 30
+            assert (np.abs(host(dw) - want) <= size * ((2 * D + 60 + depth) * 2.0 ** -24)).all(), (n, t)
+
+
 def test_infinite_and_nan_elements_stay_in_their_head():
     x = made("f32", 4, 3, 1, 64, 3)
     x["q"][1, 1, 7], x["q"][2, 0, 3] = float("nan"), float("inf")

@@ -293,3 +293,9 @@ def test_outputs_are_memory_of_the_stream_that_writes_them(monkeypatch):
         made.clear()
         call()
         assert made == [st] * n
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(32, 4, 64), (3, 1, 256), (40, 0, 16), (64, 8, 128)])
+def test_a_workspace_of_the_norms_does_for_fewer_rows(H, Hkv, D):
+    need = [B.lib().bn_qk_norm_rope_backward_workspace_size(n, H, Hkv, D) for n in [*range(0, 3000), 8191, 8192, 1 << 23]]
+    assert need[1] > 0 and all(a <= b for a, b in zip(need, need[1:]))
