@@ -470,7 +470,10 @@ int bn_gqa_decode_noalloc(int dtype, const void *q, const void *k_cache,
  * form them).  What is infinite or NaN reaches the rows that see it and no other: an
  * element of such a value makes that element of every row that sees its key
  * infinite or NaN (infinite, or NaN where its weight is 0 or infinities of both
- * signs meet), whatever the key's weight.  Any number of
+ * signs meet), whatever the key's weight.  A row's weighted values are added before
+ * they are divided by its weights' sum, the weights up to 2^14 then: values of more than
+ * 2^113 / (the row's keys, up to a multiple of 64) may overflow to an infinite or NaN
+ * output whose quotient is finite.  Any number of
  * query heads per KV head, at most 65535 heads; query head h reads KV head
  * h / (n_heads / n_kv_heads).
  *
