@@ -727,7 +727,7 @@ def _qk_weight(op, name, w, d, dtype, device):
     return w.data_ptr()
 
 
-def _qk_args(op, q, k, q_weight, k_weight, positions, stream):
+def _qk_args(op, q, k, q_weight, k_weight, positions, position_offset, stream):
     """What both directions check alike: (type's code, stream, pointers of the positions and of the
     weights, what _qk_rows wants of q's shape)."""
     if q.dim() != 3 or (k is not None and k.dim() != 3):
@@ -737,6 +737,8 @@ def _qk_args(op, q, k, q_weight, k_weight, positions, stream):
         raise ValueError(f"{op}: q must be float32 or bfloat16")
     if (k is None) != (k_weight is None):
         raise ValueError(f"{op}: k and k_weight must be given together")
+    if not -0x80000000 <= position_offset <= 0x7fffffff:  # (ctypes would keep its lowest 32 bits)
+        raise ValueError(f"{op}: position_offset must fit in 32 bits")
     wq = _qk_weight(op, "q_weight", q_weight, d, dtype, device)
     wk = None if k is None else _qk_weight(op, "k_weight", k_weight, d, dtype, device)
     import torch
@@ -771,7 +773,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, eps=1e-5, positions=None, position_of
     Heads contiguous, row strides of their own; float32 or bfloat16.  k and
     k_weight may be None.  q_out may be q, k_out k."""
     op = "qk_norm_rope"
-    code, s, pp, wq, wk, rows, heads, kind = _qk_args(op, q, k, q_weight, k_weight, positions, stream)
+    code, s, pp, wq, wk, rows, heads, kind = _qk_args(op, q, k, q_weight, k_weight, positions, position_offset, stream)
     q_out = _like(q, stream) if q_out is None else q_out
     qp, qs = _qk_rows(op, "q", q, rows, heads, *kind)
     op_, os_ = _qk_rows(op, "q_out", q_out, rows, heads, *kind)
@@ -803,7 +805,7 @@ def qk_norm_rope_backward(q, k, q_weight, k_weight, dq_out, dk_out, eps=1e-5, po
     are None."""
     import torch
     op = "qk_norm_rope_backward"
-    code, s, pp, wq, wk, rows, heads, kind = _qk_args(op, q, k, q_weight, k_weight, positions, stream)
+    code, s, pp, wq, wk, rows, heads, kind = _qk_args(op, q, k, q_weight, k_weight, positions, position_offset, stream)
     if (k is None) != (dk_out is None):
         raise ValueError(f"{op}: k and dk_out must be given together")
     d = kind[0]
