@@ -9,6 +9,7 @@
 // kernels are those of the bf16 cache behind the conversion.
 #include "bn_head_rows.hpp"
 #include "bn_paged_host.hpp"
+#include "bn_q8_plan.hpp"
 
 namespace bn {
 namespace {
@@ -382,9 +383,7 @@ struct Q8DecodeLds {
   int sums[2][kWaves], rank0, last_in[2];
 };
 
-// ONCE: rows past the caches' keeping, where no other workgroup reads their lines: pages whose rows of a
-// KV head lie one behind the other (64 caches of 4096 keys 27.9 us, else 31.5); of token-major pages two
-// heads' rows share a line (64 caches of 512..4096 23.9 us, else 26.1; 33.4 on XCDs of their own).
+// ONCE: rows past the caches' keeping (decode_reads_once).
 template <bool ONCE>
 __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodeParams p, E4m3Pages src) {
   __shared__ __attribute__((aligned(16))) Q8DecodeLds lds;
@@ -880,7 +879,7 @@ int launch_decode(const AttnParams &a, int dtype, const E4m3Scales &scales, void
   p.cuts = nullptr;
   const dim3 grid((unsigned)(d.bins * d.columns));
   if (dtype == BN_F32) hipLaunchKernelGGL(paged_q8_decode_f32_kernel, grid, dim3(256), 0, s, p, E4m3PagesF32{scales});
-  else if (a.c.row_stride == HD) hipLaunchKernelGGL(paged_q8_decode_kernel<true>, grid, dim3(64 * kWaves), 0, s, p, E4m3Pages{scales});
+  else if (decode_reads_once(a.c.row_stride, d.hblocks)) hipLaunchKernelGGL(paged_q8_decode_kernel<true>, grid, dim3(64 * kWaves), 0, s, p, E4m3Pages{scales});
   else hipLaunchKernelGGL(paged_q8_decode_kernel<false>, grid, dim3(64 * kWaves), 0, s, p, E4m3Pages{scales});
   BN_LAUNCH_CHECK();
   return BN_OK;
