@@ -13,12 +13,12 @@
 
 #include "bn_head_rows.hpp"
 #include "bn_paged_host.hpp"
+#include "bn_qk_plan.hpp"
 
 namespace bn {
 namespace {
 
 constexpr int kMaxHeadDim = 256;
-constexpr int kMostRows = 8, kJoinedRows = 16;  // rows of a workgroup at once; of backward's where one adds all sums
 struct QkParams {
   const void *q, *k, *wq, *wk, *gq, *gk;  // gq, gk: gradients of the outputs (backward)
   void *qo, *ko;                          // outputs (backward: gradients of q and k)
@@ -246,30 +246,6 @@ __global__ __launch_bounds__(256) void qk_norm_rope_weights_kernel(const float *
   s = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
   if (e < d) dwq[e] = s;
   else if (dwk) dwk[e - d] = s;
-}
-
-int rows_at_once(int n_rows) { return n_rows >= 8192 ? 8 : n_rows >= 2048 ? 4 : 1; }
-
-// Backward's launch: its workgroups, their rows at once, whether the last of them adds their sums.
-// It does for small calls, to which a second launch adds more on the host than they take (300 fp32
-// rows of 32 and 4 heads of 64 called one behind the other 15.0 -> 12.1 us; in a graph, where it
-// costs little, 8.1 -> 9.0).  Arrivals are counted one by one and one compute unit reads the sums,
-// so there are at most 128 workgroups and 64 KB of sums (512 bf16 rows in a graph 9.6 us, with 256
-// workgroups 11.8), and a workgroup has at most kJoinedWork elements (777 fp32 rows of heads of
-// 128, which have more, 18.6, now 14.8).
-constexpr size_t kArriveBytes = 256;  // (16 are used: the sums keep their lines: 16384 bf16 rows 51.2 -> 50.1 us)
-constexpr int kBackGroups = 1024, kJoinedGroups = 128, kJoinedWork = 32768;
-struct BackPlan {
-  int rows, groups;
-  bool joins;
-};
-BackPlan plan_back(int n_rows, int heads, int head_dim) {
-  BackPlan d;
-  const int most = std::min(kJoinedGroups, 8192 / head_dim);
-  d.joins = n_rows > 0 && n_rows <= most * kJoinedRows && (int64_t)n_rows * heads * head_dim <= (int64_t)most * kJoinedWork;
-  d.rows = d.joins ? (n_rows + most - 1) / most : std::max(1, std::min(n_rows / 256, kMostRows));
-  d.groups = std::min((n_rows + d.rows - 1) / d.rows, kBackGroups);
-  return d;
 }
 
 int check_qk(const std::string &op, int dtype, const void *q, const void *k, const void *wq, const void *wk,
