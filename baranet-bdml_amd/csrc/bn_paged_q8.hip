@@ -885,17 +885,6 @@ int launch_decode(const AttnParams &a, int dtype, const E4m3Scales &scales, void
   return BN_OK;
 }
 
-// Codes are turned into bf16 once a tile and workgroup, so that units of 256 rows pay
-// at fewer rows than in a cache of bf16: with 32 and 4 heads the pipelined kernel takes, and
-// units of 128, for 4 x 1024 rows (1028 units) 36.4 us and 35.3, 3 x 1500 (1128) 48.1 and 47.8,
-// 2 x 2500 (1252) 74.3 and 77.3, 5200 (1304) 166 and 189, 6 prompts of 600..1100 behind 2000
-// keys 121 and 128, 7 of 165..1500 behind up to 700 83 and 87.
-constexpr int kPipeFrom = 1200;
-
-PrefillPlan plan_q8(int dtype, int n_seq, int n_rows, int n_heads, int n_kv_heads, int cap, bool most = false) {
-  return plan_prefill(dtype, n_seq, n_rows, n_heads, n_kv_heads, cap, most, kPipeFrom);
-}
-
 int launch_prefill(const AttnParams &a, int dtype, const E4m3Scales &scales, void *ws, hipStream_t s) {
   const PrefillPlan d = plan_q8(dtype, a.c.batch, a.n_rows, a.n_heads, a.c.n_kv_heads, a.c.cap);
   PrefillParams p;
