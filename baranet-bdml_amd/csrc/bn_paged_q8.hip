@@ -364,10 +364,11 @@ struct E4m3PagesF32 : E4m3Scales {  // as fp32
 // lane's scores of two tiles are those of eight keys in a row, V's operand's order.
 //
 // Bound by memory, and for small calls by the chain lengths -> list -> table -> rows ->
-// parts -> records: 64 caches of 4096 keys (32 and 4 heads) 29 us, 4.6 TB/s; of 512..4096
-// 22.5, 3.5 TB/s, of which 6 are that chain and 3 the records; three of 34763 to 131072 31.5,
-// 4.0 TB/s; one of 640 9.4.  Four waves and two tiles each in flight: 31.5 and 41.8 us for the
-// second and third.  (Per tile the matrix cores are 6%, VALU 31%, LDS 26% busy.)
+// parts -> records: 64 caches of 4096 keys (32 and 4 heads) 29.9 us, 4.5 TB/s; of 512..4096
+// 22.5, 3.5 TB/s, of which 6 are that chain and 3 the records; three of 34763 to 131072 34.8,
+// three of 5003 to 131072 30, 4.2 TB/s; one of 640 9.4.  Four waves and two tiles each in flight,
+// before the probabilities were two values: 31.5 and 41.8 us for the second and third.  (Matrix cores 8
+// to 11%, VALU 37 to 39%, LDS 25 to 29% busy.)
 constexpr int kWaves = 8, kTile = 64;
 constexpr int kListed = 32;                  // sequences of a list
 constexpr int kHoldParts = 256;              // rows of LDS for the waves' parts of sequences
@@ -632,7 +633,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_q8_decode_kernel(DecodePara
         }
         // The probabilities are taken against a reference that is the true running maximum only when it was
         // last moved: it moves when a lane's weights against it pass 2^16 in sum (or are NaN).  They enter the
-        // products as two bf16 values each, the upper 16 bits and what is left of them (off by at most 2^-17
+        // products as two bf16 values each, the upper 16 bits and what is left of them (off by at most 2^-16
         // together; rounded to one, 3 caches of up to 131072 keys were 0.0024 off 64 bits, not 0.0017).
         float e[16], rs;
         auto weigh = [&](float ref) __attribute__((always_inline)) {
@@ -829,7 +830,11 @@ __global__ __launch_bounds__(64 * HW * KW, OCC) void paged_q8_prefill_kernel(Pre
   __shared__ __attribute__((aligned(16))) PrefillLds<HW, KW> lds;
   prefill_bf16_body<HW, KW>(p, lds, blockIdx.x, src);
 }
-// Queries in fp32: the fp32 cache's kernels, whose time the matrix cores' fp32 rate sets.
+// Queries in fp32: the fp32 cache's kernels.  A prefill's time is mostly the matrix cores' fp32 rate (64%
+// busy, VALU 20%): 8192 rows of 32 and 4 heads 2800 us, 98 TFLOP/s, 64% of an 8192^3 fp32 library
+// product's rate; 2048 rows 215 us.  A decode's is not, nor memory's: its four waves walk 16 keys a step,
+// one step's rows in flight (matrix cores 25%, VALU 15% busy, 60% of the waves' time waiting): 64
+// caches of 512..4096 keys 73 us, 1.07 TB/s, where bf16 queries take 22.5; of 4096 115; one of 640 8.6.
 __global__ __launch_bounds__(256) void paged_q8_decode_f32_kernel(DecodeParams p, E4m3PagesF32 src) {
   __shared__ __attribute__((aligned(16))) DecodeLds<float> lds;
   decode_body<float>(p, lds, blockIdx.x, src);

@@ -9,9 +9,9 @@ namespace bn {
 namespace {
 
 // Whether a decode's rows go past the caches' keeping: where no other workgroup reads their lines.
-// Of pages whose rows of a KV head lie one behind the other none does (64 caches of 4096 keys 27.9 us,
-// else 31.5); of token-major pages two heads' rows share a line (64 caches of 512..4096 23.9 us, else
-// 26.1; 33.4 on XCDs of their own); and blocks of more than one of query heads (more than 16 a KV
+// Of pages whose rows of a KV head lie one behind the other none does (64 caches of 4096 keys 29.9 us,
+// else 33.1; three of 34763 to 131072 34.8, 38.5; 64 of 512..4096 23.6, 23.1); of token-major pages two
+// heads' rows share a line (64 caches of 4096 35.3 us, else 38.4; of 512..4096 24.2, 27.9; 33.4 on XCDs of their own); and blocks of more than one of query heads (more than 16 a KV
 // head) read all rows once each (64 caches of 4096 keys, 2 KV heads of 32 query heads each, 21.9 us,
 // else 23.3; 64 of 512..4096, 4 of 32, 30.7, 32.6; of 1 of 32 18.2, 18.0).
 inline bool decode_reads_once(int64_t row_stride, int hblocks) { return row_stride == HD && hblocks == 1; }

@@ -50,7 +50,8 @@ __device__ __forceinline__ void angles(const QkParams &p, const Turns<D> &t, flo
 // `rows` rows a workgroup: their angles once, then their heads' pieces of eight
 // elements, four of a thread on their way at once, the first of them while the
 // angles are formed.  Bound by memory, VALU 87% busy: 8192 bf16 rows of 32 and 4 heads
-// 15.6 us, 4.8 TB/s, a copy's rate; 16 rows 3.1, a launch.  (Stores past the caches' keeping: 16384
+// 15.6 us, 4.8 TB/s, a large copy's rate (a copy of as many bytes, all of which the memory-side cache
+// holds, 12.3); as fp32 37, 4.1 TB/s; 16 rows 3.1, a launch.  (Stores past the caches' keeping: 16384
 // rows 35 -> 25 us, but the attention that reads them takes as much longer.)
 constexpr int kPieces = 4;
 template <typename T, int D>
